@@ -408,8 +408,9 @@ def _norm_call(st, ctx, h, gate, r, w, form, new, out, out_scales=None, **more):
     prm = ctx.block_norm_params(rows, dim, post=_codes(form["post"]), pre=_codes(form["pre"]), gate_act=_codes(form["act"]),
                                 gate_rows=0 if gate is None or gate.shape[0] == 1 else 1, eps=EPS, res_scale=form["res_scale"],
                                 branch_scale=form["branch_scale"], **more)
-    return ctx.block_norm, (prm, H(h), None if gate is None else H(gate), H(r), H(w["post"]), H(w["post_bias"]) if form["post"] == "layer" else None, H(w["pre"]),
-                            H(w["pre_bias"]) if form["pre"] == "layer" else None, H(new), H(out), None if out_scales is None else H(out_scales))
+    affine = lambda kind, name: (None if kind == "none" else H(w[name]), H(w[name + "_bias"]) if kind == "layer" else None)  # noqa: E731
+    return ctx.block_norm, (prm, H(h), None if gate is None else H(gate), H(r), *affine(form["post"], "post"), *affine(form["pre"], "pre"), H(new), H(out),
+                            None if out_scales is None else H(out_scales))
 
 
 def _calls_norm(st):
