@@ -41,6 +41,8 @@
 #ifndef LUX_CUDA_QUANT_H
 #define LUX_CUDA_QUANT_H
 
+#include <stddef.h>
+
 #include "lux/gpu/backend_plugin.h"
 #include "lux/gpu/kernel_loader.h"
 
@@ -52,6 +54,20 @@ extern "C" {
 #define LUX_CUDA_PRO_RMS_NORM 1
 #define LUX_CUDA_PRO_SUM3 2
 #define LUX_CUDA_QUANT_VERSION 7u /* 2: symm_* and qmatmul_sharded_push appended; 3: sum3, mul_rms_norm; 4: qmatmul_pro; 5: qmatmul_batch; 6: qmatmul_sharded_push_batch; 7: qmatmul_sharded_push_pro */
+/* Entries behind qmatmul_sharded_push_pro are told by the table's size, not by its version:
+ * LUX_CUDA_QUANT_HAS(q, mx4_matmul) is true where the library that filled *q has that entry. */
+#define LUX_CUDA_QUANT_HAS(q, entry) \
+    ((q)->magic == LUX_CUDA_QUANT_MAGIC && (q)->size >= offsetof(lux_gpu_quant_vtbl, entry) + sizeof((q)->entry))
+/* microscaled 4-bit formats: see mx4_scale_bytes below */
+#define LUX_CUDA_MX4_E8M0 1
+#define LUX_CUDA_MX4_E4M3 2
+/* norms and gate functions of block_norm */
+#define LUX_CUDA_NORM_NONE 0
+#define LUX_CUDA_NORM_RMS 1
+#define LUX_CUDA_NORM_LAYER 2
+#define LUX_CUDA_GATE_IDENTITY 0
+#define LUX_CUDA_GATE_SIGMOID 1
+#define LUX_CUDA_GATE_TANH 2
 #define LUX_CUDA_QMM_KERNEL_NAME "lux.qmm.affine"
 #define LUX_CUDA_NCCL_UID_BYTES 128
 
@@ -59,6 +75,20 @@ extern "C" {
 typedef struct lux_qmm_params {
     int32_t M, K, N, bits, group, x_dtype, sb_dtype, y_dtype;
 } lux_qmm_params;
+
+/* what block_norm does (see there); lds in elements, 0 = dim */
+typedef struct lux_block_norm_params {
+    uint64_t rows, dim;
+    uint64_t h_ld, gate_ld;  /* row strides of h and gate */
+    uint64_t gate_rows;      /* neighbouring rows that share a row of gate; 0: one row of gate for all */
+    int32_t post_norm, pre_norm;         /* LUX_CUDA_NORM_* */
+    int32_t gate_act;                    /* LUX_CUDA_GATE_* */
+    int32_t x_dtype, r_dtype, out_dtype; /* LuxBackendDtype of h and gate; of r and r_out; of out */
+    int32_t out_format;                  /* 0: out holds out_dtype; LUX_CUDA_MX4_*: codes, with their scales in out_scales */
+    float eps, res_scale, branch_scale;
+    float out_pre;                       /* `pre` of mx4_quantize, where out_format is set */
+    uint32_t _pad;
+} lux_block_norm_params;
 
 /* One rank of a column-sharded layer (see shard_* below). */
 typedef struct LuxCudaShardComm LuxCudaShardComm;
@@ -270,6 +300,51 @@ typedef struct lux_gpu_quant_vtbl {
                                                 LuxBackendBuffer* scales_local, LuxBackendBuffer* biases_local,
                                                 int M, int K, int N_local, int bits, int group, LuxBackendDtype y_dtype,
                                                 int prologue, size_t x_ld, float eps);
+
+    /* --- microscaled 4-bit floating point: quantisation, expansion, product (LUX_CUDA_QUANT_HAS) ---
+     * (No counterpart in the reference, which has no quantized format.)
+     * codes   uint32[rows][K/8], LSB-first along K as the 4-bit words above; a code is E2M1: sign (bit 3), then
+     *         0 0.5 1 1.5 2 3 4 6.  K is a multiple of 32.
+     * scales  one byte per block of a row:  LUX_CUDA_MX4_E8M0: 32 codes, 2^(byte-127), 255 = NaN;
+     *                                       LUX_CUDA_MX4_E4M3: 16 codes, an 8-bit float (4 exponent bits, bias 7;
+     *                                       3 mantissa bits; 0x7F = NaN).
+     *         They lie as the tensor cores read them, in tiles of 128 rows x 4 blocks: with nb = K/block and
+     *         nt = ceil(nb/4), the scale of (row r, block b) is byte
+     *             ((r/128)*nt + b/4)*512 + (r%32)*16 + (r/32%4)*4 + b%4.
+     *         Bytes of blocks past nb are zero (mx4_quantize writes them so; a host that fills tiles itself owes it);
+     *         those of rows past the last are never looked at.  A factor for the whole tensor, which E4M3 scales need to
+     *         stay in their range, is the caller's: pre = 1/factor here, post = factor or alpha = the operands' factors
+     *         multiplied there.
+     * mx4_scale_bytes: size of the scales of [rows][K] (0 for arguments that no call takes). */
+    size_t (*mx4_scale_bytes)(int rows, int K, int format);
+    /* u = in * pre (fp32, rounded once), F32 or BF16 with row stride ld (elements, 0 = K); per block, with m = max |u|:
+     *   E8M0: scale 2^(floor(log2 m) - 2), at least 2^-127; an infinite m counts as the largest finite value;
+     *   E4M3: scale = m/6 rounded to fp32, then to the nearest 8-bit float, ties to even, at most 448;
+     * codes = u / scale to the nearest, ties to the even code, at most 6 in magnitude (0 where the scale is 0).  A block with
+     * a NaN gets a NaN for its scale. */
+    LuxBackendError (*mx4_quantize)(LuxBackendContext* ctx, LuxBackendBuffer* in, LuxBackendBuffer* codes, LuxBackendBuffer* scales,
+                                    int rows, int K, size_t ld, int format, LuxBackendDtype in_dtype, float pre);
+    /* out[rows][K] = code * scale * post (fp32), as F32 or rounded to BF16. */
+    LuxBackendError (*mx4_dequantize)(LuxBackendContext* ctx, LuxBackendBuffer* codes, LuxBackendBuffer* scales, LuxBackendBuffer* out,
+                                      int rows, int K, int format, LuxBackendDtype out_dtype, float post);
+    /* y[M,N] = alpha * x[M,K] . W[N,K]^T, both operands in one format, any M; fp32 accumulation of exact products, y F32 or BF16.
+     * Needs no workspace. */
+    LuxBackendError (*mx4_matmul)(LuxBackendContext* ctx, LuxBackendBuffer* x_codes, LuxBackendBuffer* x_scales, LuxBackendBuffer* w_codes,
+                                  LuxBackendBuffer* w_scales, LuxBackendBuffer* y, int M, int K, int N, int format, LuxBackendDtype y_dtype,
+                                  float alpha);
+
+    /* --- the row step between two blocks: norm, gate, residual sum, norm (LUX_CUDA_QUANT_HAS) ---
+     * Per row, in fp32:
+     *   b     = post_norm(h)         none; rms: h / sqrt(mean(h^2) + eps) * post_w; layer: (h - mean) / sqrt(var + eps) * post_w + post_b
+     *   r_out = res_scale * r + branch_scale * act(gate) * b          rounded to r_dtype
+     *   out   = pre_norm(r_out)      with pre_w, pre_b; as out_dtype, or rounded to bf16 and quantised as mx4_quantize does
+     * Weights and biases are fp32 [dim]; NULL: ones and zeros (a bias goes with a layer norm only).  gate NULL: 1.  h NULL: r_out =
+     * res_scale * r; r NULL: the branch alone.  r_out or out may be NULL.  r_out may be r itself; otherwise what is written
+     * overlaps nothing that is read.  A multiple of 32 for dim where out_format is set.  Rows of more than 32768 elements (16384
+     * where dim is no multiple of 8) need r_out.  (op_rms_norm_f32 and op_layer_norm_f32, backend_plugin.h:175-178, are its parts.) */
+    LuxBackendError (*block_norm)(LuxBackendContext* ctx, const lux_block_norm_params* params, LuxBackendBuffer* h, LuxBackendBuffer* gate,
+                                  LuxBackendBuffer* r, LuxBackendBuffer* post_w, LuxBackendBuffer* post_b, LuxBackendBuffer* pre_w,
+                                  LuxBackendBuffer* pre_b, LuxBackendBuffer* r_out, LuxBackendBuffer* out, LuxBackendBuffer* out_scales);
 } lux_gpu_quant_vtbl;
 
 /* Entry points exported with default visibility. */

@@ -305,6 +305,37 @@ cudaError_t launch_rms_norm(const void* in, void* out, const float* weight, size
 cudaError_t launch_sum3(const void* in, void* out, size_t rows, size_t cols, size_t ld, cudaStream_t stream, bool overlap_prev = false);
 cudaError_t launch_mul_rms_norm(const void* in, void* out, size_t rows, size_t cols, size_t ld, float eps, cudaStream_t stream,
                                 bool overlap_prev = false);
+// microscaled 4-bit floating point (mx4_quant.cu, mx4_gemm.cu; the format: mx4.cuh)
+cudaError_t launch_mx4_quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, int format, int in_dtype, float pre,
+                                cudaStream_t stream, bool overlap_prev);
+cudaError_t launch_mx4_dequantize(const uint32_t* codes, const uint8_t* scales, void* out, int rows, int K, int format, int out_dtype, float post,
+                                  cudaStream_t stream);
+struct Mx4MatmulArgs {
+    const uint32_t* xq;
+    const uint8_t* xs;
+    const uint32_t* wq;
+    const uint8_t* ws;
+    void* y;
+    int M, K, N, format, y_dtype;
+    float alpha;
+    int* error;  // as QmmArgs::error
+};
+// overlap_prev: as above; the weights are then read ahead of the wait for that kernel
+cudaError_t launch_mx4_matmul(const Mx4MatmulArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
+// the row step between two blocks (block_norm.cu)
+struct BlockNormArgs {
+    const void *h, *gate, *r;
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    void *r_out, *out;
+    uint8_t* out_scales;
+    size_t rows, dim, h_ld, gate_ld, gate_rows;  // gate_rows: rows that share a row of gate (0: all)
+    int post_kind, pre_kind, gate_act, out_format;
+    bool x_bf16, r_bf16, out_bf16;
+    bool h_vec, gate_vec, r_vec, r_out_vec, out_vec, w_vec;  // every row starts on a 16-byte boundary
+    float eps, res_scale, branch_scale, out_pre;
+};
+bool block_norm_needs_stream(size_t dim);  // rows so long that r' is read back from r_out
+cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);
 cudaError_t launch_flush(void* buf, size_t bytes, cudaStream_t stream);
@@ -327,6 +358,7 @@ const lux_gpu_quant_vtbl* quant_vtbl();
 LuxBackendError qmatmul_on_stream(Context* c, const QmmArgs& a);
 void fill_shard_entries(lux_gpu_quant_vtbl* t);
 void fill_symm_entries(lux_gpu_quant_vtbl* t);
+void fill_mx4_entries(lux_gpu_quant_vtbl* t);  // mx4_api.cu: mx4_* and block_norm
 LuxBackendError ensure_qmv_workspace(Context* c, size_t bytes);  // scratch of the decode kernel, grown on demand
 LuxBackendError ensure_qmm_workspace(Context* c);                // scratch of the prefill GEMM, created on first use
 

@@ -525,6 +525,11 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.rms_norm", "rms_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.sum3", "sum3", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.mul_rms_norm", "mul_rms_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.mx4.quantize", "mx4_quantize", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.mx4.dequantize", "mx4_dequantize", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.mx4.matmul", "mx4_tile<e8m0>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.mx4.matmul", "mx4_tile<e4m3>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.block_norm", "block_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
 };
 const LuxKernelRegistry g_registry = {"cuda", g_kernels, sizeof(g_kernels) / sizeof(g_kernels[0])};
 

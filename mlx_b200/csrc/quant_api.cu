@@ -637,6 +637,7 @@ void fill_quant() {
     g_quant.mul_rms_norm = mul_rms_norm;
     g_quant.qmatmul_pro = qmatmul_pro;
     g_quant.qmatmul_batch = qmatmul_batch;
+    fill_mx4_entries(&g_quant);
 }
 
 }  // namespace

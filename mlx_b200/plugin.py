@@ -91,6 +91,12 @@ class QmmParams(C.Structure):  # include/lux_cuda_quant.h: lux_qmm_params
     _fields_ = [(n, C.c_int32) for n in ("M", "K", "N", "bits", "group", "x_dtype", "sb_dtype", "y_dtype")]
 
 
+class BlockNormParams(C.Structure):  # include/lux_cuda_quant.h: lux_block_norm_params
+    _fields_ = [(n, _u64) for n in ("rows", "dim", "h_ld", "gate_ld", "gate_rows")] + \
+               [(n, C.c_int32) for n in ("post_norm", "pre_norm", "gate_act", "x_dtype", "r_dtype", "out_dtype", "out_format")] + \
+               [(n, C.c_float) for n in ("eps", "res_scale", "branch_scale", "out_pre")] + [("_pad", _u32)]
+
+
 _QMM = _fn(_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i)
 
 
@@ -143,11 +149,20 @@ class QuantVtbl(C.Structure):  # include/lux_cuda_quant.h: lux_gpu_quant_vtbl
         ("qmatmul_batch", _fn(_i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i)),
         ("qmatmul_sharded_push_batch", _fn(_i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i)),
         ("qmatmul_sharded_push_pro", _fn(_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _sz, C.c_float)),
+        # told by `size` (LUX_CUDA_QUANT_HAS)
+        ("mx4_scale_bytes", _fn(_sz, _i, _i, _i)),
+        ("mx4_quantize", _fn(_i, _vp, _vp, _vp, _vp, _i, _i, _sz, _i, _i, C.c_float)),
+        ("mx4_dequantize", _fn(_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, C.c_float)),
+        ("mx4_matmul", _fn(_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, C.c_float)),
+        ("block_norm", _fn(_i, _vp, C.POINTER(BlockNormParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp)),
     ]
 
 
 SYMM_HANDLE_BYTES = 96  # LUX_CUDA_SYMM_HANDLE_BYTES
 PRO_RMS_NORM, PRO_SUM3 = 1, 2  # LUX_CUDA_PRO_*: prologues of qmatmul_pro
+MX4_E8M0, MX4_E4M3 = 1, 2  # LUX_CUDA_MX4_*: microscaled 4-bit formats
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2  # LUX_CUDA_NORM_*
+GATE_IDENTITY, GATE_SIGMOID, GATE_TANH = 0, 1, 2  # LUX_CUDA_GATE_*
 
 
 EXPORTED_SYMBOLS = ("lux_gpu_backend_init", "lux_gpu_cuda_quant_vtbl", "lux_gpu_cuda_abi_layout",
@@ -273,6 +288,8 @@ class Context:
         self.handle = plugin.vtbl.create_context(device)
         if not self.handle:
             raise RuntimeError(f"create_context({device}) failed: {plugin.last_error()}")
+        q = plugin.quant  # (a field of a ctypes table is a new function object at every access)
+        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = q.mx4_quantize, q.mx4_dequantize, q.mx4_matmul, q.block_norm
 
     # --- base vtable ---------------------------------------------------------
     def close(self):
@@ -390,6 +407,37 @@ class Context:
         keep = [arr(xs), arr(wqs), arr(scales), arr(biases), arr(ys), (C.c_int * n)(*Ms)]
         self.plugin.check(self.plugin.quant.qmatmul_batch(self.handle, n, *[C.cast(a, C.c_void_p) for a in keep], K, N, bits, group, y_dtype),
                           "qmatmul_batch")
+
+    # --- microscaled 4-bit floating point ------------------------------------
+    def mx4_scale_bytes(self, rows, K, fmt):
+        """Bytes of the scales of [rows][K] (MX4_E8M0 | MX4_E4M3), in tiles of 128 rows x 4 blocks."""
+        return int(self.plugin.quant.mx4_scale_bytes(rows, K, fmt))
+
+    def mx4_quantize(self, src, codes, scales, rows, K, fmt, in_dtype, pre=1.0, ld=0):
+        """src * pre into 4-bit codes and block scales; ld: row stride of src in elements (0: K)."""
+        self.plugin.check(self._mx4_quantize(self.handle, src.handle, codes.handle, scales.handle, rows, K, ld, fmt, in_dtype, pre), "mx4_quantize")
+
+    def mx4_dequantize(self, codes, scales, dst, rows, K, fmt, out_dtype, post=1.0):
+        """dst = code * scale * post."""
+        self.plugin.check(self._mx4_dequantize(self.handle, codes.handle, scales.handle, dst.handle, rows, K, fmt, out_dtype, post), "mx4_dequantize")
+
+    def mx4_matmul(self, x_codes, x_scales, w_codes, w_scales, y, M, K, N, fmt, y_dtype, alpha=1.0):
+        """y = alpha * x . W^T, both operands in the microscaled format."""
+        self.plugin.check(self._mx4_matmul(self.handle, x_codes.handle, x_scales.handle, w_codes.handle, w_scales.handle, y.handle, M, K, N, fmt,
+                                           y_dtype, alpha), "mx4_matmul")
+
+    # --- norm after a block, gate, residual, norm before the next ---------------
+    @staticmethod
+    def block_norm_params(rows, dim, post=NORM_NONE, pre=NORM_NONE, gate_act=GATE_IDENTITY, gate_rows=0, x_dtype=BF16, r_dtype=BF16, out_dtype=BF16,
+                          out_format=0, eps=1e-6, res_scale=1.0, branch_scale=1.0, out_pre=1.0, h_ld=0, gate_ld=0):
+        """What block_norm does, to be kept and used again: see lux_block_norm_params."""
+        return BlockNormParams(rows, dim, h_ld, gate_ld, gate_rows, post, pre, gate_act, x_dtype, r_dtype, out_dtype, out_format, eps, res_scale,
+                               branch_scale, out_pre, 0)
+
+    def block_norm(self, params, h, gate, r, post_w, post_b, pre_w, pre_b, r_out, out, out_scales=None):
+        """r_out = res_scale * r + branch_scale * act(gate) * post_norm(h); out = pre_norm(r_out).  None where there is no such buffer."""
+        args = [None if b is None else b.handle for b in (h, gate, r, post_w, post_b, pre_w, pre_b, r_out, out, out_scales)]
+        self.plugin.check(self._block_norm(self.handle, C.byref(params), *args), "block_norm")
 
     def timer_record(self, slot):
         self.plugin.check(self.plugin.quant.timer_record(self.handle, slot), "timer_record")
