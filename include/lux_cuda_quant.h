@@ -340,8 +340,8 @@ typedef struct lux_gpu_quant_vtbl {
      *   out   = pre_norm(r_out)      with pre_w, pre_b; as out_dtype, or rounded to bf16 and quantised as mx4_quantize does
      * Weights and biases are fp32 [dim]; NULL: ones and zeros (a bias goes with a layer norm only).  gate NULL: 1.  h NULL: r_out =
      * res_scale * r; r NULL: the branch alone.  r_out or out may be NULL.  r_out may be r itself; otherwise what is written
-     * overlaps nothing that is read.  A multiple of 32 for dim where out_format is set.  Rows of more than 32768 elements (16384
-     * where dim is no multiple of 8) need r_out.  (op_rms_norm_f32 and op_layer_norm_f32, backend_plugin.h:175-178, are its parts.) */
+     * overlaps nothing that is read.  A multiple of 32 for dim where out_format is set.  (op_rms_norm_f32 and op_layer_norm_f32,
+     * backend_plugin.h:175-178, are its parts.) */
     LuxBackendError (*block_norm)(LuxBackendContext* ctx, const lux_block_norm_params* params, LuxBackendBuffer* h, LuxBackendBuffer* gate,
                                   LuxBackendBuffer* r, LuxBackendBuffer* post_w, LuxBackendBuffer* post_b, LuxBackendBuffer* pre_w,
                                   LuxBackendBuffer* pre_b, LuxBackendBuffer* r_out, LuxBackendBuffer* out, LuxBackendBuffer* out_scales);

@@ -331,10 +331,9 @@ struct BlockNormArgs {
     size_t rows, dim, h_ld, gate_ld, gate_rows;  // gate_rows: rows that share a row of gate (0: all)
     int post_kind, pre_kind, gate_act, out_format;
     bool x_bf16, r_bf16, out_bf16;
-    bool h_vec, gate_vec, r_vec, r_out_vec, out_vec, w_vec;  // every row starts on a 16-byte boundary
-    float eps, res_scale, branch_scale, out_pre;
+    bool vec;  // every row of every buffer starts on a 16-byte boundary
+    float eps, res_scale, branch_scale, out_pre, inv_dim;
 };
-bool block_norm_needs_stream(size_t dim);  // rows so long that r' is read back from r_out
 cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);

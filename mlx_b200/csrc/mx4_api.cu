@@ -164,7 +164,6 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     const size_t h_ld = p.h_ld ? p.h_ld : p.dim, gate_ld = p.gate_ld ? p.gate_ld : p.dim;
     if (!p.dim || p.dim > INT32_MAX || p.rows > INT32_MAX || h_ld < p.dim || gate_ld < p.dim || h_ld > (1ull << 31) || gate_ld > (1ull << 31))
         return invalid("block_norm: rows, dim or a row stride out of range");
-    if (block_norm_needs_stream(p.dim) && !b[R_OUT]) return invalid("block_norm: rows this long need r_out");
     if (!p.rows) return LUX_BACKEND_OK;
     const size_t gate_n = p.gate_rows ? (p.rows + p.gate_rows - 1) / p.gate_rows : 1;
     const size_t bytes[COUNT] = {((p.rows - 1) * h_ld + p.dim) * xs, ((gate_n - 1) * gate_ld + p.dim) * xs, p.rows * p.dim * rs, p.dim * 4, p.dim * 4, p.dim * 4,
@@ -182,7 +181,7 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
             if (overlap(b[o]->ptr, bytes[o], b[i]->ptr, bytes[i])) return invalid("block_norm: what is written overlaps another buffer");
         }
     auto ptr = [&](int i) { return b[i] ? b[i]->ptr : nullptr; };
-    auto vec = [&](int i, size_t ld, size_t es) { return b[i] && aligned(b[i], 16) && ld * es % 16 == 0; };
+    auto vec = [&](int i, size_t ld, size_t es) { return !b[i] || (aligned(b[i], 16) && (ld * es % 16 == 0 || p.rows == 1)); };
     BlockNormArgs a;
     a.h = ptr(H); a.gate = ptr(GATE); a.r = ptr(R);
     a.post_w = (const float*)ptr(POST_W); a.post_b = (const float*)ptr(POST_B); a.pre_w = (const float*)ptr(PRE_W); a.pre_b = (const float*)ptr(PRE_B);
@@ -190,10 +189,9 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     a.rows = p.rows; a.dim = p.dim; a.h_ld = h_ld; a.gate_ld = gate_ld; a.gate_rows = p.gate_rows;
     a.post_kind = p.post_norm; a.pre_kind = p.pre_norm; a.gate_act = p.gate_act; a.out_format = p.out_format;
     a.x_bf16 = xs == 2; a.r_bf16 = rs == 2; a.out_bf16 = os == 2;
-    a.h_vec = vec(H, h_ld, xs); a.gate_vec = vec(GATE, gate_ld, xs); a.r_vec = vec(R, p.dim, rs); a.r_out_vec = vec(R_OUT, p.dim, rs); a.out_vec = vec(OUT, p.dim, os);
-    a.w_vec = true;
-    for (int i = POST_W; i <= PRE_B; i++) a.w_vec = a.w_vec && (!b[i] || aligned(b[i], 16));
-    a.eps = p.eps; a.res_scale = p.res_scale; a.branch_scale = p.branch_scale; a.out_pre = p.out_pre;
+    a.vec = vec(H, h_ld, xs) && vec(GATE, gate_ld, xs) && vec(R, p.dim, rs) && vec(R_OUT, p.dim, rs) && (mx || vec(OUT, p.dim, os));
+    for (int i = POST_W; i <= PRE_B; i++) a.vec = a.vec && vec(i, 0, 4);
+    a.eps = p.eps; a.res_scale = p.res_scale; a.branch_scale = p.branch_scale; a.out_pre = p.out_pre; a.inv_dim = (float)(1.0 / (double)p.dim);
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
     LUX_CUDA_TRY(launch_block_norm(a, c->dev->sm_count, c->stream, chain_is_open(c)));
