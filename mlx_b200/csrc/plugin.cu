@@ -529,6 +529,8 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.mx4.dequantize", "mx4_dequantize", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.mx4.matmul", "mx4_tile<e8m0>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.mx4.matmul", "mx4_tile<e4m3>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.mx4.matmul", "mx4_pairs<e8m0>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // many rows of x: on pairs of CTAs
+    {"lux.mx4.matmul", "mx4_pairs<e4m3>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.block_norm", "block_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
 };
 const LuxKernelRegistry g_registry = {"cuda", g_kernels, sizeof(g_kernels) / sizeof(g_kernels[0])};

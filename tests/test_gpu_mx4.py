@@ -199,7 +199,20 @@ def test_matmul(ctx, oracle, fmt, M, K, N):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M,K,N", [(3, 512, 200), (200, 544, 300)])
+@pytest.mark.parametrize("M,K,N", [(520, 32, 8192), (1300, 96, 3333), (2048, 544, 2050), (257, 4128, 9001), (700, 1024, 5004), (1100, 2880, 4096)])
+def test_matmul_pairs(ctx, oracle, fmt, M, K, N):
+    """Shapes that pairs of CTAs take (but for one, at the border): several tiles per pair, K inside a stage, rows of y on any boundary, halves of tiles without rows."""
+    rng = np.random.default_rng(M + K + N)
+    xq, xs, xv = operand(ctx, rng, M, K, fmt)
+    wq, ws, wv = operand(ctx, rng, N, K, fmt)
+    for y_dtype, alpha, shift in ((BF16, 1.0, 0), (F32, 0.3, 4), (F32, 1.0, 0), (BF16, -2.0, 2)):
+        y = matmul(ctx, (xq, xs), (wq, ws), M, K, N, fmt, y_dtype, alpha, shift)
+        assert ctx.last_kernel().startswith("mx4_tile" if (M, N) == (1100, 4096) else "mx4_pairs")  # (80 tiles for 74 pairs, 288 for single CTAs)
+        check_product(oracle, y, xv, wv, np.float64(np.float32(alpha)), y_dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,K,N", [(3, 512, 200), (200, 544, 300), (600, 288, 4100)])
 def test_matmul_places(ctx, oracle, fmt, M, K, N):
     """One value per row of x, another place each: every code, scale and row has to be read from where it lies."""
     rng = np.random.default_rng(M)
@@ -228,7 +241,7 @@ def test_matmul_nan_and_infinite_scales_stay_in_their_rows(ctx, oracle, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M,K,N", [(1, 4096, 4096), (16, 2048, 640), (300, 1024, 900)])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 4096), (16, 2048, 640), (300, 1024, 900), (600, 2048, 5000)])
 def test_matmul_is_repeatable_and_replayable(ctx, oracle, fmt, M, K, N):
     """The same bits from call to call and from a recorded graph, which follows new activations; launches one behind the other
     without a wait between them."""
