@@ -193,8 +193,9 @@ template <int CH, bool XB, bool RB, int OUT, int MODE>
 __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
     __shared__ Shared sh;
     int turn = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t dim = (uint32_t)a.dim;
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // (several rows in a block: each is a warp's, and warps share nothing)
@@ -384,8 +385,9 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_const
     static_assert(OUT == 0 || V == 8, "blocks of codes: eight neighbours");
     __shared__ Shared sh;
     int turn = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const size_t dim = a.dim, row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;
     const bool xb = a.x_bf16, rb = a.r_bf16;

@@ -117,8 +117,13 @@ struct Context {
     // the stream drains (programmatic dependent launch) only if that kernel is a decode kernel of this
     // context, is the last thing the context enqueued, and does not write those weights.
     uint64_t chain_launches = ~0ull, chain_copies = 0;  // the two counters right after the last decode launch
-    const char* chain_out_lo = nullptr;                 // what that launch writes
-    const char* chain_out_hi = nullptr;
+    // What the chain kernels may still be writing once the last one lets its dependents start: its own outputs, if it does so
+    // behind its wait for the kernel before it; those of the kernels before it, too, if it does so ahead of that wait.
+    static constexpr int kChainOuts = 8;
+    struct {
+        const char *lo, *hi;
+    } chain_out[kChainOuts];
+    int chain_outs = 0;
     bool stream_exposed = false;  // the host holds the raw stream: it may enqueue work the context cannot see
     std::mutex mu;  // one thread at a time per context
 };
@@ -266,7 +271,12 @@ cudaError_t launch_qmv_push(const QmmArgs& a, void* workspace, int sm_count, cud
 bool decode_may_overlap(const Context* c, const QmmArgs& a);
 bool decode_x_stable(const Context* c, const QmmArgs& a);  // the last chain kernel's output does not overlap x
 bool chain_is_open(const Context* c);  // the last thing the context enqueued is a chain kernel (decode matmul, rms-norm)
-void note_chain_launch(Context* c, const void* out, size_t out_bytes);  // right after such a launch, before counting it
+bool chain_writes(const Context* c, const void* p, size_t bytes);  // chain kernels that may still run write into this range
+void note_chain_launch(Context* c, const void* out, size_t out_bytes);  // right after such a launch, when it has been counted
+// the same for a kernel whose dependents may start ahead of its own wait; overlapped: it was launched as a dependent itself.  One more
+// output of that launch: add_chain_output.
+void note_early_chain_launch(Context* c, bool overlapped);
+void add_chain_output(Context* c, const void* out, size_t bytes);
 void note_decode_launch(Context* c, const QmmArgs& a);  // call right after a decode launch, before counting it
 // decode / small-M, any supported dtype combination: CUDA cores + warp shuffles
 // overlap_prev (fp32 only): as above

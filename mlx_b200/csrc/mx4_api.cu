@@ -17,13 +17,6 @@ bool aligned(const Buffer* b, size_t n) { return ((uintptr_t)b->ptr & (n - 1)) =
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
-// a launch that writes two buffers: the chain's output is what spans both
-void note_two_outputs(Context* c, const void* a, size_t na, const void* b, size_t nb) {
-    const char* lo = std::min(static_cast<const char*>(a), static_cast<const char*>(b));
-    const char* hi = std::max(static_cast<const char*>(a) + na, static_cast<const char*>(b) + nb);
-    note_chain_launch(c, lo, (size_t)(hi - lo));
-}
-
 size_t mx4_scale_bytes(int rows, int K, int format) {
     if (rows < 0 || K <= 0 || K % 32 || (format != LUX_CUDA_MX4_E8M0 && format != LUX_CUDA_MX4_E4M3)) return 0;
     return ((size_t)rows + 127) / 128 * mx4_tiles_k(K, format) * 512;
@@ -66,9 +59,12 @@ LuxBackendError mx4_quantize(LuxBackendContext* ctx, LuxBackendBuffer* in, LuxBa
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
     // (behind a chain kernel the whole kernel waits for it on the device)
-    LUX_CUDA_TRY(launch_mx4_quantize(bi->ptr, (uint32_t*)bc->ptr, (uint8_t*)bs->ptr, rows, K, ld, format, (int)in_dtype, pre, c->stream, chain_is_open(c)));
+    const bool chained = chain_is_open(c);
+    LUX_CUDA_TRY(launch_mx4_quantize(bi->ptr, (uint32_t*)bc->ptr, (uint8_t*)bs->ptr, rows, K, ld, format, (int)in_dtype, pre, c->stream, chained));
     c->launches++;
-    note_two_outputs(c, bc->ptr, code_bytes, bs->ptr, scale_bytes);
+    note_early_chain_launch(c, chained);
+    add_chain_output(c, bc->ptr, code_bytes);
+    add_chain_output(c, bs->ptr, scale_bytes);
     bi->last_stream = bc->last_stream = bs->last_stream = c->stream;
     return LUX_BACKEND_OK;
 }
@@ -119,9 +115,7 @@ LuxBackendError mx4_matmul(LuxBackendContext* ctx, LuxBackendBuffer* x_codes, Lu
     Mx4MatmulArgs a{(const uint32_t*)bx->ptr, (const uint8_t*)bxs->ptr, (const uint32_t*)bw->ptr, (const uint8_t*)bws->ptr, by->ptr, M, K, N, format, (int)y_dtype,
                     alpha, c->err_dev};
     // behind a chain kernel the weights may be fetched while it drains, unless it writes them
-    const size_t out_bytes = (size_t)(c->chain_out_hi - c->chain_out_lo);
-    const bool early = chain_is_open(c) && !overlap(a.wq, (size_t)N * K / 2, c->chain_out_lo, out_bytes) &&
-                       !overlap(a.ws, mx4_scale_bytes(N, K, format), c->chain_out_lo, out_bytes);
+    const bool early = chain_is_open(c) && !chain_writes(c, a.wq, (size_t)N * K / 2) && !chain_writes(c, a.ws, mx4_scale_bytes(N, K, format));
     const char* name = "";
     const cudaError_t r = launch_mx4_matmul(a, c->dev->sm_count, c->stream, early, &name);
     if (r != cudaSuccess) return map_cuda_error(r, name);
@@ -194,17 +188,12 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     a.eps = p.eps; a.res_scale = p.res_scale; a.branch_scale = p.branch_scale; a.out_pre = p.out_pre; a.inv_dim = (float)(1.0 / (double)p.dim);
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
-    LUX_CUDA_TRY(launch_block_norm(a, c->dev->sm_count, c->stream, chain_is_open(c)));
+    const bool chained = chain_is_open(c);
+    LUX_CUDA_TRY(launch_block_norm(a, c->dev->sm_count, c->stream, chained));
     c->launches++;
-    {   // what the launch writes: the span of its outputs
-        uintptr_t lo = UINTPTR_MAX, hi = 0;
-        for (int o = R_OUT; o < COUNT; o++)
-            if (b[o]) {
-                lo = std::min(lo, (uintptr_t)b[o]->ptr);
-                hi = std::max(hi, (uintptr_t)b[o]->ptr + bytes[o]);
-            }
-        note_chain_launch(c, (const void*)lo, hi - lo);
-    }
+    note_early_chain_launch(c, chained);
+    for (int o = R_OUT; o < COUNT; o++)
+        if (b[o]) add_chain_output(c, b[o]->ptr, bytes[o]);
     for (int i = 0; i < COUNT; i++)
         if (b[i]) b[i]->last_stream = c->stream;
     return LUX_BACKEND_OK;

@@ -210,6 +210,27 @@ __device__ __forceinline__ void store_tile(const Params& p, uint32_t part, int f
     else store_rows<kMaxSplit, 2, VEC>(p, part, first, step, m_cnt, m0, n0);
 }
 
+// A stage's scales into tensor memory and its MMAs.  WHOLE: all of its K is there.
+template <int FMT, bool WHOLE>
+__device__ __forceinline__ void issue_stage(const Params& p, int st, uint32_t d, uint64_t da, uint64_t db, uint64_t dsa, uint64_t dsb, uint32_t sf, uint32_t idesc,
+                                            bool accumulate) {
+    constexpr int ST = stage_tiles(FMT);
+    const int tiles = WHOLE ? ST : min(ST, p.tiles_k - st * ST), mmas = WHOLE ? kStageK / kMmaK : (p.K - st * kStageK + kMmaK - 1) / kMmaK;
+#pragma unroll
+    for (int i = 0; i < ST; i++)
+        if (WHOLE || i < tiles) {
+            tc_copy_scales(sf + i * kScaleCols, dsa + i * (kScaleTile >> 4));
+            tc_copy_scales(sf + (ST + i) * kScaleCols, dsb + i * (kScaleTile >> 4));
+        }
+#pragma unroll
+    for (int i = 0; i < kStageK / kMmaK; i++)
+        if (WHOLE || i < mmas) {
+            const int t = FMT == LUX_CUDA_MX4_E8M0 ? i >> 1 : i;
+            const uint32_t byte = FMT == LUX_CUDA_MX4_E8M0 ? (i & 1) * 2 : 0;
+            tc_mma<FMT>(d, da + 2 * i, db + 2 * i, idesc | byte << 29 | byte << 4, sf + t * kScaleCols, sf + (ST + t) * kScaleCols, (i > 0 || accumulate) ? 1u : 0u);
+        }
+}
+
 template <int FMT>
 __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                             const __grid_constant__ Params p) {
@@ -277,26 +298,25 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
         }
         __syncwarp();
     } else if (warp == 1) {
+        // (the clock of a bounded wait must not start before the previous kernel has ended: it may itself be waiting, for a peer, for as
+        // long as its caller allows)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        // The whole warp walks the stages and one elected lane issues: what the instructions take then lives in uniform registers.  (With
+        // loops of one lane's own around them a stage took 630 cycles, whatever its loads did: 1 x 4096 x 4096 out of L2, not split,
+        // 7.8 us.)
         int slot = 0;
         uint32_t ph = 0;
         bool ok = true;
+        const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4, sf0 = tmem + p.sf_col, idesc = mma_idesc<FMT>(n_mma, 0);
+        const uint64_t da = desc_sw128(ring), db = desc_sw128(ring + p.b_off), dsa = desc_scales(ring + p.sa_off), dsb = desc_scales(ring + p.sb_off);
         for (int st = s_lo; st < s_hi; st++) {
             if (!__all_sync(0xffffffffu, bar_wait(full + 8 * slot, ph, abort))) { ok = false; break; }
             tc_fence_after();
+            const uint32_t at = slot * stage16, sf = sf0 + slot * (2 * ST * kScaleCols);
+            const bool whole = (st + 1) * kStageK <= p.K;
             if (elect_one()) {
-                const uint32_t base = ring + slot * p.stage_bytes;
-                const uint32_t sa = tmem + p.sf_col + slot * (2 * ST * kScaleCols), sb = sa + ST * kScaleCols;
-                const int tiles = min(ST, p.tiles_k - st * ST), mmas = min(kStageK / kMmaK, (p.K - st * kStageK + kMmaK - 1) / kMmaK);
-                for (int i = 0; i < tiles; i++) {
-                    tc_copy_scales(sa + i * kScaleCols, desc_scales(base + p.sa_off + i * kScaleTile));
-                    tc_copy_scales(sb + i * kScaleCols, desc_scales(base + p.sb_off + i * kScaleTile));
-                }
-                const uint64_t da = desc_sw128(base), db = desc_sw128(base + p.b_off);
-                for (int i = 0; i < mmas; i++) {
-                    const int t = FMT == LUX_CUDA_MX4_E8M0 ? i >> 1 : i;
-                    const uint32_t byte = FMT == LUX_CUDA_MX4_E8M0 ? (i & 1) * 2 : 0;
-                    tc_mma<FMT>(tmem, da + 2 * i, db + 2 * i, mma_idesc<FMT>(n_mma, byte), sa + t * kScaleCols, sb + t * kScaleCols, (st > s_lo || i > 0) ? 1u : 0u);
-                }
+                if (whole) issue_stage<FMT, true>(p, st, tmem, da + at, db + at, dsa + at, dsb + at, sf, idesc, st > s_lo);
+                else issue_stage<FMT, false>(p, st, tmem, da + at, db + at, dsa + at, dsb + at, sf, idesc, st > s_lo);
                 tc_commit(empty + 8 * slot);
                 if (st + 1 == s_hi) tc_commit(done);
             }
@@ -304,6 +324,8 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
             if (++slot == p.stages) { slot = 0; ph ^= 1; }
         }
         if (!ok) *abort = 1;
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
     }
     // every warp: 32 lanes (rows of W) of the tile
     const bool ok = __all_sync(0xffffffffu, bar_wait(done, 0, abort));
@@ -436,6 +458,28 @@ __device__ __forceinline__ void sts_v4(uint32_t a, uint32_t x, uint32_t y, uint3
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// as issue_stage; scales in shared memory and in tensor memory: ST tiles of x; in shared memory then ST tiles of the first 128 rows of W and ST
+// of the others, in tensor memory the two side by side
+template <int FMT, bool WHOLE>
+__device__ __forceinline__ void issue_stage_pair(const PairParams& p, int st, uint32_t d, uint64_t da, uint64_t db, uint64_t ds, uint32_t sf) {
+    constexpr int ST = stage_tiles(FMT);
+    const int mmas = WHOLE ? kStageK / kMmaK : (p.K - st * kStageK + kMmaK - 1) / kMmaK;
+    const uint32_t sb = sf + ST * kScaleCols;
+#pragma unroll
+    for (int i = 0; i < ST; i++) {  // (past the last tile of a row: whatever lies there, for MMAs that are not issued)
+        tc_copy_scales_pair(sf + i * kScaleCols, ds + i * (kScaleTile >> 4));
+        tc_copy_scales_pair(sb + 2 * i * kScaleCols, ds + (ST + i) * (kScaleTile >> 4));
+        tc_copy_scales_pair(sb + (2 * i + 1) * kScaleCols, ds + (2 * ST + i) * (kScaleTile >> 4));
+    }
+#pragma unroll
+    for (int i = 0; i < kStageK / kMmaK; i++)
+        if (WHOLE || i < mmas) {
+            const int t = FMT == LUX_CUDA_MX4_E8M0 ? i >> 1 : i;
+            tc_mma_pair<FMT>(d, da + 2 * i, db + 2 * i, pair_idesc<FMT>(FMT == LUX_CUDA_MX4_E8M0 ? (i & 1) * 2 : 0), sf + t * kScaleCols, sb + 2 * t * kScaleCols,
+                             (st > 0 || i > 0) ? 1u : 0u);
+        }
+}
+
 template <int FMT, bool YBF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_xs,
@@ -471,6 +515,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     cluster_sync();  // the peer's barriers are there before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (all roles: no clock of a bounded wait starts before the previous kernel has ended)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == kEpiWarps) {
         if (lane == 0) {
@@ -478,8 +524,6 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_xs) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_ws) : "memory");
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             int slot = 0;
             uint32_t ph = 1;
             bool ok = true;
@@ -504,27 +548,18 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             int slot = 0;
             uint32_t ph = 0, tile_i = 0;
             bool ok = true;
+            const uint64_t da = desc_sw128(ring), db = desc_sw128(ring + kABytes), ds = desc_scales(ring + SA);
             for (int tile = pair; tile < p.tiles && ok; tile += pairs, tile_i++) {
                 if (!__all_sync(0xffffffffu, bar_wait(tmem_empty, (tile_i & 1) ^ 1, abort))) break;
                 tc_fence_after();
                 for (int st = 0; st < p.nst; st++) {
                     if (!__all_sync(0xffffffffu, bar_wait(full + 8 * slot, ph, abort))) { ok = false; break; }
                     tc_fence_after();
+                    const uint32_t at = slot * (STAGE >> 4), sf = tmem + 256 + slot * SLOT;
+                    const bool whole = (st + 1) * kStageK <= p.K;
                     if (elect_one()) {
-                        const uint32_t base = ring + slot * STAGE, sa = tmem + 256 + slot * SLOT, sb = sa + ST * kScaleCols;
-#pragma unroll
-                        for (int i = 0; i < ST; i++) {
-                            tc_copy_scales_pair(sa + i * kScaleCols, desc_scales(base + SA + i * kScaleTile));
-                            tc_copy_scales_pair(sb + 2 * i * kScaleCols, desc_scales(base + SB + i * kScaleTile));
-                            tc_copy_scales_pair(sb + (2 * i + 1) * kScaleCols, desc_scales(base + SB + (ST + i) * kScaleTile));
-                        }
-                        const int mmas = min(kStageK / kMmaK, (p.K - st * kStageK + kMmaK - 1) / kMmaK);
-                        const uint64_t da = desc_sw128(base), db = desc_sw128(base + kABytes);
-                        for (int i = 0; i < mmas; i++) {
-                            const int t = FMT == LUX_CUDA_MX4_E8M0 ? i >> 1 : i;
-                            const uint32_t byte = FMT == LUX_CUDA_MX4_E8M0 ? (i & 1) * 2 : 0;
-                            tc_mma_pair<FMT>(tmem, da + 2 * i, db + 2 * i, pair_idesc<FMT>(byte), sa + t * kScaleCols, sb + 2 * t * kScaleCols, (st > 0 || i > 0) ? 1u : 0u);
-                        }
+                        if (whole) issue_stage_pair<FMT, true>(p, st, tmem, da + at, db + at, ds + at, sf);
+                        else issue_stage_pair<FMT, false>(p, st, tmem, da + at, db + at, ds + at, sf);
                         tc_commit_pair(empty + 8 * slot);
                         if (st + 1 == p.nst) tc_commit_pair(tmem_full);
                     }
@@ -645,12 +680,14 @@ bool encode_codes(const void* codes, int rows, int K, int box_rows, CUtensorMap*
     return r == CUDA_SUCCESS;
 }
 
-// How a launch is cut: parts of K and stages per CTA.  All CTAs should be on the machine at once; beyond that, more and shorter parts
-// are faster up to two or three CTAs per SM with three stages each (measured, us: 1 x 4096 x 11008, 86 tiles: 9.4 whole, 7.1 in
-// two, 6.9 in four with 3 stages; 11.0 in six, which are more than fit; 8 x 4096 x 22016, 172 tiles: 12.2, in two 11.3, in three
-// 15.1; 48 rows: 9.7, in four 8.7; 128 rows: 11.4, in three 11.0, in four 17.6).  A CTA with more than six stages to go through
-// takes as many slots as there is room for (16 x 8192 x 28672, whole: 26.8 with 3, 24.4 with 5); a shorter one leaves the room to the
-// next launch of the chain, which fills its own ring meanwhile (8 x 11008 x 4096 in eight: 7.7 with 3, 8.0 with 5).
+// How a launch is cut: parts of K (CTAs of a cluster) and stages per CTA.
+// A part costs 0.22 us per stage of 256 codes, a cluster about half a microsecond each time its size doubles: parts of eight stages
+// are the best of the two, shorter ones where there are hardly any CTAs.  All CTAs have to find room at once (in four fifths of the
+// slots: a cluster's CTAs have to lie in one group of SMs), and the ring is as deep as leaves the next launch of a chain, which fills
+// its own meanwhile, some two fifths of the machine's shared memory.  Measured, us, (parts, stages):
+//   1 x 4096 x 4096     (1,6) 6.0  (2,6) 4.8  (4,4) 5.2  (8,3) 4.9        8 x 11008 x 4096   (4,6) 7.5  (6,5) 7.0  (8,3) 7.0
+//   1 x 4096 x 11008    (1,6) 7.8  (2,4) 6.9  (2,6) 11.1 (4,2) 6.7        16 x 8192 x 28672  (1,4) 22.3 (1,6) 27.1 (2,4) 27.2
+//   8 x 4096 x 22016    (1,4) 10.5 (2,3) 10.3 (2,4) 11.9 (4,3) 14.8       48 x 4096 x 11008  (1,6) 8.5  (2,4) 7.7  (4,3) 8.6
 struct TilePlan {
     int bm, m_tiles, split, stages, stage_bytes, per_sm;
     long long tiles;
@@ -672,16 +709,17 @@ TilePlan plan_tile(int M, int K, int N, int format, int sm_count) {
         for (t.tmem_cols = 32; t.tmem_cols < t.sf_col + t.stages * 2 * st * kScaleCols; t.tmem_cols *= 2) {}
         t.per_sm = std::min(kSmemMax / (t.smem + 1024), (int)(512 / t.tmem_cols));
     };
-    fit(std::min(3, nst));
-    // (four fifths of the slots: a cluster's CTAs have to find them in one group of SMs)
-    t.split = (int)std::max(1ll, std::min({(long long)kMaxSplit, (long long)nst, (long long)sm_count * t.per_sm * 4 / 5 / t.tiles}));
-    const int mine = (nst + t.split - 1) / t.split;
-    const long long want = std::min<long long>(std::max(1, t.per_sm), (t.tiles * t.split + sm_count - 1) / sm_count);
-    for (int stages = kMaxStages; mine > 6 && stages > 3; stages--) {
-        fit(stages);
-        if (t.per_sm >= want) return t;
+    auto resident = [&]() { return t.tiles * t.split <= (long long)sm_count * t.per_sm * 4 / 5; };
+    t.split = (int)std::min<long long>(std::min(kMaxSplit, nst), std::max((nst + 7) / 8, (int)(48 / std::min(48ll, t.tiles))));
+    for (;; t.split--) {
+        fit(std::min(3, (nst + t.split - 1) / t.split));
+        if (t.split == 1 || resident()) break;
     }
-    fit(std::min(3, mine));
+    for (int stages = std::min(kMaxStages, (nst + t.split - 1) / t.split); stages > 3; stages--) {
+        fit(stages);
+        if (resident() && t.tiles * t.split * t.smem <= (long long)sm_count * kSmemMax * 5 / 8) return t;
+    }
+    fit(std::min(3, (nst + t.split - 1) / t.split));
     return t;
 }
 

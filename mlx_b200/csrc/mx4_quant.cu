@@ -48,8 +48,9 @@ __device__ __forceinline__ void load16(const void* p, bool bf16, bool vec, int l
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(32 * kRows) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                 int rows, int K, size_t ld, float pre, bool vec) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int LPW = 4 * mx4_block(FMT) / 16;  // lanes per scale word
     const int lane = threadIdx.x & 31, tiles_k = mx4_tiles_k(K, FMT);
     const int k = blockIdx.x * kChunk + lane * 16;

@@ -4,6 +4,7 @@
 // (include/lux/gpu/backend_plugin.h:129) and returns INVALID_ARGUMENT on NULL
 // or undersized buffers the way the CPU backend does
 // (src/cpu_backend.cpp:243-247).
+#include <algorithm>
 #include <cstring>
 #include <new>
 
@@ -39,30 +40,45 @@ LuxBackendError check_format(int K, int bits, int group) {
 
 }  // namespace
 
-static bool ranges_overlap(const char* a_lo, size_t a_bytes, const char* b_lo, const char* b_hi) {
-    return a_lo < b_hi && b_lo < a_lo + a_bytes;
-}
 bool chain_is_open(const Context* c) {
     static const bool disabled = getenv("LUXCUDA_NO_PDL") != nullptr;
     if (disabled || c->stream_exposed) return false;
     return c->chain_launches == c->launches.load() && c->chain_copies == c->copies.load();
 }
-void note_chain_launch(Context* c, const void* out, size_t out_bytes) {
+bool chain_writes(const Context* c, const void* p, size_t bytes) {
+    const char* lo = (const char*)p;
+    for (int i = 0; i < c->chain_outs; i++)
+        if (lo < c->chain_out[i].hi && c->chain_out[i].lo < lo + bytes) return true;
+    return false;
+}
+void add_chain_output(Context* c, const void* out, size_t bytes) {
+    if (!bytes) return;
+    const char *lo = (const char*)out, *hi = lo + bytes;
+    if (c->chain_outs == Context::kChainOuts) {  // too many to tell apart: one range that spans them
+        for (int i = 0; i < c->chain_outs; i++) {
+            lo = std::min(lo, c->chain_out[i].lo);
+            hi = std::max(hi, c->chain_out[i].hi);
+        }
+        c->chain_outs = 0;
+    }
+    c->chain_out[c->chain_outs].lo = lo;
+    c->chain_out[c->chain_outs++].hi = hi;
+}
+void note_early_chain_launch(Context* c, bool overlapped) {
     c->chain_launches = c->launches.load();
     c->chain_copies = c->copies.load();
-    c->chain_out_lo = (const char*)out;
-    c->chain_out_hi = (const char*)out + out_bytes;
+    if (!overlapped) c->chain_outs = 0;
+}
+void note_chain_launch(Context* c, const void* out, size_t out_bytes) {
+    note_early_chain_launch(c, false);
+    add_chain_output(c, out, out_bytes);
 }
 bool decode_may_overlap(const Context* c, const QmmArgs& a) {
     if (!chain_is_open(c)) return false;
     const size_t sb = (size_t)a.N * (a.K / a.group) * dtype_size(a.sb_dtype);
-    return !ranges_overlap((const char*)a.wq, (size_t)a.N * a.K * a.bits / 8, c->chain_out_lo, c->chain_out_hi) &&
-           !ranges_overlap((const char*)a.scales, sb, c->chain_out_lo, c->chain_out_hi) &&
-           !ranges_overlap((const char*)a.biases, sb, c->chain_out_lo, c->chain_out_hi);
+    return !chain_writes(c, a.wq, (size_t)a.N * a.K * a.bits / 8) && !chain_writes(c, a.scales, sb) && !chain_writes(c, a.biases, sb);
 }
-bool decode_x_stable(const Context* c, const QmmArgs& a) {
-    return !ranges_overlap((const char*)a.x, (size_t)a.M * a.K * 2, c->chain_out_lo, c->chain_out_hi);
-}
+bool decode_x_stable(const Context* c, const QmmArgs& a) { return !chain_writes(c, a.x, (size_t)a.M * a.K * 2); }
 // A graph's recording, its end and its launch each end a chain: recording counts launches that do not run, and ends by
 // taking them off the counter again, which may thus come back to an earlier value.
 static void close_chain(Context* c) {
@@ -70,10 +86,7 @@ static void close_chain(Context* c) {
     c->chain_launches = ~0ull;
 }
 void note_decode_launch(Context* c, const QmmArgs& a) {
-    c->chain_launches = c->launches.load();
-    c->chain_copies = c->copies.load();
-    c->chain_out_lo = (const char*)a.y;
-    c->chain_out_hi = (const char*)a.y + (size_t)a.M * a.N * (a.y_dtype == LUX_DTYPE_BFLOAT16 ? 2 : 4);
+    note_chain_launch(c, a.y, (size_t)a.M * a.N * (a.y_dtype == LUX_DTYPE_BFLOAT16 ? 2 : 4));
 }
 
 LuxBackendError ensure_qmv_workspace(Context* c, size_t bytes) {
