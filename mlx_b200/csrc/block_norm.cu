@@ -11,6 +11,7 @@
 
 #include "internal.h"
 #include "mx4.cuh"
+#include "pair.cuh"
 
 namespace luxcuda {
 
@@ -31,11 +32,6 @@ __device__ __forceinline__ float act_of(float g, int act) {
     if (act == LUX_CUDA_GATE_TANH) return tanhf(g);
     return g;
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t w;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
-    return w;
-}
 __device__ __forceinline__ float round_bf16(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 // rows are read once and their results not again here: neither stays in L1, where the weights are
 __device__ __forceinline__ uint4 ld_row(const void* p) {
@@ -46,29 +42,6 @@ __device__ __forceinline__ uint4 ld_row(const void* p) {
 __device__ __forceinline__ void st_row(void* p, const uint4& v) {
     asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// Two neighbouring elements in a register pair: the fp32 pipe takes both in one instruction.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair_of(uint32_t lo, uint32_t hi) { return (Pair)hi << 32 | lo; }
-__device__ __forceinline__ Pair pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ float lo_of(Pair p) { return __uint_as_float((uint32_t)p); }
-__device__ __forceinline__ float hi_of(Pair p) { return __uint_as_float((uint32_t)(p >> 32)); }
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ Pair unpack2(uint32_t w) { return pair_of(w << 16, w & 0xFFFF0000u); }  // bf16 pair
-__device__ __forceinline__ uint32_t pack2(Pair p) { return pack_bf16(lo_of(p), hi_of(p)); }
 // A thread's eight elements of a chunk: neighbours, on a 16-byte boundary (kWide: kFull where no chunk is cut off by the row's end),
 // or, on any boundary, `step` apart, those at `end` and behind it zero (kApart).
 enum Mode { kWide, kFull, kApart };
@@ -358,14 +331,10 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
 #pragma unroll
         for (int j = 0; j < CH; j++) {  // (the whole warp: lanes past the row carry zeros)
             const uint32_t i = at(j).first;
-            float u[8];
+            Pair u[4];
             uint32_t c[1], byte;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const Pair t = FULL || i < dim ? mul2(unpack2(pack2(v[j][e])), pre) : 0;
-                u[2 * e] = lo_of(t);
-                u[2 * e + 1] = hi_of(t);
-            }
+            for (int e = 0; e < 4; e++) u[e] = FULL || i < dim ? mul2(unpack2(pack2(v[j][e])), pre) : 0;
             mx4_encode<F, 8>(u, c, byte);
             const uint32_t word = mx4_scale_word<F, 8>(byte, threadIdx.x & 31);
             if (FULL || i < dim) {
@@ -452,10 +421,11 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_const
         constexpr int F = OUT ? OUT : 1;
         for (size_t base = 0; base < dim; base += step) {  // (the whole warp: lanes past the row carry zeros)
             const size_t at = base + (size_t)threadIdx.x * V;
-            float u[8];
+            Pair u[4];
             uint32_t c[1], byte;
+            auto value = [&](size_t i) { return i < dim ? __fmul_rn(round_bf16(norm(pre, a.pre_kind, a.pre_w, a.pre_b, i, r_at(i))), a.out_pre) : 0.0f; };
 #pragma unroll
-            for (int e = 0; e < 8; e++) u[e] = at + e < dim ? __fmul_rn(round_bf16(norm(pre, a.pre_kind, a.pre_w, a.pre_b, at + e, r_at(at + e))), a.out_pre) : 0.0f;
+            for (int e = 0; e < 4; e++) u[e] = pair_of(value(at + 2 * e), value(at + 2 * e + 1));
             mx4_encode<F, 8>(u, c, byte);
             const uint32_t word = mx4_scale_word<F, 8>(byte, threadIdx.x & 31);
             if (at < dim) {

@@ -11,6 +11,7 @@
 #include <cstdint>
 
 #include "lux_cuda_quant.h"
+#include "pair.cuh"
 
 namespace luxcuda {
 
@@ -22,16 +23,23 @@ __host__ __device__ constexpr size_t mx4_scale_at(size_t row, int tk, int tiles_
     return ((row >> 7) * tiles_k + tk) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
 }
 
-// the larger one, NaN if either is
-__device__ __forceinline__ float max_nan(float a, float b) {
+// the largest magnitude of three, of two; NaN if one is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// two values to two codes, nearest, ties to the even code, at most +-6
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
-    uint16_t r;
-    asm("{ .reg .b8 t; cvt.rn.satfinite.e2m1x2.f32 t, %1, %2; cvt.u16.u8 %0, t; }" : "=h"(r) : "f"(hi), "f"(lo));
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+// eight values to eight codes, nearest, ties to the even code, at most +-6
+__device__ __forceinline__ uint32_t e2m1x8(Pair a, Pair b, Pair c, Pair d) {
+    uint32_t r;
+    asm("{ .reg .b8 w, x, y, z; cvt.rn.satfinite.e2m1x2.f32 w, %2, %1; cvt.rn.satfinite.e2m1x2.f32 x, %4, %3;\n"
+        "  cvt.rn.satfinite.e2m1x2.f32 y, %6, %5; cvt.rn.satfinite.e2m1x2.f32 z, %8, %7; mov.b32 %0, {w, x, y, z}; }"
+        : "=r"(r) : "f"(lo_of(a)), "f"(hi_of(a)), "f"(lo_of(b)), "f"(hi_of(b)), "f"(lo_of(c)), "f"(hi_of(c)), "f"(lo_of(d)), "f"(hi_of(d)));
     return r;
 }
 // two codes (the low byte of v) to their values, which are exact
@@ -66,38 +74,40 @@ __device__ __forceinline__ float mx4_scale_value(uint32_t b) {
 //         quotient): fp32 division would do.  It costs eight operations a value; one multiplication by the rounded
 //         reciprocal and one correction by the exact remainder gives the same number (Markstein 1990, theorem 8.1) in three.
 template <int FMT, int E>
-__device__ __forceinline__ void mx4_encode(float (&u)[E], uint32_t (&codes)[E / 8], uint32_t& byte) {
-    float m = fabsf(u[0]);
+__device__ __forceinline__ void mx4_encode(Pair (&u)[E / 2], uint32_t (&codes)[E / 8], uint32_t& byte) {
+    float m = max_abs(lo_of(u[0]), hi_of(u[0]));
 #pragma unroll
-    for (int i = 1; i < E; i++) m = max_nan(m, fabsf(u[i]));
+    for (int i = 1; i < E / 2; i++) m = max_abs(m, lo_of(u[i]), hi_of(u[i]));
 #pragma unroll
-    for (int o = 1; o < mx4_block(FMT) / E; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 1; o < mx4_block(FMT) / E; o <<= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (FMT == LUX_CUDA_MX4_E8M0) {
         const uint32_t field = min(__float_as_uint(m) >> 23, 254u);  // (an infinity as the largest finite value)
         byte = field > 2u ? field - 2u : 0u;
-        const float inv = __uint_as_float((254u - byte) << 23);
+        const uint32_t inv = (254u - byte) << 23;
         if (m != m) byte = 255u;
 #pragma unroll
-        for (int i = 0; i < E; i++) u[i] = __fmul_rn(u[i], inv);
+        for (int i = 0; i < E / 2; i++) u[i] = mul2(u[i], pair_of(inv, inv));
     } else {
-        byte = e4m3_of(__fdiv_rn(m, 6.0f));
-        const float s = e4m3_value(byte), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+        // (the same correction for m / 6, and one step for the reciprocal of a scale: 126 numbers, all of them tested)
+        const float top = m == INFINITY ? 3e38f : m, q = __fmul_rn(top, 1.0f / 6.0f);
+        byte = e4m3_of(__fmaf_rn(__fmaf_rn(-6.0f, q, top), 1.0f / 6.0f, q));
+        const float s = e4m3_value(byte);
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        inv = s > 0.0f ? __fmaf_rn(__fmaf_rn(-s, inv, 1.0f), inv, inv) : 0.0f;
         if (m == INFINITY) {  // (infinity - infinity below)
 #pragma unroll
-            for (int i = 0; i < E; i++) u[i] = fminf(fmaxf(u[i], -3e38f), 3e38f);
+            for (int i = 0; i < E / 2; i++) u[i] = pair_of(fminf(fmaxf(lo_of(u[i]), -3e38f), 3e38f), fminf(fmaxf(hi_of(u[i]), -3e38f), 3e38f));
         }
+        const Pair inv2 = pair_of(inv, inv), neg2 = pair_of(-s, -s);
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            const float t = __fmul_rn(u[i], inv);
-            u[i] = __fmaf_rn(__fmaf_rn(-t, s, u[i]), inv, t);
+        for (int i = 0; i < E / 2; i++) {
+            const Pair t = mul2(u[i], inv2);
+            u[i] = fma2(fma2(t, neg2, u[i]), inv2, t);
         }
     }
 #pragma unroll
-    for (int w = 0; w < E / 8; w++) {
-        codes[w] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) codes[w] |= e2m1x2(u[8 * w + 2 * i], u[8 * w + 2 * i + 1]) << (8 * i);
-    }
+    for (int w = 0; w < E / 8; w++) codes[w] = e2m1x8(u[4 * w], u[4 * w + 1], u[4 * w + 2], u[4 * w + 3]);
 }
 // The scale word (4 blocks) that the lane's block belongs to, from the blocks' bytes; lanes of a word side by side.
 template <int FMT, int E>

@@ -515,8 +515,8 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     cluster_sync();  // the peer's barriers are there before anything arrives on them
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // (all roles: no clock of a bounded wait starts before the previous kernel has ended)
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // No clock of a bounded wait starts before the previous kernel has ended; ahead of that the loader alone is at work, on weights.
+    if (warp != kEpiWarps) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp == kEpiWarps) {
         if (lane == 0) {
@@ -524,20 +524,29 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_xs) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(&map_ws) : "memory");
+            auto load_w = [&](int st, int tn, int slot) {
+                const uint32_t bar = full + 8 * slot, base = ring + slot * STAGE;
+                if (rank == 0) bar_expect(bar, 2 * STAGE);
+                tma_load_2d_pair(base + kABytes, &map_w, st * 128, (tn + (int)rank) * kTileN, bar);
+                tma_load_2d_pair(base + SB, &map_ws, 0, tn * p.tiles_k + st * ST, bar);
+                tma_load_2d_pair(base + SB + ST * kScaleTile, &map_ws, 0, (tn + 1) * p.tiles_k + st * ST, bar);
+            };
+            const int first = min(kPairStages, p.nst);  // stages of the first tile whose weights are fetched ahead
+            for (int st = 0; st < first; st++) load_w(st, pair / p.m_tiles * 2, st);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             int slot = 0;
             uint32_t ph = 1;
             bool ok = true;
             for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
                 const int tm = tile % p.m_tiles * 2 + (int)rank, tn = tile / p.m_tiles * 2;  // this CTA's tile of x, the pair's first of W (128 rows each)
                 for (int st = 0; st < p.nst; st++) {
-                    if (!bar_wait(empty + 8 * slot, ph, abort)) { ok = false; break; }
-                    const uint32_t bar = full + 8 * slot, base = ring + slot * STAGE;
-                    if (rank == 0) bar_expect(bar, 2 * STAGE);
-                    tma_load_2d_pair(base, &map_x, st * 128, tm * kTileN, bar);
-                    tma_load_2d_pair(base + kABytes, &map_w, st * 128, (tn + (int)rank) * kTileN, bar);
-                    tma_load_2d_pair(base + SA, &map_xs, 0, tm * p.tiles_k + st * ST, bar);
-                    tma_load_2d_pair(base + SB, &map_ws, 0, tn * p.tiles_k + st * ST, bar);
-                    tma_load_2d_pair(base + SB + ST * kScaleTile, &map_ws, 0, (tn + 1) * p.tiles_k + st * ST, bar);
+                    if (tile != pair || st >= first) {
+                        if (!bar_wait(empty + 8 * slot, ph, abort)) { ok = false; break; }
+                        load_w(st, tn, slot);
+                    }
+                    tma_load_2d_pair(ring + slot * STAGE, &map_x, st * 128, tm * kTileN, full + 8 * slot);
+                    tma_load_2d_pair(ring + slot * STAGE + SA, &map_xs, 0, tm * p.tiles_k + st * ST, full + 8 * slot);
                     if (++slot == kPairStages) { slot = 0; ph ^= 1; }
                 }
             }

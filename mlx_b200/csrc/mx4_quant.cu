@@ -8,59 +8,66 @@ namespace luxcuda {
 
 namespace {
 
-constexpr int kRows = 8;       // rows per block, a warp each
+constexpr int kWarps = 8;      // per block, a row each at a time
 constexpr int kChunk = 512;    // values of a row per warp: 16 per lane
 constexpr int kMaxGridY = 65535;
 
-__device__ __forceinline__ void load16(const void* p, bool bf16, bool vec, int left, float (&u)[16]) {
+// 16 neighbouring values as they lie; align: 32 or 16 bytes, or less
+template <bool BF16>
+struct Raw16 {
+    Words8 w[BF16 ? 1 : 2];
+    __device__ __forceinline__ void load(const void* p, int align) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) u[i] = 0.0f;
-    if (left <= 0) return;
-    if (vec) {
-        if (bf16) {
-            const uint4* q = static_cast<const uint4*>(p);
+        for (int h = 0; h < (BF16 ? 1 : 2); h++) {
+            const char* s = static_cast<const char*>(p) + 32 * h;
+            if (align == 32) {
+                w[h] = ld_once_32(s);
+            } else if (align == 16) {
+                const uint4 a = __ldcs(reinterpret_cast<const uint4*>(s)), b = __ldcs(reinterpret_cast<const uint4*>(s) + 1);
+                w[h] = Words8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+            } else {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint4 v = __ldcs(q + h);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    u[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-                    u[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                }
-            }
-        } else {
-            const float4* q = static_cast<const float4*>(p);
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-                const float4 v = __ldcs(q + h);
-                u[4 * h] = v.x; u[4 * h + 1] = v.y; u[4 * h + 2] = v.z; u[4 * h + 3] = v.w;
+                for (int i = 0; i < 8; i++)
+                    w[h].v[i] = BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(s)[2 * i] | (uint32_t)reinterpret_cast<const uint16_t*>(s)[2 * i + 1] << 16
+                                     : reinterpret_cast<const uint32_t*>(s)[i];
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) u[i] = bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
     }
-}
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int h = 0; h < (BF16 ? 1 : 2); h++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[h].v[i] = 0;
+    }
+    __device__ __forceinline__ Pair get(int i) const {  // i = 0 .. 7
+        if (BF16) return unpack2(w[0].v[i]);
+        return pair_of(w[i >> 2 & (BF16 ? 0 : 1)].v[(2 * i) & 7], w[i >> 2 & (BF16 ? 0 : 1)].v[(2 * i + 1) & 7]);
+    }
+};
 
-// HBM-bound: 4 or 2 bytes read and 0.53 or 0.56 written per value.  A lane takes 16 neighbouring values (a block of 16, or half a
-// block of 32), a warp 512 of one row.
+// HBM-bound (4 or 2 bytes read and 0.53 or 0.56 written per value) with the instructions around a value close behind: 11 at E4M3.
+// A lane takes 16 neighbouring values (a block of 16, or half a block of 32), a warp 512 of a row.  What hides the memory is the number of
+// warps: 32 registers and 64 warps on an SM, one row each, beat two rows each with 32 warps (4096 x 8192, bf16, E4M3: 17.1 us
+// against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  17.1 us is 5.0 TB/s; 11008 x 4096 fp32 31.8 us, 6.4 TB/s.
 template <int FMT, bool BF16>
-__global__ void __launch_bounds__(32 * kRows) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                int rows, int K, size_t ld, float pre, bool vec) {
+__global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                    int rows, int K, size_t ld, float pre, int align) {
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int LPW = 4 * mx4_block(FMT) / 16;  // lanes per scale word
     const int lane = threadIdx.x & 31, tiles_k = mx4_tiles_k(K, FMT);
     const int k = blockIdx.x * kChunk + lane * 16;
-    for (size_t row = (size_t)blockIdx.y * kRows + (threadIdx.x >> 5); row < (size_t)rows; row += (size_t)gridDim.y * kRows) {
-        float u[16];
-        load16(static_cast<const char*>(in) + (row * ld + k) * (BF16 ? 2 : 4), BF16, vec, K - k, u);
+    const Pair pre2 = pair_of(pre, pre);
+    for (size_t row = (size_t)blockIdx.y * kWarps + (threadIdx.x >> 5); row < (size_t)rows; row += (size_t)gridDim.y * kWarps) {
+        Raw16<BF16> raw;
+        if (k < K) raw.load(static_cast<const char*>(in) + (row * ld + k) * (BF16 ? 2 : 4), align);
+        else raw.zero();
+        Pair v[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) u[i] = __fmul_rn(u[i], pre);
+        for (int i = 0; i < 8; i++) v[i] = mul2(raw.get(i), pre2);
         uint32_t c[2], byte;
-        mx4_encode<FMT, 16>(u, c, byte);
+        mx4_encode<FMT, 16>(v, c, byte);
         const uint32_t word = mx4_scale_word<FMT, 16>(byte, lane);
         if (k >= K) continue;
         reinterpret_cast<uint2*>(codes)[(row * K + k) >> 4] = make_uint2(c[0], c[1]);
@@ -68,48 +75,96 @@ __global__ void __launch_bounds__(32 * kRows) mx4_quantize_kernel(const void* __
     }
 }
 
-template <int FMT, bool BF16>
-__global__ void __launch_bounds__(32 * kRows) mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ out,
-                                                                  int rows, int K, float post, bool vec) {
+// HBM-bound, most of it the stores; the same division of the work, but U rows per warp, all of whose loads are under way before the
+// first is used (11008 x 4096, bf16: 20.0 us, 5.7 TB/s, against 21.9 row by row; 5003 x 2880, fp32, with 32-byte instead of
+// 16-byte stores, which fill a sector: 11.9 against 19.3).
+template <int FMT, bool BF16, int U>
+__global__ void __launch_bounds__(32 * kWarps) mx4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, void* __restrict__ out,
+                                                                   int rows, int K, float post, bool aligned) {
     const int lane = threadIdx.x & 31, tiles_k = mx4_tiles_k(K, FMT);
     const int k = blockIdx.x * kChunk + lane * 16;
     if (k >= K) return;
     const int b = k / mx4_block(FMT);
-    for (size_t row = (size_t)blockIdx.y * kRows + (threadIdx.x >> 5); row < (size_t)rows; row += (size_t)gridDim.y * kRows) {
-        const uint2 c = __ldcs(reinterpret_cast<const uint2*>(codes) + ((row * K + k) >> 4));
-        const float s = mx4_scale_value<FMT>(__ldg(scales + mx4_scale_at(row, b >> 2, tiles_k) + (b & 3)));
-        float v[16];
+    const Pair post2 = pair_of(post, post);
+    for (size_t row0 = (size_t)blockIdx.y * (kWarps * U) + (threadIdx.x >> 5); row0 < (size_t)rows; row0 += (size_t)gridDim.y * (kWarps * U)) {
+        uint2 c[U];
+        uint32_t byte[U];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float2 p = e2m1x2_value((i < 4 ? c.x : c.y) >> (8 * (i & 3)) & 0xFFu);
-            v[2 * i] = __fmul_rn(__fmul_rn(p.x, s), post);  // (code * scale is exact)
-            v[2 * i + 1] = __fmul_rn(__fmul_rn(p.y, s), post);
+        for (int u = 0; u < U; u++) {
+            const size_t row = min(row0 + u * kWarps, (size_t)rows - 1);
+            c[u] = __ldcs(reinterpret_cast<const uint2*>(codes) + ((row * K + k) >> 4));
+            byte[u] = __ldg(scales + mx4_scale_at(row, b >> 2, tiles_k) + (b & 3));
         }
-        const size_t at = row * K + k;
-        if (BF16) {
-            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-            if (vec) {
-                uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at);
-                __stcs(o, make_uint4(w[0], w[1], w[2], w[3]));
-                __stcs(o + 1, make_uint4(w[4], w[5], w[6], w[7]));
-            } else {
-                uint16_t* o = static_cast<uint16_t*>(out) + at;
+        for (int u = 0; u < U; u++) {
+            const size_t row = row0 + u * kWarps, at = row * K + k;
+            if (row >= (size_t)rows) break;
+            const float s = mx4_scale_value<FMT>(byte[u]);
+            const Pair s2 = pair_of(s, s);
+            Pair v[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+            for (int i = 0; i < 8; i++) {
+                const float2 p = e2m1x2_value((i < 4 ? c[u].x : c[u].y) >> (8 * (i & 3)) & 0xFFu);
+                v[i] = mul2(mul2(pair_of(p.x, p.y), s2), post2);  // (code * scale is exact)
             }
-        } else {
-            float* o = static_cast<float*>(out) + at;
-            if (vec) {
+            Words8 w[BF16 ? 1 : 2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) __stcs(reinterpret_cast<float4*>(o) + i, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
-            } else {
+            for (int i = 0; i < 8; i++) {
+                if (BF16) {
+                    w[0].v[i] = pack2(v[i]);
+                } else {
+                    w[i >> 2 & (BF16 ? 0 : 1)].v[(2 * i) & 7] = (uint32_t)v[i];
+                    w[i >> 2 & (BF16 ? 0 : 1)].v[(2 * i + 1) & 7] = (uint32_t)(v[i] >> 32);
+                }
+            }
+            char* o = static_cast<char*>(out) + at * (BF16 ? 2 : 4);
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[i] = v[i];
+            for (int h = 0; h < (BF16 ? 1 : 2); h++) {
+                if (aligned) {
+                    st_once_32(o + 32 * h, w[h]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (BF16) {
+                            reinterpret_cast<uint16_t*>(o)[2 * i] = (uint16_t)w[h].v[i];
+                            reinterpret_cast<uint16_t*>(o)[2 * i + 1] = (uint16_t)(w[h].v[i] >> 16);
+                        } else {
+                            reinterpret_cast<uint32_t*>(o)[8 * h + i] = w[h].v[i];
+                        }
+                    }
+                }
             }
         }
     }
+}
+
+dim3 grid_of(int rows, int K, int u) { return dim3((K + kChunk - 1) / kChunk, std::min((rows + kWarps * u - 1) / (kWarps * u), kMaxGridY)); }
+// a full wave of warps, a row each
+bool many(int rows, int K) { return (long long)rows * K >= 148ll * 64 * kChunk; }
+
+template <int FMT, bool BF16>
+cudaError_t quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, float pre, cudaStream_t stream, bool overlap_prev) {
+    const size_t step = ld * (BF16 ? 2 : 4);
+    const int align = ((uintptr_t)in | step) % 32 == 0 ? 32 : ((uintptr_t)in | step) % 16 == 0 ? 16 : 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid_of(rows, K, 1);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap_prev ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, mx4_quantize_kernel<FMT, BF16>, in, codes, scales, rows, K, ld, pre, align);
+}
+
+template <int FMT, bool BF16>
+cudaError_t dequantize(const uint32_t* codes, const uint8_t* scales, void* out, int rows, int K, float post, cudaStream_t stream) {
+    constexpr int U = 4;
+    const bool aligned = (uintptr_t)out % 32 == 0;
+    if (many(rows, K)) mx4_dequantize_kernel<FMT, BF16, U><<<grid_of(rows, K, U), 32 * kWarps, 0, stream>>>(codes, scales, out, rows, K, post, aligned);
+    else mx4_dequantize_kernel<FMT, BF16, 1><<<grid_of(rows, K, 1), 32 * kWarps, 0, stream>>>(codes, scales, out, rows, K, post, aligned);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -117,30 +172,17 @@ __global__ void __launch_bounds__(32 * kRows) mx4_dequantize_kernel(const uint32
 cudaError_t launch_mx4_quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, int format, int in_dtype, float pre,
                                 cudaStream_t stream, bool overlap_prev) {
     if (!rows) return cudaSuccess;
-    const bool bf16 = in_dtype == LUX_DTYPE_BFLOAT16, vec = ((uintptr_t)in & 15) == 0 && ld % (bf16 ? 8 : 4) == 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((K + kChunk - 1) / kChunk, std::min((rows + kRows - 1) / kRows, kMaxGridY));
-    cfg.blockDim = dim3(32 * kRows);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = overlap_prev ? 1 : 0;
-    auto kern = format == LUX_CUDA_MX4_E8M0 ? (bf16 ? mx4_quantize_kernel<LUX_CUDA_MX4_E8M0, true> : mx4_quantize_kernel<LUX_CUDA_MX4_E8M0, false>)
-                                            : (bf16 ? mx4_quantize_kernel<LUX_CUDA_MX4_E4M3, true> : mx4_quantize_kernel<LUX_CUDA_MX4_E4M3, false>);
-    return cudaLaunchKernelEx(&cfg, kern, in, codes, scales, rows, K, ld, pre, vec);
+    auto f = format == LUX_CUDA_MX4_E8M0 ? (in_dtype == LUX_DTYPE_BFLOAT16 ? quantize<LUX_CUDA_MX4_E8M0, true> : quantize<LUX_CUDA_MX4_E8M0, false>)
+                                         : (in_dtype == LUX_DTYPE_BFLOAT16 ? quantize<LUX_CUDA_MX4_E4M3, true> : quantize<LUX_CUDA_MX4_E4M3, false>);
+    return f(in, codes, scales, rows, K, ld, pre, stream, overlap_prev);
 }
 
 cudaError_t launch_mx4_dequantize(const uint32_t* codes, const uint8_t* scales, void* out, int rows, int K, int format, int out_dtype, float post,
                                   cudaStream_t stream) {
     if (!rows) return cudaSuccess;
-    const bool bf16 = out_dtype == LUX_DTYPE_BFLOAT16, vec = ((uintptr_t)out & 15) == 0;
-    const dim3 grid((K + kChunk - 1) / kChunk, std::min((rows + kRows - 1) / kRows, kMaxGridY));
-    auto kern = format == LUX_CUDA_MX4_E8M0 ? (bf16 ? mx4_dequantize_kernel<LUX_CUDA_MX4_E8M0, true> : mx4_dequantize_kernel<LUX_CUDA_MX4_E8M0, false>)
-                                            : (bf16 ? mx4_dequantize_kernel<LUX_CUDA_MX4_E4M3, true> : mx4_dequantize_kernel<LUX_CUDA_MX4_E4M3, false>);
-    kern<<<grid, 32 * kRows, 0, stream>>>(codes, scales, out, rows, K, post, vec);
-    return cudaGetLastError();
+    auto f = format == LUX_CUDA_MX4_E8M0 ? (out_dtype == LUX_DTYPE_BFLOAT16 ? dequantize<LUX_CUDA_MX4_E8M0, true> : dequantize<LUX_CUDA_MX4_E8M0, false>)
+                                         : (out_dtype == LUX_DTYPE_BFLOAT16 ? dequantize<LUX_CUDA_MX4_E4M3, true> : dequantize<LUX_CUDA_MX4_E4M3, false>);
+    return f(codes, scales, out, rows, K, post, stream);
 }
 
 }  // namespace luxcuda

@@ -415,7 +415,9 @@ class Context:
 
     def mx4_quantize(self, src, codes, scales, rows, K, fmt, in_dtype, pre=1.0, ld=0):
         """src * pre into 4-bit codes and block scales; ld: row stride of src in elements (0: K)."""
-        self.plugin.check(self._mx4_quantize(self.handle, src.handle, codes.handle, scales.handle, rows, K, ld, fmt, in_dtype, pre), "mx4_quantize")
+        code = self._mx4_quantize(self.handle, src.handle, codes.handle, scales.handle, rows, K, ld, fmt, in_dtype, pre)
+        if code != OK:
+            self.plugin.check(code, "mx4_quantize")
 
     def mx4_dequantize(self, codes, scales, dst, rows, K, fmt, out_dtype, post=1.0):
         """dst = code * scale * post."""
@@ -423,8 +425,9 @@ class Context:
 
     def mx4_matmul(self, x_codes, x_scales, w_codes, w_scales, y, M, K, N, fmt, y_dtype, alpha=1.0):
         """y = alpha * x . W^T, both operands in the microscaled format."""
-        self.plugin.check(self._mx4_matmul(self.handle, x_codes.handle, x_scales.handle, w_codes.handle, w_scales.handle, y.handle, M, K, N, fmt,
-                                           y_dtype, alpha), "mx4_matmul")
+        code = self._mx4_matmul(self.handle, x_codes.handle, x_scales.handle, w_codes.handle, w_scales.handle, y.handle, M, K, N, fmt, y_dtype, alpha)
+        if code != OK:
+            self.plugin.check(code, "mx4_matmul")
 
     # --- norm after a block, gate, residual, norm before the next ---------------
     @staticmethod
@@ -436,8 +439,10 @@ class Context:
 
     def block_norm(self, params, h, gate, r, post_w, post_b, pre_w, pre_b, r_out, out, out_scales=None):
         """r_out = res_scale * r + branch_scale * act(gate) * post_norm(h); out = pre_norm(r_out).  None where there is no such buffer."""
-        args = [None if b is None else b.handle for b in (h, gate, r, post_w, post_b, pre_w, pre_b, r_out, out, out_scales)]
-        self.plugin.check(self._block_norm(self.handle, C.byref(params), *args), "block_norm")
+        code = self._block_norm(self.handle, params, h and h.handle, gate and gate.handle, r and r.handle, post_w and post_w.handle, post_b and post_b.handle,
+                                pre_w and pre_w.handle, pre_b and pre_b.handle, r_out and r_out.handle, out and out.handle, out_scales and out_scales.handle)
+        if code != OK:
+            self.plugin.check(code, "block_norm")
 
     def timer_record(self, slot):
         self.plugin.check(self.plugin.quant.timer_record(self.handle, slot), "timer_record")
