@@ -9,153 +9,11 @@
 // registers between the statistics, which are fp32 sums over threads, lanes and warps; the variance is the mean of squared differences.
 #include <algorithm>
 
-#include "internal.h"
-#include "mx4.cuh"
-#include "pair.cuh"
+#include "block_norm.cuh"
 
 namespace luxcuda {
 
 namespace {
-
-__device__ __forceinline__ float act_of(float g, int act) {
-    if (act == LUX_CUDA_GATE_SIGMOID) {
-        // 1 / (1 + 2^t), t = -g / ln 2 in two pieces, so that a large g costs no accuracy; at a third of what expf and an exact
-        // reciprocal issue, which were a quarter of the kernel
-        const float c_hi = -1.44269504f, c_lo = -1.92596299e-8f;  // -1 / ln 2
-        const float t = g * c_hi, lo = fmaf(g, c_lo, fmaf(g, c_hi, -t));
-        float e, d;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        e = fmaf(e, lo * 0.693147181f, e);
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(1.0f + e));
-        return d;
-    }
-    if (act == LUX_CUDA_GATE_TANH) return tanhf(g);
-    return g;
-}
-__device__ __forceinline__ float round_bf16(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
-// rows are read once and their results not again here: neither stays in L1, where the weights are
-__device__ __forceinline__ uint4 ld_row(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ void st_row(void* p, const uint4& v) {
-    asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-// A thread's eight elements of a chunk: neighbours, on a 16-byte boundary (kWide: kFull where no chunk is cut off by the row's end),
-// or, on any boundary, `step` apart, those at `end` and behind it zero (kApart).
-enum Mode { kWide, kFull, kApart };
-struct Place {
-    uint32_t first, step, end;
-};
-template <bool BF16, int MODE>
-struct Raw {
-    uint4 q[BF16 ? 1 : 2];
-    __device__ __forceinline__ void load(const char* row, const Place& p) {
-        if constexpr (MODE != kApart) {
-            const char* s = row + (size_t)p.first * (BF16 ? 2 : 4);
-            q[0] = ld_row(s);
-            if (!BF16) q[BF16 ? 0 : 1] = ld_row(s + 16);
-        } else {
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t i = p.first + e * p.step;
-                w[e] = i >= p.end ? 0u : BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[i] : reinterpret_cast<const uint32_t*>(row)[i];
-            }
-            if (BF16) {
-                q[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-            } else {
-                q[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                q[BF16 ? 0 : 1] = make_uint4(w[4], w[5], w[6], w[7]);
-            }
-        }
-    }
-    __device__ __forceinline__ Pair get(int i) const {  // i = 0 .. 3
-        if (BF16) return unpack2(i == 0 ? q[0].x : i == 1 ? q[0].y : i == 2 ? q[0].z : q[0].w);
-        const uint4 t = q[BF16 ? 0 : i >> 1];
-        return i & 1 ? pair_of(t.z, t.w) : pair_of(t.x, t.y);
-    }
-};
-template <bool BF16, int MODE>
-__device__ __forceinline__ void store8(char* row, const Place& p, const Pair (&v)[4]) {
-    if (MODE == kApart) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t i = p.first + e * p.step;
-            const float x = e & 1 ? hi_of(v[e >> 1]) : lo_of(v[e >> 1]);
-            if (i < p.end) {
-                if (BF16) reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(x);
-                else reinterpret_cast<float*>(row)[i] = x;
-            }
-        }
-    } else if (BF16) {
-        st_row(row + (size_t)p.first * 2, make_uint4(pack2(v[0]), pack2(v[1]), pack2(v[2]), pack2(v[3])));
-    } else {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            st_row(row + (size_t)p.first * 4 + 16 * h, make_uint4((uint32_t)v[2 * h], (uint32_t)(v[2 * h] >> 32), (uint32_t)v[2 * h + 1], (uint32_t)(v[2 * h + 1] >> 32)));
-    }
-}
-template <int MODE>
-__device__ __forceinline__ void weights8(const float* w, const Place& p, Pair (&v)[4]) {
-    if (MODE == kApart) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t i = p.first + 2 * e * p.step, k = i + p.step;
-            v[e] = pair_of(i < p.end ? __ldg(w + i) : 0.0f, k < p.end ? __ldg(w + k) : 0.0f);
-        }
-    } else {
-        const ulonglong2 a = __ldg(reinterpret_cast<const ulonglong2*>(w + p.first)), b = __ldg(reinterpret_cast<const ulonglong2*>(w + p.first) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-    }
-}
-// What the threads of a row, a warp of its own or the whole block, exchange: two places, used in turn, so that a warp may be a step
-// ahead of those that still read.
-struct Shared {
-    float2 part[2][32];
-};
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-// every lane gets the contribution of the warp of its number (zeros past the last).  All warps go on with all of them: one warp that
-// does, and tells the others, makes two waits of one (2048 x 4096, layer | layer: 51 us against 40).
-__device__ __forceinline__ float2 exchange(float2 v, Shared& sh, int& turn) {
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) sh.part[turn][threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = lane < (int)(blockDim.x >> 5) ? sh.part[turn][lane] : make_float2(0.0f, 0.0f);
-    turn ^= 1;
-    return v;
-}
-__device__ __forceinline__ float row_sum(float v, Shared& sh, int& turn) {
-    v = warp_sum(v);
-    return blockDim.x == 32 ? v : warp_sum(exchange(make_float2(v, 0.0f), sh, turn).x);
-}
-struct Stats {
-    float mean, squares;
-};
-// The row's mean and the squared differences from it, in one exchange, from every thread's own mean and squared differences over n
-// elements, the same number in all threads: two halves of 2n elements have their means' mean and, besides their own, n/2 times the
-// squared difference of the means (Chan, Golub, LeVeque 1979).
-__device__ __forceinline__ Stats row_moments(float mean, float squares, int n, float inv_dim, Shared& sh, int& turn) {
-    float half = 0.5f * n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1, half *= 2.0f) {
-        const float d = __shfl_xor_sync(0xffffffffu, mean, o) - mean;
-        squares += __shfl_xor_sync(0xffffffffu, squares, o);
-        squares = fmaf(d * d, half, squares);
-        mean = fmaf(0.5f, d, mean);
-    }
-    if (blockDim.x == 32) return Stats{mean, squares};
-    const float2 p = exchange(make_float2(mean, squares), sh, turn);
-    mean = warp_sum(p.x) * (32 * n * inv_dim);
-    const float d = (threadIdx.x & 31) < blockDim.x >> 5 ? p.x - mean : 0.0f;
-    return Stats{mean, warp_sum(fmaf(d * d, 32.0f * n, p.y))};
-}
-__device__ __forceinline__ float inv_root(float squares, float inv_dim, float eps) { return __frsqrt_rn(fmaf(squares, inv_dim, eps)); }
 
 // Rows of up to 8 * CH elements per thread, a multiple of 8, every row on a 16-byte boundary; FULL: exactly so many.  blockDim =
 // (threads of a row, rows): several rows only where a row is a warp's.  OUT: 0: fp32 or bf16, else a microscaled format.
@@ -165,7 +23,6 @@ __device__ __forceinline__ float inv_root(float squares, float inv_dim, float ep
 template <int CH, bool XB, bool RB, int OUT, int MODE>
 __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
     __shared__ Shared sh;
-    int turn = 0;
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -202,26 +59,9 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
         chunks([&](int j, const Place& p) { rg[j].load(gate, p); });
     }
     Pair v[CH][4];
-    auto total = [&]() {
-        Pair s = 0;
-        chunks([&](int j, const Place&) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) s = add2(s, v[j][e]);
-        });
-        return lo_of(s) + hi_of(s);
-    };
-    auto squares = [&](float mean) {  // of the differences from mean
-        Pair s = 0;
-        const Pair neg = pair_of(-mean, -mean);
-        chunks([&](int j, const Place&) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const Pair d = mean == 0.0f ? v[j][e] : add2(v[j][e], neg);
-                s = fma2(d, d, s);
-            }
-        });
-        return lo_of(s) + hi_of(s);
-    };
+    Group g{&sh, (int)(blockDim.x >> 5), (int)(threadIdx.x >> 5), 0, 0};
+    auto within = [&](int j) { return at(j).first < dim; };
+    RowValues<CH, FULL, decltype(within)> values{v, within, g, a};
     auto shift = [&](float mean) {
         const Pair neg = pair_of(-mean, -mean);
         chunks([&](int j, const Place& p) {
@@ -235,50 +75,13 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
             }
         });
     };
-    // 1 / sqrt(...) of a norm; its mean is taken off
-    auto scale_of = [&](int kind) {
-        if (kind == LUX_CUDA_NORM_LAYER) {
-            if (FULL) {
-                const float own = total() * (1.0f / (8 * CH));
-                const Stats st = row_moments(own, squares(own), 8 * CH, a.inv_dim, sh, turn);
-                shift(st.mean);
-                return inv_root(st.squares, a.inv_dim, a.eps);
-            }
-            shift(row_sum(total(), sh, turn) * a.inv_dim);
-        }
-        return inv_root(row_sum(squares(0.0f), sh, turn), a.inv_dim, a.eps);
-    };
-    auto norm = [&](int kind, const float* w, const float* c) {
-        if (kind == LUX_CUDA_NORM_NONE) return;
-        const float scale = scale_of(kind);
-        const Pair inv = pair_of(scale, scale);
-        if (w) {
-            chunks([&](int j, const Place& p) {
-                Pair wv[4];
-                weights8<MODE>(w, p, wv);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[j][e] = mul2(mul2(v[j][e], inv), wv[e]);
-            });
-        } else {
-            chunks([&](int j, const Place&) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[j][e] = mul2(v[j][e], inv);
-            });
-        }
-        if (c)
-            chunks([&](int j, const Place& p) {
-                Pair cv[4];
-                weights8<MODE>(c, p, cv);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[j][e] = add2(v[j][e], cv[e]);
-            });
-    };
+    auto weights = [&](const float* w, int j, Pair (&out)[4]) { weights8<MODE>(w, at(j), out); };
     if (a.h) {
         chunks([&](int j, const Place&) {
 #pragma unroll
             for (int e = 0; e < 4; e++) v[j][e] = rh[j].get(e);
         });
-        norm(a.post_kind, a.post_w, a.post_b);
+        values.norm(a.post_kind, a.post_w, a.post_b, shift, weights);
         auto gated = [&](auto&& act) {
             chunks([&](int j, const Place&) {
 #pragma unroll
@@ -293,11 +96,7 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
             else if (a.gate_act == LUX_CUDA_GATE_TANH) gated([](float g) { return act_of(g, LUX_CUDA_GATE_TANH); });
             else gated([](float g) { return g; });
         }
-        const Pair branch = pair_of(a.branch_scale, a.branch_scale);
-        chunks([&](int j, const Place&) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[j][e] = mul2(branch, v[j][e]);
-        });
+        values.scale_by(a.branch_scale);
     } else {
         chunks([&](int j, const Place&) {
 #pragma unroll
@@ -319,30 +118,14 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
             for (int e = 0; e < 4; e++) v[j][e] = unpack2(pack2(v[j][e]));
         });
     if (!a.out) return;
-    norm(a.pre_kind, a.pre_w, a.pre_b);
+    values.norm(a.pre_kind, a.pre_w, a.pre_b, shift, weights);
     if (OUT == 0) {
         char* out = static_cast<char*>(a.out) + r0 * (a.out_bf16 ? 2 : 4);
         if (a.out_bf16) chunks([&](int j, const Place& p) { store8<true, MODE>(out, p, v[j]); });
         else chunks([&](int j, const Place& p) { store8<false, MODE>(out, p, v[j]); });
     } else {
-        constexpr int F = OUT ? OUT : 1;
-        const Pair pre = pair_of(a.out_pre, a.out_pre);
-        const int tiles_k = mx4_tiles_k(dim, F);
 #pragma unroll
-        for (int j = 0; j < CH; j++) {  // (the whole warp: lanes past the row carry zeros)
-            const uint32_t i = at(j).first;
-            Pair u[4];
-            uint32_t c[1], byte;
-#pragma unroll
-            for (int e = 0; e < 4; e++) u[e] = FULL || i < dim ? mul2(unpack2(pack2(v[j][e])), pre) : 0;
-            mx4_encode<F, 8>(u, c, byte);
-            const uint32_t word = mx4_scale_word<F, 8>(byte, threadIdx.x & 31);
-            if (FULL || i < dim) {
-                static_cast<uint32_t*>(a.out)[(r0 + i) >> 3] = c[0];
-                if ((threadIdx.x & 31) % (mx4_block(F) / 2) == 0)
-                    *reinterpret_cast<uint32_t*>(a.out_scales + mx4_scale_at(row, i / (4 * mx4_block(F)), tiles_k)) = word;
-            }
-        }
+        for (int j = 0; j < CH; j++) put_codes<OUT ? OUT : 1>(a, v[j], row, at(j).first, FULL || at(j).first < dim);
     }
 }
 
@@ -353,8 +136,8 @@ template <int OUT, int V>
 __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_constant__ BlockNormArgs a) {
     static_assert(OUT == 0 || V == 8, "blocks of codes: eight neighbours");
     __shared__ Shared sh;
-    int turn = 0;
-    // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
+    Group g{&sh, (int)(blockDim.x >> 5), (int)(threadIdx.x >> 5), 0, 0};
+    // (as above)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const size_t dim = a.dim, row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -401,14 +184,14 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_const
         float s = 0.0f;
         if (kind == LUX_CUDA_NORM_LAYER) {
             elements([&](size_t i) { s += value(i); });
-            st.mean = row_sum(s, sh, turn) * a.inv_dim;
+            st.mean = row_sum(s, g) * a.inv_dim;
             s = 0.0f;
         }
         elements([&](size_t i) {
             const float d = value(i) - st.mean;
             s = fmaf(d, d, s);
         });
-        st.inv = inv_root(row_sum(s, sh, turn), a.inv_dim, a.eps);
+        st.inv = inv_root(row_sum(s, g), a.inv_dim, a.eps);
         return st;
     };
     if (a.h) post = stats(a.post_kind, h_at);
@@ -418,21 +201,13 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_const
     if (OUT == 0) {
         elements([&](size_t i) { st(a.out, a.out_bf16, r0 + i, norm(pre, a.pre_kind, a.pre_w, a.pre_b, i, r_at(i))); });
     } else {
-        constexpr int F = OUT ? OUT : 1;
         for (size_t base = 0; base < dim; base += step) {  // (the whole warp: lanes past the row carry zeros)
             const size_t at = base + (size_t)threadIdx.x * V;
             Pair u[4];
-            uint32_t c[1], byte;
-            auto value = [&](size_t i) { return i < dim ? __fmul_rn(round_bf16(norm(pre, a.pre_kind, a.pre_w, a.pre_b, i, r_at(i))), a.out_pre) : 0.0f; };
+            auto value = [&](size_t i) { return i < dim ? norm(pre, a.pre_kind, a.pre_w, a.pre_b, i, r_at(i)) : 0.0f; };
 #pragma unroll
             for (int e = 0; e < 4; e++) u[e] = pair_of(value(at + 2 * e), value(at + 2 * e + 1));
-            mx4_encode<F, 8>(u, c, byte);
-            const uint32_t word = mx4_scale_word<F, 8>(byte, threadIdx.x & 31);
-            if (at < dim) {
-                static_cast<uint32_t*>(a.out)[(r0 + at) >> 3] = c[0];
-                if ((threadIdx.x & 31) % (mx4_block(F) / 2) == 0)
-                    *reinterpret_cast<uint32_t*>(a.out_scales + mx4_scale_at(row, (int)(at / (4 * mx4_block(F))), mx4_tiles_k((int)dim, F))) = word;
-            }
+            put_codes<OUT ? OUT : 1>(a, u, row, (uint32_t)at, at < dim);
         }
     }
 }
@@ -456,6 +231,7 @@ NormKernel pick(const BlockNormArgs& a) {
 
 cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev) {
     if (!a.rows || !a.dim) return cudaSuccess;
+    if (block_norm_streams(a, sm_count)) return launch_block_norm_stream(a, sm_count, stream, overlap_prev);
     NormKernel kern;
     size_t threads;
     auto warps = [](size_t n) { return (n + 31) / 32 * 32; };

@@ -343,7 +343,10 @@ struct BlockNormArgs {
     bool x_bf16, r_bf16, out_bf16;
     bool vec;  // every row of every buffer starts on a 16-byte boundary
     float eps, res_scale, branch_scale, out_pre, inv_dim;
+    int* error;  // as QmmArgs::error
 };
+bool block_norm_streams(const BlockNormArgs& a, int sm_count);  // rows that block_norm_stream.cu takes
+cudaError_t launch_block_norm_stream(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);

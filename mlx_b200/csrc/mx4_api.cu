@@ -185,7 +185,7 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     a.x_bf16 = xs == 2; a.r_bf16 = rs == 2; a.out_bf16 = os == 2;
     a.vec = vec(H, h_ld, xs) && vec(GATE, gate_ld, xs) && vec(R, p.dim, rs) && vec(R_OUT, p.dim, rs) && (mx || vec(OUT, p.dim, os));
     for (int i = POST_W; i <= PRE_B; i++) a.vec = a.vec && vec(i, 0, 4);
-    a.eps = p.eps; a.res_scale = p.res_scale; a.branch_scale = p.branch_scale; a.out_pre = p.out_pre; a.inv_dim = (float)(1.0 / (double)p.dim);
+    a.eps = p.eps; a.res_scale = p.res_scale; a.branch_scale = p.branch_scale; a.out_pre = p.out_pre; a.inv_dim = (float)(1.0 / (double)p.dim); a.error = c->err_dev;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
     const bool chained = chain_is_open(c);

@@ -301,3 +301,40 @@ def test_refusals(ctx, plugin):
         assert e.value.code == P.ERR_INVALID, kw
     assert plugin.last_error()
     assert plugin.quant.block_norm(None, None, *[None] * 10) == P.ERR_INVALID
+
+
+@pytest.mark.parametrize("post,pre", [(0, 1), (1, 1), (2, 2), (1, 0)])
+@pytest.mark.parametrize("rows,dim,gate_rows", [(1200, 2048, None), (1300, 2880, 0), (1184, 4096, 1), (1500, 2056, 7)])
+def test_many_rows(ctx, oracle, rows, dim, gate_rows, post, pre):
+    """Rows that one block per SM takes in turn: with and without a gate, shared by all, by some or of each row's own; every type."""
+    for xd, rd, od, act in ((BF16, BF16, BF16, P.GATE_TANH), (BF16, F32, F32, P.GATE_SIGMOID), (F32, BF16, F32, P.GATE_IDENTITY), (F32, F32, BF16, P.GATE_SIGMOID)):
+        run(ctx, oracle, rows, dim, post, pre, gate_rows, act if gate_rows is not None else 0, xd, rd, od, seed=post)
+
+
+@pytest.mark.parametrize("fmt", [P.MX4_E8M0, P.MX4_E4M3])
+@pytest.mark.parametrize("rows,dim", [(1300, 2048), (1200, 2912)])
+def test_many_rows_microscaled_in_place_and_column_blocks(ctx, oracle, fmt, rows, dim):
+    rng = np.random.default_rng(dim)
+    bh, _ = place(ctx, oracle, rng.standard_normal((rows, dim + 64)), BF16)
+    stream = rng.standard_normal((rows, dim)).astype(np.float32)
+    bw, _ = place(ctx, oracle, rng.standard_normal(dim), F32)
+    kw = dict(post=P.NORM_LAYER, pre=P.NORM_RMS, r_dtype=F32, eps=EPS, branch_scale=0.5, h_ld=dim + 64)
+    n = ctx.mx4_scale_bytes(rows, dim, fmt)
+    out, new = empty(ctx, (rows, dim), BF16), ctx.upload(stream)
+    codes = [ctx.empty((rows, dim // 8), np.uint32) for _ in range(2)]
+    scales = [ctx.upload(np.full(n, 0x5A, np.uint8)) for _ in range(2)]
+    ctx.block_norm(ctx.block_norm_params(rows, dim, **kw), bh, None, new, bw, bw, bw, None, new, out)
+    ctx.mx4_quantize(out, codes[0], scales[0], rows, dim, fmt, BF16, 3.7)
+    first = new.to_host()
+    new.from_host(stream)
+    for _ in range(3):  # the stream in place: every call adds the branch again; the last of three replays after a reset is compared
+        new.from_host(stream)
+        ctx.block_norm(ctx.block_norm_params(rows, dim, out_format=fmt, out_pre=3.7, **kw), bh, None, new, bw, bw, bw, None, new, codes[1], scales[1])
+    assert np.array_equal(new.to_host(), first)
+    np.testing.assert_array_equal(scales[1].to_host(), scales[0].to_host())
+    np.testing.assert_array_equal(codes[1].to_host(), codes[0].to_host())
+    # without a block's output: the norm of the stream alone
+    ctx.block_norm(ctx.block_norm_params(rows, dim, pre=P.NORM_RMS, r_dtype=F32, eps=EPS), None, None, new, None, None, bw, None, None, out)
+    want = mx4.norm(first, 1, EPS, bw.room.to_host())
+    tol = norm_tolerance(first.astype(np.float64), 1, bw.room.to_host(), None, want)
+    assert (np.abs(host(oracle, out, BF16) - want) <= tol + rounding(np.abs(want) + tol, BF16)).all()
