@@ -159,7 +159,8 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     if (!p.dim || p.dim > INT32_MAX || p.rows > INT32_MAX || h_ld < p.dim || gate_ld < p.dim || h_ld > (1ull << 31) || gate_ld > (1ull << 31))
         return invalid("block_norm: rows, dim or a row stride out of range");
     if (!p.rows) return LUX_BACKEND_OK;
-    const size_t gate_n = p.gate_rows ? (p.rows + p.gate_rows - 1) / p.gate_rows : 1;
+    const size_t gate_rows = p.gate_rows < p.rows ? p.gate_rows : 0;  // (from here on below 2^31: all rows share one beyond)
+    const size_t gate_n = gate_rows ? (p.rows + gate_rows - 1) / gate_rows : 1;
     const size_t bytes[COUNT] = {((p.rows - 1) * h_ld + p.dim) * xs, ((gate_n - 1) * gate_ld + p.dim) * xs, p.rows * p.dim * rs, p.dim * 4, p.dim * 4, p.dim * 4,
                                  p.dim * 4, p.rows * p.dim * rs, mx ? p.rows * p.dim / 2 : p.rows * p.dim * os,
                                  mx ? mx4_scale_bytes((int)p.rows, (int)p.dim, p.out_format) : 0};
@@ -180,7 +181,7 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     a.h = ptr(H); a.gate = ptr(GATE); a.r = ptr(R);
     a.post_w = (const float*)ptr(POST_W); a.post_b = (const float*)ptr(POST_B); a.pre_w = (const float*)ptr(PRE_W); a.pre_b = (const float*)ptr(PRE_B);
     a.r_out = ptr(R_OUT); a.out = ptr(OUT); a.out_scales = (uint8_t*)ptr(SCALES);
-    a.rows = p.rows; a.dim = p.dim; a.h_ld = h_ld; a.gate_ld = gate_ld; a.gate_rows = p.gate_rows;
+    a.rows = p.rows; a.dim = p.dim; a.h_ld = h_ld; a.gate_ld = gate_ld; a.gate_rows = gate_rows;
     a.post_kind = p.post_norm; a.pre_kind = p.pre_norm; a.gate_act = p.gate_act; a.out_format = p.out_format;
     a.x_bf16 = xs == 2; a.r_bf16 = rs == 2; a.out_bf16 = os == 2;
     a.vec = vec(H, h_ld, xs) && vec(GATE, gate_ld, xs) && vec(R, p.dim, rs) && vec(R_OUT, p.dim, rs) && (mx || vec(OUT, p.dim, os));

@@ -338,3 +338,24 @@ def test_many_rows_microscaled_in_place_and_column_blocks(ctx, oracle, fmt, rows
     want = mx4.norm(first, 1, EPS, bw.room.to_host())
     tol = norm_tolerance(first.astype(np.float64), 1, bw.room.to_host(), None, want)
     assert (np.abs(host(oracle, out, BF16) - want) <= tol + rounding(np.abs(want) + tol, BF16)).all()
+
+
+@pytest.mark.parametrize("rows,dim", [(5, 96), (3, 40008), (1200, 2048)])
+@pytest.mark.parametrize("gate_rows", [1 << 31, 1 << 32, (1 << 64) - 1])
+def test_a_gate_shared_by_more_rows_than_there_are(ctx, rows, dim, gate_rows):
+    """One row of gate serves them all, as with 0; a gate with less than a row is refused however many share it."""
+    rng = np.random.default_rng(rows)
+    bits = lambda shape: ctx.upload((rng.standard_normal(shape).astype(np.float32).view(np.uint32) >> 16).astype(np.uint16))  # noqa: E731
+    h, r, g = bits((rows, dim)), bits((rows, dim)), bits((dim,))
+    got = []
+    for n in (0, gate_rows):
+        new, out = empty(ctx, (rows, dim), BF16), empty(ctx, (rows, dim), BF16)
+        ctx.block_norm(ctx.block_norm_params(rows, dim, post=P.NORM_RMS, pre=P.NORM_RMS, gate_act=P.GATE_SIGMOID, gate_rows=n, eps=EPS), h, g, r, None, None, None, None, new, out)
+        got.append((new.to_host(), out.to_host()))
+    np.testing.assert_array_equal(got[1][0], got[0][0])
+    np.testing.assert_array_equal(got[1][1], got[0][1])
+    for less in (dim - 1, 1):
+        with pytest.raises(BackendError) as e:
+            ctx.block_norm(ctx.block_norm_params(rows, dim, post=P.NORM_RMS, pre=P.NORM_RMS, gate_rows=gate_rows, eps=EPS), h, ctx.wrap(g.device_ptr, less * 2), r, None, None, None, None,
+                           new, out)
+        assert e.value.code == P.ERR_INVALID
