@@ -304,7 +304,7 @@ typedef struct lux_gpu_quant_vtbl {
     /* --- microscaled 4-bit floating point: quantisation, expansion, product (LUX_CUDA_QUANT_HAS) ---
      * (No counterpart in the reference, which has no quantized format.)
      * codes   uint32[rows][K/8], LSB-first along K as the 4-bit words above; a code is E2M1: sign (bit 3), then
-     *         0 0.5 1 1.5 2 3 4 6.  K is a multiple of 32.
+     *         0 0.5 1 1.5 2 3 4 6.  K is a multiple of 32, at most 2^31 - 512.
      * scales  one byte per block of a row:  LUX_CUDA_MX4_E8M0: 32 codes, 2^(byte-127), 255 = NaN;
      *                                       LUX_CUDA_MX4_E4M3: 16 codes, an 8-bit float (4 exponent bits, bias 7;
      *                                       3 mantissa bits; 0x7F = NaN).

@@ -17,8 +17,9 @@ bool aligned(const Buffer* b, size_t n) { return ((uintptr_t)b->ptr & (n - 1)) =
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
     return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
+constexpr int kMaxK = INT32_MAX - 511;  // rounded up to what any kernel takes at a time it is still an int
 size_t mx4_scale_bytes(int rows, int K, int format) {
-    if (rows < 0 || K <= 0 || K % 32 || (format != LUX_CUDA_MX4_E8M0 && format != LUX_CUDA_MX4_E4M3)) return 0;
+    if (rows < 0 || K <= 0 || K > kMaxK || K % 32 || (format != LUX_CUDA_MX4_E8M0 && format != LUX_CUDA_MX4_E4M3)) return 0;
     return ((size_t)rows + 127) / 128 * mx4_tiles_k(K, format) * 512;
 }
 LuxBackendError check_format(int rows, int K, int format) {
@@ -26,8 +27,8 @@ LuxBackendError check_format(int rows, int K, int format) {
         set_last_error("mx4: format must be LUX_CUDA_MX4_E8M0 or LUX_CUDA_MX4_E4M3 (got %d)", format);
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     }
-    if (rows < 0 || K <= 0 || K % 32) {
-        set_last_error("mx4: K=%d must be a positive multiple of 32, the number of rows (%d) not negative", K, rows);
+    if (rows < 0 || K <= 0 || K > kMaxK || K % 32) {
+        set_last_error("mx4: K=%d must be a positive multiple of 32, at most 2^31 - 512, the number of rows (%d) not negative", K, rows);
         return LUX_BACKEND_ERROR_INVALID_ARGUMENT;
     }
     return LUX_BACKEND_OK;
@@ -158,6 +159,8 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     const size_t h_ld = p.h_ld ? p.h_ld : p.dim, gate_ld = p.gate_ld ? p.gate_ld : p.dim;
     if (!p.dim || p.dim > INT32_MAX || p.rows > INT32_MAX || h_ld < p.dim || gate_ld < p.dim || h_ld > (1ull << 31) || gate_ld > (1ull << 31))
         return invalid("block_norm: rows, dim or a row stride out of range");
+    if (mx)
+        if (LuxBackendError e = check_format((int)p.rows, (int)p.dim, p.out_format)) return e;
     if (!p.rows) return LUX_BACKEND_OK;
     const size_t gate_rows = p.gate_rows < p.rows ? p.gate_rows : 0;  // (from here on below 2^31: all rows share one beyond)
     const size_t gate_n = gate_rows ? (p.rows + gate_rows - 1) / gate_rows : 1;

@@ -706,9 +706,9 @@ struct TilePlan {
 TilePlan plan_tile(int M, int K, int N, int format, int sm_count) {
     const int st = stage_tiles(format), nst = (K + kStageK - 1) / kStageK;
     TilePlan t;
-    t.bm = std::min(kTileM, (M + 15) & ~15);
-    t.m_tiles = (M + t.bm - 1) / t.bm;
-    t.tiles = (long long)t.m_tiles * ((N + kTileN - 1) / kTileN);
+    t.bm = M >= kTileM ? kTileM : (M + 15) & ~15;
+    t.m_tiles = (M - 1) / t.bm + 1;
+    t.tiles = (long long)t.m_tiles * ((N - 1) / kTileN + 1);
     t.stage_bytes = (kABytes + t.bm * 128 + 2 * st * kScaleTile + 1023) & ~1023;
     t.sf_col = (t.bm + 31) & ~31;
     auto fit = [&](int stages) {
@@ -788,11 +788,11 @@ cudaError_t launch_pair(const Mx4MatmulArgs& a, int sm_count, cudaStream_t strea
     PairParams p = {};
     p.y = a.y; p.error = a.error ? a.error : device_error_word();
     p.M = a.M; p.K = a.K; p.N = a.N; p.alpha = a.alpha;
-    p.m_tiles = (a.M + 2 * kTileN - 1) / (2 * kTileN);
-    const long long tiles = (long long)p.m_tiles * ((a.N + kPairN - 1) / kPairN);
+    p.m_tiles = (a.M - 1) / (2 * kTileN) + 1;
+    const long long tiles = (long long)p.m_tiles * ((a.N - 1) / kPairN + 1);
     p.tiles_k = mx4_tiles_k(a.K, FMT);
     p.nst = (a.K + kStageK - 1) / kStageK;
-    const long long x_tiles = (long long)((a.M + kTileN - 1) / kTileN) * p.tiles_k, w_tiles = (long long)((a.N + kTileN - 1) / kTileN) * p.tiles_k;
+    const long long x_tiles = (long long)((a.M - 1) / kTileN + 1) * p.tiles_k, w_tiles = (long long)((a.N - 1) / kTileN + 1) * p.tiles_k;
     if (tiles > 0x7fffffff || x_tiles > 0x7fffffff || w_tiles > 0x7fffffff) return cudaErrorInvalidValue;
     p.tiles = (int)tiles;
     CUtensorMap map_x, map_w, map_xs, map_ws, map_y;

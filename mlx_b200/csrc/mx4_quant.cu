@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * kWarps) mx4_dequantize_kernel(const uint3
     }
 }
 
-dim3 grid_of(int rows, int K, int u) { return dim3((K + kChunk - 1) / kChunk, std::min((rows + kWarps * u - 1) / (kWarps * u), kMaxGridY)); }
+dim3 grid_of(int rows, int K, int u) { return dim3((K + kChunk - 1) / kChunk, std::min((rows - 1) / (kWarps * u) + 1, kMaxGridY)); }
 // a full wave of warps, a row each
 bool many(int rows, int K) { return (long long)rows * K >= 148ll * 64 * kChunk; }
 

@@ -337,3 +337,25 @@ def test_refusals(ctx, plugin):
         assert e.value.code == P.ERR_INVALID
     assert ctx.mx4_scale_bytes(1, 48, fmt) == 0 and ctx.mx4_scale_bytes(1, 64, 7) == 0 and ctx.mx4_scale_bytes(-1, 64, fmt) == 0
     assert plugin.last_error()
+
+
+def test_refuses_lengths_past_their_range(ctx, plugin):
+    """K whose last chunk would pass 2^31: refused for that, ahead of any look at the buffers' sizes."""
+    K, fmt = 2 ** 31 - 32, P.MX4_E8M0
+    b = [ctx.alloc(4096) for _ in range(5)]
+    for call in (lambda: ctx.mx4_quantize(b[0], b[1], b[2], 1, K, fmt, BF16), lambda: ctx.mx4_dequantize(b[1], b[2], b[0], 1, K, fmt, BF16),
+                 lambda: ctx.mx4_matmul(b[0], b[1], b[2], b[3], b[4], 1, K, 1, fmt, BF16),
+                 lambda: ctx.block_norm(ctx.block_norm_params(1, K, pre=P.NORM_RMS, out_format=fmt), b[0], None, None, None, None, None, None, None, b[1], b[2])):
+        with pytest.raises(BackendError) as e:
+            call()
+        assert e.value.code == P.ERR_INVALID and "2^31 - 512" in plugin.last_error()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("K,N", [(512, 200), (2080, 1300)])
+def test_matmul_of_a_matrix_with_itself(ctx, oracle, fmt, K, N):
+    """Both operands in the same buffers."""
+    w, ws, wv = operand(ctx, np.random.default_rng(K), N, K, fmt)
+    y = ctx.empty((N, N), np.float32)
+    ctx.mx4_matmul(w, ws, w, ws, y, N, K, N, fmt, F32)
+    check_product(oracle, y.to_host(), wv, wv, 1.0, F32)

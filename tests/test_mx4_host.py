@@ -80,3 +80,13 @@ def test_oracle_round_trip(fmt):
     assert (np.abs(v - w) / s <= np.where(a > 6, a - 6, half) + 1e-12).all()
     np.testing.assert_array_equal(mx4.unpack(mx4.pack(code)), code)
     np.testing.assert_array_equal(mx4.from_tiles(mx4.to_tiles(byte), *byte.shape), byte)
+
+
+def test_extents_at_the_end_of_their_range(q):
+    """Sizes whose rounding up would leave 32 bits have no scales, so no call takes them."""
+    top = 2 ** 31 - 512
+    for fmt in (mx4.E8M0, mx4.E4M3):
+        assert q.mx4_scale_bytes(1, top, fmt) == mx4.scale_bytes(1, top, fmt)
+        assert q.mx4_scale_bytes(2 ** 31 - 1, 32, fmt) == mx4.scale_bytes(2 ** 31 - 1, 32, fmt)
+        for K in (top + 32, 2 ** 31 - 32):
+            assert q.mx4_scale_bytes(1, K, fmt) == 0
