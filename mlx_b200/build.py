@@ -8,6 +8,7 @@ declaration of the same layout (include/lux/gpu/) otherwise.
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -16,6 +17,7 @@ LIB_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(HERE, "lib", "obj")
 LIB_NAME = "libluxgpu_backend_cuda.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
+FASTCALL_PATH = os.path.join(LIB_DIR, "fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 SOURCES = ["plugin.cu", "device_state.cu", "ops_basic.cu", "ops_tensor.cu", "quant_ops.cu", "quant_api.cu", "qmv_simt.cu",
            "qmv_mma.cu", "qmv_stream.cu", "qmm_tc.cu", "shard.cu", "shard_push.cu", "mx4_quant.cu", "mx4_gemm.cu", "block_norm.cu",
@@ -59,6 +61,19 @@ def _newer(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def build_fastcall(ref_inc, verbose=False, force=False):
+    """The compiled binding of the short calls (csrc/fastcall.c), for the Python that runs this."""
+    src = os.path.join(CSRC, "fastcall.c")
+    if not (force or _newer(FASTCALL_PATH, [src, os.path.join(ROOT, "include", "lux_cuda_quant.h")])):
+        return
+    cc = "/usr/bin/gcc" if os.path.exists("/usr/bin/gcc") else "gcc"
+    cmd = [cc, "-O2", "-std=c11", "-Wall", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"], "-I", ref_inc,
+           "-I", os.path.join(ROOT, "include"), src, "-o", FASTCALL_PATH]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+
+
 def build(verbose=False, force=False, ptxas_info=False):
     ref_inc = reference_include() or os.path.join(ROOT, "include")
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -89,6 +104,7 @@ def build(verbose=False, force=False, ptxas_info=False):
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
+    build_fastcall(ref_inc, verbose, force)
     return LIB_PATH
 
 

@@ -8,6 +8,8 @@ vtable (backend_plugin.h:82-382) and the quantized-matmul extension table
 missing or reports no usable GPU, construction raises.
 """
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 import numpy as np
@@ -184,6 +186,17 @@ def load_library(path=None):
     return C.CDLL(path, mode=os.RTLD_NOW | os.RTLD_LOCAL)
 
 
+def _short_calls(quant):
+    """mx4_* and block_norm as functions: csrc/fastcall.c where it is built for this interpreter and the library has them, else the mirror's own."""
+    from .build import FASTCALL_PATH
+    if not os.path.exists(FASTCALL_PATH) or quant.size < C.sizeof(QuantVtbl):
+        return quant
+    loader = importlib.machinery.ExtensionFileLoader("fastcall", FASTCALL_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fastcall", loader))
+    loader.exec_module(module)
+    return module.Entries(C.addressof(quant))
+
+
 class Plugin:
     """The loaded backend: descriptor, base vtable, quantized-matmul table."""
 
@@ -207,6 +220,7 @@ class Plugin:
         if not qp or qp.contents.magic != QUANT_MAGIC:
             raise RuntimeError("quantized-matmul extension table missing from vtbl->_reserved[0]")
         self.quant = qp.contents
+        self.short_calls = _short_calls(self.quant)
 
     def abi_layout(self):
         out = (_u32 * 5)()
@@ -288,8 +302,8 @@ class Context:
         self.handle = plugin.vtbl.create_context(device)
         if not self.handle:
             raise RuntimeError(f"create_context({device}) failed: {plugin.last_error()}")
-        q = plugin.quant  # (a field of a ctypes table is a new function object at every access)
-        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = q.mx4_quantize, q.mx4_dequantize, q.mx4_matmul, q.block_norm
+        e = plugin.short_calls
+        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = e.mx4_quantize, e.mx4_dequantize, e.mx4_matmul, e.block_norm
 
     # --- base vtable ---------------------------------------------------------
     def close(self):

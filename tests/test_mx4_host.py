@@ -90,3 +90,28 @@ def test_extents_at_the_end_of_their_range(q):
         assert q.mx4_scale_bytes(2 ** 31 - 1, 32, fmt) == mx4.scale_bytes(2 ** 31 - 1, 32, fmt)
         for K in (top + 32, 2 ** 31 - 32):
             assert q.mx4_scale_bytes(1, K, fmt) == 0
+
+
+def test_compiled_binding_checks_its_arguments():
+    """The short calls reach the same entries without ctypes: same codes, and errors of Python's for what is no C argument."""
+    plugin = mlx_b200.Plugin(require_gpu=False)
+    e = plugin.short_calls
+    assert e is not plugin.quant  # (built)
+    prm = P.Context.block_norm_params(1, 32)
+    assert e.mx4_quantize(None, None, None, None, 1, 32, 0, 1, P.F32, 1.0) == P.ERR_INVALID
+    assert e.mx4_dequantize(None, None, None, None, 1, 32, 1, P.F32, 1) == P.ERR_INVALID
+    assert e.mx4_matmul(None, None, None, None, None, None, 1, 32, 1, 1, P.F32, 1.0) == P.ERR_INVALID
+    assert e.block_norm(None, prm, *[None] * 10) == e.block_norm(None, None, *[None] * 10) == P.ERR_INVALID
+    for args, error in (((1, 32), TypeError), ((1 << 31, 32, 0, 1, P.F32, 1.0), OverflowError), ((-(1 << 31) - 1, 32, 0, 1, P.F32, 1.0), OverflowError), ((1.5, 32, 0, 1, P.F32, 1.0), TypeError),
+                        ((1, 32, -1, 1, P.F32, 1.0), OverflowError), ((1, 32, 1 << 64, 1, P.F32, 1.0), OverflowError), ((1, 32, 0, 1, P.F32, "1"), TypeError), ((1, 32, 0, None, P.F32, 1.0), TypeError)):
+        with pytest.raises(error):
+            e.mx4_quantize(None, None, None, None, *args)
+    for bad in (b"short", C.c_int(0), 7):
+        with pytest.raises(TypeError):
+            e.block_norm(None, bad, *[None] * 10)
+    with pytest.raises(TypeError):
+        e.mx4_matmul(None, "x", None, None, None, None, 1, 32, 1, 1, P.F32, 1.0)
+    old = P.QuantVtbl(magic=P.QUANT_MAGIC, size=C.sizeof(P.QuantVtbl) - 8)
+    with pytest.raises(ValueError):
+        type(e)(C.addressof(old))
+    assert P._short_calls(old) is old
