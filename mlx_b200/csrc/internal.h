@@ -328,7 +328,8 @@ struct Mx4MatmulArgs {
     void* y;
     int M, K, N, format, y_dtype;
     float alpha;
-    int* error;  // as QmmArgs::error
+    int* error;     // as QmmArgs::error
+    bool x_stable;  // x may be read ahead of that wait, too
 };
 // overlap_prev: as above; the weights are then read ahead of the wait for that kernel
 cudaError_t launch_mx4_matmul(const Mx4MatmulArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);

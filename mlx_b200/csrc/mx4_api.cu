@@ -114,9 +114,10 @@ LuxBackendError mx4_matmul(LuxBackendContext* ctx, LuxBackendBuffer* x_codes, Lu
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
     Mx4MatmulArgs a{(const uint32_t*)bx->ptr, (const uint8_t*)bxs->ptr, (const uint32_t*)bw->ptr, (const uint8_t*)bws->ptr, by->ptr, M, K, N, format, (int)y_dtype,
-                    alpha, c->err_dev};
+                    alpha, c->err_dev, false};
     // behind a chain kernel the weights may be fetched while it drains, unless it writes them
     const bool early = chain_is_open(c) && !chain_writes(c, a.wq, (size_t)N * K / 2) && !chain_writes(c, a.ws, mx4_scale_bytes(N, K, format));
+    a.x_stable = early && !chain_writes(c, a.xq, (size_t)M * K / 2) && !chain_writes(c, a.xs, mx4_scale_bytes(M, K, format));
     const char* name = "";
     const cudaError_t r = launch_mx4_matmul(a, c->dev->sm_count, c->stream, early, &name);
     if (r != cudaSuccess) return map_cuda_error(r, name);

@@ -145,6 +145,7 @@ struct Params {
     void* y;
     int* error;
     int M, K, N, y_bf16, y_vec;  // y_vec: y on a 16-byte boundary, N a multiple of 4
+    int x_early;                 // x is not being written by a kernel before this one
     float alpha;
     int m_tiles, bm, split;  // tiles along M of bm rows of x (a multiple of 16); CTAs per cluster = parts of K
     int tiles_k;             // scale tiles along K
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
     const uint32_t full = ring + p.bar_off, empty = full + 8 * kMaxStages, done = empty + 8 * kMaxStages;
     const int rank = p.split == 1 ? 0 : blockIdx.x % p.split, tile = blockIdx.x / p.split;
     const int tm = tile % p.m_tiles, tn = tile / p.m_tiles, m0 = tm * p.bm, n0 = tn * kTileN;
-    const int s_lo = p.nst * rank / p.split, s_hi = p.nst * (rank + 1) / p.split;
+    const int s_lo = p.nst * rank / p.split, s_hi = p.nst * (rank + 1) / p.split, first = min(p.stages, s_hi - s_lo);
     if (tid == 0) {
         for (int i = 0; i < p.stages; i++) {
             bar_init(full + 8 * i, 1);
@@ -281,12 +282,14 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
                 tma_load_2d(base + p.b_off, &map_x, st * 128, m0, bar);
                 bulk_load(base + p.sb_off, p.xs + ((size_t)(m0 >> 7) * p.tiles_k + st * ST) * kScaleTile, scales(st), bar);
             };
-            // what lies ahead of the wait for the previous kernel of the stream touches weights only
-            const int first = min(p.stages, s_hi - s_lo);
+            // what lies ahead of the wait for the previous kernel of the stream touches weights only, and x where that kernel leaves it
             for (int i = 0; i < first; i++) load_w(s_lo + i, i);
+            if (p.x_early)
+                for (int i = 0; i < first; i++) load_x(s_lo + i, i);
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            for (int i = 0; i < first; i++) load_x(s_lo + i, i);
+            if (!p.x_early)
+                for (int i = 0; i < first; i++) load_x(s_lo + i, i);
             int slot = 0;
             uint32_t ph = 0;
             for (int st = s_lo + first; st < s_hi; st++) {
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
     } else if (warp == 1) {
         // (the clock of a bounded wait must not start before the previous kernel has ended: it may itself be waiting, for a peer, for as
         // long as its caller allows)
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int wait_at = p.x_early ? s_lo + first : s_lo;  // (behind what is loaded ahead of the loader's own wait)
         // The whole warp walks the stages and one elected lane issues: what the instructions take then lives in uniform registers.  (With
         // loops of one lane's own around them a stage took 630 cycles, whatever its loads did: 1 x 4096 x 4096 out of L2, not split,
         // 7.8 us.)
@@ -310,6 +313,7 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
         const uint32_t stage16 = (uint32_t)p.stage_bytes >> 4, sf0 = tmem + p.sf_col, idesc = mma_idesc<FMT>(n_mma, 0);
         const uint64_t da = desc_sw128(ring), db = desc_sw128(ring + p.b_off), dsa = desc_scales(ring + p.sa_off), dsb = desc_scales(ring + p.sb_off);
         for (int st = s_lo; st < s_hi; st++) {
+            if (st == wait_at) asm volatile("griddepcontrol.wait;" ::: "memory");
             if (!__all_sync(0xffffffffu, bar_wait(full + 8 * slot, ph, abort))) { ok = false; break; }
             tc_fence_after();
             const uint32_t at = slot * stage16, sf = sf0 + slot * (2 * ST * kScaleCols);
@@ -324,9 +328,8 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
             if (++slot == p.stages) { slot = 0; ph ^= 1; }
         }
         if (!ok) *abort = 1;
-    } else {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // every warp: 32 lanes (rows of W) of the tile
     const bool ok = __all_sync(0xffffffffu, bar_wait(done, 0, abort));
     tc_fence_after();
@@ -738,7 +741,7 @@ cudaError_t launch_tile(const Mx4MatmulArgs& a, int sm_count, cudaStream_t strea
     const TilePlan t = plan_tile(a.M, a.K, a.N, FMT, sm_count);
     Params p = {};
     p.xs = a.xs; p.ws = a.ws; p.y = a.y; p.error = a.error ? a.error : device_error_word();
-    p.M = a.M; p.K = a.K; p.N = a.N; p.y_bf16 = a.y_dtype == LUX_DTYPE_BFLOAT16; p.y_vec = ((uintptr_t)a.y & 15) == 0 && a.N % 4 == 0; p.alpha = a.alpha;
+    p.M = a.M; p.K = a.K; p.N = a.N; p.y_bf16 = a.y_dtype == LUX_DTYPE_BFLOAT16; p.y_vec = ((uintptr_t)a.y & 15) == 0 && a.N % 4 == 0; p.alpha = a.alpha; p.x_early = overlap_prev && a.x_stable;
     p.bm = t.bm; p.m_tiles = t.m_tiles; p.split = t.split;
     p.tiles_k = mx4_tiles_k(a.K, FMT);
     p.nst = (a.K + kStageK - 1) / kStageK;

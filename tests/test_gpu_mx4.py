@@ -359,3 +359,37 @@ def test_matmul_of_a_matrix_with_itself(ctx, oracle, fmt, K, N):
     y = ctx.empty((N, N), np.float32)
     ctx.mx4_matmul(w, ws, w, ws, y, N, K, N, fmt, F32)
     check_product(oracle, y.to_host(), wv, wv, 1.0, F32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 1024), (20, 2048, 2048)])
+def test_products_of_one_x_and_x_written_anew(ctx, oracle, fmt, M, K, N):
+    """Several layers on the same x (which no kernel still at work writes), then x from a layer's output, then layers again: without a
+    wait between the calls as with one after each."""
+    rng = np.random.default_rng(M)
+    ws = [operand(ctx, rng, N, K, fmt)[:2] for _ in range(6)]
+    start = ctx.upload(oracle.to_bf16(rng.standard_normal((M, K)).astype(np.float32)))
+    xq, xs = ctx.empty((M, K // 8), np.uint32), ctx.alloc(ctx.mx4_scale_bytes(M, K, fmt))
+    wide = ctx.empty((M, K), np.uint16)
+
+    def steps(after):
+        ys = [ctx.empty((M, N), np.float32) for _ in ws]
+        for i, w in enumerate(ws):
+            if i % 3 == 0:
+                if i:  # (of the last product, where it is as wide)
+                    for _ in range(2):
+                        ctx.mx4_quantize(ys[i - 1] if N >= K else wide, xq, xs, M, K, fmt, F32 if N >= K else BF16, 0.01)
+                        after()
+                else:
+                    ctx.mx4_quantize(start, xq, xs, M, K, fmt, BF16)
+                    after()
+            ctx.mx4_matmul(xq, xs, *w, ys[i], M, K, N, fmt, F32)
+            after()
+        return [y.to_host() for y in ys]
+
+    wide.from_host(oracle.to_bf16(rng.standard_normal((M, K)).astype(np.float32)))
+    want = steps(ctx.sync)
+    assert any(not np.array_equal(a, b) for a, b in zip(want[:3], want[3:]))
+    for _ in range(20):
+        for a, b in zip(steps(lambda: None), want):
+            np.testing.assert_array_equal(a, b)
