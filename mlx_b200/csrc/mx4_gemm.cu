@@ -832,17 +832,21 @@ cudaError_t launch_pair(const Mx4MatmulArgs& a, int sm_count, cudaStream_t strea
     return cudaLaunchKernelEx(&cfg, kern, map_x, map_w, map_xs, map_ws, map_y, p);
 }
 
-// Pairs or single CTAs, by estimates in microseconds that were fitted to measurements (pairs | single): 200 x 4096 x 4096 10.5 | 9.6,
-// 256 x 4096 x 11008 10.7 | 13.4, 300 x 4096 x 11008 17.6 | 13.3, 512 x 4096 x 4096 9.7 | 11.1, 777 x 2880 x 5003 15.0 | 14.3,
-// 1024 x 4096 x 4096 10.4 | 13.4, 2048 x 4096 x 4096 17.2 | 27.6, 2048 x 4096 x 11008 36.5 | 65.2, 4096 x 8192 x 28672 324 | 505.  A
-// stage of a pair's tile takes 0.385 with all pairs at work, one of a single CTA's, two to an SM, 0.5.
+// Pairs or single CTAs, by estimates in microseconds whose constants were chosen for the best choices over 62 shapes (129 .. 4096 rows, K
+// 512 .. 11008, N 256 .. 28672, both formats; the worst choice costs 15%, the mean half a percent).  A round of tiles costs a pair by its
+// stages of K, and more where y is fp32 or its rows are no multiple of 16 bytes; a wave of single CTAs by the stages of a part.
+// Measured, us, pairs | single:
+//   129 x 4096 x 4096 8.9 | 7.8     256 x 4096 x 11008 11.1 | 12.1     1024 x 4096 x 4096 10.6 | 12.1    3207 x 10272 x 465 20.9 | 21.5
+//   200 x 4096 x 4096 8.9 | 7.9     300 x 4096 x 11008 15.1 | 12.1     2048 x 4096 x 4096 16.2 | 23.0    3340 x 4256 x 24487 186 | 330
+//   512 x 4096 x 4096 9.2 | 10.2    777 x 2880 x 5003 15.0 | 13.5      158 x 1856 x 498 fp32 9.9 | 5.8   2635 x 1248 x 23907 66 | 139
 bool pairs_pay(const Mx4MatmulArgs& a, int sm_count) {
     if (a.M <= kTileN) return false;
     const TilePlan t = plan_tile(a.M, a.K, a.N, a.format, sm_count);
+    const bool f32 = a.y_dtype == LUX_DTYPE_FLOAT32, odd = (long long)a.N * (f32 ? 4 : 2) % 16 != 0;
     const long long nst = (a.K + kStageK - 1) / kStageK, slots = (long long)sm_count * std::max(1, t.per_sm);
     const long long pair_tiles = ((a.M + 255ll) / 256) * ((a.N + 255ll) / 256), rounds = (pair_tiles + sm_count / 2 - 1) / (sm_count / 2);
     const long long waves = (t.tiles * t.split + slots - 1) / slots;
-    return 2.9 + rounds * (0.385 * nst + 0.64) < 2.5 + waves * (0.5 * ((nst + t.split - 1) / t.split) + 4.5);
+    return 3.4 + rounds * (0.26 * nst + 1.8 + 1.1 * f32 + 1.5 * odd) < waves * (0.66 * ((nst + t.split - 1) / t.split) + 6.8) - 3.4;
 }
 
 }  // namespace
