@@ -21,7 +21,7 @@ namespace {
 // for all of a thread's chunks, not chunk by chunk, and rows that fill their threads (FULL) check no element: see
 // launch_block_norm for what that is worth.
 template <int CH, bool XB, bool RB, int OUT, int MODE>
-__global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
+__global__ void __launch_bounds__(512, CH == 1 ? 2 + XB + RB : CH == 2 && XB ? 2 : 1) block_norm_kernel(const __grid_constant__ BlockNormArgs a) {
     __shared__ Shared sh;
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -31,9 +31,11 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
     if (row >= a.rows) return;  // (several rows in a block: each is a warp's, and warps share nothing)
     constexpr bool FULL = MODE == kFull;
     static_assert(OUT == 0 || MODE != kApart, "blocks of codes are neighbours");
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     auto at = [&](int j) {
-        if (MODE == kApart) return Place{j * 8 * blockDim.x + threadIdx.x, blockDim.x, dim};
-        return Place{(j * blockDim.x + threadIdx.x) * 8, 1, dim};
+        if (MODE != kApart) return Place{(j * blockDim.x + threadIdx.x) * 8};
+        const uint32_t chunk = (j * (blockDim.x / 32) + warp) * 256;
+        return Place{chunk + (threadIdx.x & 31), dim, chunk + 256 <= dim};
     };
     // f(chunk, its place) for the thread's chunks that lie within the row
     auto chunks = [&](auto&& f) {
@@ -66,11 +68,12 @@ __global__ void __launch_bounds__(512, CH == 2 && XB ? 2 : 1) block_norm_kernel(
         const Pair neg = pair_of(-mean, -mean);
         chunks([&](int j, const Place& p) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[j][e] = add2(v[j][e], neg);
-                if (MODE == kApart) {  // (what is not there stays zero)
-                    const uint32_t i = p.first + 2 * e * p.step;
-                    v[j][e] = i + p.step < dim ? v[j][e] : i < dim ? v[j][e] & 0xFFFFFFFFull : 0;
+            for (int e = 0; e < 4; e++) v[j][e] = add2(v[j][e], neg);
+            if (MODE == kApart && !p.whole) {  // (what is not there stays zero)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t i = p.first + 64 * e;
+                    v[j][e] = i + 32 < dim ? v[j][e] : i < dim ? v[j][e] & 0xFFFFFFFFull : 0;
                 }
             }
         });
@@ -237,11 +240,13 @@ cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t
     auto warps = [](size_t n) { return (n + 31) / 32 * 32; };
     const bool wide = a.vec && a.dim % 8 == 0;
     if ((wide || a.dim % 8) && a.dim <= 16384) {
-        // two chunks per thread as far as 512 threads hold the row (2048 x 4096, rms | rms, bf16: 17.5 us against 19.2 with four)
-        const int ch = a.dim <= 8192 ? 2 : 4;
+        // Two chunks per thread as far as 512 threads hold the row (2048 x 4096, rms | rms, bf16: 17.5 us against 19.2 with four; one: 8192 x
+        // 1024 18.5 against 15.4).  Single elements wait for memory one chunk at a time, and want twice as many warps for it:
+        // one chunk (4000 x 1031 15.2 us, two 19.0; 8 x 4095 4.0 against 4.8).
+        const int ch = !wide && a.dim <= 4096 ? 1 : a.dim <= 8192 ? 2 : 4;
         threads = warps((a.dim + 8 * ch - 1) / (8 * ch));
         const bool full = a.dim == threads * 8 * ch;
-        kern = ch == 2 ? (!wide ? pick<2, kApart>(a) : full ? pick<2, kFull>(a) : pick<2, kWide>(a))
+        kern = ch == 1 ? pick<1, kApart>(a) : ch == 2 ? (!wide ? pick<2, kApart>(a) : full ? pick<2, kFull>(a) : pick<2, kWide>(a))
                        : (!wide ? pick<4, kApart>(a) : full ? pick<4, kFull>(a) : pick<4, kWide>(a));
     } else if (a.dim % 8 == 0) {
         kern = a.out_format == LUX_CUDA_MX4_E8M0   ? block_norm_any_kernel<LUX_CUDA_MX4_E8M0, 8>

@@ -32,26 +32,37 @@ __device__ __forceinline__ void st_row(void* p, const uint4& v) {
     asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 // A thread's eight elements of a chunk: neighbours, on a 16-byte boundary (kWide: kFull where no chunk is cut off by the row's end),
-// or, on any boundary, `step` apart, those at `end` and behind it zero (kApart).
+// or, on any boundary, 32 apart (kApart: a warp's chunk is 256 neighbours, of which each access takes 32; those at `end` and behind
+// it are zero, and nobody asks where the whole chunk lies ahead of it).
 enum Mode { kWide, kFull, kApart };
 struct Place {
-    uint32_t first, step, end;
+    uint32_t first, end;
+    bool whole;  // (the same in all lanes)
 };
+// f(element 0 .. 7 of the thread's, whether it lies within the row)
+template <class F>
+__device__ __forceinline__ void apart8(const Place& p, F&& f) {
+    if (p.whole) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f(e, true);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f(e, p.first + 32 * e < p.end);
+    }
+}
 template <bool BF16, int MODE>
 struct Raw {
     uint4 q[BF16 ? 1 : 2];
     __device__ __forceinline__ void load(const char* row, const Place& p) {
+        const char* s = row + (size_t)p.first * (BF16 ? 2 : 4);
         if constexpr (MODE != kApart) {
-            const char* s = row + (size_t)p.first * (BF16 ? 2 : 4);
             q[0] = ld_row(s);
             if (!BF16) q[BF16 ? 0 : 1] = ld_row(s + 16);
         } else {
             uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t i = p.first + e * p.step;
-                w[e] = i >= p.end ? 0u : BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(row)[i] : reinterpret_cast<const uint32_t*>(row)[i];
-            }
+            apart8(p, [&](int e, bool in) {
+                w[e] = !in ? 0u : BF16 ? (uint32_t)reinterpret_cast<const uint16_t*>(s)[32 * e] : reinterpret_cast<const uint32_t*>(s)[32 * e];
+            });
             if (BF16) {
                 q[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
             } else {
@@ -69,15 +80,13 @@ struct Raw {
 template <bool BF16, int MODE>
 __device__ __forceinline__ void store8(char* row, const Place& p, const Pair (&v)[4]) {
     if (MODE == kApart) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t i = p.first + e * p.step;
+        char* const d = row + (size_t)p.first * (BF16 ? 2 : 4);
+        apart8(p, [&](int e, bool in) {
             const float x = e & 1 ? hi_of(v[e >> 1]) : lo_of(v[e >> 1]);
-            if (i < p.end) {
-                if (BF16) reinterpret_cast<__nv_bfloat16*>(row)[i] = __float2bfloat16_rn(x);
-                else reinterpret_cast<float*>(row)[i] = x;
-            }
-        }
+            if (!in) return;
+            if (BF16) reinterpret_cast<__nv_bfloat16*>(d)[32 * e] = __float2bfloat16_rn(x);
+            else reinterpret_cast<float*>(d)[32 * e] = x;
+        });
     } else if (BF16) {
         st_row(row + (size_t)p.first * 2, make_uint4(pack2(v[0]), pack2(v[1]), pack2(v[2]), pack2(v[3])));
     } else {
@@ -89,11 +98,10 @@ __device__ __forceinline__ void store8(char* row, const Place& p, const Pair (&v
 template <int MODE>
 __device__ __forceinline__ void weights8(const float* w, const Place& p, Pair (&v)[4]) {
     if (MODE == kApart) {
+        uint32_t u[8];
+        apart8(p, [&](int e, bool in) { u[e] = in ? __float_as_uint(__ldg(w + p.first + 32 * e)) : 0u; });
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t i = p.first + 2 * e * p.step, k = i + p.step;
-            v[e] = pair_of(i < p.end ? __ldg(w + i) : 0.0f, k < p.end ? __ldg(w + k) : 0.0f);
-        }
+        for (int e = 0; e < 4; e++) v[e] = pair_of(u[2 * e], u[2 * e + 1]);
     } else {
         const ulonglong2 a = __ldg(reinterpret_cast<const ulonglong2*>(w + p.first)), b = __ldg(reinterpret_cast<const ulonglong2*>(w + p.first) + 1);
         v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;

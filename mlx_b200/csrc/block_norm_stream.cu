@@ -218,14 +218,14 @@ __global__ void __launch_bounds__(kMaxThreads + 32) block_norm_stream_kernel(con
                     if (a.r_out) st_row(static_cast<char*>(a.r_out) + (r0 + at(j)) * 2, q);
                     v[j][0] = unpack2(q.x); v[j][1] = unpack2(q.y); v[j][2] = unpack2(q.z); v[j][3] = unpack2(q.w);
                 } else if (a.r_out) {
-                    store8<false, kWide>(static_cast<char*>(a.r_out) + r0 * 4, Place{at(j), 1, dim}, v[j]);
+                    store8<false, kWide>(static_cast<char*>(a.r_out) + r0 * 4, Place{at(j)}, v[j]);
                 }
             });
             if (!a.out) continue;
             values.norm(a.pre_kind, placed(2), placed(3), shift, weights);
             if (OUT == 0) {
-                if (a.out_bf16) values.each([&](int j) { store8<true, kWide>(static_cast<char*>(a.out) + r0 * 2, Place{at(j), 1, dim}, v[j]); });
-                else values.each([&](int j) { store8<false, kWide>(static_cast<char*>(a.out) + r0 * 4, Place{at(j), 1, dim}, v[j]); });
+                if (a.out_bf16) values.each([&](int j) { store8<true, kWide>(static_cast<char*>(a.out) + r0 * 2, Place{at(j)}, v[j]); });
+                else values.each([&](int j) { store8<false, kWide>(static_cast<char*>(a.out) + r0 * 4, Place{at(j)}, v[j]); });
             } else {
 #pragma unroll
                 for (int j = 0; j < kChunks; j++) put_codes<OUT ? OUT : 1>(a, v[j], row, at(j), FULL || at(j) < dim);
