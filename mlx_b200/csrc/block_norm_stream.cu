@@ -281,12 +281,16 @@ StreamKernel pick(const BlockNormArgs& a) {
 
 }  // namespace
 
-// Measured, us, here | a row per block: 2048 x 4096 rms | rms bf16 15.7 | 17.5, layer | layer with fp32 stream and a sigmoid gate per
-// row 25.5 | 35.5, rms | rms into the microscaled format 17.2 | 18.1; 8192 x 4096 rms | rms 52.2 | 56.1; 1200 x 8192 21.2 | 22.2;
-// 2048 x 2880 12.0 | 14.6; but 8192 x 1024 24.3 | 15.7: the one warp that asks for the rows takes 0.4 us for each.
+// It pays by what a row brings with it: the one warp that asks for the rows takes 0.4 us for each, and the weights are on their way for
+// a microsecond before the first.  Measured, us, here | a row per block (A: rms | rms, bf16; B: layer | layer, fp32 stream, a sigmoid gate
+// per row; KB a row):
+//   2048 x 4096 A (16) 14.0 | 17.5    B (32) 24.5 | 35.2     600 x 4096 A 7.0 | 7.6     B 10.8 | 14.8     300 x 4096 A 5.8 | 5.5
+//   2048 x 2880 A (11.3) 12.1 | 15.1  B (22.5) 19.4 | 26.8   600 x 2880 A 6.7 | 6.2     B 9.8 | 10.6      8192 x 4096 A 51 | 56
+//   2048 x 2048 A (8) 9.7 | 9.9       B (16) 13.6 | 19.1     1184 x 2048 A 7.0 | 6.3    B 9.6 | 11.4      4096 x 1024 A (4) 13.0 | 9.6
 bool block_norm_streams(const BlockNormArgs& a, int sm_count) {
     StreamPlan p;
-    return a.vec && a.dim % 8 == 0 && a.dim >= 2048 && a.rows >= (size_t)8 * sm_count && make_plan(a, &p);
+    if (!a.vec || a.dim % 8 || a.rows < (size_t)4 * sm_count || !make_plan(a, &p)) return false;
+    return p.slot_bytes >= 11 * 1024 || (p.slot_bytes >= 8 * 1024 && a.rows >= (size_t)12 * sm_count);
 }
 
 cudaError_t launch_block_norm_stream(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev) {

@@ -5,9 +5,15 @@
 // by the copy engine into shared memory, the scale tiles from there by tcgen05.cp into tensor memory, and the tile
 // D[n, m] = sum_k W[n, k] x[m, k] (128 rows of W x bm rows of x) accumulates there.
 //
-// Few rows of x: HBM-bound on the weights (K/2 + K/block bytes per row of W).  With few tiles K is cut over a cluster of up to
-// eight CTAs; each leaves its fp32 tile in its shared memory and all add up an equal share of it in the order of K, out of one
-// another's shared memory: no workspace, no atomics, and the sum's order follows from the shape alone.
+// Few rows of x (mx4_tile_kernel): HBM-bound on the weights (K/2 + K/block bytes per row of W), and on the latency of a launch where
+// they are few.  With few tiles K is cut over a cluster of up to eight CTAs; each leaves its fp32 tile in its shared memory and all
+// add up an equal share of it in the order of K, out of one another's shared memory: no workspace, no atomics, and the sum's order
+// follows from the shape alone.  A launch fills its ring with weights while the kernels before it still run.
+//   16 x 8192 x 28672, E4M3: 23.5 us, 5.7 TB/s.  One after another, each with its own weights: 1 x 4096 x 11008 6.9 us (floor 3.7),
+//   8 x 4096 x 22016 10.9 (7.4), 1 x 1024 x 1024 2.5; behind its quantisation 1 x 4096 x 11008 takes 8.2 with it.
+// Many rows (mx4_pair_kernel, further down): bound by what shared memory and L2 give the tensor cores.
+//   4096 x 8192 x 28672 304-318 us, 6.1-6.3 PFLOP/s while the chip is cool (under its power limit: 390); 2048 x 4096 x 4096 16.2 us,
+//   4.2 PFLOP/s (two rounds of tiles for 1.7 rounds' worth).
 #include <cuda.h>
 
 #include <algorithm>
@@ -368,8 +374,9 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
 
 // ---- many rows of x: pairs of CTAs (cta_group::2) ----------------------------------------------------------------------------
 // Two CTAs of a cluster share one stream of MMAs: 256 rows of x (128 from each) times 256 rows of W, of which each stages half.  A
-// stage of 256 codes is 32 KB of codes per CTA for 512 cycles of the tensor core at its rate; with tiles of 128 x 128 on single CTAs
-// L2 would have to bring the same in 256.  D takes 256 columns of tensor memory, the scales of the stages in flight the others: those
+// stage of 256 codes is 32 KB of codes per CTA for 512 cycles of the tensor core at its rate (it takes 700, the tensor pipe is busy
+// two thirds of the time and L2 gives 13 TB/s); with tiles of 128 x 128 on single CTAs L2 would have to bring the same in 256.  Rows of codes on
+// odd 16-byte boundaries (K / 32 odd) touch five sectors for four: 59.5 us at 3829 x 10272 x 3232, 47.4 at K = 10304.  D takes 256 columns of tensor memory, the scales of the stages in flight the others: those
 // of the CTA's own rows of x, and of all 256 rows of W in both CTAs.
 //
 // One pair per pair of SMs, tiles round robin, x innermost.  10 warps: 0-7 epilogue (warp w: lanes 32*(w%4).., half w/4 of the columns;
@@ -378,7 +385,7 @@ constexpr int kPairStages = 5, kPairN = 256, kEpiWarps = 8;
 constexpr int kPairThreads = (kEpiWarps + 2) * 32;
 constexpr int kPairRowBytes = 128;                        // a row of a block of y on its way out: 64 bf16 or 32 fp32, swizzled
 constexpr int kPairBlockBytes = kTileN * kPairRowBytes;   // and the block: 128 rows; two of them, filled and emptied in turn
-constexpr int kPairYBytes = 2 * kPairBlockBytes;          // (room for the whole tile would cost a stage: 41.7 us against 38 at 2048 x 4096 x 11008)
+constexpr int kPairYBytes = 2 * kPairBlockBytes;          // (room for the whole tile would cost a stage: 41.7 us against 40.0 at 2048 x 4096 x 11008)
 constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;            // a shared::cluster address with this bit cleared is CTA 0's copy
 constexpr int kEpiBar = 1;
 
@@ -583,7 +590,7 @@ mx4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     } else {
         // This thread's row of the CTA's 128 rows of x; its columns: half of each block of y that leaves as one.  All 128 of them come into
         // registers first, so that the accumulator is free again after the time of the loads and the next tile's MMAs run while this
-        // one is converted and stored.  (Block by block out of tensor memory: 333 us against 299 at 4096 x 8192 x 28672.)
+        // one is converted and stored.  (Block by block out of tensor memory: 333 us against 322 at 4096 x 8192 x 28672.)
         const int q = warp & 3, half = warp >> 2, row = q * 32 + lane;
         constexpr int kCols = kPairRowBytes / (YBF16 ? 2 : 4), kBlocks = kPairN / kCols, kMine = kCols / 2;
         uint32_t tile_i = 0;
@@ -696,7 +703,7 @@ bool encode_codes(const void* codes, int rows, int K, int box_rows, CUtensorMap*
 // A part costs 0.22 us per stage of 256 codes, a cluster about half a microsecond each time its size doubles: parts of eight stages
 // are the best of the two, shorter ones where there are hardly any CTAs.  All CTAs have to find room at once (in four fifths of the
 // slots: a cluster's CTAs have to lie in one group of SMs), and the ring is as deep as leaves the next launch of a chain, which fills
-// its own meanwhile, some two fifths of the machine's shared memory.  Measured, us, (parts, stages):
+// its own meanwhile, some two fifths of the machine's shared memory.  Measured one after another, x behind the wait, us, (parts, stages):
 //   1 x 4096 x 4096     (1,6) 6.0  (2,6) 4.8  (4,4) 5.2  (8,3) 4.9        8 x 11008 x 4096   (4,6) 7.5  (6,5) 7.0  (8,3) 7.0
 //   1 x 4096 x 11008    (1,6) 7.8  (2,4) 6.9  (2,6) 11.1 (4,2) 6.7        16 x 8192 x 28672  (1,4) 22.3 (1,6) 27.1 (2,4) 27.2
 //   8 x 4096 x 22016    (1,4) 10.5 (2,3) 10.3 (2,4) 11.9 (4,3) 14.8       48 x 4096 x 11008  (1,6) 8.5  (2,4) 7.7  (4,3) 8.6

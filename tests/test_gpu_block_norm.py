@@ -304,7 +304,7 @@ def test_refusals(ctx, plugin):
 
 
 @pytest.mark.parametrize("post,pre", [(0, 1), (1, 1), (2, 2), (1, 0)])
-@pytest.mark.parametrize("rows,dim,gate_rows", [(1200, 2048, None), (1300, 2880, 0), (1184, 4096, 1), (1500, 2056, 7)])
+@pytest.mark.parametrize("rows,dim,gate_rows", [(1200, 2048, None), (1300, 2880, 0), (1184, 4096, 1), (1500, 2056, 7), (600, 4096, 0), (650, 1536, 1), (1800, 2048, None)])
 def test_many_rows(ctx, oracle, rows, dim, gate_rows, post, pre):
     """Rows that one block per SM takes in turn: with and without a gate, shared by all, by some or of each row's own; every type."""
     for xd, rd, od, act in ((BF16, BF16, BF16, P.GATE_TANH), (BF16, F32, F32, P.GATE_SIGMOID), (F32, BF16, F32, P.GATE_IDENTITY), (F32, F32, BF16, P.GATE_SIGMOID)):
