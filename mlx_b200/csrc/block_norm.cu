@@ -30,7 +30,6 @@ __global__ void __launch_bounds__(512, CH == 1 ? 2 + XB + RB : CH == 2 && XB ? 2
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // (several rows in a block: each is a warp's, and warps share nothing)
     constexpr bool FULL = MODE == kFull;
-    static_assert(OUT == 0 || MODE != kApart, "blocks of codes are neighbours");
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     auto at = [&](int j) {
         if (MODE != kApart) return Place{(j * blockDim.x + threadIdx.x) * 8};
@@ -127,13 +126,29 @@ __global__ void __launch_bounds__(512, CH == 1 ? 2 + XB + RB : CH == 2 && XB ? 2
         if (a.out_bf16) chunks([&](int j, const Place& p) { store8<true, MODE>(out, p, v[j]); });
         else chunks([&](int j, const Place& p) { store8<false, MODE>(out, p, v[j]); });
     } else {
+        // (blocks of codes are neighbours: elements that lie 32 apart change places within the warp first)
+        __shared__ uint4 turn[MODE == kApart && OUT ? 512 : 1];
+        const uint32_t lane = threadIdx.x & 31;
+        uint4* const mine = turn + (threadIdx.y * (blockDim.x >> 5) + warp) * 32;
 #pragma unroll
-        for (int j = 0; j < CH; j++) put_codes<OUT ? OUT : 1>(a, v[j], row, at(j).first, FULL || at(j).first < dim);
+        for (int j = 0; j < CH; j++) {
+            uint32_t i = at(j).first;
+            if (MODE == kApart) {
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    reinterpret_cast<__nv_bfloat16*>(mine)[32 * e + lane] = __float2bfloat16_rn(e & 1 ? hi_of(v[j][e >> 1]) : lo_of(v[j][e >> 1]));
+                __syncwarp();
+                const uint4 q = mine[lane];
+                v[j][0] = unpack2(q.x); v[j][1] = unpack2(q.y); v[j][2] = unpack2(q.z); v[j][3] = unpack2(q.w);
+                i += 7 * lane;
+            }
+            put_codes<OUT ? OUT : 1>(a, v[j], row, i, FULL || i < dim);
+        }
     }
 }
 
-// Longer rows, and rows of a multiple of 8 on odd boundaries: nothing is kept, what is needed is read (or, without r_out, computed) again
-// for every step.  V neighbours to a thread.  (V = 8 with and without OUT: the same sums, so the same stream whatever becomes of the
+// Longer rows: nothing is kept, what is needed is read (or, without r_out, computed) again for every step.  V neighbours to a thread.  (V = 8 with and without OUT: the same sums, so the same stream whatever becomes of the
 // output.)
 template <int OUT, int V>
 __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_constant__ BlockNormArgs a) {
@@ -218,10 +233,8 @@ __global__ void __launch_bounds__(1024) block_norm_any_kernel(const __grid_const
 using NormKernel = void (*)(BlockNormArgs);
 template <int CH, bool XB, bool RB, int MODE>
 NormKernel pick_out(int format) {
-    if constexpr (MODE != kApart) {
-        if (format == LUX_CUDA_MX4_E8M0) return block_norm_kernel<CH, XB, RB, LUX_CUDA_MX4_E8M0, MODE>;
-        if (format == LUX_CUDA_MX4_E4M3) return block_norm_kernel<CH, XB, RB, LUX_CUDA_MX4_E4M3, MODE>;
-    }
+    if (format == LUX_CUDA_MX4_E8M0) return block_norm_kernel<CH, XB, RB, LUX_CUDA_MX4_E8M0, MODE>;
+    if (format == LUX_CUDA_MX4_E4M3) return block_norm_kernel<CH, XB, RB, LUX_CUDA_MX4_E4M3, MODE>;
     return block_norm_kernel<CH, XB, RB, 0, MODE>;
 }
 template <int CH, int MODE>
@@ -239,7 +252,7 @@ cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t
     size_t threads;
     auto warps = [](size_t n) { return (n + 31) / 32 * 32; };
     const bool wide = a.vec && a.dim % 8 == 0;
-    if ((wide || a.dim % 8) && a.dim <= 16384) {
+    if (a.dim <= 16384) {
         // Two chunks per thread as far as 512 threads hold the row (2048 x 4096, rms | rms, bf16: 17.5 us against 19.2 with four; one: 8192 x
         // 1024 18.5 against 15.4).  Single elements wait for memory one chunk at a time, and want twice as many warps for it:
         // one chunk (4000 x 1031 15.2 us, two 19.0; 8 x 4095 4.0 against 4.8).
