@@ -93,6 +93,17 @@ constexpr uint32_t kBufMagic = 0x4C425546u;  // "LBUF"
 constexpr uint32_t kKernMagic = 0x4C4B524Eu; // "LKRN"
 constexpr int kTimerSlots = 16;
 
+// A few ranges of device memory; with no room for one more, one range that spans them all.
+struct Ranges {
+    static constexpr int kMax = 12;
+    struct {
+        const char *lo, *hi;
+    } r[kMax];
+    int n = 0;
+    void add(const void* p, size_t bytes);
+    bool overlaps(const void* p, size_t bytes) const;
+};
+
 struct Context {
     uint32_t magic = kCtxMagic;
     std::shared_ptr<DeviceState> dev;
@@ -117,13 +128,10 @@ struct Context {
     // the stream drains (programmatic dependent launch) only if that kernel is a decode kernel of this
     // context, is the last thing the context enqueued, and does not write those weights.
     uint64_t chain_launches = ~0ull, chain_copies = 0;  // the two counters right after the last decode launch
-    // What the chain kernels may still be writing once the last one lets its dependents start: its own outputs, if it does so
+    // What the chain kernels may still be writing, and reading, once the last one lets its dependents start: its own buffers, if it does so
     // behind its wait for the kernel before it; those of the kernels before it, too, if it does so ahead of that wait.
-    static constexpr int kChainOuts = 8;
-    struct {
-        const char *lo, *hi;
-    } chain_out[kChainOuts];
-    int chain_outs = 0;
+    Ranges chain_out, chain_in;
+    bool chain_in_known = false;  // chain_in has all of them
     bool stream_exposed = false;  // the host holds the raw stream: it may enqueue work the context cannot see
     std::mutex mu;  // one thread at a time per context
 };
@@ -272,11 +280,11 @@ bool decode_may_overlap(const Context* c, const QmmArgs& a);
 bool decode_x_stable(const Context* c, const QmmArgs& a);  // the last chain kernel's output does not overlap x
 bool chain_is_open(const Context* c);  // the last thing the context enqueued is a chain kernel (decode matmul, rms-norm)
 bool chain_writes(const Context* c, const void* p, size_t bytes);  // chain kernels that may still run write into this range
+bool chain_reads(const Context* c, const void* p, size_t bytes);   // they read from it, for all that is known
 void note_chain_launch(Context* c, const void* out, size_t out_bytes);  // right after such a launch, when it has been counted
-// the same for a kernel whose dependents may start ahead of its own wait; overlapped: it was launched as a dependent itself.  One more
-// output of that launch: add_chain_output.
+// the same for a kernel whose dependents may start ahead of its own wait; overlapped: it was launched as a dependent itself.  Its buffers:
+// chain_out, and chain_in if chain_in_known is to be true.
 void note_early_chain_launch(Context* c, bool overlapped);
-void add_chain_output(Context* c, const void* out, size_t bytes);
 void note_decode_launch(Context* c, const QmmArgs& a);  // call right after a decode launch, before counting it
 // decode / small-M, any supported dtype combination: CUDA cores + warp shuffles
 // overlap_prev (fp32 only): as above
@@ -316,8 +324,11 @@ cudaError_t launch_sum3(const void* in, void* out, size_t rows, size_t cols, siz
 cudaError_t launch_mul_rms_norm(const void* in, void* out, size_t rows, size_t cols, size_t ld, float eps, cudaStream_t stream,
                                 bool overlap_prev = false);
 // microscaled 4-bit floating point (mx4_quant.cu, mx4_gemm.cu; the format: mx4.cuh)
+// ahead: nothing that may still run touches what it reads and writes, so that it need not wait for that (mx4_quantize_is_short: and it
+// leaves the machine to that meanwhile)
+bool mx4_quantize_is_short(int rows, int K, int sm_count);
 cudaError_t launch_mx4_quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, int format, int in_dtype, float pre,
-                                cudaStream_t stream, bool overlap_prev);
+                                cudaStream_t stream, bool overlap_prev, bool ahead);
 cudaError_t launch_mx4_dequantize(const uint32_t* codes, const uint8_t* scales, void* out, int rows, int K, int format, int out_dtype, float post,
                                   cudaStream_t stream);
 struct Mx4MatmulArgs {

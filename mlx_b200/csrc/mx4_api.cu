@@ -59,13 +59,17 @@ LuxBackendError mx4_quantize(LuxBackendContext* ctx, LuxBackendBuffer* in, LuxBa
     if (!rows) return LUX_BACKEND_OK;
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
-    // (behind a chain kernel the whole kernel waits for it on the device)
-    const bool chained = chain_is_open(c);
-    LUX_CUDA_TRY(launch_mx4_quantize(bi->ptr, (uint32_t*)bc->ptr, (uint8_t*)bs->ptr, rows, K, ld, format, (int)in_dtype, pre, c->stream, chained));
+    // behind a chain kernel: at work beside it where neither touches what the other writes, else after it
+    const bool chained = chain_is_open(c), known = !chained || c->chain_in_known;
+    const bool ahead = chained && mx4_quantize_is_short(rows, K, c->dev->sm_count) && !chain_writes(c, bi->ptr, in_bytes) && !chain_writes(c, bc->ptr, code_bytes) &&
+                       !chain_writes(c, bs->ptr, scale_bytes) && !chain_reads(c, bc->ptr, code_bytes) && !chain_reads(c, bs->ptr, scale_bytes);
+    LUX_CUDA_TRY(launch_mx4_quantize(bi->ptr, (uint32_t*)bc->ptr, (uint8_t*)bs->ptr, rows, K, ld, format, (int)in_dtype, pre, c->stream, chained, ahead));
     c->launches++;
     note_early_chain_launch(c, chained);
-    add_chain_output(c, bc->ptr, code_bytes);
-    add_chain_output(c, bs->ptr, scale_bytes);
+    c->chain_out.add(bc->ptr, code_bytes);
+    c->chain_out.add(bs->ptr, scale_bytes);
+    c->chain_in.add(bi->ptr, in_bytes);
+    c->chain_in_known = known;
     bi->last_stream = bc->last_stream = bs->last_stream = c->stream;
     return LUX_BACKEND_OK;
 }
@@ -123,6 +127,11 @@ LuxBackendError mx4_matmul(LuxBackendContext* ctx, LuxBackendBuffer* x_codes, Lu
     if (r != cudaSuccess) return map_cuda_error(r, name);
     c->launches++;
     note_chain_launch(c, by->ptr, y_bytes);
+    c->chain_in.add(a.xq, (size_t)M * K / 2);
+    c->chain_in.add(a.xs, mx4_scale_bytes(M, K, format));
+    c->chain_in.add(a.wq, (size_t)N * K / 2);
+    c->chain_in.add(a.ws, mx4_scale_bytes(N, K, format));
+    c->chain_in_known = true;
     c->last_kernel = name;
     bx->last_stream = bxs->last_stream = bw->last_stream = bws->last_stream = by->last_stream = c->stream;
     return LUX_BACKEND_OK;
@@ -198,7 +207,7 @@ LuxBackendError block_norm(LuxBackendContext* ctx, const lux_block_norm_params* 
     c->launches++;
     note_early_chain_launch(c, chained);
     for (int o = R_OUT; o < COUNT; o++)
-        if (b[o]) add_chain_output(c, b[o]->ptr, bytes[o]);
+        if (b[o]) c->chain_out.add(b[o]->ptr, bytes[o]);
     for (int i = 0; i < COUNT; i++)
         if (b[i]) b[i]->last_stream = c->stream;
     return LUX_BACKEND_OK;

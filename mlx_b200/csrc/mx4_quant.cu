@@ -51,10 +51,10 @@ struct Raw16 {
 // against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  17.1 us is 5.0 TB/s; 11008 x 4096 fp32 31.8 us, 6.4 TB/s.
 template <int FMT, bool BF16>
 __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                    int rows, int K, size_t ld, float pre, int align) {
+                                                                    int rows, int K, size_t ld, float pre, int align, bool ahead) {
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int LPW = 4 * mx4_block(FMT) / 16;  // lanes per scale word
     const int lane = threadIdx.x & 31, tiles_k = mx4_tiles_k(K, FMT);
     const int k = blockIdx.x * kChunk + lane * 16;
@@ -73,6 +73,8 @@ __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void
         reinterpret_cast<uint2*>(codes)[(row * K + k) >> 4] = make_uint2(c[0], c[1]);
         if (lane % LPW == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, k / (4 * mx4_block(FMT)), tiles_k)) = word;
     }
+    // (whoever waits for this kernel relies on all before it having ended, too)
+    if (ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // HBM-bound, most of it the stores; the same division of the work, but U rows per warp, all of whose loads are under way before the
@@ -143,7 +145,7 @@ dim3 grid_of(int rows, int K, int u) { return dim3((K + kChunk - 1) / kChunk, st
 bool many(int rows, int K) { return (long long)rows * K >= 148ll * 64 * kChunk; }
 
 template <int FMT, bool BF16>
-cudaError_t quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, float pre, cudaStream_t stream, bool overlap_prev) {
+cudaError_t quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, float pre, cudaStream_t stream, bool overlap_prev, bool ahead) {
     const size_t step = ld * (BF16 ? 2 : 4);
     const int align = ((uintptr_t)in | step) % 32 == 0 ? 32 : ((uintptr_t)in | step) % 16 == 0 ? 16 : 0;
     cudaLaunchConfig_t cfg = {};
@@ -155,7 +157,7 @@ cudaError_t quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = overlap_prev ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, mx4_quantize_kernel<FMT, BF16>, in, codes, scales, rows, K, ld, pre, align);
+    return cudaLaunchKernelEx(&cfg, mx4_quantize_kernel<FMT, BF16>, in, codes, scales, rows, K, ld, pre, align, overlap_prev && ahead);
 }
 
 template <int FMT, bool BF16>
@@ -169,12 +171,19 @@ cudaError_t dequantize(const uint32_t* codes, const uint8_t* scales, void* out, 
 
 }  // namespace
 
+// At work beside the kernel before it, the quantisation costs a run of independent layers hardly anything: 8 of 1 x 4096 x 11008 with their
+// products 61.8 us against 71.  But its blocks stay until that kernel has ended: at most one per SM.
+bool mx4_quantize_is_short(int rows, int K, int sm_count) {
+    const dim3 g = grid_of(rows, K, 1);
+    return (long long)g.x * g.y <= sm_count;
+}
+
 cudaError_t launch_mx4_quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows, int K, size_t ld, int format, int in_dtype, float pre,
-                                cudaStream_t stream, bool overlap_prev) {
+                                cudaStream_t stream, bool overlap_prev, bool ahead) {
     if (!rows) return cudaSuccess;
     auto f = format == LUX_CUDA_MX4_E8M0 ? (in_dtype == LUX_DTYPE_BFLOAT16 ? quantize<LUX_CUDA_MX4_E8M0, true> : quantize<LUX_CUDA_MX4_E8M0, false>)
                                          : (in_dtype == LUX_DTYPE_BFLOAT16 ? quantize<LUX_CUDA_MX4_E4M3, true> : quantize<LUX_CUDA_MX4_E4M3, false>);
-    return f(in, codes, scales, rows, K, ld, pre, stream, overlap_prev);
+    return f(in, codes, scales, rows, K, ld, pre, stream, overlap_prev, ahead);
 }
 
 cudaError_t launch_mx4_dequantize(const uint32_t* codes, const uint8_t* scales, void* out, int rows, int K, int format, int out_dtype, float post,

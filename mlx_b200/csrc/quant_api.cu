@@ -45,33 +45,36 @@ bool chain_is_open(const Context* c) {
     if (disabled || c->stream_exposed) return false;
     return c->chain_launches == c->launches.load() && c->chain_copies == c->copies.load();
 }
-bool chain_writes(const Context* c, const void* p, size_t bytes) {
+void Ranges::add(const void* p, size_t bytes) {
+    if (!bytes) return;
+    const char *lo = (const char*)p, *hi = lo + bytes;
+    if (n == kMax) {
+        for (int i = 0; i < n; i++) {
+            lo = std::min(lo, r[i].lo);
+            hi = std::max(hi, r[i].hi);
+        }
+        n = 0;
+    }
+    r[n].lo = lo;
+    r[n++].hi = hi;
+}
+bool Ranges::overlaps(const void* p, size_t bytes) const {
     const char* lo = (const char*)p;
-    for (int i = 0; i < c->chain_outs; i++)
-        if (lo < c->chain_out[i].hi && c->chain_out[i].lo < lo + bytes) return true;
+    for (int i = 0; i < n; i++)
+        if (lo < r[i].hi && r[i].lo < lo + bytes) return true;
     return false;
 }
-void add_chain_output(Context* c, const void* out, size_t bytes) {
-    if (!bytes) return;
-    const char *lo = (const char*)out, *hi = lo + bytes;
-    if (c->chain_outs == Context::kChainOuts) {  // too many to tell apart: one range that spans them
-        for (int i = 0; i < c->chain_outs; i++) {
-            lo = std::min(lo, c->chain_out[i].lo);
-            hi = std::max(hi, c->chain_out[i].hi);
-        }
-        c->chain_outs = 0;
-    }
-    c->chain_out[c->chain_outs].lo = lo;
-    c->chain_out[c->chain_outs++].hi = hi;
-}
+bool chain_writes(const Context* c, const void* p, size_t bytes) { return c->chain_out.overlaps(p, bytes); }
+bool chain_reads(const Context* c, const void* p, size_t bytes) { return !c->chain_in_known || c->chain_in.overlaps(p, bytes); }
 void note_early_chain_launch(Context* c, bool overlapped) {
     c->chain_launches = c->launches.load();
     c->chain_copies = c->copies.load();
-    if (!overlapped) c->chain_outs = 0;
+    if (!overlapped) c->chain_out.n = c->chain_in.n = 0;
+    c->chain_in_known = false;
 }
 void note_chain_launch(Context* c, const void* out, size_t out_bytes) {
     note_early_chain_launch(c, false);
-    add_chain_output(c, out, out_bytes);
+    c->chain_out.add(out, out_bytes);
 }
 bool decode_may_overlap(const Context* c, const QmmArgs& a) {
     if (!chain_is_open(c)) return false;

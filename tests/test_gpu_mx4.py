@@ -396,3 +396,70 @@ def test_products_of_one_x_and_x_written_anew(ctx, oracle, fmt, M, K, N):
     for _ in range(20):
         for a, b in zip(steps(lambda: None), want):
             np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("seed,M,K", [(0, 8, 1024), (1, 1, 4096), (2, 40, 512), (3, 300, 1024), (4, 16, 2048), (5, 700, 2048)])
+def test_any_order_of_calls_is_as_with_a_wait_after_each(ctx, oracle, seed, M, K):
+    """Random programs over a few buffers, so that calls read what the one before writes, write what it reads, or have nothing to do with
+    it: quantisations of activations and of weights, products, row steps, older chain kernels.  Eagerly and as a replayed graph, against one call at a time."""
+    rng = np.random.default_rng(seed)
+    fmt = P.MX4_E8M0 if seed % 2 else P.MX4_E4M3
+    bits = lambda shape: oracle.to_bf16(rng.standard_normal(shape).astype(np.float32))  # noqa: E731
+    acts = [ctx.upload(bits((M, K))) for _ in range(4)]
+    raw = [ctx.upload(bits((K, K))) for _ in range(2)]  # weights before the format
+    codes = [(ctx.empty((M, K // 8), np.uint32), ctx.alloc(ctx.mx4_scale_bytes(M, K, fmt))) for _ in range(3)]
+    layers = [(ctx.empty((K, K // 8), np.uint32), ctx.alloc(ctx.mx4_scale_bytes(K, K, fmt))) for _ in range(3)]
+    start = [(b, b.to_host()) for b in acts]
+    prm = ctx.block_norm_params(M, K, post=P.NORM_RMS, pre=P.NORM_RMS, eps=1e-5, res_scale=0.5)
+    prm_mx = ctx.block_norm_params(M, K, post=P.NORM_RMS, pre=P.NORM_RMS, eps=1e-5, res_scale=0.5, out_format=fmt)
+    pick = lambda a: int(rng.integers(len(a)))  # noqa: E731
+    steps = [lambda q=c: ctx.mx4_quantize(acts[0], *q, M, K, fmt, BF16) for c in codes] + [lambda q=w: ctx.mx4_quantize(raw[0], *q, K, K, fmt, BF16) for w in layers]
+    for _ in range(70):
+        kind = rng.random()
+        a, b, c, w = pick(acts), pick(acts), codes[pick(codes)], layers[pick(layers)]
+        if kind < 0.35:
+            steps.append(lambda a=a, c=c: ctx.mx4_quantize(acts[a], *c, M, K, fmt, BF16))
+        elif kind < 0.75:
+            steps.append(lambda a=a, c=c, w=w: ctx.mx4_matmul(*c, *w, acts[a], M, K, K, fmt, BF16, 1.0 / K ** 0.5))
+        elif kind < 0.8:
+            steps.append(lambda r=raw[pick(raw)], w=w: ctx.mx4_quantize(r, *w, K, K, fmt, BF16))
+        elif kind < 0.9:
+            d = (a + 1 + pick(acts[1:])) % len(acts)
+            r = next(i for i in range(len(acts)) if i not in (a, d))
+            steps.append(lambda a=a, d=d, r=r: ctx.block_norm(prm, acts[a], None, acts[r], None, None, None, None, acts[r], acts[d]))
+        elif kind < 0.95:
+            r = (a + 1) % len(acts)
+            steps.append(lambda a=a, r=r, c=c: ctx.block_norm(prm_mx, acts[a], None, acts[r], None, None, None, None, acts[r], *c))
+        else:
+            if a != b:
+                steps.append(lambda a=a, b=b: ctx.rms_norm(acts[a], acts[b], M, K, 1e-5, BF16, BF16))
+
+    def reset():
+        for b, v in start:
+            b.from_host(v)
+
+    def state():
+        return [b.to_host() for b in acts] + [x.to_host() for c in codes + layers for x in c[:1]]
+
+    reset()
+    for s in steps:
+        s()
+        ctx.sync()
+    want = state()
+    for _ in range(4):
+        reset()
+        for s in steps:
+            s()
+        for got, w in zip(state(), want):
+            np.testing.assert_array_equal(got, w)
+    reset()
+    ctx.graph_begin()
+    for s in steps:
+        s()
+    g = ctx.graph_end()
+    for _ in range(4):
+        reset()
+        ctx.graph_launch(g)
+        for got, w in zip(state(), want):
+            np.testing.assert_array_equal(got, w)
+    ctx.graph_destroy(g)
