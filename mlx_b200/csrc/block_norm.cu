@@ -26,10 +26,11 @@ __global__ void __launch_bounds__(512, CH == 1 ? 2 + XB + RB : CH == 2 && XB ? 2
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t dim = (uint32_t)a.dim;
-    const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= a.rows) return;  // (several rows in a block: each is a warp's, and warps share nothing)
     constexpr bool FULL = MODE == kFull;
+    const int lanes = MODE == kWide && blockDim.x < 32 ? 16 : 32;  // of a warp, for a row
+    const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
+    if (lanes == 32 && row >= a.rows) return;  // (several rows in a block: each is a warp's, and warps share nothing)
+    const uint32_t dim = MODE == kWide && row >= a.rows ? 0 : (uint32_t)a.dim;  // (a warp's second row that is not there has no elements)
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     auto at = [&](int j) {
         if (MODE != kApart) return Place{(j * blockDim.x + threadIdx.x) * 8};
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(512, CH == 1 ? 2 + XB + RB : CH == 2 && XB ? 2
         chunks([&](int j, const Place& p) { rg[j].load(gate, p); });
     }
     Pair v[CH][4];
-    Group g{&sh, (int)(blockDim.x >> 5), (int)(threadIdx.x >> 5), 0, 0};
+    Group g{&sh, lanes == 32 ? (int)(blockDim.x >> 5) : 1, (int)(threadIdx.x >> 5), 0, 0, lanes};
     auto within = [&](int j) { return at(j).first < dim; };
     RowValues<CH, FULL, decltype(within)> values{v, within, g, a};
     auto shift = [&](float mean) {
@@ -270,7 +271,10 @@ cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t
         kern = block_norm_any_kernel<0, 1>;
         threads = 1024;
     }
-    const unsigned rows_per_block = threads == 32 ? 4 : 1;
+    // Many short rows on 16-byte boundaries: two to a warp (the 16 lanes that a scale word's blocks have at most).  65536 x 128, a norm
+    // alone, 16.6 us against 28.9, 8192 x 256 rms | rms 5.9 against 7.2; but 8 x 256 2.65 against 2.4.
+    if (wide && a.dim <= 256 && a.rows >= (size_t)8 * sm_count) threads = 16;
+    const unsigned rows_per_block = threads <= 32 ? 128 / threads : 1;
     const size_t blocks = (a.rows + rows_per_block - 1) / rows_per_block;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);

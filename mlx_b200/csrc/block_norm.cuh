@@ -111,14 +111,17 @@ __device__ __forceinline__ void weights8(const float* w, const Place& p, Pair (&
 struct Shared {
     float2 part[2][32];
 };
-// The threads of a row: `warps` warps, of which this is the `warp`-th, with a barrier of their own (none where it is one warp).
+// The threads of a row: `warps` warps, of which this is the `warp`-th, with a barrier of their own (none where it is one warp); or the 16
+// `lanes` of a half of a warp.
 struct Group {
     Shared* sh;
     int warps, warp, barrier, turn;
+    int lanes = 32;
 };
-__device__ __forceinline__ float warp_sum(float v) {
+__device__ __forceinline__ float warp_sum(float v, int lanes = 32) {
+    if (lanes == 32) v += __shfl_xor_sync(0xffffffffu, v, 16);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 // every lane gets the contribution of the warp of its number (zeros past the last).  All warps go on with all of them: one warp that
@@ -132,7 +135,7 @@ __device__ __forceinline__ float2 exchange(float2 v, Group& g) {
     return v;
 }
 __device__ __forceinline__ float row_sum(float v, Group& g) {
-    v = warp_sum(v);
+    v = warp_sum(v, g.lanes);
     return g.warps == 1 ? v : warp_sum(exchange(make_float2(v, 0.0f), g).x);
 }
 struct Stats {

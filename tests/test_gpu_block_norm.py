@@ -359,3 +359,28 @@ def test_a_gate_shared_by_more_rows_than_there_are(ctx, rows, dim, gate_rows):
             ctx.block_norm(ctx.block_norm_params(rows, dim, post=P.NORM_RMS, pre=P.NORM_RMS, gate_rows=gate_rows, eps=EPS), h, ctx.wrap(g.device_ptr, less * 2), r, None, None, None, None,
                            new, out)
         assert e.value.code == P.ERR_INVALID
+
+
+@pytest.mark.parametrize("post,pre", list(itertools.product(KINDS, KINDS)))
+@pytest.mark.parametrize("rows,dim", [(5, 64), (1201, 8), (1185, 64), (1299, 128), (1500, 200), (1187, 256), (2000, 136)])
+def test_short_rows(ctx, oracle, rows, dim, post, pre):
+    """Two rows to a warp, the last of them alone."""
+    run(ctx, oracle, rows, dim, post, pre, 3, P.GATE_TANH, BF16, F32, BF16, seed=rows)
+    run(ctx, oracle, rows, dim, post, pre, None, 0, F32, BF16, F32, seed=rows, in_place=True)
+
+
+@pytest.mark.parametrize("fmt", [P.MX4_E8M0, P.MX4_E4M3])
+@pytest.mark.parametrize("rows,dim", [(3, 128), (1201, 64), (1185, 128), (1311, 160), (1400, 256)])
+def test_short_rows_microscaled(ctx, oracle, fmt, rows, dim):
+    """As a bf16 output and its quantisation, bit for bit; nothing is written for a row that is not there."""
+    rng = np.random.default_rng(dim)
+    bh, _ = place(ctx, oracle, rng.standard_normal((rows, dim)), BF16)
+    out, n = empty(ctx, (rows, dim), BF16), ctx.mx4_scale_bytes(rows, dim, fmt)
+    codes = [ctx.upload(np.full((rows + 1, dim // 8), 0x5A5A5A5A, np.uint32)) for _ in range(2)]
+    scales = [ctx.upload(np.full(n, 0x5A, np.uint8)) for _ in range(2)]
+    kw = dict(pre=P.NORM_LAYER, eps=EPS, post=P.NORM_RMS)
+    ctx.block_norm(ctx.block_norm_params(rows, dim, **kw), bh, None, None, None, None, None, None, None, out)
+    ctx.mx4_quantize(out, codes[0], scales[0], rows, dim, fmt, BF16)
+    ctx.block_norm(ctx.block_norm_params(rows, dim, out_format=fmt, **kw), bh, None, None, None, None, None, None, None, codes[1], scales[1])
+    np.testing.assert_array_equal(scales[1].to_host(), scales[0].to_host())
+    np.testing.assert_array_equal(codes[1].to_host(), codes[0].to_host())
