@@ -62,8 +62,10 @@ def _newer(target, deps):
 
 
 def build_fastcall(ref_inc, verbose=False, force=False):
-    """The compiled binding of the short calls (csrc/fastcall.c), for the Python that runs this."""
+    """The compiled binding of the short calls (csrc/fastcall.c), for the Python that runs this, where its headers lie."""
     src = os.path.join(CSRC, "fastcall.c")
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return  # (plugin.py then makes these calls as all others, through ctypes)
     if not (force or _newer(FASTCALL_PATH, [src, os.path.join(ROOT, "include", "lux_cuda_quant.h")])):
         return
     cc = "/usr/bin/gcc" if os.path.exists("/usr/bin/gcc") else "gcc"
