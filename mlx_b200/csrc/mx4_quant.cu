@@ -47,19 +47,20 @@ struct Raw16 {
 
 // HBM-bound (4 or 2 bytes read and 0.53 or 0.56 written per value) with the instructions around a value close behind: 11 at E4M3.
 // A lane takes 16 neighbouring values (a block of 16, or half a block of 32), a warp 512 of a row.  What hides the memory is the number of
-// warps: 32 registers and 64 warps on an SM, one row each, beat two rows each with 32 warps (4096 x 8192, bf16, E4M3: 17.1 us
-// against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  17.1 us is 5.0 TB/s; 11008 x 4096 fp32 31.8 us, 6.4 TB/s.
-template <int FMT, bool BF16>
+// warps: 32 registers and 64 warps on an SM, one row each, beat two rows each with 32 warps (4096 x 8192, bf16, E4M3: 16.7 us
+// against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  16.7 us is 5.1 TB/s; 11008 x 4096 fp32 31.8 us, 6.4 TB/s.
+// AHEAD: see mx4_quantize_is_short.
+template <int FMT, bool BF16, bool AHEAD>
 __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                                    int rows, int K, size_t ld, float pre, int align, bool ahead) {
+                                                                    int rows, int K, size_t ld, float pre, int align) {
     // (dependents first: a matmul behind this kernel fetches its weights while the kernel before it still runs; see note_early_chain_launch)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (!ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!AHEAD) asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int LPW = 4 * mx4_block(FMT) / 16;  // lanes per scale word
     const int lane = threadIdx.x & 31, tiles_k = mx4_tiles_k(K, FMT);
     const int k = blockIdx.x * kChunk + lane * 16;
     const Pair pre2 = pair_of(pre, pre);
-    for (size_t row = (size_t)blockIdx.y * kWarps + (threadIdx.x >> 5); row < (size_t)rows; row += (size_t)gridDim.y * kWarps) {
+    for (uint32_t row = blockIdx.y * kWarps + (threadIdx.x >> 5); row < (uint32_t)rows; row += gridDim.y * kWarps) {
         Raw16<BF16> raw;
         if (k < K) raw.load(static_cast<const char*>(in) + (row * ld + k) * (BF16 ? 2 : 4), align);
         else raw.zero();
@@ -70,11 +71,11 @@ __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void
         mx4_encode<FMT, 16>(v, c, byte);
         const uint32_t word = mx4_scale_word<FMT, 16>(byte, lane);
         if (k >= K) continue;
-        reinterpret_cast<uint2*>(codes)[(row * K + k) >> 4] = make_uint2(c[0], c[1]);
+        reinterpret_cast<uint2*>(codes)[((size_t)row * (uint32_t)K + k) >> 4] = make_uint2(c[0], c[1]);
         if (lane % LPW == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, k / (4 * mx4_block(FMT)), tiles_k)) = word;
     }
     // (whoever waits for this kernel relies on all before it having ended, too)
-    if (ahead) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (AHEAD) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // HBM-bound, most of it the stores; the same division of the work, but U rows per warp, all of whose loads are under way before the
@@ -157,7 +158,8 @@ cudaError_t quantize(const void* in, uint32_t* codes, uint8_t* scales, int rows,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = overlap_prev ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, mx4_quantize_kernel<FMT, BF16>, in, codes, scales, rows, K, ld, pre, align, overlap_prev && ahead);
+    return cudaLaunchKernelEx(&cfg, overlap_prev && ahead ? mx4_quantize_kernel<FMT, BF16, true> : mx4_quantize_kernel<FMT, BF16, false>, in, codes, scales, rows, K, ld,
+                              pre, align);
 }
 
 template <int FMT, bool BF16>
