@@ -8,13 +8,15 @@ namespace luxcuda {
 
 __device__ __forceinline__ float act_of(float g, int act) {
     if (act == LUX_CUDA_GATE_SIGMOID) {
-        // 1 / (1 + 2^t), t = -g / ln 2 in two pieces, so that a large g costs no accuracy; at a third of what expf and an exact
-        // reciprocal issue, which were a quarter of the kernel
+        // 1 / (1 + 2^t), t = -g / ln 2 in two pieces, so that a large g costs no accuracy; at half of what expf and an exact
+        // reciprocal issue, which were a quarter of the kernel.  From |t| = 127 on the result is 0 (below the normal numbers) or 1
+        // whatever the second piece says, which is then no small number or none at all (infinity - infinity); a NaN passes through
+        // ex2.
         const float c_hi = -1.44269504f, c_lo = -1.92596299e-8f;  // -1 / ln 2
         const float t = g * c_hi, lo = fmaf(g, c_lo, fmaf(g, c_hi, -t));
         float e, d;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        e = fmaf(e, lo * 0.693147181f, e);
+        if (fabsf(t) < 127.0f) e = fmaf(e, lo * 0.693147181f, e);
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(1.0f + e));
         return d;
     }
