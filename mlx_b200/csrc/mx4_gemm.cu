@@ -22,23 +22,16 @@
 
 #include "internal.h"
 #include "mx4.cuh"
+#include "mx4_plan.h"
 
 namespace luxcuda {
 
 namespace {
 
-constexpr int kStageK = 256;              // codes along K per stage: 128 bytes of a row, one swizzle span
-constexpr int kTileN = 128;               // rows of W per tile
-constexpr int kTileM = 128;               // rows of x per tile, at most
-constexpr int kMmaK = 64;                 // codes along K per MMA
-constexpr int kMaxStages = 6;
-constexpr int kMaxSplit = 8;              // CTAs of a cluster
+using namespace mx4_plan;
+
 constexpr int kThreads = 128;
-constexpr int kScaleTile = 512;           // bytes of a scale tile (128 rows x 4 blocks)
-constexpr int kScaleCols = 4;             // and its columns of tensor memory
-constexpr int kABytes = kTileN * 128;
 constexpr uint32_t kWaitClocks = 4000000000u;
-constexpr int kSmemMax = 227 * 1024;
 
 // scale tiles along K per stage
 constexpr int stage_tiles(int format) { return kStageK / (4 * mx4_block(format)); }
@@ -349,16 +342,8 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
 #pragma unroll
             for (int j = 0; j < 16; j++) asm volatile("st.shared.u32 [%0], %1;" ::"r"(ring + ((c0 + j) * kTileN + tid) * 4), "r"(v[j]) : "memory");
         }
-    __syncwarp();
-    if (p.split == 1) __syncthreads();
-    else cluster_sync();
-    if (ok) {
-        const int first = rank + p.split * warp, step = p.split * (kThreads / 32);
-        if (p.y_vec) store_tile<true>(p, ring, first, step, m_cnt, m0, n0);
-        else store_tile<false>(p, ring, first, step, m_cnt, m0, n0);
-    }
-    __syncwarp();
-    if (p.split > 1) cluster_sync();  // nobody leaves while another may still read its shared memory
+    // Tensor memory goes back before this CTA waits for another: one that is still waiting for room in it (tcgen05.alloc has no limit)
+    // waits only for CTAs that need nothing but their own copies and MMAs, whatever else lies on the SM.
     tc_fence_before();
     __syncthreads();
     if (s_abort) {  // copies and MMAs in flight get two milliseconds to land
@@ -371,6 +356,14 @@ __global__ void __launch_bounds__(kThreads) mx4_tile_kernel(const __grid_constan
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     }
+    if (p.split > 1) cluster_sync();
+    if (ok) {
+        const int first = rank + p.split * warp, step = p.split * (kThreads / 32);
+        if (p.y_vec) store_tile<true>(p, ring, first, step, m_cnt, m0, n0);
+        else store_tile<false>(p, ring, first, step, m_cnt, m0, n0);
+    }
+    __syncwarp();
+    if (p.split > 1) cluster_sync();  // nobody leaves while another may still read its shared memory
 }
 
 // ---- many rows of x: pairs of CTAs (cta_group::2) ----------------------------------------------------------------------------
@@ -700,53 +693,10 @@ bool encode_codes(const void* codes, int rows, int K, int box_rows, CUtensorMap*
     return r == CUDA_SUCCESS;
 }
 
-// How a launch is cut: parts of K (CTAs of a cluster) and stages per CTA.
-// A part costs 0.22 us per stage of 256 codes, a cluster about half a microsecond each time its size doubles: parts of eight stages
-// are the best of the two, shorter ones where there are hardly any CTAs.  All CTAs have to find room at once (in four fifths of the
-// slots: a cluster's CTAs have to lie in one group of SMs), and the ring is as deep as leaves the next launch of a chain, which fills
-// its own meanwhile, some two fifths of the machine's shared memory.  Measured one after another, x behind the wait, us, (parts, stages):
-//   1 x 4096 x 4096     (1,6) 6.0  (2,6) 4.8  (4,4) 5.2  (8,3) 4.9        8 x 11008 x 4096   (4,6) 7.5  (6,5) 7.0  (8,3) 7.0
-//   1 x 4096 x 11008    (1,6) 7.8  (2,4) 6.9  (2,6) 11.1 (4,2) 6.7        16 x 8192 x 28672  (1,4) 22.3 (1,6) 27.1 (2,4) 27.2
-//   8 x 4096 x 22016    (1,4) 10.5 (2,3) 10.3 (2,4) 11.9 (4,3) 14.8       48 x 4096 x 11008  (1,6) 8.5  (2,4) 7.7  (4,3) 8.6
-struct TilePlan {
-    int bm, m_tiles, split, stages, stage_bytes, per_sm;
-    long long tiles;
-    uint32_t sf_col, tmem_cols;
-    int smem;
-};
-TilePlan plan_tile(int M, int K, int N, int format, int sm_count) {
-    const int st = stage_tiles(format), nst = (K + kStageK - 1) / kStageK;
-    TilePlan t;
-    t.bm = M >= kTileM ? kTileM : (M + 15) & ~15;
-    t.m_tiles = (M - 1) / t.bm + 1;
-    t.tiles = (long long)t.m_tiles * ((N - 1) / kTileN + 1);
-    t.stage_bytes = (kABytes + t.bm * 128 + 2 * st * kScaleTile + 1023) & ~1023;
-    t.sf_col = (t.bm + 31) & ~31;
-    auto fit = [&](int stages) {
-        t.stages = std::max(2, stages);
-        while (t.stages * t.stage_bytes < kTileN * t.bm * 4) t.stages++;  // (the sums take the ring's place)
-        t.smem = t.stages * t.stage_bytes + 8 * (2 * kMaxStages + 1) + 1024;
-        for (t.tmem_cols = 32; t.tmem_cols < t.sf_col + t.stages * 2 * st * kScaleCols; t.tmem_cols *= 2) {}
-        t.per_sm = std::min(kSmemMax / (t.smem + 1024), (int)(512 / t.tmem_cols));
-    };
-    auto resident = [&]() { return t.tiles * t.split <= (long long)sm_count * t.per_sm * 4 / 5; };
-    t.split = (int)std::min<long long>(std::min(kMaxSplit, nst), std::max((nst + 7) / 8, (int)(48 / std::min(48ll, t.tiles))));
-    for (;; t.split--) {
-        fit(std::min(3, (nst + t.split - 1) / t.split));
-        if (t.split == 1 || resident()) break;
-    }
-    for (int stages = std::min(kMaxStages, (nst + t.split - 1) / t.split); stages > 3; stages--) {
-        fit(stages);
-        if (resident() && t.tiles * t.split * t.smem <= (long long)sm_count * kSmemMax * 5 / 8) return t;
-    }
-    fit(std::min(3, (nst + t.split - 1) / t.split));
-    return t;
-}
-
 template <int FMT>
 cudaError_t launch_tile(const Mx4MatmulArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name) {
     constexpr int ST = stage_tiles(FMT);
-    const TilePlan t = plan_tile(a.M, a.K, a.N, FMT, sm_count);
+    const TilePlan t = plan_tile(a.M, a.K, a.N, ST, sm_count);
     Params p = {};
     p.xs = a.xs; p.ws = a.ws; p.y = a.y; p.error = a.error ? a.error : device_error_word();
     p.M = a.M; p.K = a.K; p.N = a.N; p.y_bf16 = a.y_dtype == LUX_DTYPE_BFLOAT16; p.y_vec = ((uintptr_t)a.y & 15) == 0 && a.N % 4 == 0; p.alpha = a.alpha; p.x_early = overlap_prev && a.x_stable;
@@ -849,7 +799,7 @@ cudaError_t launch_pair(const Mx4MatmulArgs& a, int sm_count, cudaStream_t strea
 //   512 x 4096 x 4096 9.2 | 10.2    777 x 2880 x 5003 15.0 | 13.5      158 x 1856 x 498 fp32 9.9 | 5.8   2635 x 1248 x 23907 66 | 139
 bool pairs_pay(const Mx4MatmulArgs& a, int sm_count) {
     if (a.M <= kTileN) return false;
-    const TilePlan t = plan_tile(a.M, a.K, a.N, a.format, sm_count);
+    const TilePlan t = plan_tile(a.M, a.K, a.N, stage_tiles(a.format), sm_count);
     const bool f32 = a.y_dtype == LUX_DTYPE_FLOAT32, odd = (long long)a.N * (f32 ? 4 : 2) % 16 != 0;
     const long long nst = (a.K + kStageK - 1) / kStageK, slots = (long long)sm_count * std::max(1, t.per_sm);
     const long long pair_tiles = ((a.M + 255ll) / 256) * ((a.N + 255ll) / 256), rounds = (pair_tiles + sm_count / 2 - 1) / (sm_count / 2);
