@@ -197,6 +197,17 @@ def _short_calls(quant):
     return module.Entries(C.addressof(quant))
 
 
+def _entry(plugin, table, name):
+    """Entry `name` of a table whose end LUX_CUDA_QUANT_HAS tells; where the library's ends ahead of it, what lies there is not looked at."""
+    field = getattr(QuantVtbl, name)
+    if plugin.quant.size >= field.offset + field.size:
+        return getattr(table, name)
+
+    def missing(*_):
+        raise BackendError(ERR_NOT_SUPPORTED, name, "this library's table ends ahead of it")
+    return missing
+
+
 class Plugin:
     """The loaded backend: descriptor, base vtable, quantized-matmul table."""
 
@@ -302,8 +313,9 @@ class Context:
         self.handle = plugin.vtbl.create_context(device)
         if not self.handle:
             raise RuntimeError(f"create_context({device}) failed: {plugin.last_error()}")
-        e = plugin.short_calls
-        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = e.mx4_quantize, e.mx4_dequantize, e.mx4_matmul, e.block_norm
+        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = (
+            _entry(plugin, plugin.short_calls, name) for name in ("mx4_quantize", "mx4_dequantize", "mx4_matmul", "block_norm"))
+        self._mx4_scale_bytes = _entry(plugin, plugin.quant, "mx4_scale_bytes")
 
     # --- base vtable ---------------------------------------------------------
     def close(self):
@@ -425,7 +437,7 @@ class Context:
     # --- microscaled 4-bit floating point ------------------------------------
     def mx4_scale_bytes(self, rows, K, fmt):
         """Bytes of the scales of [rows][K] (MX4_E8M0 | MX4_E4M3), in tiles of 128 rows x 4 blocks."""
-        return int(self.plugin.quant.mx4_scale_bytes(rows, K, fmt))
+        return int(self._mx4_scale_bytes(rows, K, fmt))
 
     def mx4_quantize(self, src, codes, scales, rows, K, fmt, in_dtype, pre=1.0, ld=0):
         """src * pre into 4-bit codes and block scales; ld: row stride of src in elements (0: K)."""
