@@ -73,7 +73,12 @@ def build_fastcall(ref_inc, verbose=False, force=False):
            "-I", os.path.join(ROOT, "include"), src, "-o", FASTCALL_PATH]
     if verbose:
         print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    try:
+        subprocess.run(cmd, check=True)
+    except (OSError, subprocess.CalledProcessError) as e:  # (as without the headers; an earlier build's has an earlier interface)
+        print(f"fastcall: not built ({e}); its calls go through ctypes", file=sys.stderr)
+        if os.path.exists(FASTCALL_PATH):
+            os.remove(FASTCALL_PATH)
 
 
 def build(verbose=False, force=False, ptxas_info=False):

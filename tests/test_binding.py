@@ -43,3 +43,27 @@ def test_entries_past_the_end_of_the_table_are_not_called(table, last):
             with pytest.raises(P.BackendError) as e:
                 CALLS[name](ctx, SimpleNamespace(handle=1))
             assert e.value.code == P.ERR_NOT_SUPPORTED and name in str(e.value) and not called
+
+
+@pytest.mark.parametrize("compiler", ["fails", "is not there"])
+def test_a_build_without_the_compiled_binding(monkeypatch, tmp_path, compiler):
+    """The compiled binding is an extra: where it cannot be built the build goes on, none of an earlier build stays, and the calls go through ctypes."""
+    import subprocess
+
+    from mlx_b200 import build
+    path = tmp_path / "fastcall.so"
+    path.write_bytes(b"an earlier build's")
+    monkeypatch.setattr(build, "FASTCALL_PATH", str(path))
+    commands = []
+
+    def run(cmd, **kw):
+        commands.append(cmd)
+        if compiler == "fails":
+            raise subprocess.CalledProcessError(1, cmd)
+        raise FileNotFoundError(cmd[0])
+    monkeypatch.setattr(build.subprocess, "run", run)
+    monkeypatch.setattr(build.os.path, "exists", lambda p, exists=build.os.path.exists: p.endswith("Python.h") or exists(p))
+    build.build_fastcall("include", force=True)
+    assert len(commands) == 1 and not path.exists()
+    t = P.QuantVtbl(magic=P.QUANT_MAGIC, size=C.sizeof(P.QuantVtbl))
+    assert P._short_calls(t) is t
