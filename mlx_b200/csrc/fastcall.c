@@ -28,7 +28,10 @@ static int as_int(PyObject* o, int* v) {
     return 0;
 }
 static int as_size(PyObject* o, size_t* v) {
-    *v = PyLong_AsSize_t(o);
+    PyObject* const n = PyNumber_Index(o); /* (PyLong_AsSize_t takes Python's own integers only) */
+    if (!n) return 0;
+    *v = PyLong_AsSize_t(n);
+    Py_DECREF(n);
     return *v != (size_t)-1 || !PyErr_Occurred();
 }
 static int as_float(PyObject* o, float* v) {

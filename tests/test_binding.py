@@ -67,3 +67,18 @@ def test_a_build_without_the_compiled_binding(monkeypatch, tmp_path, compiler):
     assert len(commands) == 1 and not path.exists()
     t = P.QuantVtbl(magic=P.QUANT_MAGIC, size=C.sizeof(P.QuantVtbl))
     assert P._short_calls(t) is t
+
+
+@pytest.mark.parametrize("kind", ["int32", "int64", "uint64"])
+def test_sizes_that_are_numpy_integers(kind):
+    """As with ctypes: whatever Python takes for an index is a size, floats are not."""
+    import numpy as np
+
+    import mlx_b200
+    plugin = mlx_b200.Plugin(require_gpu=False)
+    T = getattr(np, kind)
+    for table in (plugin.quant, plugin.short_calls):
+        assert table.mx4_quantize(None, None, None, None, T(1), T(32), T(32), T(1), T(P.F32), np.float32(1)) == P.ERR_INVALID
+        assert table.mx4_matmul(None, None, None, None, None, None, T(1), T(32), T(1), T(1), T(P.F32), np.float32(1)) == P.ERR_INVALID
+        with pytest.raises((TypeError, C.ArgumentError)):
+            table.mx4_quantize(None, None, None, None, 1, 32, 32.0, 1, P.F32, 1.0)
