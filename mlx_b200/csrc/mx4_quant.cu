@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void
         for (int i = 0; i < 8; i++) v[i] = mul2(raw.get(i), pre2);
         uint32_t c[2], byte;
         mx4_encode<FMT, 16>(v, c, byte);
-        const uint32_t word = mx4_scale_word<FMT, 16>(byte, lane);
+        const uint32_t word = mx4_scale_word<FMT, 16>(k < K ? byte : 0u, lane);  // (a factor that is infinite or NaN leaves one in lanes past the row)
         if (k >= K) continue;
         reinterpret_cast<uint2*>(codes)[((size_t)row * (uint32_t)K + k) >> 4] = make_uint2(c[0], c[1]);
         if (lane % LPW == 0) *reinterpret_cast<uint32_t*>(scales + mx4_scale_at(row, k / (4 * mx4_block(FMT)), tiles_k)) = word;
