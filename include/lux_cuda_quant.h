@@ -307,7 +307,7 @@ typedef struct lux_gpu_quant_vtbl {
      *         0 0.5 1 1.5 2 3 4 6.  K is a multiple of 32, at most 2^31 - 512.
      * scales  one byte per block of a row:  LUX_CUDA_MX4_E8M0: 32 codes, 2^(byte-127), 255 = NaN;
      *                                       LUX_CUDA_MX4_E4M3: 16 codes, an 8-bit float (4 exponent bits, bias 7;
-     *                                       3 mantissa bits; 0x7F = NaN).
+     *                                       3 mantissa bits; 0x7F = NaN; top bit zero).
      *         They lie as the tensor cores read them, in tiles of 128 rows x 4 blocks: with nb = K/block and
      *         nt = ceil(nb/4), the scale of (row r, block b) is byte
      *             ((r/128)*nt + b/4)*512 + (r%32)*16 + (r/32%4)*4 + b%4.
@@ -320,7 +320,8 @@ typedef struct lux_gpu_quant_vtbl {
     /* u = in * pre (fp32, rounded once), F32 or BF16 with row stride ld (elements, 0 = K); per block, with m = max |u|:
      *   E8M0: scale 2^(floor(log2 m) - 2), at least 2^-127; an infinite m counts as the largest finite value;
      *   E4M3: scale = m/6 rounded to fp32, then to the nearest 8-bit float, ties to even, at most 448;
-     * codes = u / scale to the nearest, ties to the even code, at most 6 in magnitude (0 where the scale is 0).  A block with
+     * codes = u / scale to the nearest, ties to the even code, at most 6 in magnitude (0 where the scale is 0; a code of zero
+     * may have either sign).  A block with
      * a NaN gets a NaN for its scale. */
     LuxBackendError (*mx4_quantize)(LuxBackendContext* ctx, LuxBackendBuffer* in, LuxBackendBuffer* codes, LuxBackendBuffer* scales,
                                     int rows, int K, size_t ld, int format, LuxBackendDtype in_dtype, float pre);

@@ -6,7 +6,8 @@
 // o leaves as fp32, as bf16, or rounded to bf16 and from there in the microscaled format (mx4.cuh) that the product takes.
 //
 // HBM-bound: h, r, (gate) read and r', o written once.  A group of threads takes a row, asks for all of it at once and keeps it in
-// registers between the statistics, which are fp32 sums over threads, lanes and warps; the variance is the mean of squared differences.
+// registers (rows of 8193 to 16384 elements, in part, in local memory: see launch_block_norm) between the statistics, which are fp32 sums
+// over threads, lanes and warps; the variance is the mean of squared differences.
 #include <algorithm>
 
 #include "block_norm.cuh"
@@ -257,6 +258,7 @@ cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t
         // Two chunks per thread as far as 512 threads hold the row (2048 x 4096, rms | rms, bf16: 17.5 us against 19.2 with four; one: 8192 x
         // 1024 18.5 against 15.4).  Single elements wait for memory one chunk at a time, and want twice as many warps for it:
         // one chunk (4000 x 1031 15.2 us, two 19.0; 8 x 4095 4.0 against 4.8).
+        // Four chunks of fp32 h and r do not fit 128 registers: up to 800 bytes a thread spill (512 x 12288 50 us, bf16 18.5).
         const int ch = !wide && a.dim <= 4096 ? 1 : a.dim <= 8192 ? 2 : 4;
         threads = warps((a.dim + 8 * ch - 1) / (8 * ch));
         const bool full = a.dim == threads * 8 * ch;
@@ -271,8 +273,8 @@ cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t
         kern = block_norm_any_kernel<0, 1>;
         threads = 1024;
     }
-    // Many short rows on 16-byte boundaries: two to a warp (the 16 lanes that a scale word's blocks have at most).  65536 x 128, a norm
-    // alone, 16.6 us against 28.9, 8192 x 256 rms | rms 5.9 against 7.2; but 8 x 256 2.65 against 2.4.
+    // Many short rows on 16-byte boundaries: two to a warp (the 16 lanes that a scale word's blocks have at most).  65536 x 128, h,
+    // the stream and one norm, 16.6 us against 28.9, 8192 x 256 rms | rms 5.9 against 7.2; but 8 x 256 2.65 against 2.4.
     if (wide && a.dim <= 256 && a.rows >= (size_t)8 * sm_count) threads = 16;
     const unsigned rows_per_block = threads <= 32 ? 128 / threads : 1;
     const size_t blocks = (a.rows + rows_per_block - 1) / rows_per_block;

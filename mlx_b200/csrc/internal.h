@@ -277,7 +277,7 @@ cudaError_t launch_decode(const QmmArgs& a, const DecodePlan& pl, void* workspac
 cudaError_t launch_qmv_push(const QmmArgs& a, void* workspace, int sm_count, cudaStream_t stream, const char** name,
                             bool overlap_prev, const ShardPush& push);
 bool decode_may_overlap(const Context* c, const QmmArgs& a);
-bool decode_x_stable(const Context* c, const QmmArgs& a);  // the last chain kernel's output does not overlap x
+bool decode_x_stable(const Context* c, const QmmArgs& a);  // no chain kernel that may still run writes x
 bool chain_is_open(const Context* c);  // the last thing the context enqueued is a chain kernel (decode matmul, rms-norm)
 bool chain_writes(const Context* c, const void* p, size_t bytes);  // chain kernels that may still run write into this range
 bool chain_reads(const Context* c, const void* p, size_t bytes);   // they read from it, for all that is known
@@ -285,7 +285,7 @@ void note_chain_launch(Context* c, const void* out, size_t out_bytes);  // right
 // the same for a kernel whose dependents may start ahead of its own wait; overlapped: it was launched as a dependent itself.  Its buffers:
 // chain_out, and chain_in if chain_in_known is to be true.
 void note_early_chain_launch(Context* c, bool overlapped);
-void note_decode_launch(Context* c, const QmmArgs& a);  // call right after a decode launch, before counting it
+void note_decode_launch(Context* c, const QmmArgs& a);  // right after a decode launch, when it has been counted
 // decode / small-M, any supported dtype combination: CUDA cores + warp shuffles
 // overlap_prev (fp32 only): as above
 cudaError_t launch_qmv_simt(const QmmArgs& a, int sm_count, cudaStream_t stream, const char** name, bool overlap_prev = false);

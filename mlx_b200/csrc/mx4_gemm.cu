@@ -9,8 +9,8 @@
 // they are few.  With few tiles K is cut over a cluster of up to eight CTAs; each leaves its fp32 tile in its shared memory and all
 // add up an equal share of it in the order of K, out of one another's shared memory: no workspace, no atomics, and the sum's order
 // follows from the shape alone.  A launch fills its ring with weights while the kernels before it still run.
-//   16 x 8192 x 28672, E4M3: 23.5 us, 5.7 TB/s.  One after another, each with its own weights: 1 x 4096 x 11008 6.9 us (floor 3.7),
-//   8 x 4096 x 22016 10.9 (7.4), 1 x 1024 x 1024 2.5; 1 x 4096 x 11008 with its quantisation 8.2, 7.5 where
+//   16 x 8192 x 28672, E4M3: 23.5 us, 5.7 TB/s.  One after another, each with its own weights: 1 x 4096 x 11008 6.7 us (floor 3.7),
+//   8 x 4096 x 22016 10.7 (7.4), 1 x 1024 x 1024 2.4; 1 x 4096 x 11008 with its quantisation 8.2, 7.6 where
 //   that runs beside the product before.
 // Many rows (mx4_pair_kernel, further down): bound by what shared memory and L2 give the tensor cores.
 //   4096 x 8192 x 28672 304-318 us, 6.1-6.3 PFLOP/s while the chip is cool (under its power limit: 390); 2048 x 4096 x 4096 16.2 us,

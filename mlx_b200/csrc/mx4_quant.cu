@@ -48,7 +48,7 @@ struct Raw16 {
 // HBM-bound (4 or 2 bytes read and 0.53 or 0.56 written per value) with the instructions around a value close behind: 11 at E4M3.
 // A lane takes 16 neighbouring values (a block of 16, or half a block of 32), a warp 512 of a row.  What hides the memory is the number of
 // warps: 32 registers and 64 warps on an SM, one row each, beat two rows each with 32 warps (4096 x 8192, bf16, E4M3: 16.7 us
-// against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  16.7 us is 5.1 TB/s; 11008 x 4096 fp32 31.8 us, 6.4 TB/s.
+// against 18.3; four rows: 22.9; one row with 44 registers: 22.3).  Now 16.9 us, 5.1 TB/s; 11008 x 4096 fp32 31.9 us, 6.4 TB/s.
 // AHEAD: see mx4_quantize_is_short.
 template <int FMT, bool BF16, bool AHEAD>
 __global__ void __launch_bounds__(32 * kWarps, 8) mx4_quantize_kernel(const void* __restrict__ in, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales,
