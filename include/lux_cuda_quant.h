@@ -68,6 +68,18 @@ extern "C" {
 #define LUX_CUDA_GATE_IDENTITY 0
 #define LUX_CUDA_GATE_SIGMOID 1
 #define LUX_CUDA_GATE_TANH 2
+/* activations of qmatmul_epi and qmatmul_experts: v; max(v, 0); v / (1 + exp(-v)); v * (1 + erf(v / sqrt 2)) / 2;
+ * v * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) / 2 */
+#define LUX_CUDA_ACT_NONE 0
+#define LUX_CUDA_ACT_RELU 1
+#define LUX_CUDA_ACT_SILU 2
+#define LUX_CUDA_ACT_GELU 3
+#define LUX_CUDA_ACT_GELU_TANH 4
+/* scores of moe_route */
+#define LUX_CUDA_SCORE_SOFTMAX 0
+#define LUX_CUDA_SCORE_SIGMOID 1
+#define LUX_CUDA_MAX_EXPERTS 1024
+#define LUX_CUDA_MAX_TOP_K 32
 #define LUX_CUDA_QMM_KERNEL_NAME "lux.qmm.affine"
 #define LUX_CUDA_NCCL_UID_BYTES 128
 
@@ -89,6 +101,42 @@ typedef struct lux_block_norm_params {
     float out_pre;                       /* `pre` of mx4_quantize, where out_format is set */
     uint32_t _pad;
 } lux_block_norm_params;
+
+/* what qmatmul_epi does */
+typedef struct lux_qmm_epi_params {
+    int32_t M, K, N, bits, group;
+    int32_t act;              /* LUX_CUDA_ACT_* */
+    int32_t r_dtype, y_dtype; /* LuxBackendDtype of residual (looked at where there is one) and of y */
+} lux_qmm_epi_params;
+
+/* what moe_route does */
+typedef struct lux_moe_route_params {
+    uint64_t tokens, ld;      /* rows of logits, their stride in elements (0 = experts) */
+    int32_t experts, top_k;
+    int32_t score;            /* LUX_CUDA_SCORE_* */
+    int32_t renorm;           /* not 0: a token's weights sum to `scale` */
+    int32_t logits_dtype;     /* LuxBackendDtype */
+    float scale;
+} lux_moe_route_params;
+
+/* what qmatmul_experts does */
+typedef struct lux_experts_params {
+    uint64_t rows;            /* rows of y (and of order) */
+    uint64_t x_rows;          /* rows of x */
+    int32_t experts, K, N, bits, group;
+    int32_t top_k;            /* with order: row i of y comes from row order[i] / top_k of x */
+    int32_t act, gated;       /* LUX_CUDA_ACT_*; gated: not 0 */
+    int32_t y_dtype, _pad;
+} lux_experts_params;
+
+/* what moe_combine does */
+typedef struct lux_moe_combine_params {
+    uint64_t tokens, dim;
+    uint64_t y_rows;          /* rows of y */
+    int32_t top_k;
+    int32_t y_dtype;          /* LuxBackendDtype of y */
+    int32_t out_dtype, _pad;  /* of residual and out */
+} lux_moe_combine_params;
 
 /* One rank of a column-sharded layer (see shard_* below). */
 typedef struct LuxCudaShardComm LuxCudaShardComm;
@@ -346,6 +394,52 @@ typedef struct lux_gpu_quant_vtbl {
     LuxBackendError (*block_norm)(LuxBackendContext* ctx, const lux_block_norm_params* params, LuxBackendBuffer* h, LuxBackendBuffer* gate,
                                   LuxBackendBuffer* r, LuxBackendBuffer* post_w, LuxBackendBuffer* post_b, LuxBackendBuffer* pre_w,
                                   LuxBackendBuffer* pre_b, LuxBackendBuffer* r_out, LuxBackendBuffer* out, LuxBackendBuffer* out_scales);
+
+    /* --- a product with its epilogue (LUX_CUDA_QUANT_HAS) ---
+     * y[M,N] = act(x[M,K] . dequant(wq[N,K])^T + bias[n]) + residual[M,N]
+     * x, scales and biases BF16; bias fp32 [N]; residual F32 or BF16; y F32 or BF16.  The sum, the bias, the activation and the residual
+     * are taken in fp32 and rounded once.  bias or residual may be NULL: nothing is added.  y may be residual itself (of the same
+     * type); otherwise it overlaps nothing that is read.  Any M.  (The reference has op_matmul_f32, backend_plugin.h:129, then op_add_f32
+     * and the unary ops as calls of their own.) */
+    LuxBackendError (*qmatmul_epi)(LuxBackendContext* ctx, const lux_qmm_epi_params* params, LuxBackendBuffer* x, LuxBackendBuffer* wq,
+                                   LuxBackendBuffer* scales, LuxBackendBuffer* biases, LuxBackendBuffer* bias, LuxBackendBuffer* residual,
+                                   LuxBackendBuffer* y);
+
+    /* --- a layer of experts: router, products grouped by expert, weighted sum (LUX_CUDA_QUANT_HAS) ---
+     * (No counterpart in the reference.)  A pair p = token * top_k + slot is one of the top_k experts of a token.  The calls leave out pairs
+     * that go to no expert; all indices are int32, tokens * top_k < 2^31, experts at most LUX_CUDA_MAX_EXPERTS, top_k at most LUX_CUDA_MAX_TOP_K.
+     *
+     * moe_route: logits F32 or BF16 [tokens][experts].  A token's experts, best first, are those of the top_k largest logits or, with `bias`
+     * (fp32 [experts], SCORE_SIGMOID only), of the largest sigmoid(logit) + bias, taken in fp64; of equals the lowest index first.  An
+     * expert whose logit is -infinity or NaN is not chosen, nor one whose bias is; a slot for which no expert is left gets id -1 and weight 0.
+     *   SCORE_SOFTMAX: weight = exp(logit - max) / sum over the token's experts (logits equal to the largest count as exp(0), infinite ones too);
+     *   SCORE_SIGMOID: weight = 1 / (1 + exp(-logit));
+     *   renorm: divided by the sum of the token's weights (0 where that is 0);     all times `scale`.
+     * ids int32 [tokens][top_k], weights fp32 [tokens][top_k];
+     * offsets int32 [experts+1]: offsets[e] pairs go to the experts before e;
+     * order int32 [tokens*top_k]: the pairs by expert, for one expert in rising order; order[i] for i >= offsets[experts] is left as it was;
+     * pos int32 [tokens*top_k]: where in order a pair stands, -1: nowhere.
+     * With logits NULL, ids and weights are somebody else's: ids is read (a value outside [0, experts) goes nowhere, one token may name
+     * an expert twice), weights is not looked at and may be NULL, bias is NULL; only order, pos and offsets are written. */
+    LuxBackendError (*moe_route)(LuxBackendContext* ctx, const lux_moe_route_params* params, LuxBackendBuffer* logits, LuxBackendBuffer* bias,
+                                 LuxBackendBuffer* ids, LuxBackendBuffer* weights, LuxBackendBuffer* order, LuxBackendBuffer* pos,
+                                 LuxBackendBuffer* offsets);
+    /* For every expert e and every row i in [offsets[e], offsets[e+1]):
+     *   v = x[row] . dequant(wq[e])^T + bias[e],    row = i, or order[i] / top_k where order is not NULL
+     *   y[i] = act(v)                               [N]
+     *   y[i] = act(v[:N/2]) * v[N/2:]               [N/2], gated: the first half of an expert's rows of wq are its gate's; N is a multiple of 16
+     * wq, scales and biases as qmatmul's, one expert's [N][...] after the other's; x, scales, biases BF16; bias fp32 [experts][N] or NULL; y F32
+     * or BF16, sums, bias and activation in fp32 and rounded once.  Rows of y that belong to no expert are left as they were.  Offsets
+     * are cut to [0, rows], an expert whose offsets fall has no rows, and x counts as zero where a row of it does not exist.
+     * K a multiple of the group.  A row's result depends on nothing but the row and its expert. */
+    LuxBackendError (*qmatmul_experts)(LuxBackendContext* ctx, const lux_experts_params* params, LuxBackendBuffer* x, LuxBackendBuffer* order,
+                                       LuxBackendBuffer* offsets, LuxBackendBuffer* wq, LuxBackendBuffer* scales, LuxBackendBuffer* biases,
+                                       LuxBackendBuffer* bias, LuxBackendBuffer* y);
+    /* out[t] = residual[t] + sum over slots j of weights[t][j] * y[pos[t][j]], in fp32, the slots in turn, rounded once.  A pos outside
+     * [0, y_rows) adds nothing.  weights NULL: ones; residual NULL: zeros; out may be residual itself, otherwise it overlaps nothing that
+     * is read.  y, residual, out F32 or BF16, [y_rows][dim] and [tokens][dim]. */
+    LuxBackendError (*moe_combine)(LuxBackendContext* ctx, const lux_moe_combine_params* params, LuxBackendBuffer* y, LuxBackendBuffer* pos,
+                                   LuxBackendBuffer* weights, LuxBackendBuffer* residual, LuxBackendBuffer* out);
 } lux_gpu_quant_vtbl;
 
 /* Entry points exported with default visibility. */

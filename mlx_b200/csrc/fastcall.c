@@ -1,9 +1,11 @@
-/* The short calls of lux_gpu_quant_vtbl for Python: mx4_quantize, mx4_dequantize, mx4_matmul, block_norm.
+/* The short calls of lux_gpu_quant_vtbl for Python: mx4_quantize, mx4_dequantize, mx4_matmul, block_norm, qmatmul_epi, moe_route,
+ * qmatmul_experts, moe_combine.
  *
  * plugin.py mirrors the whole interface with ctypes, which takes 1.1 us to turn a dozen arguments into C ones (0.2 us here): a
  * third of the time of a call whose kernel takes two or three.  Same entries, same arguments, same codes. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <string.h>
 
 #include "lux_cuda_quant.h"
 
@@ -85,33 +87,47 @@ static PyObject* matmul(Entries* self, PyObject* const* a, Py_ssize_t n) {
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(r);
 }
-static PyObject* block_norm(Entries* self, PyObject* const* a, Py_ssize_t n) {
-    void *ctx, *p[10];
-    lux_block_norm_params prm; /* (copied: another thread may change the caller's while this one is in the call) */
+/* A parameter block (None: no block), copied: another thread may change the caller's while this one is in the call.  1: there is one. */
+static int block(PyObject* o, void* dst, size_t size, const char* what) {
     Py_buffer b;
-    int r;
-    if (!count(n, 12) || !as_pointer(a[0], &ctx) || !pointers(a + 2, p, 10)) return NULL;
-    if (a[1] != Py_None) {
-        if (PyObject_GetBuffer(a[1], &b, PyBUF_SIMPLE)) return NULL;
-        const int fits = b.len == (Py_ssize_t)sizeof prm;
-        if (fits) prm = *(const lux_block_norm_params*)b.buf;
-        PyBuffer_Release(&b);
-        if (!fits) {
-            PyErr_SetString(PyExc_TypeError, "block_norm: not a BlockNormParams");
-            return NULL;
-        }
-    }
-    Py_BEGIN_ALLOW_THREADS
-    r = self->q->block_norm(ctx, a[1] == Py_None ? NULL : &prm, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9]);
-    Py_END_ALLOW_THREADS
-    return PyLong_FromLong(r);
+    if (o == Py_None) return 0;
+    if (PyObject_GetBuffer(o, &b, PyBUF_SIMPLE)) return -1;
+    const int fits = b.len == (Py_ssize_t)size;
+    if (fits) memcpy(dst, b.buf, size);
+    PyBuffer_Release(&b);
+    if (fits) return 1;
+    PyErr_SetString(PyExc_TypeError, what);
+    return -1;
 }
+/* entry(context, parameters, N buffers) */
+#define WITH_BLOCK(NAME, TYPE, N, CLASS, ...)                                                              \
+    static PyObject* NAME(Entries* self, PyObject* const* a, Py_ssize_t n) {                               \
+        void *ctx, *p[N];                                                                                  \
+        TYPE prm;                                                                                          \
+        int r;                                                                                             \
+        if (!count(n, N + 2) || !as_pointer(a[0], &ctx) || !pointers(a + 2, p, N)) return NULL;            \
+        const int there = block(a[1], &prm, sizeof prm, #NAME ": not a " CLASS);                           \
+        if (there < 0) return NULL;                                                                        \
+        Py_BEGIN_ALLOW_THREADS                                                                             \
+        r = self->q->NAME(ctx, there ? &prm : NULL, __VA_ARGS__);                                          \
+        Py_END_ALLOW_THREADS                                                                               \
+        return PyLong_FromLong(r);                                                                         \
+    }
+WITH_BLOCK(block_norm, lux_block_norm_params, 10, "BlockNormParams", p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9])
+WITH_BLOCK(qmatmul_epi, lux_qmm_epi_params, 7, "QmmEpiParams", p[0], p[1], p[2], p[3], p[4], p[5], p[6])
+WITH_BLOCK(moe_route, lux_moe_route_params, 7, "MoeRouteParams", p[0], p[1], p[2], p[3], p[4], p[5], p[6])
+WITH_BLOCK(qmatmul_experts, lux_experts_params, 8, "ExpertsParams", p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7])
+WITH_BLOCK(moe_combine, lux_moe_combine_params, 5, "MoeCombineParams", p[0], p[1], p[2], p[3], p[4])
 
 static PyMethodDef methods[] = {
     {"mx4_quantize", (PyCFunction)(void (*)(void))quantize, METH_FASTCALL, NULL},
     {"mx4_dequantize", (PyCFunction)(void (*)(void))dequantize, METH_FASTCALL, NULL},
     {"mx4_matmul", (PyCFunction)(void (*)(void))matmul, METH_FASTCALL, NULL},
     {"block_norm", (PyCFunction)(void (*)(void))block_norm, METH_FASTCALL, NULL},
+    {"qmatmul_epi", (PyCFunction)(void (*)(void))qmatmul_epi, METH_FASTCALL, NULL},
+    {"moe_route", (PyCFunction)(void (*)(void))moe_route, METH_FASTCALL, NULL},
+    {"qmatmul_experts", (PyCFunction)(void (*)(void))qmatmul_experts, METH_FASTCALL, NULL},
+    {"moe_combine", (PyCFunction)(void (*)(void))moe_combine, METH_FASTCALL, NULL},
     {NULL, NULL, 0, NULL},
 };
 /* Entries(address of a lux_gpu_quant_vtbl) */
@@ -121,7 +137,7 @@ static PyObject* entries_new(PyTypeObject* type, PyObject* args, PyObject* kw) {
     if (kw && PyDict_GET_SIZE(kw)) return PyErr_Format(PyExc_TypeError, "no keywords");
     if (!PyArg_ParseTuple(args, "O", &o) || !as_pointer(o, &p)) return NULL;
     const lux_gpu_quant_vtbl* q = p;
-    if (!q || !LUX_CUDA_QUANT_HAS(q, block_norm)) return PyErr_Format(PyExc_ValueError, "no table of a library with these entries");
+    if (!q || !LUX_CUDA_QUANT_HAS(q, moe_combine)) return PyErr_Format(PyExc_ValueError, "no table of a library with these entries");
     Entries* self = (Entries*)type->tp_alloc(type, 0);
     if (self) self->q = q;
     return (PyObject*)self;

@@ -115,6 +115,7 @@ struct Context {
     // Outgrown workspaces stay allocated until the context goes: launches recorded in CUDA graphs keep
     // using the block they were recorded with.
     std::vector<Block*> qmv_ws_retired;
+    Block* moe_ws = nullptr;  // counts of moe_route's blocks, made on first use
     // scratch of the prefill GEMM (partial accumulators of tiles shared between CTAs + their flags)
     Block* qmm_ws = nullptr;
     // A kernel that gives up on a bounded wait says so here (page-locked host memory mapped into the device's
@@ -224,6 +225,11 @@ struct QmmArgs {
     // row with eps; 2: bf16(sum of the column blocks [0,K), [K,2K), [2K,3K)); x_ld = row stride of the buffer)
     int pro = 0, x_ld = 0;
     float eps = 0.0f;
+    // epilogue of qmatmul_epi: y = act(sum + bias[n]) + residual, each where there is one
+    bool epi = false;
+    const float* bias = nullptr;
+    const void* residual = nullptr;
+    int act = 0, r_bf16 = 0;
     // where the kernels raise a time-out of one of their bounded waits: the calling context's word (device
     // address of page-locked, mapped host memory); null: the word shared by the process
     int* error = nullptr;
@@ -360,6 +366,48 @@ struct BlockNormArgs {
 bool block_norm_streams(const BlockNormArgs& a, int sm_count);  // rows that block_norm_stream.cu takes
 cudaError_t launch_block_norm_stream(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 cudaError_t launch_block_norm(const BlockNormArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
+// a layer of experts (moe.cu): the router, the weighted sum
+struct MoeRouteArgs {
+    const void* logits;  // null: ids are given
+    const float* bias;
+    int* ids;
+    float* weights;
+    int *order, *pos, *offsets, *hist;  // hist: moe_route_workspace_bytes
+    size_t tokens, ld;
+    int experts, top_k, score, renorm;
+    bool logits_bf16;
+    float scale;
+};
+int moe_route_blocks(const MoeRouteArgs& a, int sm_count);  // more than one: the workspace is needed
+size_t moe_route_workspace_bytes(int sm_count);
+cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, int* launches);
+struct MoeCombineArgs {
+    const void* y;
+    const int* pos;
+    const float* weights;
+    const void* residual;
+    void* out;
+    size_t tokens, dim, y_rows;
+    int top_k;
+    bool y_bf16, out_bf16, vec;  // vec: every row of every buffer starts on a 16-byte boundary and is whole pieces of 8
+};
+cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev);
+// products grouped by expert (qmv_stream.cu: few rows an expert)
+struct ExpertsArgs {
+    const void* x;
+    const int *order, *offsets;  // order null: row i of y comes from row i of x
+    const uint32_t* wq;
+    const void *scales, *biases;
+    const float* bias;
+    void* y;
+    size_t rows, x_rows;
+    int experts, K, N, bits, group, top_k, act;
+    bool gated;
+    int y_dtype;
+    int* error;  // as QmmArgs::error
+};
+bool qmv_experts_supported(const ExpertsArgs& a, int sm_count);
+cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);
 cudaError_t launch_flush(void* buf, size_t bytes, cudaStream_t stream);
@@ -383,6 +431,8 @@ LuxBackendError qmatmul_on_stream(Context* c, const QmmArgs& a);
 void fill_shard_entries(lux_gpu_quant_vtbl* t);
 void fill_symm_entries(lux_gpu_quant_vtbl* t);
 void fill_mx4_entries(lux_gpu_quant_vtbl* t);  // mx4_api.cu: mx4_* and block_norm
+void fill_moe_entries(lux_gpu_quant_vtbl* t);  // moe_api.cu: qmatmul_epi, moe_*, qmatmul_experts
+LuxBackendError qmatmul_epi_on_stream(Context* c, const QmmArgs& a);
 LuxBackendError ensure_qmv_workspace(Context* c, size_t bytes);  // scratch of the decode kernel, grown on demand
 LuxBackendError ensure_qmm_workspace(Context* c);                // scratch of the prefill GEMM, created on first use
 

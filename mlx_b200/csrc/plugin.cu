@@ -79,6 +79,7 @@ void destroy_context(LuxBackendContext* ctx) {
     if (c->qmv_ws) c->dev->release(c->qmv_ws, c->stream);
     for (Block* b : c->qmv_ws_retired) c->dev->release(b, c->stream);
     if (c->qmm_ws) c->dev->release(c->qmm_ws, c->stream);
+    if (c->moe_ws) c->dev->release(c->moe_ws, c->stream);
     if (c->err_host) cudaFreeHost(c->err_host);
     c->dev->release_stream(c->stream);
     c->magic = 0;
@@ -532,6 +533,12 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.mx4.matmul", "mx4_pairs<e8m0>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // many rows of x: on pairs of CTAs
     {"lux.mx4.matmul", "mx4_pairs<e4m3>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.block_norm", "block_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.route", "moe_route", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.combine", "moe_combine", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmv_experts<4,m8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // few rows an expert: 8 or 16 at a time
+    {"lux.moe.experts", "qmv_experts<4,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmv_experts<8,m8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmv_experts<8,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
 };
 const LuxKernelRegistry g_registry = {"cuda", g_kernels, sizeof(g_kernels) / sizeof(g_kernels[0])};
 

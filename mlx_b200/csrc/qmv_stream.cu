@@ -26,12 +26,22 @@
 //
 // K need not be a multiple of the k-block: x reads as zero past K, and the last box of a row is cut off there.
 //
+// The epilogue of qmatmul_epi (bias, activation, residual) is the summing warps': a tile's bias and residual are requested ahead of its sums.
+//
+// Products grouped by expert (qmatmul_experts): the items are runs of 8 or 16 rows of one expert, which every CTA works out from the
+// offsets in device memory; the row tiles of all of them, item after item, are cut into one range per CTA, so that a CTA reloads x two or
+// three times a launch (dealt out per item, as in a batch, it reads 64 KB of x for every 32 KB of weights).  Rows of a gated product: a
+// tile is eight rows of gate and the eight of up that go with them, one box of the weights seen as [expert][half][row]; the MMA's
+// layout leaves both in one lane.
+//
 // More than 16 rows of x (the prefill kernel takes them where K is a multiple of 64) are items of 16 rows on the same
 // weights, dealt over the grid's y as far as few row tiles leave SMs over.  (A launch for every 16 rows: 4096 x 96 x 16 took
 // 544 us; the CUDA-core kernel 12; this way 6.)
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
+#include "epilogue.cuh"
 #include "internal.h"
 #include "qmv_frag.cuh"
 
@@ -91,6 +101,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
@@ -128,15 +142,34 @@ struct Item {
     void* y;
     int M;
 };
-// NI: how many matmuls of a batch, at most; 1: one; 0: one whose rows of x are n_items items of 16 (M: all of them).
+// Epilogue: bias and activation; EPI 1: and residual, where the items are no experts' (y's shape)
+template <int EPI>
+struct EpiParams {
+    const float* bias;
+    const void* residual;
+    int act, r_bf16;
+};
+template <>
+struct EpiParams<0> {};
+// Items that are an expert's rows
 template <int NI>
-struct Params {
-    static constexpr bool kRows = NI == 0;
-    static constexpr int kArray = kRows ? 1 : NI;
+struct GroupParams {};
+constexpr int kGroups = -1;
+template <>
+struct GroupParams<kGroups> {
+    const int *offsets, *order;
+    int experts, rows, x_rows, n_rt, tables_off;  // row tiles of an expert; offset of the tables in shared memory
+    uint32_t top_k;
+};
+// NI: how many matmuls of a batch, at most; 1: one; 0: one whose rows of x are n_items items of 16 (M: all of them); kGroups: experts.
+template <int NI, int EPI>
+struct Params : EpiParams<EPI>, GroupParams<NI> {
+    static constexpr bool kRows = NI == 0, kExperts = NI == kGroups;
+    static constexpr int kArray = NI > 0 ? NI : 1;
     alignas(64) CUtensorMap maps[kArray];  // the packed weights
     Item items[kArray];
     int n_items, K, N, gshift, y_bf16;
-    __device__ __forceinline__ const Item& item(int i) const { return items[kRows ? 0 : i]; }
+    __device__ __forceinline__ const Item& item(int i) const { return items[NI > 0 ? i : 0]; }
     int rt_q, rt_rem;       // row tiles per CTA, and how many CTAs have one more
     int ts_inv, kbc_inv;    // 65536 / ts, 65536 / kbc, rounded up
     int nkb, nch, kbc, ts, tb;  // k-blocks; chunks of K and k-blocks per chunk (at most); row tiles per stage, and per pass over K
@@ -194,11 +227,103 @@ struct Walk {
     __device__ __forceinline__ int kb_cnt(const P& p) const { return min(p.kbc, p.nkb - c * p.kbc); }  // k-blocks of this chunk
 };
 
+// The same for experts: the row tiles of all items, item after item, in one range per CTA.  off: the experts' first rows (cut to what there
+// is), first: their first items, both in shared memory, experts + 1 of them (group_tables).  ROWS: rows of an item.
+template <int ROWS>
+struct GroupWalk {
+    int item, lo, hi, b0, c, ng;
+    int e, m0, M;  // the item's expert, its first row of y and how many it has
+    int left;      // row tiles of this CTA behind the item
+    template <class P>
+    __device__ __forceinline__ static const int* off(const P& p) {
+        extern __shared__ __align__(1024) unsigned char smem[];
+        return reinterpret_cast<const int*>(smem + p.tables_off);
+    }
+    template <class P>
+    __device__ __forceinline__ static const int* first(const P& p) { return off(p) + p.experts + 1; }
+    template <class P>
+    __device__ __forceinline__ void range(const P& p, int from) {
+        const int j = item - first(p)[e];
+        m0 = off(p)[e] + j * ROWS;
+        M = min(ROWS, off(p)[e + 1] - m0);
+        lo = b0 = from;
+        hi = min(p.n_rt, from + left);
+        left -= hi - from;
+        groups(p);
+    }
+    template <class P>
+    __device__ __forceinline__ void groups(const P& p) {
+        ng = (int)((uint32_t)((min(p.tb, hi - b0) + p.ts - 1) * p.ts_inv) >> 16);
+    }
+    template <class P>
+    __device__ __forceinline__ bool init(const P& p) {  // false: nothing for this CTA
+        const long long total = (long long)first(p)[p.experts] * p.n_rt, at = total * blockIdx.x / gridDim.x;
+        left = (int)(total * (blockIdx.x + 1) / gridDim.x - at);
+        if (!left) return false;
+        item = (int)(at / p.n_rt);
+        e = 0;
+        for (int n = p.experts; n > 1;) {  // the last expert whose first item is not past this one
+            const int half = n >> 1;
+            if (first(p)[e + half] <= item) e += half;
+            n -= half;
+        }
+        c = 0;
+        range(p, (int)(at - (long long)item * p.n_rt));
+        return true;
+    }
+    template <class P>
+    __device__ __forceinline__ bool next_run(const P& p) {
+        if (++c < p.nch) return true;
+        c = 0;
+        b0 += p.tb;
+        if (b0 < hi) {
+            groups(p);
+            return true;
+        }
+        if (!left) return false;
+        item++;
+        while (first(p)[e + 1] <= item) e++;
+        range(p, 0);
+        return true;
+    }
+    template <class P>
+    __device__ __forceinline__ int tile_end(const P& p) const { return min(b0 + p.tb, hi); }
+    template <class P>
+    __device__ __forceinline__ int kb_cnt(const P& p) const { return min(p.kbc, p.nkb - c * p.kbc); }
+};
+// Whole block: the tables of GroupWalk from the offsets.
+template <int ROWS, class P>
+__device__ __forceinline__ void group_tables(const P& p, unsigned char* smem) {
+    int* off = reinterpret_cast<int*>(smem + p.tables_off);
+    int* first = off + p.experts + 1;
+    for (int e = threadIdx.x; e <= p.experts; e += kThreads) off[e] = min(max(__ldcg(p.offsets + e), 0), p.rows);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int e0 = 0; e0 < p.experts; e0 += 32) {
+            const int e = e0 + (int)threadIdx.x, n = e < p.experts ? (max(off[e + 1] - off[e], 0) + ROWS - 1) / ROWS : 0;
+            int sum = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, sum, d);
+                if ((int)threadIdx.x >= d) sum += v;
+            }
+            if (e < p.experts) first[e] = before + sum - n;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) first[p.experts] = before;
+    }
+    __syncthreads();
+}
+
 // SPL: scales per lane and row of a task (2 for 4-bit weights in groups of 32).  PRO: what x is (0: as it lies; 1: the
-// rms-norm of its rows, for K within one chunk; 2: the sum of three column blocks; 1 and 2 for M <= 8).
-template <int BITS, int MT, int SPL, int PRO, int NI>
-__global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_constant__ Params<NI> p) {
+// rms-norm of its rows, for K within one chunk; 2: the sum of three column blocks; 1 and 2 for M <= 8).  EPI: 0 none; 1 bias,
+// activation, residual; 2 gated (experts).
+template <int BITS, int MT, int SPL, int PRO, int NI, int EPI>
+__global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_constant__ Params<NI, EPI> p) {
     static_assert(PRO == 0 || MT == 1, "prologues are built for M <= 8");
+    constexpr bool kExperts = NI == kGroups, kGated = EPI == 2;
+    static_assert(!kGated || kExperts, "gated products are built for experts");
     constexpr int XV = x_frags(BITS), KB = kb_weights(BITS), KL = lane_weights(BITS), SROW = sb_row(SPL);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ int s_abort;
@@ -218,8 +343,21 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
     }
     __syncthreads();
 
-    Walk wk;
-    wk.init(p);
+    std::conditional_t<kExperts, GroupWalk<8 * MT>, Walk> wk;
+    if constexpr (kExperts) {
+        // (which weights are wanted is the previous kernel's answer: there is nothing to fetch ahead of it)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        group_tables<8 * MT>(p, smem);
+        if (!wk.init(p)) return;
+    } else {
+        wk.init(p);
+    }
+    // row of wq, scales and biases that is row 0 of a tile; rows 8 .. 15 of a gated one lie p.N / 2 further on
+    auto tile_row = [&](int tile) {
+        if constexpr (kExperts) return (uint32_t)wk.e * p.N + (uint32_t)tile * (kGated ? 8 : 16);
+        else return (uint32_t)tile * 16;
+    };
     const int role = __shfl_sync(0xffffffffu, warp, 0);  // (uniform for the compiler too: the helpers' registers are few)
     if (role >= kWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
@@ -236,10 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             // Pieces are cut off at the row's end and filled up with zeros.  Where K ends inside a k-block, the groups that the
             // lanes past K would have read their scales from are zeros, too (for those a piece of nothing else, if need be): zero
             // codes with the last group's own scale and bias would add 0 * infinity where these are infinite.
-            const uint32_t gpr = (uint32_t)p.K >> p.gshift, half = 16u * gpr, k16 = 16u * (lane % LPR);
+            const uint32_t gpr = (uint32_t)p.K >> p.gshift, half = (kGated ? (uint32_t)p.N : 16u) * gpr, k16 = 16u * (lane % LPR);
+            const uint32_t next_tile = (kGated ? 16u : 32u) * gpr;
             do {
                 const int t_end = wk.tile_end(p), kb0 = wk.c * p.kbc, ops = p.k_tail ? wk.kb_cnt(p) : 1;
-                const CUtensorMap* map = &p.maps[p.kRows ? 0 : wk.item];
+                const CUtensorMap* map = &p.maps[NI > 0 ? wk.item : 0];
                 const uint32_t g0 = (uint32_t)(wk.c * p.kbc) * KB >> p.gshift, bytes = 2u * min((uint32_t)wk.kb_cnt(p) * KB >> p.gshift, gpr - g0);
                 const char *sc = reinterpret_cast<const char*>(p.item(wk.item).scales), *bi = reinterpret_cast<const char*>(p.item(wk.item).biases);
                 const uint32_t need = bytes + (p.k_tail && wk.c + 1 == p.nch ? 2u * SPL : 0u);
@@ -247,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 uint32_t lo[NB], cnt[NB], some = 0, odd = 0;
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    const uint32_t at = 2u * (((uint32_t)wk.b0 * 16 + i * RPI + lane / LPR) * gpr + g0);
+                    const uint32_t at = 2u * ((tile_row(wk.b0) + i * RPI + lane / LPR) * gpr + g0);
                     lo[i] = (at & ~15u) + k16;
                     cnt[i] = lo[i] < at + bytes ? min(16u, at + bytes - lo[i]) : 0u;
                     some |= (lo[i] < at + need ? 1u : 0u) << i;
@@ -263,7 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                     if (lane == 0) bar_expect(full + 8 * st, tiles * (p.k_tail ? ops : p.kbc) * 2048);
                     __syncwarp();
                     const uint32_t stage = ring + st * p.stage_bytes;
-                    if (!p.k_tail) {
+                    if constexpr (kExperts) {
+                        const int z = kGated ? 2 * wk.e : wk.e;
+                        if (!p.k_tail) {
+                            if (lane < tiles) tma_load_4d(stage + lane * p.tile_bytes, map, 0, (tile0 + lane) * (kGated ? 8 : 16), z, kb0, full + 8 * st);
+                        } else {
+                            for (int ti = 0; ti < tiles; ti++)
+                                if (lane < ops)
+                                    tma_load_3d(stage + ti * p.tile_bytes + lane * 2048, map, (kb0 + lane) * 128, (tile0 + ti) * (kGated ? 8 : 16), z, full + 8 * st);
+                        }
+                    } else if (!p.k_tail) {
                         if (lane < tiles) tma_load_3d(stage + lane * p.tile_bytes, map, 0, (tile0 + lane) * 16, kb0, full + 8 * st);
                     } else {
                         for (int ti = 0; ti < tiles; ti++)
@@ -272,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                     issued++;
                     uint32_t dst = stage + p.sb_off + (lane / LPR) * SROW + k16;
                     for (int ti = 0; ti < tiles; ti++, dst += 32 * SROW) {
-                        if ((tile0 + ti) * 16 + 16 <= p.N) {
+                        if (kGated || (tile0 + ti) * 16 + 16 <= p.N) {
 #pragma unroll
                             for (int i = 0; i < NB; i++)
                                 if (some >> i & 1) {
@@ -293,16 +441,17 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                                 }
                         }
                         if (odd && lane < 16) {
-                            const uint32_t n = (tile0 + ti) * 16 + lane, at = 2u * (n * gpr + g0), src = (at & ~15u) + 16 * LPR;
+                            const uint32_t n = (tile0 + ti) * 16 + lane, row = tile_row(tile0 + ti) + (kGated ? (lane & 7) + (lane >> 3) * (p.N >> 1) : lane);
+                            const uint32_t at = 2u * (row * gpr + g0), src = (at & ~15u) + 16 * LPR;
                             const uint32_t d = stage + p.sb_off + ti * (32 * SROW) + (lane >> 3) * (16 * SROW) + (lane & 7) * SROW + 16 * LPR;
-                            if (n < (uint32_t)p.N && src < at + need) {
+                            if ((kGated || n < (uint32_t)p.N) && src < at + need) {
                                 const uint32_t c = src < at + bytes ? min(16u, at + bytes - src) : 0u;
                                 cp_async16(d, sc + src, c);
                                 cp_async16(d + 8 * SROW, bi + src, c);
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < NB; i++) lo[i] += 2 * half;
+                        for (int i = 0; i < NB; i++) lo[i] += next_tile;
                     }
                     cp_async_arrive(full + 8 * st);
                     next_stage();
@@ -324,11 +473,18 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 // the sums carried from chunk to chunk change hands (all these warps come here in every run, after an abort too)
                 if (p.nch > 1) asm volatile("bar.sync 2, %0;" ::"r"(p.sum_warps * 32) : "memory");
                 const int kn = wk.kb_cnt(p), t_end = wk.tile_end(p);
-                int M = p.item(wk.item).M;
+                const size_t n_out = kGated ? p.N >> 1 : p.N;
+                int M;
                 void* y = p.item(wk.item).y;
-                if (p.kRows) {
-                    M = min(M - kItemRows * wk.item, kItemRows);
-                    y = static_cast<char*>(y) + (size_t)wk.item * kItemRows * p.N * (p.y_bf16 ? 2 : 4);
+                if constexpr (kExperts) {
+                    M = wk.M;
+                    y = static_cast<char*>(y) + (size_t)wk.m0 * n_out * (p.y_bf16 ? 2 : 4);
+                } else {
+                    M = p.item(wk.item).M;
+                    if (p.kRows) {
+                        M = min(M - kItemRows * wk.item, kItemRows);
+                        y = static_cast<char*>(y) + (size_t)wk.item * kItemRows * p.N * (p.y_bf16 ? 2 : 4);
+                    }
                 }
                 // lane (g, t) of the MMA: rows n = g, g+8 of the tile, rows of x 2t, 2t+1 (and 8 more)
                 const int m0 = 2 * (lane & 3), n0 = lane >> 2;
@@ -345,6 +501,31 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                         const int ti = MT == 1 ? i : i >> 1, mt = MT == 1 ? 0 : i & 1;
                         uint32_t src = ring + st * p.stage_bytes + ti * p.tile_bytes + mt * 512 + lane * 16;
                         const uint32_t run = ring + p.run_off + ((tile0 - wk.b0 + ti) * MT + mt) * 512 + lane * 16;
+                        // what the epilogue adds: row n0 of the tile and row n0 + 8
+                        float bias[2] = {0.0f, 0.0f}, res[2][2] = {};
+                        if constexpr (EPI != 0) {
+                            if (wk.c + 1 == p.nch) {
+                                const int n = (tile0 + ti) * (kGated ? 8 : 16) + n0, m = mt * 8 + m0;
+                                if (p.bias) {
+                                    const float* q = p.bias + tile_row(tile0 + ti) + n0;
+                                    if (n < p.N) bias[0] = q[0];
+                                    if (kGated) bias[1] = q[p.N >> 1];
+                                    else if (n + 8 < p.N) bias[1] = q[8];
+                                }
+                                if constexpr (!kExperts) {
+                                    if (p.residual) {
+                                        const size_t at = ((size_t)(p.kRows ? wk.item * kItemRows : 0) + m) * p.N + n;
+#pragma unroll
+                                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                                            for (int h = 0; h < 2; h++)
+                                                if (m + j < M && n + 8 * h < p.N)
+                                                    res[h][j] = p.r_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at + (size_t)j * p.N + 8 * h])
+                                                                         : static_cast<const float*>(p.residual)[at + (size_t)j * p.N + 8 * h];
+                                    }
+                                }
+                            }
+                        }
                         uint4 s = make_uint4(0, 0, 0, 0);
                         if (wk.c) s = lds_v4(run);
                         int k = kn;
@@ -359,16 +540,25 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                         if (wk.c + 1 < p.nch) {
                             sts_v4(run, s);
                         } else {
-                            const int n = (tile0 + ti) * 16 + n0, m = mt * 8 + m0;
-                            const bool two = n + 8 < p.N;
-                            if (n < p.N && m < M) {
-                                const size_t idx = (size_t)m * p.N + n;
+                            if constexpr (EPI == 1) {
+                                s.x = __float_as_uint(activate(p.act, __uint_as_float(s.x) + bias[0]) + res[0][0]);
+                                s.y = __float_as_uint(activate(p.act, __uint_as_float(s.y) + bias[0]) + res[0][1]);
+                                s.z = __float_as_uint(activate(p.act, __uint_as_float(s.z) + bias[1]) + res[1][0]);
+                                s.w = __float_as_uint(activate(p.act, __uint_as_float(s.w) + bias[1]) + res[1][1]);
+                            } else if constexpr (kGated) {
+                                s.x = __float_as_uint(activate(p.act, __uint_as_float(s.x) + bias[0]) * (__uint_as_float(s.z) + bias[1]));
+                                s.y = __float_as_uint(activate(p.act, __uint_as_float(s.y) + bias[0]) * (__uint_as_float(s.w) + bias[1]));
+                            }
+                            const int n = (tile0 + ti) * (kGated ? 8 : 16) + n0, m = mt * 8 + m0;
+                            const bool two = !kGated && n + 8 < p.N;
+                            if ((kGated || n < p.N) && m < M) {
+                                const size_t idx = (size_t)m * n_out + n;
                                 if (p.y_bf16) {
                                     __nv_bfloat16* q = static_cast<__nv_bfloat16*>(y) + idx;
                                     q[0] = __float2bfloat16_rn(__uint_as_float(s.x));
                                     if (two) q[8] = __float2bfloat16_rn(__uint_as_float(s.z));
                                     if (m + 1 < M) {
-                                        q += p.N;
+                                        q += n_out;
                                         q[0] = __float2bfloat16_rn(__uint_as_float(s.y));
                                         if (two) q[8] = __float2bfloat16_rn(__uint_as_float(s.w));
                                     }
@@ -377,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                                     q[0] = __uint_as_float(s.x);
                                     if (two) q[8] = __uint_as_float(s.z);
                                     if (m + 1 < M) {
-                                        q += p.N;
+                                        q += n_out;
                                         q[0] = __uint_as_float(s.y);
                                         if (two) q[8] = __uint_as_float(s.w);
                                     }
@@ -414,9 +604,23 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             constexpr int PP = XP / 2, CPR = 4 * PP, RPI = 32 / CPR, NL = 8 / RPI;
             const Item& it = p.item(wk.item);
             const int first = p.kRows ? wk.item * kItemRows : 0;  // row of the matmul that is the item's row 0
+            int rows;
+            if constexpr (kExperts) rows = wk.M;
+            else rows = it.M;
             const int pr = lane % PP, tt = lane / PP % 4, row = row0 + lane / CPR, ld = PRO == 0 ? p.K : p.x_ld;
             const int k0 = (wk.c * p.kbc + kq) * KB + tt * KL + pr * 16;
             V8 v[PASS][NL];
+            int src[NL];  // row of x
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                src[i] = first + row + i * RPI;
+                if constexpr (kExperts) {
+                    int at = -1;
+                    if (src[i] < rows) at = p.order ? __ldcg(p.order + wk.m0 + src[i]) : wk.m0 + src[i];
+                    if (p.order && at >= 0) at = (uint32_t)at / p.top_k;
+                    src[i] = at < p.x_rows ? at : -1;
+                }
+            }
 #pragma unroll
             for (int h = 0; h < PASS; h++)
 #pragma unroll
@@ -424,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                     const int k = k0 + h * (KL / PASS);
 #pragma unroll
                     for (int e = 0; e < 8; e++) v[h][i].v[e] = 0;
-                    if (first + row + i * RPI < it.M && k < p.K) {
-                        const __nv_bfloat16* s = it.x + (size_t)(first + row + i * RPI) * ld + k;
+                    if ((kExperts ? src[i] >= 0 : src[i] < rows) && k < p.K) {
+                        const __nv_bfloat16* s = it.x + (size_t)src[i] * ld + k;
                         v[h][i] = ldg_32(s, p.x32);
                         if (PRO == 2) {
                             const V8 b = ldg_32(s + p.K, p.x32), d = ldg_32(s + 2 * p.K, p.x32);
@@ -440,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < NL; i++) {
                     const int slot = (i * RPI + lane / CPR) * 4 + tt, j = h * XP + 2 * pr;
-                    if (first + row0 + i * RPI >= it.M) break;  // (rows past M: their columns of the result are never stored)
+                    if (first + row0 + i * RPI >= rows) break;  // (rows past M: their columns of the result are never stored)
                     sts_v4(frag_addr(j, slot), permute_x8<BITS>(make_uint4(v[h][i].v[0], v[h][i].v[1], v[h][i].v[2], v[h][i].v[3])));
                     sts_v4(frag_addr(j + 1, slot), permute_x8<BITS>(make_uint4(v[h][i].v[4], v[h][i].v[5], v[h][i].v[6], v[h][i].v[7])));
                 }
@@ -499,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             uint32_t sb_lane;
             {
                 const int kb0 = wk.c * p.kbc, gpr = p.K >> p.gshift, g0 = kb0 * KB >> p.gshift, gi = min(((kb0 + kq) * KB + t * KL) >> p.gshift, gpr);
-                const int n = (wk.b0 + tsub) * 16 + g;
+                const uint32_t n = tile_row(wk.b0 + tsub) + g;
                 sb_lane = p.sb_off + tsub * (32 * SROW - p.tile_bytes) + g * SROW + ((uint32_t)((n * gpr + g0) * 2) & 15u) + 2 * (gi - g0) - in_tile;
             }
 #pragma unroll 1
@@ -549,7 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
 // ---- host side ------------------------------------------------------------------------------------------------------
 using Plan = QmvStreamPlan;
 
-bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl) {
+// experts: 0, or how many a.N rows of W there are of (and the launch is a qmatmul_experts)
+bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl, int experts = 0) {
     if (a.x_dtype != LUX_DTYPE_BFLOAT16 || a.sb_dtype != LUX_DTYPE_BFLOAT16 || (a.bits != 4 && a.bits != 8)) return false;
     if (mmax < 1 || mmax > 16 || a.N < 1 || sm_count < 1 || (a.group != 32 && a.group != 64 && a.group != 128) || a.K % a.group) return false;
     if (((uintptr_t)a.wq | (uintptr_t)a.x | (uintptr_t)a.scales | (uintptr_t)a.biases) & 15) return false;
@@ -557,10 +762,10 @@ bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl) {
     const int KB = 1024 / a.bits, mt = mmax <= 8 ? 1 : 2;
     pl->nkb = (a.K + KB - 1) / KB;
     pl->n_rt = (a.N + 15) / 16;
-    if ((long long)a.N * (a.K / a.group) > (1ll << 30) || (long long)pl->n_rt * pl->nkb > (1ll << 26)) return false;  // 32-bit indices
-    pl->grid = std::min(pl->n_rt, sm_count);
+    if ((long long)a.N * std::max(experts, 1) * (a.K / a.group) > (1ll << 30) || (long long)pl->n_rt * pl->nkb > (1ll << 26)) return false;  // 32-bit indices
+    pl->grid = experts ? sm_count : std::min(pl->n_rt, sm_count);
     pl->grid_y = 1;
-    const int tiles_max = (pl->n_rt + pl->grid - 1) / pl->grid;
+    const int tiles_max = experts ? pl->n_rt : (pl->n_rt + pl->grid - 1) / pl->grid, tables = experts ? 8 * (experts + 1) : 0;
     pl->nch = (pl->nkb + kWarps - 1) / kWarps;
     pl->kbc = (pl->nkb + pl->nch - 1) / pl->nch;
     pl->nch = (pl->nkb + pl->kbc - 1) / pl->kbc;
@@ -573,14 +778,14 @@ bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl) {
     for (pl->ts = std::max(1, std::min(kWarps / pl->kbc, tiles_max));; pl->ts--) {
         pl->sb_off = pl->ts * pl->tile_bytes;
         pl->stage_bytes = (pl->sb_off + pl->ts * sb + 1023) & ~1023;
-        pl->stages = std::min(kMaxStages, (kSmemLimit - run - xs - bars) / pl->stage_bytes);
+        pl->stages = std::min(kMaxStages, (kSmemLimit - run - xs - bars - tables) / pl->stage_bytes);
         if (pl->stages >= 2) break;
         if (pl->ts == 1) return false;
     }
     pl->xs_off = pl->stages * pl->stage_bytes;
     pl->run_off = pl->xs_off + xs;
     pl->bar_off = pl->run_off + run;
-    pl->smem = (size_t)pl->bar_off + bars;
+    pl->smem = (size_t)pl->bar_off + bars + tables;  // (the tables are the last)
     return true;
 }
 
@@ -608,9 +813,9 @@ bool encode_weights(const QmmArgs& a, const Plan& pl, CUtensorMap* map) {
     return r == CUDA_SUCCESS;
 }
 
-template <int BITS, int MT, int SPL, int PRO, int NI>
-cudaError_t launch_t(const Params<NI>& p, const Plan& pl, cudaStream_t stream, bool overlap_prev) {
-    auto kern = qmv_stream_kernel<BITS, MT, SPL, PRO, NI>;
+template <int BITS, int MT, int SPL, int PRO, int NI, int EPI>
+cudaError_t launch_t(const Params<NI, EPI>& p, const Plan& pl, cudaStream_t stream, bool overlap_prev) {
+    auto kern = qmv_stream_kernel<BITS, MT, SPL, PRO, NI, EPI>;
     static std::atomic<bool> attr_set[64];
     if (cudaError_t e = allow_smem(kern, kSmemLimit, attr_set)) return e;
     cudaLaunchConfig_t cfg = {};
@@ -628,33 +833,50 @@ cudaError_t launch_t(const Params<NI>& p, const Plan& pl, cudaStream_t stream, b
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <int BITS, int SPL, int NI>
-cudaError_t launch_rows(const Params<NI>& p, const Plan& pl, int mmax, int pro, cudaStream_t stream, bool overlap_prev) {
-    if constexpr (NI > 0) {
-        constexpr int P1 = NI == 1 ? 1 : 0, P2 = NI == 1 ? 2 : 0;  // (prologues: single calls only)
+template <int BITS, int SPL, int NI, int EPI>
+cudaError_t launch_rows(const Params<NI, EPI>& p, const Plan& pl, int mmax, int pro, cudaStream_t stream, bool overlap_prev) {
+    if constexpr (NI != 0) {
+        constexpr int P1 = NI == 1 && EPI == 0 ? 1 : 0, P2 = NI == 1 && EPI == 0 ? 2 : 0;  // (prologues: single calls without an epilogue only)
         if (mmax <= 8)
-            return pro == 1   ? launch_t<BITS, 1, SPL, P1, NI>(p, pl, stream, overlap_prev)
-                   : pro == 2 ? launch_t<BITS, 1, SPL, P2, NI>(p, pl, stream, overlap_prev)
-                              : launch_t<BITS, 1, SPL, 0, NI>(p, pl, stream, overlap_prev);
+            return pro == 1   ? launch_t<BITS, 1, SPL, P1, NI, EPI>(p, pl, stream, overlap_prev)
+                   : pro == 2 ? launch_t<BITS, 1, SPL, P2, NI, EPI>(p, pl, stream, overlap_prev)
+                              : launch_t<BITS, 1, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
     }
-    return launch_t<BITS, 2, SPL, 0, NI>(p, pl, stream, overlap_prev);
+    return launch_t<BITS, 2, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
 }
-
-template <int NI>
-cudaError_t launch_items(const QmmArgs* items, int n, int mmax, const Plan& pl, cudaStream_t stream, bool overlap_prev, bool x_stable) {
-    const QmmArgs& a0 = items[0];
-    Params<NI> p;
-    p.n_items = p.kRows ? (a0.M + kItemRows - 1) / kItemRows : n;
-    p.K = a0.K; p.N = a0.N; p.gshift = pl.gshift; p.y_bf16 = a0.y_dtype == LUX_DTYPE_BFLOAT16;
+template <int NI, int EPI>
+cudaError_t launch_bits(const Params<NI, EPI>& p, const Plan& pl, int bits, int group, int mmax, int pro, cudaStream_t stream, bool overlap_prev) {
+    return bits == 8     ? launch_rows<8, 1, NI, EPI>(p, pl, mmax, pro, stream, overlap_prev)
+           : group == 32 ? launch_rows<4, 2, NI, EPI>(p, pl, mmax, pro, stream, overlap_prev)
+                         : launch_rows<4, 1, NI, EPI>(p, pl, mmax, pro, stream, overlap_prev);
+}
+// what follows from the plan
+template <int NI, int EPI>
+void fill_plan(Params<NI, EPI>& p, const QmmArgs& a, const Plan& pl) {
+    p.K = a.K; p.N = a.N; p.gshift = pl.gshift; p.y_bf16 = a.y_dtype == LUX_DTYPE_BFLOAT16;
     p.rt_q = pl.n_rt / pl.grid; p.rt_rem = pl.n_rt % pl.grid;
     p.ts_inv = (65536 + pl.ts - 1) / pl.ts; p.kbc_inv = (65536 + pl.kbc - 1) / pl.kbc;
     p.nkb = pl.nkb; p.nch = pl.nch; p.kbc = pl.kbc; p.ts = pl.ts; p.tb = pl.tb;
-    p.stages = pl.stages; p.sum_warps = std::min(kSumWarps, pl.stages); p.stage_bytes = pl.stage_bytes; p.tile_bytes = pl.tile_bytes; p.k_tail = a0.K % (1024 / a0.bits) != 0;
+    p.stages = pl.stages; p.sum_warps = std::min(kSumWarps, pl.stages); p.stage_bytes = pl.stage_bytes; p.tile_bytes = pl.tile_bytes; p.k_tail = a.K % (1024 / a.bits) != 0;
     p.sb_off = pl.sb_off; p.xs_off = pl.xs_off; p.run_off = pl.run_off; p.bar_off = pl.bar_off;
+    p.error = a.error ? a.error : device_error_word();
+}
+
+template <int NI, int EPI>
+cudaError_t launch_items(const QmmArgs* items, int n, int mmax, const Plan& pl, cudaStream_t stream, bool overlap_prev, bool x_stable) {
+    const QmmArgs& a0 = items[0];
+    Params<NI, EPI> p;
+    p.n_items = p.kRows ? (a0.M + kItemRows - 1) / kItemRows : n;
+    fill_plan(p, a0, pl);
+    if constexpr (EPI != 0) {
+        p.bias = a0.bias;
+        p.residual = a0.residual;
+        p.act = a0.act;
+        p.r_bf16 = a0.r_bf16;
+    }
     p.x_early = (!overlap_prev || x_stable) ? 1 : 0;
     p.x_ld = a0.pro ? a0.x_ld : a0.K;
     p.eps = a0.eps;
-    p.error = a0.error ? a0.error : device_error_word();
     p.x32 = p.x_ld % 16 == 0;
     for (int i = 0; i < n; i++) {
         if ((uintptr_t)items[i].x & 31) p.x32 = 0;
@@ -662,9 +884,34 @@ cudaError_t launch_items(const QmmArgs* items, int n, int mmax, const Plan& pl, 
         p.items[i] = Item{(const __nv_bfloat16*)items[i].x, (const __nv_bfloat16*)items[i].scales,
                           (const __nv_bfloat16*)items[i].biases, items[i].y, items[i].M};
     }
-    return a0.bits == 8     ? launch_rows<8, 1, NI>(p, pl, mmax, a0.pro, stream, overlap_prev)
-           : a0.group == 32 ? launch_rows<4, 2, NI>(p, pl, mmax, a0.pro, stream, overlap_prev)
-                            : launch_rows<4, 1, NI>(p, pl, mmax, a0.pro, stream, overlap_prev);
+    return launch_bits<NI, EPI>(p, pl, a0.bits, a0.group, mmax, a0.pro, stream, overlap_prev);
+}
+
+// ---- experts ----
+// Rows of an item: 8 as long as an expert has four rows on average or fewer, else 16 (which takes 1.3 times as long per weight, and eight
+// twice where there are more than eight).
+int group_rows(const ExpertsArgs& a) { return a.rows <= (size_t)4 * a.experts ? 8 : 16; }
+QmmArgs one_expert(const ExpertsArgs& a) {
+    QmmArgs q{a.x, a.wq, a.scales, a.biases, a.y, 0, a.K, a.N, a.bits, a.group, (int)LUX_DTYPE_BFLOAT16, (int)LUX_DTYPE_BFLOAT16, a.y_dtype};
+    q.error = a.error;
+    return q;
+}
+template <int EPI>
+cudaError_t launch_experts(const ExpertsArgs& a, const Plan& pl, const CUtensorMap& map, cudaStream_t stream, bool overlap_prev) {
+    Params<kGroups, EPI> p;
+    p.maps[0] = map;
+    fill_plan(p, one_expert(a), pl);
+    p.n_items = 0;  // (known on the device)
+    p.x_early = 0; p.x_ld = a.K; p.eps = 0.0f;
+    p.x32 = a.K % 16 == 0 && ((uintptr_t)a.x & 31) == 0;
+    p.items[0] = Item{(const __nv_bfloat16*)a.x, (const __nv_bfloat16*)a.scales, (const __nv_bfloat16*)a.biases, a.y, 0};
+    p.bias = a.bias;
+    p.residual = nullptr;
+    p.act = a.act;
+    p.r_bf16 = 0;
+    p.offsets = a.offsets; p.order = a.order; p.experts = a.experts; p.rows = (int)a.rows; p.x_rows = (int)a.x_rows;
+    p.n_rt = pl.n_rt; p.tables_off = (int)pl.smem - 8 * (a.experts + 1); p.top_k = a.order ? a.top_k : 1;
+    return launch_bits<kGroups, EPI>(p, pl, a.bits, a.group, group_rows(a), 0, stream, overlap_prev);
 }
 
 }  // namespace
@@ -680,8 +927,46 @@ int qmv_batch_max() { return kMaxBatch; }
 cudaError_t launch_qmv_stream(const QmmArgs& a, const QmvStreamPlan& pl, cudaStream_t stream, bool overlap_prev, bool x_stable) {
     // the rms-norm prologue needs the whole of x in the first fragments of the CTA's warps
     if (a.pro && (a.M > 8 || (a.pro == 1 && pl.nch != 1))) return cudaErrorNotSupported;
-    return a.M > kItemRows ? launch_items<0>(&a, 1, a.M, pl, stream, overlap_prev, x_stable)
-                           : launch_items<1>(&a, 1, a.M, pl, stream, overlap_prev, x_stable);
+    if (a.epi)
+        return a.M > kItemRows ? launch_items<0, 1>(&a, 1, a.M, pl, stream, overlap_prev, x_stable)
+                               : launch_items<1, 1>(&a, 1, a.M, pl, stream, overlap_prev, x_stable);
+    return a.M > kItemRows ? launch_items<0, 0>(&a, 1, a.M, pl, stream, overlap_prev, x_stable)
+                           : launch_items<1, 0>(&a, 1, a.M, pl, stream, overlap_prev, x_stable);
+}
+
+bool qmv_experts_supported(const ExpertsArgs& a, int sm_count) {
+    Plan pl;
+    // (a CTA's share of the row tiles is counted in 32 bits)
+    return make_plan(one_expert(a), group_rows(a), sm_count, &pl, a.experts) && (long long)(a.rows / 8 + a.experts) * pl.n_rt / sm_count < (1ll << 30);
+}
+
+cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name) {
+    Plan pl;
+    const EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode || !make_plan(one_expert(a), group_rows(a), sm_count, &pl, a.experts)) return cudaErrorInvalidValue;
+    // The packed weights [expert][half][row][byte], a tile being eight rows of either half, or 16 of the only one: boxes as encode_weights'
+    const cuuint64_t row_bytes = (cuuint64_t)a.K * a.bits / 8, halves = a.gated ? 2 : 1, rows = a.N / halves;
+    const cuuint32_t estr[4] = {1, 1, 1, 1}, box_rows = 16 / (cuuint32_t)halves;
+    CUtensorMap map;
+    CUresult r;
+    if (row_bytes % 128 == 0) {
+        const cuuint64_t dims[4] = {128, rows, halves * a.experts, row_bytes / 128}, strides[3] = {row_bytes, rows * row_bytes, 128};
+        const cuuint32_t box[4] = {128, box_rows, (cuuint32_t)halves, (cuuint32_t)pl.kbc};
+        r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else {
+        const cuuint64_t dims[3] = {row_bytes, rows, halves * a.experts}, strides[2] = {row_bytes, rows * row_bytes};
+        const cuuint32_t box[3] = {128, box_rows, (cuuint32_t)halves};
+        r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
+    if (r != CUDA_SUCCESS) {
+        set_last_error("cuTensorMapEncodeTiled (experts' weights) failed (%d)", (int)r);
+        return cudaErrorInvalidValue;
+    }
+    const bool m8 = group_rows(a) == 8;
+    *name = a.bits == 4 ? (m8 ? "qmv_experts<4,m8>" : "qmv_experts<4,m16>") : (m8 ? "qmv_experts<8,m8>" : "qmv_experts<8,m16>");
+    return a.gated ? launch_experts<2>(a, pl, map, stream, overlap_prev) : launch_experts<1>(a, pl, map, stream, overlap_prev);
 }
 
 cudaError_t launch_qmv_stream_batch(const QmmArgs* items, int n, int sm_count, cudaStream_t stream) {
@@ -698,7 +983,7 @@ cudaError_t launch_qmv_stream_batch(const QmmArgs* items, int n, int sm_count, c
     }
     Plan pl;
     if (mmax > kItemRows || !make_plan(a0, mmax, sm_count, &pl)) return cudaErrorNotSupported;
-    return n == 1 ? launch_items<1>(items, n, mmax, pl, stream, false, false) : launch_items<kMaxBatch>(items, n, mmax, pl, stream, false, false);
+    return n == 1 ? launch_items<1, 0>(items, n, mmax, pl, stream, false, false) : launch_items<kMaxBatch, 0>(items, n, mmax, pl, stream, false, false);
 }
 
 }  // namespace luxcuda

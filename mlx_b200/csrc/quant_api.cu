@@ -137,6 +137,23 @@ LuxBackendError ensure_qmm_workspace(Context* c) {
     return LUX_BACKEND_OK;
 }
 
+// The product with its epilogue: the prefill GEMM where qmatmul would take it, else the decode kernel in one pass over K (a K split over CTAs
+// has no place for an epilogue).
+LuxBackendError qmatmul_epi_on_stream(Context* c, const QmmArgs& a) {
+    const char* name = "";
+    QmvStreamPlan pl;
+    if (!plan_qmv_stream(a, c->dev->sm_count, &pl)) {
+        set_last_error("qmatmul_epi: M=%d K=%d N=%d in groups of %d is past the kernels' 32-bit index ranges", a.M, a.K, a.N, a.group);
+        return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    }
+    const cudaError_t e = launch_qmv_stream(a, pl, c->stream, decode_may_overlap(c, a), decode_x_stable(c, a));
+    if (e != cudaSuccess) return map_cuda_error(e, "qmatmul_epi");
+    c->launches++;
+    note_decode_launch(c, a);
+    c->last_kernel = name;
+    return LUX_BACKEND_OK;
+}
+
 LuxBackendError qmatmul_on_stream(Context* c, const QmmArgs& a) {
     if (a.M == 0 || a.N == 0) return LUX_BACKEND_OK;
     const char* name = "";
@@ -654,6 +671,7 @@ void fill_quant() {
     g_quant.qmatmul_pro = qmatmul_pro;
     g_quant.qmatmul_batch = qmatmul_batch;
     fill_mx4_entries(&g_quant);
+    fill_moe_entries(&g_quant);
 }
 
 }  // namespace

@@ -99,6 +99,23 @@ class BlockNormParams(C.Structure):  # include/lux_cuda_quant.h: lux_block_norm_
                [(n, C.c_float) for n in ("eps", "res_scale", "branch_scale", "out_pre")] + [("_pad", _u32)]
 
 
+class QmmEpiParams(C.Structure):  # include/lux_cuda_quant.h: lux_qmm_epi_params
+    _fields_ = [(n, C.c_int32) for n in ("M", "K", "N", "bits", "group", "act", "r_dtype", "y_dtype")]
+
+
+class MoeRouteParams(C.Structure):  # lux_moe_route_params
+    _fields_ = [(n, _u64) for n in ("tokens", "ld")] + [(n, C.c_int32) for n in ("experts", "top_k", "score", "renorm", "logits_dtype")] + [("scale", C.c_float)]
+
+
+class ExpertsParams(C.Structure):  # lux_experts_params
+    _fields_ = [(n, _u64) for n in ("rows", "x_rows")] + \
+               [(n, C.c_int32) for n in ("experts", "K", "N", "bits", "group", "top_k", "act", "gated", "y_dtype", "_pad")]
+
+
+class MoeCombineParams(C.Structure):  # lux_moe_combine_params
+    _fields_ = [(n, _u64) for n in ("tokens", "dim", "y_rows")] + [(n, C.c_int32) for n in ("top_k", "y_dtype", "out_dtype", "_pad")]
+
+
 _QMM = _fn(_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i)
 
 
@@ -157,6 +174,10 @@ class QuantVtbl(C.Structure):  # include/lux_cuda_quant.h: lux_gpu_quant_vtbl
         ("mx4_dequantize", _fn(_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, C.c_float)),
         ("mx4_matmul", _fn(_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, C.c_float)),
         ("block_norm", _fn(_i, _vp, C.POINTER(BlockNormParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp)),
+        ("qmatmul_epi", _fn(_i, _vp, C.POINTER(QmmEpiParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp)),
+        ("moe_route", _fn(_i, _vp, C.POINTER(MoeRouteParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp)),
+        ("qmatmul_experts", _fn(_i, _vp, C.POINTER(ExpertsParams), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp)),
+        ("moe_combine", _fn(_i, _vp, C.POINTER(MoeCombineParams), _vp, _vp, _vp, _vp, _vp)),
     ]
 
 
@@ -165,6 +186,9 @@ PRO_RMS_NORM, PRO_SUM3 = 1, 2  # LUX_CUDA_PRO_*: prologues of qmatmul_pro
 MX4_E8M0, MX4_E4M3 = 1, 2  # LUX_CUDA_MX4_*: microscaled 4-bit formats
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2  # LUX_CUDA_NORM_*
 GATE_IDENTITY, GATE_SIGMOID, GATE_TANH = 0, 1, 2  # LUX_CUDA_GATE_*
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = range(5)  # LUX_CUDA_ACT_*
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1  # LUX_CUDA_SCORE_*
+SHORT_CALLS = ("mx4_quantize", "mx4_dequantize", "mx4_matmul", "block_norm", "qmatmul_epi", "moe_route", "qmatmul_experts", "moe_combine")
 
 
 EXPORTED_SYMBOLS = ("lux_gpu_backend_init", "lux_gpu_cuda_quant_vtbl", "lux_gpu_cuda_abi_layout",
@@ -187,7 +211,7 @@ def load_library(path=None):
 
 
 def _short_calls(quant):
-    """mx4_* and block_norm as functions: csrc/fastcall.c where it is built for this interpreter and the library has them, else the mirror's own."""
+    """SHORT_CALLS as functions: csrc/fastcall.c where it is built for this interpreter and the library has them, else the mirror's own."""
     from .build import FASTCALL_PATH
     if not os.path.exists(FASTCALL_PATH) or quant.size < C.sizeof(QuantVtbl):
         return quant
@@ -313,8 +337,8 @@ class Context:
         self.handle = plugin.vtbl.create_context(device)
         if not self.handle:
             raise RuntimeError(f"create_context({device}) failed: {plugin.last_error()}")
-        self._mx4_quantize, self._mx4_dequantize, self._mx4_matmul, self._block_norm = (
-            _entry(plugin, plugin.short_calls, name) for name in ("mx4_quantize", "mx4_dequantize", "mx4_matmul", "block_norm"))
+        for name in SHORT_CALLS:
+            setattr(self, "_" + name, _entry(plugin, plugin.short_calls, name))
         self._mx4_scale_bytes = _entry(plugin, plugin.quant, "mx4_scale_bytes")
 
     # --- base vtable ---------------------------------------------------------
@@ -469,6 +493,53 @@ class Context:
                                 pre_w and pre_w.handle, pre_b and pre_b.handle, r_out and r_out.handle, out and out.handle, out_scales and out_scales.handle)
         if code != OK:
             self.plugin.check(code, "block_norm")
+
+    # --- a product with its epilogue; a layer of experts -------------------------
+    @staticmethod
+    def qmm_epi_params(M, K, N, bits, group, act=ACT_NONE, r_dtype=BF16, y_dtype=BF16):
+        """What qmatmul_epi does, to be kept and used again: see lux_qmm_epi_params."""
+        return QmmEpiParams(M, K, N, bits, group, act, r_dtype, y_dtype)
+
+    def qmatmul_epi(self, params, x, wq, scales, biases, bias, residual, y):
+        """y = act(x . dequant(Wq)^T + bias) + residual.  None where there is no such buffer."""
+        code = self._qmatmul_epi(self.handle, params, x.handle, wq.handle, scales.handle, biases.handle, bias and bias.handle, residual and residual.handle, y.handle)
+        if code != OK:
+            self.plugin.check(code, "qmatmul_epi")
+
+    @staticmethod
+    def moe_route_params(tokens, experts, top_k, score=SCORE_SOFTMAX, renorm=True, logits_dtype=F32, scale=1.0, ld=0):
+        """What moe_route does: see lux_moe_route_params."""
+        return MoeRouteParams(tokens, ld, experts, top_k, score, int(renorm), logits_dtype, scale)
+
+    def moe_route(self, params, logits, bias, ids, weights, order, pos, offsets):
+        """A token's top_k experts and their weights, and the pairs (token, slot) sorted by expert.  logits None: the experts are given in ids."""
+        code = self._moe_route(self.handle, params, logits and logits.handle, bias and bias.handle, ids.handle, weights and weights.handle, order.handle,
+                               pos.handle, offsets.handle)
+        if code != OK:
+            self.plugin.check(code, "moe_route")
+
+    @staticmethod
+    def experts_params(rows, x_rows, experts, K, N, bits, group, top_k=1, act=ACT_NONE, gated=False, y_dtype=BF16):
+        """What qmatmul_experts does: see lux_experts_params."""
+        return ExpertsParams(rows, x_rows, experts, K, N, bits, group, top_k, act, int(gated), y_dtype, 0)
+
+    def qmatmul_experts(self, params, x, order, offsets, wq, scales, biases, bias, y):
+        """Rows offsets[e] .. offsets[e+1] of y = epilogue(x rows . dequant(Wq[e])^T); with order, row i comes from row order[i] / top_k of x."""
+        code = self._qmatmul_experts(self.handle, params, x.handle, order and order.handle, offsets.handle, wq.handle, scales.handle, biases.handle,
+                                     bias and bias.handle, y.handle)
+        if code != OK:
+            self.plugin.check(code, "qmatmul_experts")
+
+    @staticmethod
+    def moe_combine_params(tokens, dim, top_k, y_rows, y_dtype=BF16, out_dtype=BF16):
+        """What moe_combine does: see lux_moe_combine_params."""
+        return MoeCombineParams(tokens, dim, y_rows, top_k, y_dtype, out_dtype, 0)
+
+    def moe_combine(self, params, y, pos, weights, residual, out):
+        """out = residual + the sum over a token's slots of weights * y[pos]."""
+        code = self._moe_combine(self.handle, params, y.handle, pos.handle, weights and weights.handle, residual and residual.handle, out.handle)
+        if code != OK:
+            self.plugin.check(code, "moe_combine")
 
     def timer_record(self, slot):
         self.plugin.check(self.plugin.quant.timer_record(self.handle, slot), "timer_record")
