@@ -414,7 +414,7 @@ typedef struct lux_gpu_quant_vtbl {
      * expert whose logit is -infinity or NaN is not chosen, nor one whose bias is; a slot for which no expert is left gets id -1 and weight 0.
      *   SCORE_SOFTMAX: weight = exp(logit - max) / sum over the token's experts (logits equal to the largest count as exp(0), infinite ones too);
      *   SCORE_SIGMOID: weight = 1 / (1 + exp(-logit));
-     *   renorm: divided by the sum of the token's weights (0 where that is 0);     all times `scale`.
+     *   renorm: divided by the sum of the token's weights (0 where that is 0);     all times `scale`.  Weights are taken in fp32.
      * ids int32 [tokens][top_k], weights fp32 [tokens][top_k];
      * offsets int32 [experts+1]: offsets[e] pairs go to the experts before e;
      * order int32 [tokens*top_k]: the pairs by expert, for one expert in rising order; order[i] for i >= offsets[experts] is left as it was;
@@ -430,8 +430,9 @@ typedef struct lux_gpu_quant_vtbl {
      *   y[i] = act(v[:N/2]) * v[N/2:]               [N/2], gated: the first half of an expert's rows of wq are its gate's; N is a multiple of 16
      * wq, scales and biases as qmatmul's, one expert's [N][...] after the other's; x, scales, biases BF16; bias fp32 [experts][N] or NULL; y F32
      * or BF16, sums, bias and activation in fp32 and rounded once.  Rows of y that belong to no expert are left as they were.  Offsets
-     * are cut to [0, rows], an expert whose offsets fall has no rows, and x counts as zero where a row of it does not exist.
-     * K a multiple of the group.  A row's result depends on nothing but the row and its expert. */
+     * are cut to [0, rows] and an expert whose offsets fall has no rows (where the cut ones overlap, it is not said which rows are computed); x
+     * counts as zero where a row of it does not exist.  K a multiple of the group.  A row's result depends on nothing but the row and its
+     * expert, in calls with the same parameters. */
     LuxBackendError (*qmatmul_experts)(LuxBackendContext* ctx, const lux_experts_params* params, LuxBackendBuffer* x, LuxBackendBuffer* order,
                                        LuxBackendBuffer* offsets, LuxBackendBuffer* wq, LuxBackendBuffer* scales, LuxBackendBuffer* biases,
                                        LuxBackendBuffer* bias, LuxBackendBuffer* y);

@@ -21,7 +21,7 @@ FASTCALL_PATH = os.path.join(LIB_DIR, "fastcall" + (sysconfig.get_config_var("EX
 
 SOURCES = ["plugin.cu", "device_state.cu", "ops_basic.cu", "ops_tensor.cu", "quant_ops.cu", "quant_api.cu", "qmv_simt.cu",
            "qmv_mma.cu", "qmv_stream.cu", "qmm_tc.cu", "shard.cu", "shard_push.cu", "mx4_quant.cu", "mx4_gemm.cu", "block_norm.cu",
-           "block_norm_stream.cu", "mx4_api.cu", "moe.cu", "moe_api.cu"]
+           "block_norm_stream.cu", "mx4_api.cu", "moe.cu", "moe_api.cu", "qmm_experts.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall", "--expt-relaxed-constexpr"]
 

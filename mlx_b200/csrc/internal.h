@@ -274,6 +274,7 @@ bool plan_decode(const QmmArgs& a, int sm_count, DecodePlan* pl);  // false: for
 bool qmv_mma_supported(const QmmArgs& a, int sm_count);
 size_t qmv_mma_workspace_bytes(const QmmArgs& a, int sm_count);
 bool plan_qmv_stream(const QmmArgs& a, int sm_count, QmvStreamPlan* pl);
+const char* qmv_stream_name(const QmmArgs& a);  // as last_kernel tells it
 cudaError_t launch_qmv_stream(const QmmArgs& a, const QmvStreamPlan& pl, cudaStream_t stream, bool overlap_prev, bool x_stable);
 cudaError_t launch_qmv_stream_batch(const QmmArgs* items, int n, int sm_count, cudaStream_t stream);
 // overlap_prev: launch as a programmatic dependent of the previous kernel in the stream (see Context);
@@ -392,7 +393,7 @@ struct MoeCombineArgs {
     bool y_bf16, out_bf16, vec;  // vec: every row of every buffer starts on a 16-byte boundary and is whole pieces of 8
 };
 cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev);
-// products grouped by expert (qmv_stream.cu: few rows an expert)
+// products grouped by expert (qmv_stream.cu: few rows an expert; qmm_experts.cu: many)
 struct ExpertsArgs {
     const void* x;
     const int *order, *offsets;  // order null: row i of y comes from row i of x
@@ -408,6 +409,8 @@ struct ExpertsArgs {
 };
 bool qmv_experts_supported(const ExpertsArgs& a, int sm_count);
 cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
+bool qmm_experts_supported(const ExpertsArgs& a);
+cudaError_t launch_qmm_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);
 cudaError_t launch_flush(void* buf, size_t bytes, cudaStream_t stream);

@@ -1,6 +1,6 @@
 // Entry points of the product with an epilogue and of a layer of experts (lux_gpu_quant_vtbl): argument checks, then the launches on the
 // context's stream.
-#include <cstring>
+#include <cstdlib>
 
 #include "internal.h"
 
@@ -66,6 +66,9 @@ void note_use(Context* c, const Operand* o, int n) {
     for (int i = 0; i < n; i++)
         if (o[i].b) o[i].b->last_stream = c->stream;
 }
+// Rows an expert on average (what the host knows) from which on the GEMM is the faster.
+bool experts_have_many_rows(const ExpertsArgs& a) { return a.rows >= (size_t)16 * a.experts; }
+
 // after a launch whose dependents start behind its wait: what it writes
 void note_outputs(Context* c, const Operand* o, int n) {
     note_early_chain_launch(c, false);
@@ -198,12 +201,18 @@ LuxBackendError qmatmul_experts(LuxBackendContext* ctx, const lux_experts_params
     ExpertsArgs a{o[X].ptr(), (const int*)o[ORDER].ptr(), (const int*)o[OFFSETS].ptr(), (const uint32_t*)o[WQ].ptr(), o[SCALES].ptr(), o[BIASES].ptr(),
                   (const float*)o[BIAS].ptr(), o[Y].ptr(), (size_t)p.rows, (size_t)p.x_rows, p.experts, p.K, p.N, p.bits, p.group, p.top_k, p.act,
                   p.gated != 0, p.y_dtype, c->err_dev};
-    if (!qmv_experts_supported(a, c->dev->sm_count)) {
+    // Few rows an expert: the decode kernel, which reads weights as fast as they come; many: the prefill GEMM.  LUXCUDA_EXPERTS = "few" | "many"
+    // (experiments)
+    const char* force = getenv("LUXCUDA_EXPERTS");
+    const bool many = qmm_experts_supported(a), few = qmv_experts_supported(a, c->dev->sm_count);
+    if (!many && !few) {
         set_last_error("qmatmul_experts: experts=%d K=%d N=%d in groups of %d is past the kernels' 32-bit index ranges", p.experts, p.K, p.N, p.group);
         return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     }
+    const bool use_many = many && (!few || (force ? force[0] == 'm' : experts_have_many_rows(a)));
     const char* name = "";
-    const cudaError_t e = launch_qmv_experts(a, c->dev->sm_count, c->stream, chain_is_open(c), &name);
+    const cudaError_t e = use_many ? launch_qmm_experts(a, c->dev->sm_count, c->stream, chain_is_open(c), &name)
+                                   : launch_qmv_experts(a, c->dev->sm_count, c->stream, chain_is_open(c), &name);
     if (e != cudaSuccess) return map_cuda_error(e, name);
     c->launches++;
     c->last_kernel = name;

@@ -539,6 +539,8 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.moe.experts", "qmv_experts<4,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.experts", "qmv_experts<8,m8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.experts", "qmv_experts<8,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmm_experts<4>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // many rows an expert (tcgen05)
+    {"lux.moe.experts", "qmm_experts<8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
 };
 const LuxKernelRegistry g_registry = {"cuda", g_kernels, sizeof(g_kernels) / sizeof(g_kernels[0])};
 

@@ -35,160 +35,18 @@
 //   warp 22     TMA producer for the packed weights (weight_producer).
 // Hand-over uses mbarriers; every wait is bounded: on a time-out the kernel
 // raises an error word (host-visible) and all roles drain and return.
-#include <cuda.h>
-#include <cuda_bf16.h>
-
 #include <algorithm>
 #include <atomic>
 
-#include "dequant.cuh"
-#include "internal.h"
-#include "qmm_plan.h"
+#include "epilogue.cuh"
+#include "qmm_roles.cuh"
 
 namespace luxcuda {
 
 namespace {
 
-constexpr int kDqWarps = 4 * kDqGroups;
-static_assert(kDqGroups == kStagesB, "a group always owns the same slot (and its waits, by parity, cannot alias)");
-constexpr int kTmaWarp = kEpiWarps + kDqWarps, kMmaWarp = kTmaWarp + 1, kWWarp = kMmaWarp + 1;
-constexpr int kNumThreads = (kWWarp + 1) * 32;
-constexpr uint32_t kTmemCols = 512, kAColBase = 256, kAColsPerSub = kBK / 2, kAColsPerSlot = kSub * kAColsPerSub;
-constexpr uint32_t kWaitClocks = 4000000000u;
 constexpr uint32_t kSpinLimit = 1u << 22;  // polls of a flag in global memory, 100 ns and more apart
 constexpr size_t kWsFlagBytes = 1024;  // flag words of the stream-K workspace (one per CTA), ahead of the partials
-
-__device__ __forceinline__ uint32_t s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t n) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(b)), "r"(n));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(b)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
-    uint32_t ok;
-    // (the hint, in ns, lets the hardware hold a waiting warp instead of having it poll: polls take issue slots)
-    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(ok) : "r"(s32(b)), "r"(parity), "r"(20000u) : "memory");
-    return ok != 0;
-}
-// Bounded wait, about two seconds of SM clock (a poll may itself last 20 us: counting polls would not bound it).  Returns
-// false (and raises *abort_flag) when the barrier does not flip within the limit or another role has already given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try(b, parity)) return true;
-    const uint32_t t0 = clock();
-    uint32_t i = 0;
-    do {
-#pragma unroll 1
-        for (uint32_t end = i + 64; i < end; i++) {
-            if (i > 4) __nanosleep(40);  // waiting roles must not steal issue slots from the working ones
-            if (mbar_try(b, parity)) return true;
-        }
-    } while (!*abort_flag && (uint32_t)clock() - t0 < kWaitClocks);
-    *abort_flag = 1;
-    return false;
-}
-
-// Same bound, no back-off, for the warp whose wake-up latency is on the tensor pipe's critical path.  Whole warp; the vote
-// makes the answer, and with it the control flow behind it, uniform for the compiler.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
-    if (__all_sync(0xffffffffu, mbar_try(b, parity))) return true;
-    const uint32_t t0 = clock();
-    do {
-#pragma unroll 1
-        for (uint32_t i = 0; i < 64; i++)
-            if (__all_sync(0xffffffffu, mbar_try(b, parity))) return true;
-    } while (__all_sync(0xffffffffu, !*abort_flag && (uint32_t)clock() - t0 < kWaitClocks));
-    *abort_flag = 1;
-    return false;
-}
-// After an abort nobody waits for the copies and MMAs in flight any more; before the CTA frees its tensor memory and ends
-// they get two milliseconds, far more than they take.  Every thread, behind the barrier at which all roles have returned.
-__device__ __forceinline__ void settle_after_abort(volatile int* abort_flag) {
-    if (!*abort_flag) return;
-    const uint32_t t0 = clock();
-    while ((uint32_t)clock() - t0 < 4000000u) __nanosleep(1000);
-}
-__device__ __forceinline__ bool elect_one() {  // whole warp: true in one lane, always the same
-    uint32_t r;
-    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
-    return r != 0;
-}
-
-// ---- tcgen05 / TMEM ------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {  // whole warp
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(dst_smem)), "r"(ncols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {  // whole warp
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem desc], bf16 inputs, fp32 accumulate
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-        "  tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-// 16 consecutive 32-bit columns of this thread's TMEM lane <- 16 registers
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor: K-major tile, rows of 128 bytes, 128-byte swizzle,
-// 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);   // start address, 16-byte units
-    d |= (uint64_t)1 << 16;                          // leading-dimension byte offset (unused for swizzled K-major)
-    d |= (uint64_t)(1024 >> 4) << 32;                // stride-dimension byte offset: 8 rows x 128 B
-    d |= (uint64_t)1 << 46;                          // descriptor version (sm_100)
-    d |= (uint64_t)2 << 61;                          // layout: SWIZZLE_128B
-    return d;
-}
-// Instruction descriptor, kind::f16: D = F32, A = B = BF16, both K-major, M x N.
-__host__ __device__ constexpr uint32_t umma_idesc(int M, int N) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// ---- TMA -----------------------------------------------------------------------
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(s32(dst)), "l"(map), "r"(x), "r"(y), "r"(s32(bar)) : "memory");
-}
 
 struct GemmParams {
     const uint32_t* wq;
@@ -206,7 +64,28 @@ struct GemmParams {
     int y_tma;               // pair kernel: y leaves through shared memory; 1: by a TMA store (bf16, one copy of y, N % 8 == 0),
                              // 2: by 16-byte stores into every rank's copy (column-sharded, ld and col0 multiples of 8)
     uint32_t* ws_flags;      // [CTA]: 1 while that CTA's partial waits to be added (zero between launches)
+    const float* bias;       // epilogue (EPI): null where there is none
+    const void* residual;    // as y: [M][N]
+    int act, r_bf16;
 };
+
+// The epilogue of qmatmul_epi on CNT rows of x from row m (of which `rows` are there) of column n: act(sum + bias) + residual.  The lanes of a warp
+// hold neighbouring columns: a residual row is read in whole 64- or 128-byte pieces, CNT of them under way.
+template <int CNT>
+__device__ __forceinline__ void finish(const GemmParams& p, uint32_t* v, int m, int rows, int n) {
+    if (n >= p.N) return;
+    const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
+    float r[CNT];
+#pragma unroll
+    for (int j = 0; j < CNT; j++) {
+        const size_t at = (size_t)(m + j) * p.N + n;
+        r[j] = !p.residual || j >= rows ? 0.0f
+               : p.r_bf16              ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at])
+                                       : static_cast<const float*>(p.residual)[at];
+    }
+#pragma unroll
+    for (int j = 0; j < CNT; j++) v[j] = __float_as_uint(activate(p.act, __uint_as_float(v[j]) + b) + r[j]);
+}
 
 // The work of a launch is the sequence of (tile, k-stage) units, tile after tile.  Two schedules:
 //   * whole tiles, round robin: CTA c takes tiles c, c + G, c + 2G, ... (neighbouring CTAs work on neighbouring
@@ -245,247 +124,7 @@ struct SmemLayout {
     int abort_flag;
 };
 
-__device__ __forceinline__ uint32_t ldg_u16(const uint16_t* p) {  // zero-extended straight into a 32-bit register
-    uint32_t v;
-    asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
-}
-
-// 32 weights of one row (one scale) -> 16 registers of bf16 pairs in natural k order.
-// The matrix instruction wants neighbours in k side by side, which dequant.cuh's masks do not yield (they pair weights 4
-// apart, and a byte permute per pair put them in order afterwards: 9 integer operations per 8 weights at 4 bit, 10 at 8
-// bit).  Here a permute comes first.  4 bit: byte i of the word into both halves, one mask, q_2i in the low half and
-// 16 * q_2i+1 in the high one, whose scale is 2^-4 of the low one's: 8 operations.  8 bit: two bytes into the two halves,
-// which is all: 4 operations.  The products are the same (see dequant.cuh for the 2^-133 form).
-template <int BITS, bool FAST>
-__device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s_bits, uint32_t b_bits, uint32_t (&out)[16]) {
-    const uint32_t b2 = dup_bf16(b_bits);
-    if (BITS == 4) {
-        const uint32_t s2 = FAST ? imad(s_bits, 0x00010001u, 0x40804280u) : dup_bf16(s_bits);  // FAST: (s * 2^133, s * 2^129)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            if (FAST) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) out[4 * c + i] = fma_bf16x2(prmt(w[c], 0u, 0x4040u + 0x0101u * i) & 0x00F0000Fu, s2, b2);
-            } else {
-                uint32_t r[4];  // r[i] = (w^_i, w^_{i+4})
-                dequant4_general(w[c], s2, b2, r);
-                out[4 * c + 0] = prmt(r[0], r[1], 0x5410u);
-                out[4 * c + 1] = prmt(r[2], r[3], 0x5410u);
-                out[4 * c + 2] = prmt(r[0], r[1], 0x7632u);
-                out[4 * c + 3] = prmt(r[2], r[3], 0x7632u);
-            }
-        }
-    } else {
-        const uint32_t s2 = FAST ? scale_x2_133(s_bits) : dup_bf16(s_bits);
-#pragma unroll
-        for (int c = 0; c < 8; c++) {
-            if (FAST) {
-                out[2 * c] = fma_bf16x2(prmt(w[c], 0u, 0x4140u), s2, b2);
-                out[2 * c + 1] = fma_bf16x2(prmt(w[c], 0u, 0x4342u), s2, b2);
-            } else {
-                uint32_t r[2];  // (w^_0, w^_2), (w^_1, w^_3)
-                dequant8_general(w[c], s2, b2, r);
-                out[2 * c] = prmt(r[0], r[1], 0x5410u);
-                out[2 * c + 1] = prmt(r[0], r[1], 0x7632u);
-            }
-        }
-    }
-}
-
-// ---- roles common to the kernels ----
-// Whole tiles, every `step`-th one from `tile` on (the interface of SegIter).
-struct TileIter {
-    int tile_, step, total, nst;
-    __device__ __forceinline__ bool valid() const { return tile_ < total; }
-    __device__ __forceinline__ int tile() const { return tile_; }
-    __device__ __forceinline__ int s_lo() const { return 0; }
-    __device__ __forceinline__ int s_hi() const { return nst; }
-    __device__ __forceinline__ void next() { tile_ += step; }
-};
-// The CTA's stages are counted 0, 1, 2, ... along its sequence of segments, alike in every role; dequantising group g owns
-// the counts = g (mod kDqGroups).
-//
-// One thread: the packed weights, unit after unit into the ring of the group that owns the stage.  Three stages at a time,
-// one for each group: first units first, so that with a single slot per group no group waits for another's second unit
-// (8 bit).  Every stage is UPS units, so that the rings advance alike; the odd sub-block's partner is announced without a load.
-template <int BITS, class Seg, class RowOf>
-__device__ __forceinline__ void weight_producer(const GemmParams& p, const CUtensorMap* tmap_w, Seg seg, int nks, unsigned char* ring,
-                                                uint64_t* wfull, uint64_t* wempty, volatile int* abort_flag, const RowOf& row_of) {
-    constexpr int UPS = BITS == 8 ? 2 : 1;  // weight units (128 rows x 64 packed bytes) per pipeline stage
-    int row[kDqGroups], stage[kDqGroups], cnt = 0, slot = 0;
-    uint32_t ph = 1;
-    auto flush = [&]() {
-#pragma unroll
-        for (int u = 0; u < UPS; u++) {
-#pragma unroll
-            for (int g = 0; g < kDqGroups; g++) {
-                if (g >= cnt) break;
-                const int i = g * kMaxWSlots + slot;
-                if (!mbar_wait(wempty + i, ph, abort_flag)) return false;
-                if (u == 0 || stage[g] * kSub + u < nks) {
-                    mbar_expect_tx(wfull + i, kWUnitBytes);
-                    tma_load_2d(ring + (g * p.w_slots + slot) * kWUnitBytes, tmap_w, stage[g] * (kSub * kBK * BITS / 8) + u * 64, row[g], wfull + i);
-                } else {
-                    mbar_arrive(wfull + i);
-                }
-            }
-            if (++slot == p.w_slots) { slot = 0; ph ^= 1; }
-        }
-        cnt = 0;
-        return true;
-    };
-    for (; seg.valid(); seg.next()) {
-        const int n0 = row_of(seg.tile()), s_hi = seg.s_hi();
-        for (int st = seg.s_lo(); st < s_hi; st++) {
-#pragma unroll
-            for (int g = 0; g < kDqGroups; g++)
-                if (g == cnt) { row[g] = n0; stage[g] = st; }
-            if (++cnt == kDqGroups && !flush()) return;
-        }
-    }
-    flush();
-}
-// One warp (lane quarter of group grp; a warp may only touch its own quarter of the TMEM lanes): the thread owns row r of
-// every tile.  There are as many stages in flight as groups, so a group always writes the same slot.
-// What bounds it is its instructions, three such warps to a scheduler, and the instruction caches that all roles share;
-// hence row pointers per tile (a division each), one copy of the code for both sub-blocks, one arrival per warp.
-template <int BITS, class Seg, class RowOf, class Arrive>
-__device__ __forceinline__ void dequant_role(const GemmParams& p, Seg seg, int grp, int r, int nks, const unsigned char* wring, uint64_t* wfull,
-                                             uint64_t* wempty, uint64_t* empty, uint32_t a_tmem, volatile int* abort_flag,
-                                             const RowOf& row_of, const Arrive& arrive) {
-    constexpr int WPS = kBK * BITS / 32;    // packed words per row per sub-block: 8 | 16
-    constexpr int UPS = BITS == 8 ? 2 : 1;  // weight units (128 rows x 64 packed bytes) per pipeline stage
-    const int gpr = p.K >> p.gshift;
-    const int ng_full = (kSub * kBK) >> p.gshift;  // scale groups per full stage: 4, 2 or 1
-    const bool vec_ok = (gpr % ng_full) == 0;      // then a stage's scales of one row are one aligned vector
-    // row r of a unit in shared memory is 64 bytes, its 16-byte chunk c sits at c ^ ((r >> 1) & 3)
-    const uint32_t wsw = (uint32_t)(r >> 1) & 3u;
-    const unsigned char* wrow0 = wring + r * 64;
-    const uint16_t *srow = nullptr, *brow = nullptr;  // scales / biases of this thread's row of the tile
-    int st, end;
-    bool more = true;
-    auto new_rows = [&]() {
-        const size_t at = (size_t)min(row_of(seg.tile()) + r, p.N - 1) * gpr;
-        srow = reinterpret_cast<const uint16_t*>(p.scales) + at;
-        brow = reinterpret_cast<const uint16_t*>(p.biases) + at;
-    };
-    auto settle = [&]() {  // st lies past the segment's end: the stage as far into the segments after it
-        do {
-            const int over = st - end;
-            seg.next();
-            if (!seg.valid()) {
-                more = false;
-                return;
-            }
-            st = seg.s_lo() + over;
-            end = seg.s_hi();
-        } while (st >= end);
-        new_rows();
-    };
-    uint32_t sp[2], bp[2];  // scales / biases of the next owned stage of this row, bf16 pairs in group order
-    auto fetch_sb = [&]() {
-        const int g0 = (st * kSub * kBK) >> p.gshift;
-        const uint16_t *sr = srow + g0, *br = brow + g0;
-        sp[1] = 0; bp[1] = 0;
-        if (vec_ok && ng_full == 4) {
-            asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(sp[0]), "=r"(sp[1]) : "l"(sr));
-            asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(bp[0]), "=r"(bp[1]) : "l"(br));
-        } else if (vec_ok && ng_full == 2) {
-            asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(sp[0]) : "l"(sr));
-            asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(bp[0]) : "l"(br));
-        } else if (ng_full == 4 && (gpr & 1) == 0) {  // (a load is one line per lane: four of pairs, not eight)
-            asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(sp[0]) : "l"(sr));
-            asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(bp[0]) : "l"(br));
-            if (gpr - g0 > 2) {
-                asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(sp[1]) : "l"(sr + 2));
-                asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(bp[1]) : "l"(br + 2));
-            }
-        } else {
-            const int ng = min(gpr - g0, ng_full);
-            sp[0] = ldg_u16(sr); bp[0] = ldg_u16(br);
-            if (ng > 1) { sp[0] |= ldg_u16(sr + 1) << 16; bp[0] |= ldg_u16(br + 1) << 16; }
-            if (ng > 2) { sp[1] = ldg_u16(sr + 2); bp[1] = ldg_u16(br + 2); }
-            if (ng > 3) { sp[1] |= ldg_u16(sr + 3) << 16; bp[1] |= ldg_u16(br + 3) << 16; }
-        }
-    };
-    if (!seg.valid()) return;
-    st = seg.s_lo() + grp;
-    end = seg.s_hi();
-    if (st >= end) settle();
-    else new_rows();
-    if (more) fetch_sb();
-    const int half_shift = p.gshift == 5 ? 16 : 0, sub_shift = p.gshift == 6 ? 16 : 0;  // where the next half's, the next sub-block's scale is
-    int wslot = 0;
-    uint32_t wphase = 0, phase = 1;
-    while (more) {
-        const int nsub = min(kSub, nks - st * kSub);
-        uint32_t s_lo = sp[0], b_lo = bp[0];
-        const uint32_t s_hi = sp[1], b_hi = bp[1];
-        st += kDqGroups;
-        if (st >= end) settle();
-        // Three stages ahead of its use.  At 4 bit behind the proxy fence, which would wait for these loads too (777 rows in
-        // groups of 32: 30.9 against 33-40 us); at 8 bit, with a fence per sub-block, here (512 x 8192 x 28672: 204 against 257).
-        if (UPS == 2 && more) fetch_sb();
-        uint32_t w[WPS], wn[8];  // this sub-block's words; 4 bit: the next one's, from the same unit
-        bool ok = true;
-#pragma unroll 1
-        for (int u = 0; u < kSub; u++) {
-            if (UPS == 1 && u >= nsub) break;
-            if (UPS == 2 || u == 0) {
-                ok = mbar_wait(wfull + wslot, wphase, abort_flag) && ok;
-                const unsigned char* wrow = wrow0 + wslot * kWUnitBytes;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((c ^ wsw) << 4));
-                    uint32_t* d = UPS == 2 ? w + (4 * c) % WPS : (c < 2 ? w + 4 * c : wn + 4 * (c - 2));
-                    d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
-                }
-                // The reads above are generic-proxy accesses, the refill is an async-proxy write: the proxy
-                // fence orders the two (without it a read still in the load pipe could see the next unit).
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if ((r & 31) == 0) mbar_arrive(wempty + wslot);
-                if (++wslot == p.w_slots) { wslot = 0; wphase ^= 1; }
-                if (UPS == 1 && more) fetch_sb();
-            }
-            if (u >= nsub) break;  // (the odd sub-block's partner at 8 bit: nothing in it)
-            if (u == 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
-                phase ^= 1;
-                tc_fence_after();
-                if (!ok) break;
-            }
-            // the two 32-weight halves of the sub-block: in one group, or (groups of 32) in one each
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t sv = (h ? s_lo >> half_shift : s_lo) & 0xFFFFu, bv = (h ? b_lo >> half_shift : b_lo) & 0xFFFFu;
-                uint32_t out[16];
-                if (scale_fast_ok(sv)) dequant_32<BITS, true>(w + h * (WPS / 2), sv, bv, out);
-                else dequant_32<BITS, false>(w + h * (WPS / 2), sv, bv, out);  // whole-block branch: not if-converted
-                __syncwarp();
-                tmem_st16(a_tmem + u * kAColsPerSub + h * 16, out);
-            }
-            if (UPS == 1) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = wn[i];
-            }
-            s_lo = half_shift ? s_hi : s_lo >> sub_shift;
-            b_lo = half_shift ? b_hi : b_lo >> sub_shift;
-        }
-        ok = __all_sync(0xFFFFFFFFu, ok);  // (8 bit: the second unit's wait)
-        if (!ok) {
-            *abort_flag = 1;
-            break;
-        }
-        tmem_st_wait();  // once per stage: both sub-blocks are in tensor memory
-        tc_fence_before();
-        __syncwarp();
-        if ((r & 31) == 0) arrive();
-    }
-}
-
-template <int BITS>
+template <int BITS, bool EPI>
 __global__ void __launch_bounds__(kNumThreads, 1)
 qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
               const __grid_constant__ GemmParams p) {
@@ -589,7 +228,8 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
         // ---------------- TMA producer: packed weights ----------------
         SegIter seg;
         seg.init(total_units, nst);
-        if (lane == 0) weight_producer<BITS>(p, &tmap_w, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, [&](int tile) { return (tile / p.m_tiles) * kTileN; });
+        if (lane == 0) weight_producer<BITS>(p, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, [&](const auto& s) { return make_int2((s.tile() / p.m_tiles) * kTileN, 0); },
+                                              [&](void* dst, int x, int2 at, uint64_t* bar) { tma_load_2d(dst, &tmap_w, x, at.x, bar); });
     } else if (warp >= kEpiWarps) {
         // ---------------- dequantisers ----------------
         const int q = warp & 3, grp = (warp - kEpiWarps) >> 2;
@@ -598,7 +238,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](int tile) { return (tile / p.m_tiles) * kTileN; }, [&]() { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -722,6 +362,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                         uint32_t v[16];
                         __syncwarp();
                         tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
+                        if constexpr (EPI) finish<16>(p, v, m0 + c0, m_end - c0, n);
                         store_rows(v, c0, 16);
                     }
                 } else if (parts == 0) {
@@ -729,6 +370,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                         uint32_t v[32];
                         __syncwarp();
                         tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + blk * 32, v);
+                        if constexpr (EPI) finish<32>(p, v, m0 + blk * 32, m_end - blk * 32, n);
                         store_rows(v, blk * 32, 32);
                     }
                 } else {
@@ -751,6 +393,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                                 for (int j = 0; j < 16; j++) pv[j] = __ldcg(ws + (size_t)j * kTileN);
                             }
                         }
+                        if constexpr (EPI) finish<16>(p, v, m0 + c0, m_end - c0, n);
                         store_rows(v, c0, 16);
                     }
                 }
@@ -779,7 +422,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
 // body for both schedules ran this one 5 % slower, and so did every addition tried here -- 16-byte stores through
 // shared memory in the epilogue, the look-ahead of the MMA issuer: the launch is sensitive to the amount of code
 // its roles execute side by side.)
-template <int BITS>
+template <int BITS, bool EPI>
 __global__ void __launch_bounds__(kNumThreads, 1)
 qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
               const __grid_constant__ GemmParams p) {
@@ -873,7 +516,8 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
     } else if (warp == kWWarp) {
         // ---------------- TMA producer: packed weights ----------------
         const TileIter seg{(int)blockIdx.x, (int)gridDim.x, total_tiles, nst};
-        if (lane == 0) weight_producer<BITS>(p, &tmap_w, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, [&](int tile) { return (tile / p.m_tiles) * kTileN; });
+        if (lane == 0) weight_producer<BITS>(p, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, [&](const auto& s) { return make_int2((s.tile() / p.m_tiles) * kTileN, 0); },
+                                              [&](void* dst, int x, int2 at, uint64_t* bar) { tma_load_2d(dst, &tmap_w, x, at.x, bar); });
     } else if (warp >= kEpiWarps) {
         // ---------------- dequantisers ----------------
         const int q = warp & 3, grp = (warp - kEpiWarps) >> 2;
@@ -881,7 +525,7 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](int tile) { return (tile / p.m_tiles) * kTileN; }, [&]() { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -899,6 +543,7 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
+                if constexpr (EPI) finish<32>(p, v, m0 + c0, m_end - c0, n);
                 if (n < p.N) {
                     // column-sharded layers: the tile goes into every rank's copy of y (peer stores over NVLink)
                     const size_t idx0 = (size_t)(m0 + c0) * p.ld + p.col0 + n;
@@ -992,7 +637,7 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
         ::"r"(s32(dst)), "l"(map), "r"(x), "r"(y), "r"(s32(bar) & kPeerBitMask) : "memory");
 }
 
-template <int BITS>
+template <int BITS, bool EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                    const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ GemmParams p) {
@@ -1099,7 +744,8 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     } else if (warp == kWWarp) {
         // ---------------- TMA producer: packed weights ----------------
         const TileIter seg{cl, ncl, total_tiles, nst};
-        if (lane == 0) weight_producer<BITS>(p, &tmap_w, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, n0_of);
+        if (lane == 0) weight_producer<BITS>(p, seg, nks, sW, sl->wfull, sl->wempty, abort_flag, [&](const auto& s) { return make_int2(n0_of(s.tile()), 0); },
+                                              [&](void* dst, int x, int2 at, uint64_t* bar) { tma_load_2d(dst, &tmap_w, x, at.x, bar); });
     } else if (warp >= kEpiWarps) {
         // ---------------- dequantisers ----------------
         const int q = warp & 3, grp = (warp - kEpiWarps) >> 2;
@@ -1107,7 +753,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           n0_of, [&]() { mbar_arrive_cta0(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min(n0_of(s.tile()) + r, p.N - 1); }, [&]() { mbar_arrive_cta0(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -1131,6 +777,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
+                    if constexpr (EPI) finish<32>(p, v, m0 + c0, min(p.bm, p.M - m0) - c0, n);
                     __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(sY + (size_t)c0 * 256) + q * 32 + lane;
 #pragma unroll
                     for (int j = 0; j < 32; j++) dst[j * 128] = __float2bfloat16_rn(__uint_as_float(v[j]));
@@ -1174,6 +821,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
+                if constexpr (EPI) finish<32>(p, v, m0 + c0, m_end - c0, n);
                 if (n < p.N) {
                     // column-sharded layers: the tile goes into every rank's copy of y (peer stores over NVLink)
                     const size_t idx0 = (size_t)(m0 + c0) * p.ld + p.col0 + n;
@@ -1265,9 +913,9 @@ bool make_gemm_plan(const QmmArgs& a, int sm_count, const ShardPush* push, GemmP
     return choose_gemm_plan(shape, sm_count, force, getenv("LUXCUDA_QMM_NO_YTMA") != nullptr, pl) && encode_tiled_fn() != nullptr;
 }
 
-template <int BITS>
+template <int BITS, bool EPI>
 cudaError_t launch_gemm_pair_t(const CUtensorMap& tmap, const CUtensorMap& tmap_w, const CUtensorMap& tmap_y, const GemmParams& p, const GemmPlan& pl, int sm_count, cudaStream_t stream) {
-    auto kern = qmm_tc_pair_kernel<BITS>;
+    auto kern = qmm_tc_pair_kernel<BITS, EPI>;
     static std::atomic<bool> attr_set[64];
     if (cudaError_t e = allow_smem(kern, kGemmSmemLimit, attr_set)) return e;
     // one pair of CTAs per pair of SMs (the kernel carries its cluster shape), unless there are fewer pair tiles
@@ -1278,9 +926,9 @@ cudaError_t launch_gemm_pair_t(const CUtensorMap& tmap, const CUtensorMap& tmap_
 }
 
 // SK: stream-K, else whole tiles
-template <int BITS, bool SK>
+template <int BITS, bool SK, bool EPI>
 cudaError_t launch_gemm_t(const CUtensorMap& tmap, const CUtensorMap& tmap_w, const GemmParams& p, const GemmPlan& pl, int sm_count, cudaStream_t stream) {
-    auto kern = SK ? qmm_tc_kernel<BITS> : qmm_tc_tiles_kernel<BITS>;
+    auto kern = SK ? qmm_tc_kernel<BITS, EPI> : qmm_tc_tiles_kernel<BITS, EPI>;
     static std::atomic<bool> attr_set[64];
     if (cudaError_t e = allow_smem(kern, kGemmSmemLimit, attr_set)) return e;
     // one CTA per SM, unless the launch has fewer units of work (tiles, or k-stages under stream-K) than that
@@ -1358,6 +1006,7 @@ cudaError_t launch_qmm_tc(const QmmArgs& a, void* workspace, int sm_count, cudaS
         for (int r = 0; r < push->world; r++)
             if (r != push->me) p.y_all[k++] = push->y[r];
     }
+    p.bias = a.bias; p.residual = a.residual; p.act = a.act; p.r_bf16 = a.r_bf16;
     p.bm = pl.bm; p.w_slots = pl.w_slots; p.n_tiles = pl.n_tiles; p.m_tiles = pl.m_tiles;
     p.ws_flags = static_cast<uint32_t*>(workspace);
     p.ws = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kWsFlagBytes);
@@ -1379,17 +1028,19 @@ cudaError_t launch_qmm_tc(const QmmArgs& a, void* workspace, int sm_count, cudaS
             }
         }
         if (name) *name = a.bits == 4 ? "qmm_tc<4,pairs>" : "qmm_tc<8,pairs>";
-        return a.bits == 4 ? launch_gemm_pair_t<4>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream)
-                           : launch_gemm_pair_t<8>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream);
+        if (a.epi)
+            return a.bits == 4 ? launch_gemm_pair_t<4, true>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream)
+                               : launch_gemm_pair_t<8, true>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream);
+        return a.bits == 4 ? launch_gemm_pair_t<4, false>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream)
+                           : launch_gemm_pair_t<8, false>(tmap, tmap_w, tmap_y, p, pl, sm_count, stream);
     }
-    if (a.bits == 4) {
-        if (name) *name = pl.streamk ? "qmm_tc<4,stream-k>" : "qmm_tc<4>";
-        return pl.streamk ? launch_gemm_t<4, true>(tmap, tmap_w, p, pl, sm_count, stream)
-                          : launch_gemm_t<4, false>(tmap, tmap_w, p, pl, sm_count, stream);
+    if (name) *name = a.bits == 4 ? (pl.streamk ? "qmm_tc<4,stream-k>" : "qmm_tc<4>") : (pl.streamk ? "qmm_tc<8,stream-k>" : "qmm_tc<8>");
+    if (a.epi) {
+        if (a.bits == 4) return pl.streamk ? launch_gemm_t<4, true, true>(tmap, tmap_w, p, pl, sm_count, stream) : launch_gemm_t<4, false, true>(tmap, tmap_w, p, pl, sm_count, stream);
+        return pl.streamk ? launch_gemm_t<8, true, true>(tmap, tmap_w, p, pl, sm_count, stream) : launch_gemm_t<8, false, true>(tmap, tmap_w, p, pl, sm_count, stream);
     }
-    if (name) *name = pl.streamk ? "qmm_tc<8,stream-k>" : "qmm_tc<8>";
-    return pl.streamk ? launch_gemm_t<8, true>(tmap, tmap_w, p, pl, sm_count, stream)
-                      : launch_gemm_t<8, false>(tmap, tmap_w, p, pl, sm_count, stream);
+    if (a.bits == 4) return pl.streamk ? launch_gemm_t<4, true, false>(tmap, tmap_w, p, pl, sm_count, stream) : launch_gemm_t<4, false, false>(tmap, tmap_w, p, pl, sm_count, stream);
+    return pl.streamk ? launch_gemm_t<8, true, false>(tmap, tmap_w, p, pl, sm_count, stream) : launch_gemm_t<8, false, false>(tmap, tmap_w, p, pl, sm_count, stream);
 }
 
 // Device-side address of the host-visible error word (the same on every GPU: portable mapped memory).

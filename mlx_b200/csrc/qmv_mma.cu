@@ -1077,6 +1077,7 @@ static cudaError_t launch_split(const QmmArgs& a, const Plan& pl, void* workspac
          : a.pro == 2 ? launch_t<8, 1, 2>(p, pl, stream, overlap_prev) : launch_t<8, 1, 0>(p, pl, stream, overlap_prev);
 }
 
+const char* qmv_stream_name(const QmmArgs& a) { return stream_name(a.bits, a.M, a.pro); }
 cudaError_t launch_decode(const QmmArgs& a, const DecodePlan& pl, void* workspace, cudaStream_t stream, const char** name,
                           bool overlap_prev, bool x_stable) {
     if (pl.split) return launch_split(a, pl.s, workspace, stream, name, overlap_prev, nullptr, x_stable);

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "epilogue.cuh"
+#include "groups.cuh"
 #include "internal.h"
 #include "qmv_frag.cuh"
 
@@ -158,13 +159,13 @@ constexpr int kGroups = -1;
 template <>
 struct GroupParams<kGroups> {
     const int *offsets, *order;
-    int experts, rows, x_rows, n_rt, tables_off;  // row tiles of an expert; offset of the tables in shared memory
+    int experts, rows, x_rows, n_rt, most, tables_off;  // row tiles of an expert; items, at most; offset of the tables in shared memory
     uint32_t top_k;
 };
 // NI: how many matmuls of a batch, at most; 1: one; 0: one whose rows of x are n_items items of 16 (M: all of them); kGroups: experts.
 template <int NI, int EPI>
 struct Params : EpiParams<EPI>, GroupParams<NI> {
-    static constexpr bool kRows = NI == 0, kExperts = NI == kGroups;
+    static constexpr bool kRows = NI == 0;
     static constexpr int kArray = NI > 0 ? NI : 1;
     alignas(64) CUtensorMap maps[kArray];  // the packed weights
     Item items[kArray];
@@ -291,31 +292,6 @@ struct GroupWalk {
     template <class P>
     __device__ __forceinline__ int kb_cnt(const P& p) const { return min(p.kbc, p.nkb - c * p.kbc); }
 };
-// Whole block: the tables of GroupWalk from the offsets.
-template <int ROWS, class P>
-__device__ __forceinline__ void group_tables(const P& p, unsigned char* smem) {
-    int* off = reinterpret_cast<int*>(smem + p.tables_off);
-    int* first = off + p.experts + 1;
-    for (int e = threadIdx.x; e <= p.experts; e += kThreads) off[e] = min(max(__ldcg(p.offsets + e), 0), p.rows);
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int before = 0;
-        for (int e0 = 0; e0 < p.experts; e0 += 32) {
-            const int e = e0 + (int)threadIdx.x, n = e < p.experts ? (max(off[e + 1] - off[e], 0) + ROWS - 1) / ROWS : 0;
-            int sum = n;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, sum, d);
-                if ((int)threadIdx.x >= d) sum += v;
-            }
-            if (e < p.experts) first[e] = before + sum - n;
-            before += __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (threadIdx.x == 0) first[p.experts] = before;
-    }
-    __syncthreads();
-}
-
 // SPL: scales per lane and row of a task (2 for 4-bit weights in groups of 32).  PRO: what x is (0: as it lies; 1: the
 // rms-norm of its rows, for K within one chunk; 2: the sum of three column blocks; 1 and 2 for M <= 8).  EPI: 0 none; 1 bias,
 // activation, residual; 2 gated (experts).
@@ -348,7 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
         // (which weights are wanted is the previous kernel's answer: there is nothing to fetch ahead of it)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        group_tables<8 * MT>(p, smem);
+        int* const off = reinterpret_cast<int*>(smem + p.tables_off);
+        group_tables(off, off + p.experts + 1, p.offsets, p.experts, p.rows, p.most, [](int n) { return (n + 8 * MT - 1) / (8 * MT); });
         if (!wk.init(p)) return;
     } else {
         wk.init(p);
@@ -910,7 +887,7 @@ cudaError_t launch_experts(const ExpertsArgs& a, const Plan& pl, const CUtensorM
     p.act = a.act;
     p.r_bf16 = 0;
     p.offsets = a.offsets; p.order = a.order; p.experts = a.experts; p.rows = (int)a.rows; p.x_rows = (int)a.x_rows;
-    p.n_rt = pl.n_rt; p.tables_off = (int)pl.smem - 8 * (a.experts + 1); p.top_k = a.order ? a.top_k : 1;
+    p.n_rt = pl.n_rt; p.most = (int)(a.rows / group_rows(a)) + a.experts; p.tables_off = (int)pl.smem - 8 * (a.experts + 1); p.top_k = a.order ? a.top_k : 1;
     return launch_bits<kGroups, EPI>(p, pl, a.bits, a.group, group_rows(a), 0, stream, overlap_prev);
 }
 

@@ -141,15 +141,26 @@ LuxBackendError ensure_qmm_workspace(Context* c) {
 // has no place for an epilogue).
 LuxBackendError qmatmul_epi_on_stream(Context* c, const QmmArgs& a) {
     const char* name = "";
-    QmvStreamPlan pl;
-    if (!plan_qmv_stream(a, c->dev->sm_count, &pl)) {
-        set_last_error("qmatmul_epi: M=%d K=%d N=%d in groups of %d is past the kernels' 32-bit index ranges", a.M, a.K, a.N, a.group);
-        return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    cudaError_t e;
+    if (a.M > 16 && qmm_tc_supported(a, c->dev->sm_count)) {
+        LuxBackendError le = ensure_qmm_workspace(c);
+        if (le != LUX_BACKEND_OK) return le;
+        e = launch_qmm_tc(a, c->qmm_ws->ptr, c->dev->sm_count, c->stream, &name);
+        if (e == cudaSuccess) c->launches++;
+    } else {
+        QmvStreamPlan pl;
+        if (!plan_qmv_stream(a, c->dev->sm_count, &pl)) {
+            set_last_error("qmatmul_epi: M=%d K=%d N=%d in groups of %d is past the kernels' 32-bit index ranges", a.M, a.K, a.N, a.group);
+            return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+        }
+        name = qmv_stream_name(a);
+        e = launch_qmv_stream(a, pl, c->stream, decode_may_overlap(c, a), decode_x_stable(c, a));
+        if (e == cudaSuccess) {
+            c->launches++;
+            note_decode_launch(c, a);
+        }
     }
-    const cudaError_t e = launch_qmv_stream(a, pl, c->stream, decode_may_overlap(c, a), decode_x_stable(c, a));
-    if (e != cudaSuccess) return map_cuda_error(e, "qmatmul_epi");
-    c->launches++;
-    note_decode_launch(c, a);
+    if (e != cudaSuccess) return map_cuda_error(e, name);
     c->last_kernel = name;
     return LUX_BACKEND_OK;
 }

@@ -78,7 +78,7 @@ def test_in_place(ctx, oracle, M, dtype, N):
     np.testing.assert_array_equal(run(ctx, oracle, M, 1024, N, 4, 64, act=P.ACT_GELU, res=dtype, y_dtype=dtype, in_place=True), apart)
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 1024, 300), (16, 4096, 512), (33, 96, 50)])
+@pytest.mark.parametrize("M,K,N", [(1, 1024, 300), (16, 4096, 512), (64, 1024, 512), (600, 1024, 4096), (33, 96, 50)])
 def test_nothing_but_the_product(ctx, oracle, M, K, N):
     """Without bias, activation and residual: the bits of qmatmul (the shapes are none whose K qmatmul splits over CTAs)."""
     wq, s, b = oracle.make_layer(N, K, 4, 32, oracle.BF16, config_id=42)
