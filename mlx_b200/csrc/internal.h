@@ -116,6 +116,8 @@ struct Context {
     // using the block they were recorded with.
     std::vector<Block*> qmv_ws_retired;
     Block* moe_ws = nullptr;  // counts of moe_route's blocks, made on first use
+    Block* gather_ws = nullptr;  // rows of x that qmatmul_experts puts side by side, grown on demand
+    std::vector<Block*> gather_ws_retired;  // (as qmv_ws_retired)
     // scratch of the prefill GEMM (partial accumulators of tiles shared between CTAs + their flags)
     Block* qmm_ws = nullptr;
     // A kernel that gives up on a bounded wait says so here (page-locked host memory mapped into the device's
@@ -379,8 +381,8 @@ struct MoeRouteArgs {
     bool logits_bf16;
     float scale;
 };
-int moe_route_blocks(const MoeRouteArgs& a, int sm_count);  // more than one: the workspace is needed
-size_t moe_route_workspace_bytes(int sm_count);
+int moe_route_blocks(const MoeRouteArgs& a);  // more than one: the workspace is needed
+size_t moe_route_workspace_bytes();
 cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, int* launches);
 struct MoeCombineArgs {
     const void* y;
@@ -410,7 +412,8 @@ struct ExpertsArgs {
 bool qmv_experts_supported(const ExpertsArgs& a, int sm_count);
 cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
 bool qmm_experts_supported(const ExpertsArgs& a);
-cudaError_t launch_qmm_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
+size_t qmm_experts_workspace_bytes(const ExpertsArgs& a);  // rows of x side by side, where there is an order: a launch more
+cudaError_t launch_qmm_experts(const ExpertsArgs& a, void* workspace, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name);
 cudaError_t launch_gather_columns(const void* staging, void* y_full, int world, int M, int n_local, int elem_size,
                                   cudaStream_t stream);
 cudaError_t launch_flush(void* buf, size_t bytes, cudaStream_t stream);

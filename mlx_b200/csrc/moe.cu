@@ -6,13 +6,15 @@
 // the order of the pairs: a block ranks its own pairs (ballots of equal experts within 32 pairs, counts per warp and expert in shared memory),
 // and adds where its share of each expert begins.
 //   * Few tokens: one block does it all, one launch.
-//   * More: up to one block per SM, each with a run of neighbouring tokens; it leaves its counts per expert in a workspace, and a second
-//     launch, every block for itself, adds up the counts of the blocks before it.  (No atomics: their order would change nothing here, but
-//     a pair's rank must not depend on it.)
-// Bytes: tokens * experts logits once, 16 bytes a pair out.  Few tokens are bound by the latency of a launch and of top_k dependent
-// reductions.
+//   * More: a block takes as many neighbouring tokens as it has warps (more where that would be over kMaxBlocks blocks) and leaves its counts per
+//     expert in a workspace; a second launch adds them up along the blocks, for 32 experts a block; a third puts the pairs in their places.  Up to
+//     kFewBlocks blocks the last two are one launch, whose blocks each add up for themselves.  No atomics: a pair's rank must not depend
+//     on who comes first.
+// Bytes: tokens * experts logits once, 16 bytes a pair out.  Bound by the instructions of the choice (about a thousand a token at 256 experts, best
+// 8; 60 % of the issue slots): 8192 tokens 20.5 us, with sigmoid and bias 22.7.  Few tokens: by the latency of a launch, 4 us.
 //
-// moe_combine.  HBM-bound: a thread takes 8 neighbouring columns of a token, with the loads of up to 8 slots under way.
+// moe_combine.  HBM-bound: a thread takes 8 neighbouring columns of a token, with the loads of up to 8 slots under way (4096 tokens x 8 x 4096,
+// fp32 stream: 65 us, 6.0 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -43,6 +45,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f), k = b & 0x80000000u ? ~b : b | 0x80000000u;
     return v > -INFINITY ? k : 0u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 __device__ __forceinline__ unsigned long long order_key(double v) {
     const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0), top = 1ull << 63;
     return v > -(double)INFINITY ? (b & top ? ~b : b | top) : 0ull;
@@ -60,53 +63,122 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The experts of one token (whole warp): lane j < top_k gets slot j's expert (-1: none) and weight.  VPT: logits per lane.  WIDE: keys are the
-// fp64 sums of sigmoid and bias; in fp32 two experts next to a border could change places with the rounding of the exponential.
+// One round of a choice (whole warp): the expert with the largest key, the lowest of equals, is taken out of the lanes' keys; key i of a lane is
+// expert lane + 32 i's.  -1: all keys are 0.
+template <int VPT, class Key>
+__device__ __forceinline__ int take_best(Key (&key)[VPT], int lane) {
+    Key best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+        if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+    const Key top = warp_max(best);
+    if (!top) return -1;
+    const int e = (int)__reduce_min_sync(kFull, best == top ? (uint32_t)at : 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+        if (lane + 32 * i == e) key[i] = 0;
+    return e;
+}
+__device__ __forceinline__ double wide_score(float v, float bias) { return 1.0 / (1.0 + exp(-(double)v)) + (double)bias; }
+
+// The experts of one token (whole warp).  A lane gets an expert, its slot (-1: none of the top_k) and weight.  VPT: logits per lane.
+//
+// A threshold first: the top_k-th largest of the lanes' largest keys.  The chosen are among the experts that reach it, mostly two or three more
+// than top_k of them; they are gathered, one a lane, in the order of their numbers, and each counts those ahead of it.  Where more reach
+// it than a warp has lanes: top_k rounds over all keys.  (Always the rounds: 8192 tokens x 256 experts, best 8: 19 us of a launch.)
+//
+// WIDE: by sigmoid + bias in fp64; in fp32 two experts next to a border could change places with the rounding of the exponential.  The fp32 keys
+// are off by less than 1e-6 (1 + |key|) (the machine's exponential: |v| / 4 + 1/2 U of e^-v's share of at most 1/4, U each from quotient and sums),
+// so the chosen are among those that come within twice that of the threshold; only these are looked at in fp64.
 template <int VPT, bool BF16, bool WIDE>
-__device__ __forceinline__ void choose(const MoeRouteArgs& a, size_t token, int lane, int* id, float* weight) {
-    using Key = std::conditional_t<WIDE, unsigned long long, uint32_t>;
+__device__ __forceinline__ void choose(const MoeRouteArgs& a, size_t token, int lane, uint32_t* room, int* id, int* slot, float* weight) {
     const size_t row = token * a.ld;
-    Key key[VPT];
+    uint32_t key[VPT], best = 0;
     float mine[WIDE ? 1 : VPT];
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int e = lane + 32 * i;
-        float v = e < a.experts ? load_logit<BF16>(a.logits, row + e) : -INFINITY;
+        const float v = e < a.experts ? load_logit<BF16>(a.logits, row + e) : -INFINITY;
+        key[i] = order_key(v);
         if constexpr (WIDE) {
-            key[i] = 0;
-            if (v > -INFINITY) key[i] = order_key(1.0 / (1.0 + exp(-(double)v)) + (double)a.bias[e]);
+            if (key[i]) key[i] = order_key(__fdividef(1.0f, 1.0f + __expf(-v)) + a.bias[e]);
         } else {
             mine[i] = v;
-            key[i] = order_key(v);
         }
+        best = max(best, key[i]);
     }
+    uint32_t least = best;
+    for (int j = 1; j < a.top_k; j++) {  // (one lane out per round, of equals the lowest)
+        const uint32_t top = __reduce_max_sync(kFull, least);
+        if (!top) break;
+        if (lane == __ffs(__ballot_sync(kFull, least == top)) - 1) least = 0;
+    }
+    least = max(__reduce_max_sync(kFull, least), 1u);
+    if (WIDE && least > 1) {
+        const float t = key_value(least);
+        least = max(order_key(t - 2e-6f * (1.0f + fabsf(t))), 1u);
+    }
+    int n = 0;  // experts that reach it
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const unsigned there = __ballot_sync(kFull, key[i] >= least);
+        const int at = n + __popc(there & ((1u << lane) - 1));
+        if (key[i] >= least && at < 32) {
+            room[at] = key[i];
+            room[32 + at] = lane + 32 * i;
+        }
+        n += __popc(there);
+    }
+    __syncwarp();
     *id = -1;
-    for (int j = 0; j < a.top_k; j++) {
-        Key best = 0;
-        int at = 0;
+    if (n <= 32) {
+        if (lane < n) *id = (int)room[32 + lane];
+        int ahead = 0;
+        if constexpr (WIDE) {
+            const unsigned long long w = *id >= 0 ? order_key(wide_score(load_logit<BF16>(a.logits, row + *id), a.bias[*id])) : 0ull;
+            for (int j = 0; j < n; j++) {
+                const unsigned long long other = __shfl_sync(kFull, w, j);
+                ahead += other > w || (other == w && j < lane);
+            }
+            if (!w) ahead = 32;
+        } else {
+            const uint32_t w = lane < n ? room[lane] : 0u;
+            for (int j = 0; j < n; j++) {
+                const uint32_t other = __shfl_sync(kFull, w, j);
+                ahead += other > w || (other == w && j < lane);
+            }
+        }
+        *slot = *id >= 0 && ahead < a.top_k ? ahead : -1;
+    } else {
+        using Key = std::conditional_t<WIDE, unsigned long long, uint32_t>;
+        Key all[VPT];
 #pragma unroll
-        for (int i = 0; i < VPT; i++)
-            if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
-        const Key top = warp_max(best);
-        if (!top) break;  // (the same for the whole warp)
-        const int e = (int)__reduce_min_sync(kFull, best == top ? (uint32_t)at : 0x7fffffffu);
-        if (lane == j) *id = e;
-#pragma unroll
-        for (int i = 0; i < VPT; i++)
-            if (lane + 32 * i == e) key[i] = 0;
+        for (int i = 0; i < VPT; i++) {
+            if constexpr (WIDE) all[i] = key[i] >= least ? order_key(wide_score(load_logit<BF16>(a.logits, row + lane + 32 * i), a.bias[lane + 32 * i])) : 0ull;
+            else all[i] = key[i];
+        }
+        for (int j = 0; j < a.top_k; j++) {
+            const int e = take_best<VPT>(all, lane);
+            if (e < 0) break;
+            if (lane == j) *id = e;
+        }
+        *slot = *id >= 0 ? lane : -1;
     }
-    const bool got = *id >= 0;
+    __syncwarp();  // (room has been read)
+    const bool got = *slot >= 0;
     const float v = got ? load_logit<BF16>(a.logits, row + *id) : 0.0f;
     float w = 0.0f, total = 1.0f;
     if (a.score == LUX_CUDA_SCORE_SIGMOID) {
         w = got ? 1.0f / (1.0f + expf(-v)) : 0.0f;
         if (a.renorm) total = warp_sum(w);
     } else {
-        const float top = __shfl_sync(kFull, v, 0);  // slot 0 has the largest (or there is none at all)
+        const unsigned first = __ballot_sync(kFull, *slot == 0);  // slot 0 has the largest (or there is none at all)
+        const float top = __shfl_sync(kFull, v, first ? __ffs(first) - 1 : 0);
         w = got ? (v == top ? 1.0f : expf(v - top)) : 0.0f;
         if (a.renorm) {
             total = warp_sum(w);
-        } else if constexpr (!WIDE) {
+        } else if constexpr (!WIDE) {  // (a bias goes with sigmoids only)
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < VPT; i++) s += !(mine[i] > -INFINITY) ? 0.0f : mine[i] == top ? 1.0f : expf(mine[i] - top);
@@ -145,39 +217,45 @@ __device__ __forceinline__ void scan_experts(const int* n, int* base, int expert
 // cnt[warp][e] (the warps before, 16 bits: a round has fewer pairs) + its rank within the warp's run of pairs.
 template <int VPT, bool BF16, bool WIDE, int THREADS>
 __global__ void __launch_bounds__(THREADS) moe_route_kernel(const MoeRouteArgs a, int chunk, bool one) {
-    constexpr int W = THREADS / 32;
     extern __shared__ int smem[];
-    const int E = a.experts, k = a.top_k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int E = a.experts, k = a.top_k, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, W = threads >> 5;
     int* start = smem;              // [E + 1]
     int* s_id = start + E + 1;      // [kRoundPairs]
     int* s_rank = s_id + kRoundPairs;
     uint16_t* cnt = reinterpret_cast<uint16_t*>(s_rank + kRoundPairs);  // [W + 1][E]; the last row: the round's counts
-    for (int e = threadIdx.x; e <= E; e += THREADS) start[e] = 0;
+    for (int e = threadIdx.x; e <= E; e += threads) start[e] = 0;
     wait_previous();
     const size_t t_lo = (size_t)blockIdx.x * chunk, t_hi = min(t_lo + (size_t)chunk, a.tokens);
     const int per_round = min(chunk, kRoundPairs / k);
     for (size_t t0 = t_lo; t0 < t_hi; t0 += per_round) {
         const int tokens = (int)min((size_t)per_round, t_hi - t0), pairs = tokens * k;
-        for (int i = threadIdx.x; i < W * E; i += THREADS) cnt[i] = 0;
+        const int seg = (pairs + W * 32 - 1) / (W * 32) * 32, used = (pairs + seg - 1) / seg;  // pairs a warp ranks; warps that have any
+        for (int i = threadIdx.x; i < used * E; i += threads) cnt[i] = 0;
         if constexpr (VPT == 0) {
-            for (int i = threadIdx.x; i < pairs; i += THREADS) {
+            for (int i = threadIdx.x; i < pairs; i += threads) {
                 const int e = a.ids[t0 * k + i];
                 s_id[i] = e >= 0 && e < E ? e : -1;
             }
         } else {
             for (int t = warp; t < tokens; t += W) {
-                int id;
+                int id, slot;
                 float w;
-                choose<VPT, BF16, WIDE>(a, t0 + t, lane, &id, &w);
-                if (lane < k) {
-                    s_id[t * k + lane] = id;
-                    a.ids[(t0 + t) * k + lane] = id;
-                    a.weights[(t0 + t) * k + lane] = w;
+                choose<VPT, BF16, WIDE>(a, t0 + t, lane, reinterpret_cast<uint32_t*>(s_rank) + warp * 64, &id, &slot, &w);
+                const int n = __popc(__ballot_sync(kFull, slot >= 0));  // slots 0 .. n-1
+                if (slot >= 0) {
+                    s_id[t * k + slot] = id;
+                    a.ids[(t0 + t) * k + slot] = id;
+                    a.weights[(t0 + t) * k + slot] = w;
+                }
+                if (lane >= n && lane < k) {  // slots without an expert
+                    s_id[t * k + lane] = -1;
+                    a.ids[(t0 + t) * k + lane] = -1;
+                    a.weights[(t0 + t) * k + lane] = 0.0f;
                 }
             }
         }
         __syncthreads();
-        const int seg = (pairs + W * 32 - 1) / (W * 32) * 32, lo = min(warp * seg, pairs), hi = min(lo + seg, pairs);
+        const int lo = min(warp * seg, pairs), hi = min(lo + seg, pairs);
         for (int i0 = lo; i0 < hi; i0 += 32) {
             const int i = i0 + lane, e = i < hi ? s_id[i] : -1;
             const unsigned same = __match_any_sync(kFull, e);
@@ -191,15 +269,20 @@ __global__ void __launch_bounds__(THREADS) moe_route_kernel(const MoeRouteArgs a
             __syncwarp();
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < E; e += THREADS) {
+        for (int e = threadIdx.x; e < E; e += threads) {
             int s = 0;
-            for (int w = 0; w < W; w++) {
-                const int c = cnt[w * E + e];
-                cnt[w * E + e] = (uint16_t)s;
-                s += c;
+            for (int w0 = 0; w0 < used; w0 += 8) {
+                int c[8];
+#pragma unroll
+                for (int w = 0; w < 8; w++) c[w] = w0 + w < used ? cnt[(w0 + w) * E + e] : 0;
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    if (w0 + w < used) cnt[(w0 + w) * E + e] = (uint16_t)s;
+                    s += c[w];
+                }
             }
-            cnt[W * E + e] = (uint16_t)s;
             if (one) start[e] = s;
+            else cnt[W * E + e] = (uint16_t)s;
         }
         if (one) scan_experts(start, start, E);  // (one round: the counts are the whole)
         else __syncthreads();
@@ -208,23 +291,69 @@ __global__ void __launch_bounds__(THREADS) moe_route_kernel(const MoeRouteArgs a
             a.pos[t0 * k + i] = at;
             if (one && e >= 0) a.order[at] = i;
         }
-        __syncthreads();
-        if (!one)
-            for (int e = threadIdx.x; e < E; e += THREADS) start[e] += cnt[W * E + e];
-        __syncthreads();
+        if (!one) {
+            __syncthreads();
+            for (int e = threadIdx.x; e < E; e += threads) start[e] += cnt[W * E + e];
+            __syncthreads();
+        }
     }
     if (one)
-        for (int e = threadIdx.x; e <= E; e += THREADS) a.offsets[e] = start[e];
+        for (int e = threadIdx.x; e <= E; e += threads) a.offsets[e] = start[e];
     else
-        for (int e = threadIdx.x; e < E; e += THREADS) a.hist[(size_t)blockIdx.x * E + e] = start[e];
+        for (int e = threadIdx.x; e < E; e += threads) a.hist[(size_t)blockIdx.x * E + e] = start[e];
 }
 
-// The second launch: where each block's share of an expert begins, then the places.  Shared memory: two counts per expert and part of
-// the blocks.
-constexpr int kPlaceThreads = 1024;
-__global__ void __launch_bounds__(kPlaceThreads) moe_place_kernel(const MoeRouteArgs a, int chunk) {
+// The second launch: 32 experts a block, warp w a run of the B blocks' counts.  Behind it hist[b][e] is the sum of the blocks before b, hist[B][e] that of
+// all.
+constexpr int kMaxBlocks = 296;  // two of 1024 threads on each of 148 SMs
+__global__ void __launch_bounds__(1024) moe_count_kernel(int* hist, int E, int B) {
+    __shared__ int part[32][33];
+    wait_previous();
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    const int lo = w * B / 32, hi = (w + 1) * B / 32;
+    int c[(kMaxBlocks + 31) / 32], sum = 0;
+#pragma unroll
+    for (int i = 0; i < (kMaxBlocks + 31) / 32; i++) c[i] = e < E && lo + i < hi ? __ldcg(hist + (size_t)(lo + i) * E + e) : 0;
+#pragma unroll
+    for (int i = 0; i < (kMaxBlocks + 31) / 32; i++) sum += c[i];
+    part[w][lane] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int i = 0; i < w; i++) before += part[i][lane];
+    if (e >= E) return;
+#pragma unroll
+    for (int i = 0; i < (kMaxBlocks + 31) / 32; i++)
+        if (lo + i < hi) {
+            hist[(size_t)(lo + i) * E + e] = before;
+            before += c[i];
+        }
+    if (w == 31) hist[(size_t)B * E + e] = before;
+}
+
+// The last: the places.
+constexpr int kPlaceThreads = 512;
+__global__ void __launch_bounds__(kPlaceThreads) moe_place_kernel(const MoeRouteArgs a, int chunk, int B) {
+    extern __shared__ int all[];  // [E + 1]
+    const int E = a.experts;
+    wait_previous();
+    for (int e = threadIdx.x; e < E; e += kPlaceThreads) all[e] = __ldcg(a.hist + (size_t)B * E + e);
+    scan_experts(all, all, E);
+    const uint32_t per = (uint32_t)chunk * a.top_k, pairs = (uint32_t)a.tokens * a.top_k;  // (below 2^31)
+    for (uint32_t p = blockIdx.x * kPlaceThreads + threadIdx.x; p < pairs; p += gridDim.x * kPlaceThreads) {
+        const int rank = a.pos[p];
+        if (rank < 0) continue;
+        const int id = a.ids[p], at = all[id] + __ldcg(a.hist + (size_t)(p / per) * E + id) + rank;
+        a.pos[p] = at;
+        a.order[at] = (int)p;
+    }
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= E; i += kPlaceThreads) a.offsets[i] = all[i];
+}
+// Few blocks: every block adds up the counts itself, for its own pairs.  One launch less.
+constexpr int kFewBlocks = 64, kCountThreads = 1024;
+__global__ void __launch_bounds__(kCountThreads) moe_count_place_kernel(const MoeRouteArgs a, int chunk) {
     extern __shared__ int smem[];
-    const int E = a.experts, B = gridDim.x, EP = (E + 31) & ~31, parts = kPlaceThreads / EP;  // (EP <= 1024)
+    const int E = a.experts, B = gridDim.x, EP = (E + 31) & ~31, parts = kCountThreads / EP;  // (EP <= 1024)
     int* all = smem;                    // [E + 1]
     int* mine = all + E + 1;            // [E]: of the blocks before this one
     int* part = mine + E;               // [2][parts][E]
@@ -255,7 +384,7 @@ __global__ void __launch_bounds__(kPlaceThreads) moe_place_kernel(const MoeRoute
     }
     scan_experts(all, all, E);
     const size_t k = a.top_k, lo = (size_t)blockIdx.x * chunk * k, hi = min(lo + (size_t)chunk * k, a.tokens * k);
-    for (size_t p = lo + threadIdx.x; p < hi; p += kPlaceThreads) {
+    for (size_t p = lo + threadIdx.x; p < hi; p += kCountThreads) {
         const int rank = a.pos[p];
         if (rank < 0) continue;
         const int id = a.ids[p], at = all[id] + mine[id] + rank;
@@ -263,7 +392,7 @@ __global__ void __launch_bounds__(kPlaceThreads) moe_place_kernel(const MoeRoute
         a.order[at] = (int)p;
     }
     if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= E; i += kPlaceThreads) a.offsets[i] = all[i];
+        for (int i = threadIdx.x; i <= E; i += kCountThreads) a.offsets[i] = all[i];
 }
 
 // ---- the weighted sum -------------------------------------------------------------------------------------------------
@@ -361,14 +490,17 @@ cudaLaunchConfig_t config(unsigned grid, unsigned threads, size_t smem, cudaStre
 
 constexpr size_t route_smem(int experts, int warps) { return ((size_t)experts + 1 + 2 * kRoundPairs) * 4 + ((size_t)warps + 1) * experts * 2; }
 
+constexpr int route_warps(int experts) { return experts > 256 ? 16 : 32; }  // of a block (registers for up to 32 logits a lane)
 template <int VPT, bool BF16, bool WIDE>
 cudaError_t launch_route_t(const MoeRouteArgs& a, int blocks, int chunk, cudaStream_t stream, bool overlap_prev) {
-    constexpr int THREADS = VPT > 8 || WIDE ? 512 : 1024;  // (registers for up to 32 logits a lane)
+    constexpr int THREADS = 32 * route_warps(VPT * 32);
     auto kern = moe_route_kernel<VPT, BF16, WIDE, THREADS>;
     static std::atomic<bool> attr_set[64];
-    if (cudaError_t e = allow_smem(kern, (int)route_smem(LUX_CUDA_MAX_EXPERTS, THREADS / 32), attr_set)) return e;
+    if (cudaError_t e = allow_smem(kern, (int)route_smem(LUX_CUDA_MAX_EXPERTS, 32), attr_set)) return e;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = config(blocks, THREADS, route_smem(a.experts, THREADS / 32), stream, overlap_prev, &attr);
+    // few tokens: few warps, whose barriers and prefix sums are short (one token, 64 experts: 5.0 us with 32)
+    const int threads = blocks > 1 ? THREADS : std::min(THREADS, 32 * std::max(4, chunk));
+    const cudaLaunchConfig_t cfg = config(blocks, threads, route_smem(a.experts, threads / 32), stream, overlap_prev, &attr);
     return cudaLaunchKernelEx(&cfg, kern, a, chunk, blocks == 1);
 }
 template <int VPT>
@@ -379,17 +511,16 @@ cudaError_t launch_route_v(const MoeRouteArgs& a, int blocks, int chunk, cudaStr
 
 }  // namespace
 
-// One block: as long as its warps have no more than two tokens each and the pairs fit a round.
-int moe_route_blocks(const MoeRouteArgs& a, int sm_count) {
-    if (a.tokens <= 64 && a.tokens * a.top_k <= (size_t)kRoundPairs) return 1;
-    const size_t per = std::max<size_t>(16, (a.tokens + sm_count - 1) / sm_count);
-    const size_t blocks = (a.tokens + per - 1) / per;
-    return (int)std::max<size_t>(blocks, 2);
+// One block: as long as its warps have no more than a token each (64 tokens, two each: 10.4 us against 9.0 in several) and the pairs fit a round.
+int moe_route_blocks(const MoeRouteArgs& a) {
+    if (a.tokens <= 32 && a.tokens * a.top_k <= (size_t)kRoundPairs) return 1;
+    const size_t per = std::max<size_t>(route_warps(a.experts), (a.tokens + kMaxBlocks - 1) / kMaxBlocks);
+    return (int)std::max<size_t>((a.tokens + per - 1) / per, 2);
 }
-size_t moe_route_workspace_bytes(int sm_count) { return (size_t)sm_count * LUX_CUDA_MAX_EXPERTS * sizeof(int); }
+size_t moe_route_workspace_bytes() { return (size_t)(kMaxBlocks + 1) * LUX_CUDA_MAX_EXPERTS * sizeof(int); }
 
 cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, int* launches) {
-    const int blocks = moe_route_blocks(a, sm_count), chunk = std::max(1, (int)((a.tokens + blocks - 1) / blocks));
+    const int blocks = moe_route_blocks(a), chunk = std::max(1, (int)((a.tokens + blocks - 1) / blocks));
     cudaError_t e;
     *launches = 1;
     if (!a.logits) e = launch_route_t<0, false, false>(a, blocks, chunk, stream, overlap_prev);
@@ -400,11 +531,19 @@ cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t s
     else if (a.experts <= 512) e = launch_route_v<16>(a, blocks, chunk, stream, overlap_prev);
     else e = launch_route_v<32>(a, blocks, chunk, stream, overlap_prev);
     if (e != cudaSuccess || blocks == 1) return e;
-    *launches = 2;
     cudaLaunchAttribute attr;
-    const int parts = kPlaceThreads / ((a.experts + 31) & ~31);
-    const cudaLaunchConfig_t cfg = config(blocks, kPlaceThreads, ((size_t)2 * a.experts + 1 + 2 * (size_t)parts * a.experts) * 4, stream, true, &attr);
-    return cudaLaunchKernelEx(&cfg, moe_place_kernel, a, chunk);
+    if (blocks <= kFewBlocks) {
+        *launches = 2;
+        const int parts = kCountThreads / ((a.experts + 31) & ~31);
+        const cudaLaunchConfig_t cfg = config(blocks, kCountThreads, ((size_t)2 * a.experts + 1 + 2 * (size_t)parts * a.experts) * 4, stream, true, &attr);
+        return cudaLaunchKernelEx(&cfg, moe_count_place_kernel, a, chunk);
+    }
+    *launches = 3;
+    const cudaLaunchConfig_t count = config((a.experts + 31) / 32, 1024, 0, stream, true, &attr);
+    if ((e = cudaLaunchKernelEx(&count, moe_count_kernel, a.hist, a.experts, blocks)) != cudaSuccess) return e;
+    const unsigned grid = (unsigned)std::min<size_t>(2 * (size_t)sm_count, (a.tokens * a.top_k + kPlaceThreads - 1) / kPlaceThreads);
+    const cudaLaunchConfig_t place = config(grid, kPlaceThreads, ((size_t)a.experts + 1) * 4, stream, true, &attr);
+    return cudaLaunchKernelEx(&place, moe_place_kernel, a, chunk, blocks);
 }
 
 cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {

@@ -1,5 +1,6 @@
 // Entry points of the product with an epilogue and of a layer of experts (lux_gpu_quant_vtbl): argument checks, then the launches on the
 // context's stream.
+#include <algorithm>
 #include <cstdlib>
 
 #include "internal.h"
@@ -74,6 +75,25 @@ void note_outputs(Context* c, const Operand* o, int n) {
     note_early_chain_launch(c, false);
     for (int i = 0; i < n; i++)
         if (o[i].b && o[i].written) c->chain_out.add(o[i].b->ptr, o[i].bytes);
+}
+
+// A workspace of the context of at least `bytes`: never made or grown while the stream is being recorded; an outgrown one stays for the graphs
+// that were recorded with it.
+LuxBackendError grow_workspace(Context* c, Block** ws, std::vector<Block*>* retired, size_t bytes, const char* call) {
+    if (*ws && (*ws)->size >= bytes) return LUX_BACKEND_OK;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
+        set_last_error("%s: this shape needs a larger workspace (%zu bytes); run it once outside the graph capture first", call, bytes);
+        return LUX_BACKEND_ERROR_NOT_SUPPORTED;
+    }
+    // (twice the old one at least, where there is room: what is kept for graphs then stays below the one in use)
+    cudaError_t e = cudaSuccess;
+    Block* b = *ws ? c->dev->acquire(std::max(bytes, 2 * (*ws)->size), c->stream, &e) : nullptr;
+    if (!b) b = c->dev->acquire(bytes, c->stream, &e);
+    if (!b) return map_cuda_error(e, call);
+    if (*ws) retired->push_back(*ws);
+    *ws = b;
+    return LUX_BACKEND_OK;
 }
 
 LuxBackendError check_format(const char* call, int K, int bits, int group) {
@@ -153,17 +173,8 @@ LuxBackendError moe_route(LuxBackendContext* ctx, const lux_moe_route_params* pa
     DeviceGuard g(c->dev->device());
     MoeRouteArgs a{o[LOGITS].ptr(), (const float*)o[BIAS].ptr(), (int*)o[IDS].ptr(), (float*)o[WEIGHTS].ptr(), (int*)o[ORDER].ptr(), (int*)o[POS].ptr(),
                    (int*)o[OFFSETS].ptr(), nullptr, (size_t)p.tokens, ld, p.experts, p.top_k, p.score, p.renorm, ls == 2, p.scale};
-    if (moe_route_blocks(a, c->dev->sm_count) > 1) {
-        if (!c->moe_ws) {
-            cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-            if (cudaStreamIsCapturing(c->stream, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone) {
-                set_last_error("moe_route: the workspace does not exist yet; run one call of this size outside the graph capture first");
-                return LUX_BACKEND_ERROR_NOT_SUPPORTED;
-            }
-            cudaError_t e = cudaSuccess;
-            c->moe_ws = c->dev->acquire(moe_route_workspace_bytes(c->dev->sm_count), c->stream, &e);
-            if (!c->moe_ws) return map_cuda_error(e, "moe_route workspace");
-        }
+    if (moe_route_blocks(a) > 1) {
+        if (LuxBackendError e = grow_workspace(c, &c->moe_ws, nullptr, moe_route_workspace_bytes(), "moe_route")) return e;
         a.hist = (int*)c->moe_ws->ptr;
     }
     int launches = 0;
@@ -210,9 +221,13 @@ LuxBackendError qmatmul_experts(LuxBackendContext* ctx, const lux_experts_params
         return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     }
     const bool use_many = many && (!few || (force ? force[0] == 'm' : experts_have_many_rows(a)));
+    const size_t room = use_many ? qmm_experts_workspace_bytes(a) : 0;
+    if (room)
+        if (LuxBackendError le = grow_workspace(c, &c->gather_ws, &c->gather_ws_retired, room, "qmatmul_experts")) return le;
     const char* name = "";
-    const cudaError_t e = use_many ? launch_qmm_experts(a, c->dev->sm_count, c->stream, chain_is_open(c), &name)
+    const cudaError_t e = use_many ? launch_qmm_experts(a, room ? c->gather_ws->ptr : nullptr, c->dev->sm_count, c->stream, chain_is_open(c), &name)
                                    : launch_qmv_experts(a, c->dev->sm_count, c->stream, chain_is_open(c), &name);
+    if (room) c->launches++;
     if (e != cudaSuccess) return map_cuda_error(e, name);
     c->launches++;
     c->last_kernel = name;

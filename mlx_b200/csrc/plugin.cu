@@ -80,6 +80,8 @@ void destroy_context(LuxBackendContext* ctx) {
     for (Block* b : c->qmv_ws_retired) c->dev->release(b, c->stream);
     if (c->qmm_ws) c->dev->release(c->qmm_ws, c->stream);
     if (c->moe_ws) c->dev->release(c->moe_ws, c->stream);
+    if (c->gather_ws) c->dev->release(c->gather_ws, c->stream);
+    for (Block* b : c->gather_ws_retired) c->dev->release(b, c->stream);
     if (c->err_host) cudaFreeHost(c->err_host);
     c->dev->release_stream(c->stream);
     c->magic = 0;
@@ -541,6 +543,8 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.moe.experts", "qmv_experts<8,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.experts", "qmm_experts<4>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // many rows an expert (tcgen05)
     {"lux.moe.experts", "qmm_experts<8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmm_experts<4,pairs>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // the same on pairs of CTAs
+    {"lux.moe.experts", "qmm_experts<8,pairs>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
 };
 const LuxKernelRegistry g_registry = {"cuda", g_kernels, sizeof(g_kernels) / sizeof(g_kernels[0])};
 

@@ -149,6 +149,43 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
         ::"r"(s32(dst)), "l"(map), "r"(x), "r"(y), "r"(s32(bar)) : "memory");
 }
 
+// ---- pairs of CTAs (cta_group::2) --------------------------------------------------
+constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;  // a shared::cluster address with this bit cleared is CTA 0's copy
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {  // whole warp, the same warp in both CTAs
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(dst_smem)), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// arrive on CTA 0's copy of a barrier (from either CTA)
+__device__ __forceinline__ void mbar_arrive_cta0(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(s32(b) & kPeerBitMask) : "memory");
+}
+// arrives once on the barrier at this offset in both CTAs when the MMAs issued so far have completed
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(s32(bar)), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    const uint32_t z = 0;
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+        "  tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p; }"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(z) : "memory");
+}
+// this CTA's half of an x tile into its own shared memory, completion counted on CTA 0's barrier (no multicast)
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(s32(dst)), "l"(map), "r"(x), "r"(y), "r"(s32(bar) & kPeerBitMask) : "memory");
+}
+
+
 __device__ __forceinline__ uint32_t ldg_u16(const uint16_t* p) {  // zero-extended straight into a 32-bit register
     uint32_t v;
     asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p));
@@ -254,11 +291,12 @@ __device__ __forceinline__ void weight_producer(const Prm& p, Seg seg, int nks, 
     flush();
 }
 // One warp (lane quarter of group grp; a warp may only touch its own quarter of the TMEM lanes): the thread owns row r of
-// every tile.  There are as many stages in flight as groups, so a group always writes the same slot.
+// every tile.  A group always writes the same slots.
 // What bounds it is its instructions, three such warps to a scheduler, and the instruction caches that all roles share;
 // hence row pointers per tile (a division each), one copy of the code for both sub-blocks, one arrival per warp.
+// SLOTS: how many slots of the A ring the group owns, kDqGroups apart; `empty` and a_tmem are the first one's, arrive(i) says that the i-th is full.
 // row_of(seg, r): the row of wq, scales and biases that is row r of the tile.
-template <int BITS, class Prm, class Seg, class RowOf, class Arrive>
+template <int BITS, int SLOTS = 1, class Prm, class Seg, class RowOf, class Arrive>
 __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int r, int nks, const unsigned char* wring, uint64_t* wfull,
                                              uint64_t* wempty, uint64_t* empty, uint32_t a_tmem, volatile int* abort_flag,
                                              const RowOf& row_of, const Arrive& arrive) {
@@ -325,7 +363,7 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
     if (more) fetch_sb();
     const int half_shift = p.gshift == 5 ? 16 : 0, sub_shift = p.gshift == 6 ? 16 : 0;  // where the next half's, the next sub-block's scale is
     int wslot = 0;
-    uint32_t wphase = 0, phase = 1;
+    uint32_t wphase = 0, phase = 1, own = 0;
     while (more) {
         const int nsub = min(kSub, nks - st * kSub);
         uint32_t s_lo = sp[0], b_lo = bp[0];
@@ -359,8 +397,8 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
             }
             if (u >= nsub) break;  // (the odd sub-block's partner at 8 bit: nothing in it)
             if (u == 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
-                phase ^= 1;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty + own * kDqGroups, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
+                if (SLOTS == 1) phase ^= 1;
                 tc_fence_after();
                 if (!ok) break;
             }
@@ -372,7 +410,7 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
                 if (scale_fast_ok(sv)) dequant_32<BITS, true>(w + h * (WPS / 2), sv, bv, out);
                 else dequant_32<BITS, false>(w + h * (WPS / 2), sv, bv, out);  // whole-block branch: not if-converted
                 __syncwarp();
-                tmem_st16(a_tmem + u * kAColsPerSub + h * 16, out);
+                tmem_st16(a_tmem + own * (kDqGroups * kAColsPerSlot) + u * kAColsPerSub + h * 16, out);
             }
             if (UPS == 1) {
 #pragma unroll
@@ -389,7 +427,11 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
         tmem_st_wait();  // once per stage: both sub-blocks are in tensor memory
         tc_fence_before();
         __syncwarp();
-        if ((r & 31) == 0) arrive();
+        if ((r & 31) == 0) arrive((int)own);
+        if (SLOTS > 1 && ++own == SLOTS) {
+            own = 0;
+            phase ^= 1;
+        }
     }
 }
 

@@ -238,7 +238,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&](int) { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -525,7 +525,7 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&](int) { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -589,40 +589,12 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
 constexpr int kPairEpiBar = 1 + kDqGroups;       // named barrier of the epilogue warps
 static_assert(kDqGroups == kStagesP, "a group always owns the same slot");
 static_assert(kAColBase + kStagesP * kAColsPerSlot <= kTmemCols, "A ring does not fit");
-constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;  // a shared::cluster address with this bit cleared is CTA 0's copy
 struct PairSmemLayout {
     uint64_t full[kStagesP], empty[kStagesP], wfull[kDqGroups * kMaxWSlots], wempty[kDqGroups * kMaxWSlots], tmem_full, tmem_empty;
     uint32_t tmem_base;
     int abort_flag;
 };
 static_assert(sizeof(SmemLayout) <= kGemmCtlBytes && sizeof(PairSmemLayout) <= kGemmCtlBytes, "the plan's share of shared memory");
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {  // whole warp, the same warp in both CTAs
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(dst_smem)), "r"(ncols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// arrive on CTA 0's copy of a barrier (from either CTA)
-__device__ __forceinline__ void mbar_arrive_cta0(uint64_t* b) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(s32(b) & kPeerBitMask) : "memory");
-}
-// arrives once on the barrier at this offset in both CTAs when the MMAs issued so far have completed
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(s32(bar)), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void tc_mma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    const uint32_t z = 0;
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
-        "  tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p; }"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(z) : "memory");
-}
 // a finished tile of y from shared memory ([row of x][128 columns] bf16) to global memory; rows and columns past
 // the ends of y are clipped by the copy engine
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
@@ -630,13 +602,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                  ::"l"(map), "r"(x), "r"(y), "r"(s32(src)) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// this CTA's half of an x tile into its own shared memory, completion counted on CTA 0's barrier (no multicast)
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(s32(dst)), "l"(map), "r"(x), "r"(y), "r"(s32(bar) & kPeerBitMask) : "memory");
-}
-
 template <int BITS, bool EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
@@ -753,7 +718,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min(n0_of(s.tile()) + r, p.N - 1); }, [&]() { mbar_arrive_cta0(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min(n0_of(s.tile()) + r, p.N - 1); }, [&](int) { mbar_arrive_cta0(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;

@@ -217,6 +217,38 @@ def test_recorded(ctx, oracle, rows):
     ctx.graph_destroy(g)
 
 
+def test_workspace_of_a_gathered_product(ctx, oracle):
+    """It grows between calls and not while a graph is recorded; a graph recorded with the outgrown one still gives its bits."""
+    E, K, N = 2, 128, 64
+    w, values = layer(oracle, E, N, K, 4, 64)
+    bufs = [ctx.upload(a) for a in w]
+
+    def call(rows):
+        x = oracle.make_x(rows, K, oracle.BF16, tag=rows)
+        order = np.random.default_rng(rows).permutation(rows).astype(np.int32)
+        y = ctx.empty((rows, N), np.uint16)
+        keep = (ctx.upload(x), ctx.upload(order), ctx.upload(groups(None, E, rows, "even")))
+        return lambda: ctx.qmatmul_experts(ctx.experts_params(rows, rows, E, K, N, 4, 64), keep[0], keep[1], keep[2], *bufs, None, y), y
+    small, y_small = call(200)
+    big, y_big = call(3000)
+    small()
+    want = y_small.to_host()
+    ctx.graph_begin()
+    small()
+    with pytest.raises(BackendError) as e:
+        big()
+    assert e.value.code == P.ERR_NOT_SUPPORTED
+    g = ctx.graph_end()
+    big()
+    want_big = y_big.to_host()
+    y_small.from_host(np.zeros_like(want))
+    ctx.graph_launch(g)
+    big()
+    np.testing.assert_array_equal(y_small.to_host(), want)
+    np.testing.assert_array_equal(y_big.to_host(), want_big)
+    ctx.graph_destroy(g)
+
+
 def test_refusals(ctx, oracle):
     E, K, N, rows = 2, 64, 32, 6
     w, _ = layer(oracle, E, N, K, 4, 32)

@@ -37,7 +37,7 @@ def check(got, want, T, k, E):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("score,renorm,with_bias", [(P.SCORE_SOFTMAX, True, False), (P.SCORE_SOFTMAX, False, False), (P.SCORE_SIGMOID, True, True), (P.SCORE_SIGMOID, False, False)])
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 64, 8), (3, 5, 5), (16, 33, 4), (64, 32, 32), (65, 100, 7), (777, 40, 3), (300, 513, 6), (40, 1024, 32), (5000, 256, 8)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 64, 8), (3, 5, 5), (16, 33, 4), (64, 32, 32), (32, 64, 8), (65, 100, 7), (777, 40, 3), (300, 513, 6), (40, 1024, 32), (5000, 256, 8)])
 def test_route(ctx, oracle, dtype, score, renorm, with_bias, T, E, k):
     rng = np.random.default_rng(T * E + k)
     v = (rng.standard_normal((T, E)) * 2).astype(np.float32)
@@ -69,6 +69,23 @@ def test_extremes(ctx, T):
     bias = np.array([-inf, np.nan, 0.5, 0.25], np.float32)
     got = run(ctx, ctx.moe_route_params(T, 4, 3, score=P.SCORE_SIGMOID, renorm=False), ctx.upload(v), ctx.upload(bias), T, 3, 4)
     check(got, moe.route(v, 3, False, False, 1.0, bias), T, 3, 4)
+
+
+@pytest.mark.parametrize("T,E,k", [(3, 64, 8), (100, 300, 6)])
+def test_scores_next_to_a_border(ctx, T, E, k):
+    """sigmoid + bias that differ in the last bits of fp32, or only beyond them: few such experts, and more than a warp has lanes."""
+    rng = np.random.default_rng(E)
+    v = rng.standard_normal((T, E)).astype(np.float32)
+    prm = ctx.moe_route_params(T, E, k, score=P.SCORE_SIGMOID)
+    for near in (4, 20, E):
+        one = v.copy()
+        one[:, :near] = 2.0 + np.arange(near, dtype=np.float32) % 5 * np.float32(2.0 ** -22)
+        bias = np.where(np.arange(E) < near, 3.0, 0.0).astype(np.float32)   # (the sum has 22 bits behind the point)
+        got = run(ctx, prm, ctx.upload(one), ctx.upload(bias), T, k, E)
+        check(got, moe.route(one, k, False, True, 1.0, bias), T, k, E)
+        bias = np.where(np.arange(E) < near, 1e6, 0.0).astype(np.float32)   # all alike in fp32
+        got = run(ctx, prm, ctx.upload(one), ctx.upload(bias), T, k, E)
+        check(got, moe.route(one, k, False, True, 1.0, bias), T, k, E)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
