@@ -1,0 +1,78 @@
+// Which kernel takes a product grouped by expert, and the GEMM's tiles (qmm_experts.cu), as plain host arithmetic.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstddef>
+
+#include "qmm_plan.h"
+
+namespace luxcuda {
+
+struct ExpertsShape {
+    size_t rows;  // of y: what the experts get together, at most
+    int experts, K, N, bits;
+    bool gather;  // rows of x are fetched by index
+};
+constexpr int kPairMean = 65;  // rows an expert on average from which on the GEMM runs on pairs of CTAs
+inline bool experts_in_pairs(const ExpertsShape& s, int sm_count) {
+    const size_t mean = (s.rows + s.experts - 1) / s.experts;
+    return sm_count % 2 == 0 && s.N > 128 && mean >= (size_t)kPairMean;
+}
+
+// Estimates of the times in microseconds, for experts that share the rows evenly: the host does not know better.  Fitted to 130 shapes (2 to 128
+// experts, K 512 to 4096, N 128 to 8192, 0.5 to 90 rows an expert, 4 and 8 bit; calls from a host, launches included): the faster of the two is
+// taken on 128 of them or one within 5 % of it, within 8 % at worst; the times are off by a sixth on average.
+//   few rows (qmv_stream.cu): the row tiles of all items of eight rows, dealt over the SMs, a tile at the rate of its packed bytes but
+//   not below what starting one costs; x is loaded again for every item a CTA works on;
+//   many (qmm_experts.cu): rounds of tiles, a k-stage of 128 bound by dequantisation until the tiles are high; gathered rows first.
+inline void experts_estimates(const ExpertsShape& s, int sm_count, double* few, double* many) {
+    const double mean = (double)s.rows / s.experts, active = s.experts * (1.0 - std::exp(-mean)), m = s.rows / active;
+    const double row_tiles = (s.N + 15) / 16, items = active * std::max(1.0, m / 8 + 0.23), tiles = items * row_tiles / sm_count;
+    const double tile = std::max(0.22 + 0.055 * (s.K * (double)s.bits / 1024), 0.56);
+    *few = 6.1 + std::max(1.0, tiles) * tile + 0.28 * std::max(1.0, tiles / row_tiles);
+    const bool pairs = experts_in_pairs(s, sm_count);
+    const double n_tiles = (s.N + 127) / 128, G = pairs ? sm_count / 2 : sm_count, bm = std::min(pairs ? 256.0 : 128.0, std::max(32.0, 2 * mean));
+    const double T = active * std::max(1.0, m / bm + 0.35) * (pairs ? std::ceil(n_tiles / 2) : n_tiles);
+    const double stage = pairs ? 0.77 + 0.0063 * std::max(0.0, std::min(m, bm) - 48) : 0.47 + 0.009 * std::max(0.0, std::min(m, bm) - 48);
+    *many = 6.6 + (s.gather ? 0.7 + s.rows * (double)s.K * 4 / 3.0e6 : 0.0) + std::ceil(T / G) * (std::ceil(s.K / 128.0) * stage + 1.4);
+}
+inline bool experts_have_many_rows(const ExpertsShape& s, int sm_count) {
+    if (!s.rows) return false;
+    double few, many;
+    experts_estimates(s, sm_count, &few, &many);
+    return many < few;
+}
+
+// The GEMM: stages of its ring (see qmm_experts.cu), rows of x per tile, at most.
+constexpr int stages(bool pair) { return pair ? 3 : 6; }
+constexpr int kLowRows = 128, kTwoAccRows = 64;  // tiles of single CTAs; with two accumulators
+constexpr int y_pitch(bool gated) { return (gated ? kTileN / 2 : kTileN) * 2 + 16; }  // of a finished tile in shared memory, bytes a row of x
+struct ExpertsPlan {
+    int bm, box, w_slots, n_tiles;  // box: rows of x per TMA box, a divisor of what a CTA fetches; n_tiles: of pairs two
+    bool pair, y_staged;
+    size_t smem;
+};
+// bm: an expert of twice the average still takes one tile, as far as there is room; lower tiles leave shared memory to L1, which holds the rows'
+// scales.  Weight rings: a stage of each group's, one unit at 4 bit, two at 8 bit (one: 89 us against 70 at 8 x 32 rows, 4096 x 8192; more than a
+// stage: the same).  y_pieces: y leaves in 16-byte pieces of its rows.
+inline ExpertsPlan plan_experts(const ExpertsShape& s, bool gated, bool y_pieces, int sm_count, int force_pair = -1) {
+    ExpertsPlan p;
+    const size_t mean = (s.rows + s.experts - 1) / s.experts;
+    const int n_tiles = (s.N + kTileN - 1) / kTileN;
+    p.pair = force_pair >= 0 ? force_pair == 1 && sm_count % 2 == 0 : experts_in_pairs(s, sm_count);
+    p.n_tiles = p.pair ? (n_tiles + 1) / 2 : n_tiles;
+    p.y_staged = p.pair && y_pieces;
+    p.w_slots = s.bits == 8 ? 2 : 1;
+    const int step = p.pair ? 32 : 16;
+    p.bm = (int)std::min<size_t>(p.pair ? kMaxBM : kLowRows, std::max<size_t>(32, (2 * mean + step - 1) / step * step));
+    for (;; p.bm -= step) {  // (single CTAs: 8 bit and long tables cost some rows)
+        p.smem = 1024 + kGemmCtlBytes + (size_t)stages(p.pair) * kSub * (p.pair ? p.bm / 2 : p.bm) * 128 + (size_t)p.w_slots * kDqGroups * kWUnitBytes +
+                 (p.pair ? (size_t)(p.y_staged ? p.bm * y_pitch(gated) : 0) : (size_t)kEpiWarps * kEpiStageBytes) + (size_t)8 * (s.experts + 1);
+        if (p.smem <= (size_t)kGemmSmemLimit) break;
+    }
+    const int half = p.pair ? p.bm / 2 : p.bm;  // rows a CTA fetches
+    for (p.box = 64; half % p.box; p.box -= 16) {}
+    return p;
+}
+
+}  // namespace luxcuda

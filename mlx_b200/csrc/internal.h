@@ -262,6 +262,7 @@ struct QmvSplitPlan {
 };
 struct QmvStreamPlan {
     int gshift, nkb, n_rt, grid, grid_y, nch, kbc, ts, tb, stages, stage_bytes, tile_bytes, sb_off, xs_off, run_off, bar_off;
+    bool sb_bulk;  // scales by bulk copies (qmatmul_experts)
     size_t smem;
 };
 struct DecodePlan {

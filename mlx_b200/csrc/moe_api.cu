@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstdlib>
 
+#include "experts_plan.h"
 #include "internal.h"
 
 namespace luxcuda {
@@ -67,9 +68,6 @@ void note_use(Context* c, const Operand* o, int n) {
     for (int i = 0; i < n; i++)
         if (o[i].b) o[i].b->last_stream = c->stream;
 }
-// Rows an expert on average (what the host knows) from which on the GEMM is the faster.
-bool experts_have_many_rows(const ExpertsArgs& a) { return a.rows >= (size_t)16 * a.experts; }
-
 // after a launch whose dependents start behind its wait: what it writes
 void note_outputs(Context* c, const Operand* o, int n) {
     note_early_chain_launch(c, false);
@@ -220,7 +218,7 @@ LuxBackendError qmatmul_experts(LuxBackendContext* ctx, const lux_experts_params
         set_last_error("qmatmul_experts: experts=%d K=%d N=%d in groups of %d is past the kernels' 32-bit index ranges", p.experts, p.K, p.N, p.group);
         return LUX_BACKEND_ERROR_NOT_SUPPORTED;
     }
-    const bool use_many = many && (!few || (force ? force[0] == 'm' : experts_have_many_rows(a)));
+    const bool use_many = many && (!few || (force ? force[0] == 'm' : experts_have_many_rows({a.rows, a.experts, a.K, a.N, a.bits, a.order != nullptr}, c->dev->sm_count)));
     const size_t room = use_many ? qmm_experts_workspace_bytes(a) : 0;
     if (room)
         if (LuxBackendError le = grow_workspace(c, &c->gather_ws, &c->gather_ws_retired, room, "qmatmul_experts")) return le;

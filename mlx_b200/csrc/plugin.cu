@@ -537,10 +537,8 @@ const LuxEmbeddedKernel g_kernels[] = {
     {"lux.block_norm", "block_norm", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.route", "moe_route", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.combine", "moe_combine", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
-    {"lux.moe.experts", "qmv_experts<4,m8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // few rows an expert: 8 or 16 at a time
-    {"lux.moe.experts", "qmv_experts<4,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
-    {"lux.moe.experts", "qmv_experts<8,m8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
-    {"lux.moe.experts", "qmv_experts<8,m16>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
+    {"lux.moe.experts", "qmv_experts<4>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // few rows an expert
+    {"lux.moe.experts", "qmv_experts<8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.experts", "qmm_experts<4>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // many rows an expert (tcgen05)
     {"lux.moe.experts", "qmm_experts<8>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},
     {"lux.moe.experts", "qmm_experts<4,pairs>", LUX_KERNEL_LANG_CUDA, nullptr, 0, nullptr, 0},   // the same on pairs of CTAs

@@ -20,6 +20,7 @@
 #include <cstdlib>
 
 #include "epilogue.cuh"
+#include "experts_plan.h"
 #include "groups.cuh"
 #include "qmm_roles.cuh"
 
@@ -30,9 +31,7 @@ namespace {
 // A ring of stages: A in tensor memory (64 columns a stage), B in shared memory.  Low tiles leave room for twice as many, two to a group of
 // dequantising warps, which then does not wait for the MMAs of its last stage before it writes the next; and tiles of up to 64 rows for a
 // second accumulator, whose MMAs run under the epilogue of the first.
-constexpr int stages(bool pair) { return pair ? 3 : 6; }
 constexpr uint32_t acc_cols(bool pair) { return pair ? 256 : 128; }  // of tensor memory; the ring lies behind them
-constexpr int kLowRows = 128, kTwoAccRows = 64;                      // tiles of single CTAs; with two accumulators
 static_assert(stages(true) % kDqGroups == 0 && stages(false) % kDqGroups == 0, "a group always owns the same slots");
 static_assert(acc_cols(true) + stages(true) * kAColsPerSlot <= kTmemCols && acc_cols(false) + stages(false) * kAColsPerSlot <= kTmemCols, "tensor memory");
 
@@ -48,8 +47,6 @@ struct ExpertGemm {
     int bm, n_tiles, w_slots, most;  // rows of x per tile, at most; tiles along N; tiles in all, at most
     int y_staged;  // pairs: the tile goes through shared memory (bf16 y, 16-byte pieces of its rows)
 };
-
-constexpr int y_pitch(bool gated) { return (gated ? kTileN / 2 : kTileN) * 2 + 16; }
 
 struct Control {
     uint64_t full[stages(false)], empty[stages(false)], wfull[kDqGroups * kMaxWSlots], wempty[kDqGroups * kMaxWSlots], tmem_full[2], tmem_empty[2];
@@ -416,35 +413,7 @@ qmm_experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid
     experts_body<BITS, GATED, true>(tmap_x, tmap_w, p);
 }
 
-struct Plan {
-    int bm, box, w_slots, n_tiles;  // n_tiles: of a pair two
-    bool pair, y_staged;
-    size_t smem;
-};
 bool y_in_pieces(const ExpertsArgs& a) { return a.y_dtype == LUX_DTYPE_BFLOAT16 && ((uintptr_t)a.y & 15) == 0 && (a.gated ? a.N / 2 : a.N) % 8 == 0; }
-// bm: an expert of twice the average still takes one tile, as far as there is room; lower tiles leave shared memory to L1, which holds the rows'
-// scales.  Weight rings as in qmm_plan.h.
-void make_plan(const ExpertsArgs& a, int sm_count, Plan* pl) {
-    const size_t mean = (a.rows + a.experts - 1) / a.experts;
-    const int n_tiles = (a.N + kTileN - 1) / kTileN;
-    const char* force = getenv("LUXCUDA_EXPERTS_PAIR");  // "0" | "1" (experiments)
-    pl->pair = sm_count % 2 == 0 && (force ? force[0] == '1' : n_tiles > 1 && 2 * mean > (size_t)kLowRows);
-    pl->n_tiles = pl->pair ? (n_tiles + 1) / 2 : n_tiles;
-    pl->y_staged = pl->pair && y_in_pieces(a);
-    const int step = pl->pair ? 32 : 16;
-    pl->bm = (int)std::min<size_t>(pl->pair ? kMaxBM : kLowRows, std::max<size_t>(32, (2 * mean + step - 1) / step * step));
-    const size_t slots = a.bits == 8 ? 2 : 1;
-    size_t fixed;
-    for (;; pl->bm -= step) {
-        fixed = 1024 + kGemmCtlBytes + (size_t)stages(pl->pair) * kSub * (pl->pair ? pl->bm / 2 : pl->bm) * 128 +
-                (pl->pair ? (size_t)(pl->y_staged ? pl->bm * y_pitch(a.gated) : 0) : (size_t)kEpiWarps * kEpiStageBytes) + (size_t)8 * (a.experts + 1);
-        if (fixed + slots * kDqGroups * kWUnitBytes <= (size_t)kGemmSmemLimit) break;  // (single CTAs: 8 bit and long tables cost some rows)
-    }
-    pl->w_slots = (int)slots;
-    pl->smem = fixed + slots * kDqGroups * kWUnitBytes;
-    const int half = pl->pair ? pl->bm / 2 : pl->bm;  // rows a CTA fetches
-    for (pl->box = 64; half % pl->box; pl->box -= 16) {}
-}
 template <int BITS, bool GATED, bool PAIR>
 cudaError_t launch_t(const CUtensorMap& tmap_x, const CUtensorMap& tmap_w, const ExpertGemm& p, size_t smem, int grid, cudaStream_t stream, bool overlap_prev) {
     auto kern = PAIR ? qmm_experts_pair_kernel<BITS, GATED> : qmm_experts_kernel<BITS, GATED>;
@@ -500,8 +469,8 @@ bool qmm_experts_supported(const ExpertsArgs& a) {
 }
 
 cudaError_t launch_qmm_experts(const ExpertsArgs& a, void* workspace, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name) {
-    Plan pl;
-    make_plan(a, sm_count, &pl);
+    const char* force = getenv("LUXCUDA_EXPERTS_PAIR");  // "0" | "1" (experiments)
+    const ExpertsPlan pl = plan_experts({a.rows, a.experts, a.K, a.N, a.bits, a.order != nullptr}, a.gated, y_in_pieces(a), sm_count, force ? force[0] == '1' : -1);
     int* err = a.error ? a.error : device_error_word();
     if (!err) return cudaErrorMemoryAllocation;
     const EncodeTiledFn encode = encode_tiled_fn();

@@ -28,7 +28,7 @@
 //
 // The epilogue of qmatmul_epi (bias, activation, residual) is the summing warps': a tile's bias and residual are requested ahead of its sums.
 //
-// Products grouped by expert (qmatmul_experts): the items are runs of 8 or 16 rows of one expert, which every CTA works out from the
+// Products grouped by expert (qmatmul_experts): the items are runs of eight rows of one expert, which every CTA works out from the
 // offsets in device memory; the row tiles of all of them, item after item, are cut into one range per CTA, so that a CTA reloads x two or
 // three times a launch (dealt out per item, as in a batch, it reads 64 KB of x for every 32 KB of weights).  Rows of a gated product: a
 // tile is eight rows of gate and the eight of up that go with them, one box of the weights seen as [expert][half][row]; the MMA's
@@ -106,6 +106,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
+// contiguous bytes, a multiple of 16 from 16-byte boundaries
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
@@ -136,6 +140,7 @@ __device__ __forceinline__ void add_f32x4(uint4& s, const uint4& v) {
         : "+r"(s.x), "+r"(s.y), "+r"(s.z), "+r"(s.w) : "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w));
 }
 constexpr int kItemRows = 16;  // rows of x of an item, at most (more of one matmul: several items, see Params)
+constexpr int kGroupRows = 8;  // of an expert's item.  (16, too, were built: on 9 of 130 shapes 1 to 17 % faster than the better of this and qmm_experts.cu, on the others slower)
 struct Item {
     const __nv_bfloat16* x;
     const __nv_bfloat16* scales;
@@ -161,6 +166,12 @@ struct GroupParams<kGroups> {
     const int *offsets, *order;
     int experts, rows, x_rows, n_rt, most, tables_off;  // row tiles of an expert; items, at most; offset of the tables in shared memory
     uint32_t top_k;
+    // The scales of a tile's rows lie side by side, and its biases: one bulk copy each (two where gated) into [16 rows][groups], without padding; for K
+    // in one chunk and N in whole tiles.  (By pieces as above the one warp that fetches them takes 0.5 us per tile, whatever K.)
+    int sb_bulk;
+    // K inside a k-block: the boxes are whole all the same, and what they hold behind a row's end is the row after it (with scales of zero); but the
+    // last tile of all, behind which nothing need be, takes single k-blocks of this map, which ends with the rows.
+    alignas(64) CUtensorMap map_end;
 };
 // NI: how many matmuls of a batch, at most; 1: one; 0: one whose rows of x are n_items items of 16 (M: all of them); kGroups: experts.
 template <int NI, int EPI>
@@ -300,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
     static_assert(PRO == 0 || MT == 1, "prologues are built for M <= 8");
     constexpr bool kExperts = NI == kGroups, kGated = EPI == 2;
     static_assert(!kGated || kExperts, "gated products are built for experts");
+    static_assert(!kExperts || 8 * MT == kGroupRows, "rows of an item");
     constexpr int XV = x_frags(BITS), KB = kb_weights(BITS), KL = lane_weights(BITS), SROW = sb_row(SPL);
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ int s_abort;
@@ -319,13 +331,13 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
     }
     __syncthreads();
 
-    std::conditional_t<kExperts, GroupWalk<8 * MT>, Walk> wk;
+    std::conditional_t<kExperts, GroupWalk<kGroupRows>, Walk> wk;
     if constexpr (kExperts) {
         // (which weights are wanted is the previous kernel's answer: there is nothing to fetch ahead of it)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         int* const off = reinterpret_cast<int*>(smem + p.tables_off);
-        group_tables(off, off + p.experts + 1, p.offsets, p.experts, p.rows, p.most, [](int n) { return (n + 8 * MT - 1) / (8 * MT); });
+        group_tables(off, off + p.experts + 1, p.offsets, p.experts, p.rows, p.most, [](int n) { return (n + kGroupRows - 1) / kGroupRows; });
         if (!wk.init(p)) return;
     } else {
         wk.init(p);
@@ -353,7 +365,40 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             // codes with the last group's own scale and bias would add 0 * infinity where these are infinite.
             const uint32_t gpr = (uint32_t)p.K >> p.gshift, half = (kGated ? (uint32_t)p.N : 16u) * gpr, k16 = 16u * (lane % LPR);
             const uint32_t next_tile = (kGated ? 16u : 32u) * gpr;
-            do {
+            // experts: the boxes of a stage, which expects `more` bytes besides
+            [[maybe_unused]] auto expert_boxes = [&](uint32_t stage, int tile0, int tiles, uint32_t more) {
+                if constexpr (kExperts) {
+                    constexpr int TR = kGated ? 8 : 16;
+                    const int z = kGated ? 2 * wk.e : wk.e, kb0 = wk.c * p.kbc, ops = wk.kb_cnt(p);
+                    const int whole = p.k_tail && wk.e + 1 == p.experts && tile0 + tiles == p.n_rt ? tiles - 1 : tiles;
+                    if (lane == 0) bar_expect(full + 8 * st, (whole * p.kbc + (tiles - whole) * ops) * 2048 + more);
+                    __syncwarp();
+                    if (lane < whole) tma_load_4d(stage + lane * p.tile_bytes, &p.maps[0], 0, (tile0 + lane) * TR, z, kb0, full + 8 * st);
+                    if (whole < tiles && lane < ops) tma_load_3d(stage + whole * p.tile_bytes + lane * 2048, &p.map_end, (kb0 + lane) * 128, (tile0 + whole) * TR, z, full + 8 * st);
+                }
+            };
+            bool bulk = false;
+            if constexpr (kExperts) bulk = p.sb_bulk;
+            if (bulk) {
+                // lane: tile lane / 4 of eight; half of its rows (lane & 2, gated only); scales or biases
+                const int h = kGated ? lane >> 1 & 1 : 0;
+                const char* src = static_cast<const char*>(lane & 1 ? static_cast<const void*>(p.item(0).biases) : p.item(0).scales) + (size_t)h * p.N * gpr;
+                const uint32_t dst = p.sb_off + (lane & 1) * 32 * gpr + h * 16 * gpr;
+                do {
+                    for (int g = 0; g < wk.ng && ok; g++) {
+                        const int tile0 = wk.b0 + g * p.ts, tiles = min(p.ts, wk.tile_end(p) - tile0);
+                        ok = bar_wait<true>(empty + 8 * st, ph ^ 1, abort);
+                        if (!ok) break;
+                        const uint32_t stage = ring + st * p.stage_bytes;
+                        expert_boxes(stage, tile0, tiles, tiles * 64 * gpr);
+                        for (int ti = lane >> 2; ti < tiles && (kGated || !(lane & 2)); ti += 8)
+                            bulk_load(stage + dst + ti * 64 * gpr, src + 2 * (size_t)tile_row(tile0 + ti) * gpr, (kGated ? 16 : 32) * gpr, full + 8 * st);
+                        issued++;
+                        cp_async_arrive(full + 8 * st);
+                        next_stage();
+                    }
+                } while (ok && wk.next_run(p));
+            } else do {
                 const int t_end = wk.tile_end(p), kb0 = wk.c * p.kbc, ops = p.k_tail ? wk.kb_cnt(p) : 1;
                 const CUtensorMap* map = &p.maps[NI > 0 ? wk.item : 0];
                 const uint32_t g0 = (uint32_t)(wk.c * p.kbc) * KB >> p.gshift, bytes = 2u * min((uint32_t)wk.kb_cnt(p) * KB >> p.gshift, gpr - g0);
@@ -376,23 +421,18 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                     if (issued == p.stages) asm volatile("griddepcontrol.wait;" ::: "memory");
                     ok = bar_wait<true>(empty + 8 * st, ph ^ 1, abort);
                     if (!ok) break;
-                    if (lane == 0) bar_expect(full + 8 * st, tiles * (p.k_tail ? ops : p.kbc) * 2048);
-                    __syncwarp();
                     const uint32_t stage = ring + st * p.stage_bytes;
                     if constexpr (kExperts) {
-                        const int z = kGated ? 2 * wk.e : wk.e;
+                        expert_boxes(stage, tile0, tiles, 0);
+                    } else {
+                        if (lane == 0) bar_expect(full + 8 * st, tiles * (p.k_tail ? ops : p.kbc) * 2048);
+                        __syncwarp();
                         if (!p.k_tail) {
-                            if (lane < tiles) tma_load_4d(stage + lane * p.tile_bytes, map, 0, (tile0 + lane) * (kGated ? 8 : 16), z, kb0, full + 8 * st);
+                            if (lane < tiles) tma_load_3d(stage + lane * p.tile_bytes, map, 0, (tile0 + lane) * 16, kb0, full + 8 * st);
                         } else {
                             for (int ti = 0; ti < tiles; ti++)
-                                if (lane < ops)
-                                    tma_load_3d(stage + ti * p.tile_bytes + lane * 2048, map, (kb0 + lane) * 128, (tile0 + ti) * (kGated ? 8 : 16), z, full + 8 * st);
+                                if (lane < ops) tma_load_2d(stage + ti * p.tile_bytes + lane * 2048, map, (kb0 + lane) * 128, (tile0 + ti) * 16, full + 8 * st);
                         }
-                    } else if (!p.k_tail) {
-                        if (lane < tiles) tma_load_3d(stage + lane * p.tile_bytes, map, 0, (tile0 + lane) * 16, kb0, full + 8 * st);
-                    } else {
-                        for (int ti = 0; ti < tiles; ti++)
-                            if (lane < ops) tma_load_2d(stage + ti * p.tile_bytes + lane * 2048, map, (kb0 + lane) * 128, (tile0 + ti) * 16, full + 8 * st);
                     }
                     issued++;
                     uint32_t dst = stage + p.sb_off + (lane / LPR) * SROW + k16;
@@ -650,6 +690,15 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
         // this lane's place in the stage that comes next: 16-byte pieces 2t and 2t+1 of row g of the k-block
         const uint32_t in_tile = kq * 2048 + g * 128 + (((2 * t) ^ g) << 4), sa0 = ring + tsub * p.tile_bytes + in_tile;
         const uint32_t stage_bytes = p.stage_bytes, full_end = full + 8 * p.stages;
+        // from the scales of row g to those of row g + 8, and to its biases
+        bool bulk = false;
+        uint32_t sb_half = 16 * SROW, sb_bias = 8 * SROW;
+        if constexpr (kExperts) {
+            if ((bulk = p.sb_bulk)) {
+                sb_half = 16 * ((uint32_t)p.K >> p.gshift);
+                sb_bias = 2 * sb_half;
+            }
+        }
         uint32_t sa = sa0, bar = full, ph = 0;
         bool ok = true;
         auto next_stage = [&]() {
@@ -677,11 +726,19 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             }
             // this lane's scales in a stage, from its weights: its group (the zeros behind the row's last one where K ends before
             // it) in the row's pieces, which begin up to 14 bytes ahead of the chunk's first one (the same for rows 8 apart)
-            uint32_t sb_lane;
+            uint32_t sb_lane, sb_keep[SPL];  // sb_keep: 0 for a group behind K (bulk copies have the next row's there)
             {
                 const int kb0 = wk.c * p.kbc, gpr = p.K >> p.gshift, g0 = kb0 * KB >> p.gshift, gi = min(((kb0 + kq) * KB + t * KL) >> p.gshift, gpr);
                 const uint32_t n = tile_row(wk.b0 + tsub) + g;
-                sb_lane = p.sb_off + tsub * (32 * SROW - p.tile_bytes) + g * SROW + ((uint32_t)((n * gpr + g0) * 2) & 15u) + 2 * (gi - g0) - in_tile;
+                if (kExperts && bulk) {
+                    sb_lane = p.sb_off + tsub * (64 * gpr - p.tile_bytes) + g * 2 * gpr + 2 * gi - in_tile;
+#pragma unroll
+                    for (int i = 0; i < SPL; i++) sb_keep[i] = gi + i < gpr ? 0xFFFFu : 0u;
+                } else {
+                    sb_lane = p.sb_off + tsub * (32 * SROW - p.tile_bytes) + g * SROW + ((uint32_t)((n * gpr + g0) * 2) & 15u) + 2 * (gi - g0) - in_tile;
+#pragma unroll
+                    for (int i = 0; i < SPL; i++) sb_keep[i] = 0xFFFFu;
+                }
             }
 #pragma unroll 1
             for (int gi = 0; gi < mine; gi++) {
@@ -691,8 +748,13 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 for (int r = 0; r < 2; r++)
 #pragma unroll
                     for (int i = 0; i < SPL; i++) {
-                        s[r][i] = lds_u16(sa + sb_lane + 2 * i + r * 16 * SROW);
-                        b[r][i] = lds_u16(sa + sb_lane + 2 * i + r * 16 * SROW + 8 * SROW);
+                        if constexpr (kExperts) {
+                            s[r][i] = lds_u16(sa + sb_lane + 2 * i + r * sb_half) & sb_keep[i];
+                            b[r][i] = lds_u16(sa + sb_lane + 2 * i + r * sb_half + sb_bias) & sb_keep[i];
+                        } else {
+                            s[r][i] = lds_u16(sa + sb_lane + 2 * i + r * 16 * SROW);
+                            b[r][i] = lds_u16(sa + sb_lane + 2 * i + r * 16 * SROW + 8 * SROW);
+                        }
                     }
 #pragma unroll
                 for (int r = 0; r < 2; r++)
@@ -747,7 +809,10 @@ bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl, int experts =
     pl->kbc = (pl->nkb + pl->nch - 1) / pl->nch;
     pl->nch = (pl->nkb + pl->kbc - 1) / pl->kbc;
     pl->tile_bytes = pl->kbc * 2048;
-    const int sb = 32 * sb_row(a.bits == 4 && a.group == 32 ? 2 : 1), xs = kWarps * x_frags(a.bits) * 512 / (mt == 1 ? 2 : 1), bars = 8 * 3 * kMaxStages;
+    // bulk copies of scales where a stage holds several tiles; one long tile's leave the warp time enough, and their rows meet in the same banks
+    // (64 experts x 4 rows: 1408 x 4096 54.8 us against 81.3, 2048 x 4096 65.4 against 70.3; 4096 x 4096 113.6 against 101.6)
+    pl->sb_bulk = experts && pl->kbc <= kWarps / 2 && pl->nch == 1 && a.N % 16 == 0;
+    const int sb = pl->sb_bulk ? 64 * (a.K / a.group) : 32 * sb_row(a.bits == 4 && a.group == 32 ? 2 : 1), xs = kWarps * x_frags(a.bits) * 512 / (mt == 1 ? 2 : 1), bars = 8 * 3 * kMaxStages;
     // K in one chunk: nothing is kept per tile (4096: as far as Walk::groups divides exactly); in several: the tiles' running sums
     pl->tb = std::min(tiles_max, pl->nch == 1 ? 4096 : 16 * 1024 / (mt * 512));
     const int run = pl->nch == 1 ? 0 : pl->tb * mt * 512;
@@ -812,14 +877,16 @@ cudaError_t launch_t(const Params<NI, EPI>& p, const Plan& pl, cudaStream_t stre
 
 template <int BITS, int SPL, int NI, int EPI>
 cudaError_t launch_rows(const Params<NI, EPI>& p, const Plan& pl, int mmax, int pro, cudaStream_t stream, bool overlap_prev) {
-    if constexpr (NI != 0) {
+    if constexpr (NI == kGroups) {
+        return launch_t<BITS, 1, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
+    } else if constexpr (NI != 0) {
         constexpr int P1 = NI == 1 && EPI == 0 ? 1 : 0, P2 = NI == 1 && EPI == 0 ? 2 : 0;  // (prologues: single calls without an epilogue only)
         if (mmax <= 8)
             return pro == 1   ? launch_t<BITS, 1, SPL, P1, NI, EPI>(p, pl, stream, overlap_prev)
                    : pro == 2 ? launch_t<BITS, 1, SPL, P2, NI, EPI>(p, pl, stream, overlap_prev)
                               : launch_t<BITS, 1, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
     }
-    return launch_t<BITS, 2, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
+    if constexpr (NI != kGroups) return launch_t<BITS, 2, SPL, 0, NI, EPI>(p, pl, stream, overlap_prev);
 }
 template <int NI, int EPI>
 cudaError_t launch_bits(const Params<NI, EPI>& p, const Plan& pl, int bits, int group, int mmax, int pro, cudaStream_t stream, bool overlap_prev) {
@@ -865,18 +932,16 @@ cudaError_t launch_items(const QmmArgs* items, int n, int mmax, const Plan& pl, 
 }
 
 // ---- experts ----
-// Rows of an item: 8 as long as an expert has four rows on average or fewer, else 16 (which takes 1.3 times as long per weight, and eight
-// twice where there are more than eight).
-int group_rows(const ExpertsArgs& a) { return a.rows <= (size_t)4 * a.experts ? 8 : 16; }
 QmmArgs one_expert(const ExpertsArgs& a) {
     QmmArgs q{a.x, a.wq, a.scales, a.biases, a.y, 0, a.K, a.N, a.bits, a.group, (int)LUX_DTYPE_BFLOAT16, (int)LUX_DTYPE_BFLOAT16, a.y_dtype};
     q.error = a.error;
     return q;
 }
 template <int EPI>
-cudaError_t launch_experts(const ExpertsArgs& a, const Plan& pl, const CUtensorMap& map, cudaStream_t stream, bool overlap_prev) {
+cudaError_t launch_experts(const ExpertsArgs& a, const Plan& pl, const CUtensorMap& map, const CUtensorMap& map_end, cudaStream_t stream, bool overlap_prev) {
     Params<kGroups, EPI> p;
     p.maps[0] = map;
+    p.map_end = map_end;
     fill_plan(p, one_expert(a), pl);
     p.n_items = 0;  // (known on the device)
     p.x_early = 0; p.x_ld = a.K; p.eps = 0.0f;
@@ -887,8 +952,8 @@ cudaError_t launch_experts(const ExpertsArgs& a, const Plan& pl, const CUtensorM
     p.act = a.act;
     p.r_bf16 = 0;
     p.offsets = a.offsets; p.order = a.order; p.experts = a.experts; p.rows = (int)a.rows; p.x_rows = (int)a.x_rows;
-    p.n_rt = pl.n_rt; p.most = (int)(a.rows / group_rows(a)) + a.experts; p.tables_off = (int)pl.smem - 8 * (a.experts + 1); p.top_k = a.order ? a.top_k : 1;
-    return launch_bits<kGroups, EPI>(p, pl, a.bits, a.group, group_rows(a), 0, stream, overlap_prev);
+    p.n_rt = pl.n_rt; p.most = (int)(a.rows / kGroupRows) + a.experts; p.sb_bulk = pl.sb_bulk; p.tables_off = (int)pl.smem - 8 * (a.experts + 1); p.top_k = a.order ? a.top_k : 1;
+    return launch_bits<kGroups, EPI>(p, pl, a.bits, a.group, kGroupRows, 0, stream, overlap_prev);
 }
 
 }  // namespace
@@ -914,36 +979,34 @@ cudaError_t launch_qmv_stream(const QmmArgs& a, const QmvStreamPlan& pl, cudaStr
 bool qmv_experts_supported(const ExpertsArgs& a, int sm_count) {
     Plan pl;
     // (a CTA's share of the row tiles is counted in 32 bits)
-    return make_plan(one_expert(a), group_rows(a), sm_count, &pl, a.experts) && (long long)(a.rows / 8 + a.experts) * pl.n_rt / sm_count < (1ll << 30);
+    return make_plan(one_expert(a), kGroupRows, sm_count, &pl, a.experts) && (long long)(a.rows / 8 + a.experts) * pl.n_rt / sm_count < (1ll << 30);
 }
 
 cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, const char** name) {
     Plan pl;
     const EncodeTiledFn encode = encode_tiled_fn();
-    if (!encode || !make_plan(one_expert(a), group_rows(a), sm_count, &pl, a.experts)) return cudaErrorInvalidValue;
+    if (!encode || !make_plan(one_expert(a), kGroupRows, sm_count, &pl, a.experts)) return cudaErrorInvalidValue;
     // The packed weights [expert][half][row][byte], a tile being eight rows of either half, or 16 of the only one: boxes as encode_weights'
     const cuuint64_t row_bytes = (cuuint64_t)a.K * a.bits / 8, halves = a.gated ? 2 : 1, rows = a.N / halves;
     const cuuint32_t estr[4] = {1, 1, 1, 1}, box_rows = 16 / (cuuint32_t)halves;
-    CUtensorMap map;
-    CUresult r;
-    if (row_bytes % 128 == 0) {
-        const cuuint64_t dims[4] = {128, rows, halves * a.experts, row_bytes / 128}, strides[3] = {row_bytes, rows * row_bytes, 128};
-        const cuuint32_t box[4] = {128, box_rows, (cuuint32_t)halves, (cuuint32_t)pl.kbc};
-        r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    } else {
-        const cuuint64_t dims[3] = {row_bytes, rows, halves * a.experts}, strides[2] = {row_bytes, rows * row_bytes};
-        const cuuint32_t box[3] = {128, box_rows, (cuuint32_t)halves};
-        r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    CUtensorMap map, map_end;
+    const cuuint64_t dims[4] = {128, rows, halves * a.experts, (row_bytes + 127) / 128}, strides[3] = {row_bytes, rows * row_bytes, 128};
+    const cuuint32_t box[4] = {128, box_rows, (cuuint32_t)halves, (cuuint32_t)pl.kbc};
+    CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    map_end = map;
+    if (r == CUDA_SUCCESS && row_bytes % 128) {  // (see GroupParams::map_end)
+        const cuuint64_t edims[3] = {row_bytes, rows, halves * a.experts}, estrides[2] = {row_bytes, rows * row_bytes};
+        const cuuint32_t ebox[3] = {128, box_rows, (cuuint32_t)halves};
+        r = encode(&map_end, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint32_t*>(a.wq), edims, estrides, ebox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     }
     if (r != CUDA_SUCCESS) {
         set_last_error("cuTensorMapEncodeTiled (experts' weights) failed (%d)", (int)r);
         return cudaErrorInvalidValue;
     }
-    const bool m8 = group_rows(a) == 8;
-    *name = a.bits == 4 ? (m8 ? "qmv_experts<4,m8>" : "qmv_experts<4,m16>") : (m8 ? "qmv_experts<8,m8>" : "qmv_experts<8,m16>");
-    return a.gated ? launch_experts<2>(a, pl, map, stream, overlap_prev) : launch_experts<1>(a, pl, map, stream, overlap_prev);
+    *name = a.bits == 4 ? "qmv_experts<4>" : "qmv_experts<8>";
+    return a.gated ? launch_experts<2>(a, pl, map, map_end, stream, overlap_prev) : launch_experts<1>(a, pl, map, map_end, stream, overlap_prev);
 }
 
 cudaError_t launch_qmv_stream_batch(const QmmArgs* items, int n, int sm_count, cudaStream_t stream) {
