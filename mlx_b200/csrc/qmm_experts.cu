@@ -297,28 +297,26 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                     tmem_ld_16x256b_x2(quarter + blk * 16, v[0]);
                     tmem_ld_16x256b_x2(quarter + (16u << 16) + blk * 16, v[1]);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    float o[2][4];  // rows of x: 2(t%4), the next, and those eight further on
+                    float o[8];  // two columns of y times rows of x: 2(t%4), the next, and those eight further on
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int k = 0; k < 8; k++) o[k] = __uint_as_float(v[k >> 2][(k >> 1 & 1) * 4 + (k & 1)]) + bg[k >> 2];
+                    activate(p.act, o);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int at = (i >> 1) * 4 + (i & 1);
-                            o[j][i] = activate(p.act, __uint_as_float(v[j][at]) + bg[j]) * (__uint_as_float(v[j][at + 2]) + bu[j]);
-                        }
+                    for (int k = 0; k < 8; k++) o[k] *= __uint_as_float(v[k >> 2][(k >> 1 & 1) * 4 + (k & 1) + 2]) + bu[k >> 2];
                     const int m = seg.m0 + blk * 16, rows = seg.rows - blk * 16;
                     if (staged) {
 #pragma unroll
                         for (int j = 0; j < 2; j++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                *reinterpret_cast<__nv_bfloat16*>(sEpi + (blk * 16 + (i >> 1) * 8 + (lane & 3) * 2 + (i & 1)) * kYPitch + (q * 16 + j * 8 + (lane >> 2)) * 2) = __float2bfloat16_rn(o[j][i]);
+                                *reinterpret_cast<__nv_bfloat16*>(sEpi + (blk * 16 + (i >> 1) * 8 + (lane & 3) * 2 + (i & 1)) * kYPitch + (q * 16 + j * 8 + (lane >> 2)) * 2) = __float2bfloat16_rn(o[4 * j + i]);
                     } else if (!PAIR && p.y_vec) {
                         // [16 rows of x][16 columns] through shared memory: a lane stores eight columns of a row
 #pragma unroll
                         for (int j = 0; j < 2; j++)
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                *reinterpret_cast<__nv_bfloat16*>(stg + ((i >> 1) * 8 + (lane & 3) * 2 + (i & 1)) * 32 + j * 16 + (lane >> 2) * 2) = __float2bfloat16_rn(o[j][i]);
+                                *reinterpret_cast<__nv_bfloat16*>(stg + ((i >> 1) * 8 + (lane & 3) * 2 + (i & 1)) * 32 + j * 16 + (lane >> 2) * 2) = __float2bfloat16_rn(o[4 * j + i]);
                         __syncwarp();
                         const int row = lane >> 1, col = tile_n * 64 + q * 16 + (lane & 1) * 8;
                         if (row < rows && col < F)
@@ -331,8 +329,8 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                                 const int row = (i >> 1) * 8 + (lane & 3) * 2 + (i & 1);
                                 if (row >= rows || f[j] >= F) continue;
                                 const size_t at = (size_t)(m + row) * ld + f[j];
-                                if (p.y_bf16) static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(o[j][i]);
-                                else static_cast<float*>(p.y)[at] = o[j][i];
+                                if (p.y_bf16) static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(o[4 * j + i]);
+                                else static_cast<float*>(p.y)[at] = o[4 * j + i];
                             }
                     }
                 }
@@ -346,14 +344,16 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                     __syncwarp();
                     tmem_ld16(quarter + blk * 16, v);
                     const int m = seg.m0 + blk * 16, rows = seg.rows - blk * 16;
+                    float o[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) v[j] = __float_as_uint(activate(p.act, __uint_as_float(v[j]) + b));
+                    for (int j = 0; j < 16; j++) o[j] = __uint_as_float(v[j]) + b;
+                    activate(p.act, o);
                     if (staged) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) *reinterpret_cast<__nv_bfloat16*>(sEpi + (blk * 16 + j) * kYPitch + (q * 32 + lane) * 2) = __float2bfloat16_rn(__uint_as_float(v[j]));
+                        for (int j = 0; j < 16; j++) *reinterpret_cast<__nv_bfloat16*>(sEpi + (blk * 16 + j) * kYPitch + (q * 32 + lane) * 2) = __float2bfloat16_rn(o[j]);
                     } else if (!PAIR && p.y_vec) {
 #pragma unroll
-                        for (int j = 0; j < 16; j++) *reinterpret_cast<__nv_bfloat16*>(stg + j * 64 + lane * 2) = __float2bfloat16_rn(__uint_as_float(v[j]));
+                        for (int j = 0; j < 16; j++) *reinterpret_cast<__nv_bfloat16*>(stg + j * 64 + lane * 2) = __float2bfloat16_rn(o[j]);
                         __syncwarp();
                         const int col = tile_n * kTileN + q * 32 + (lane & 3) * 8;
 #pragma unroll
@@ -367,8 +367,8 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                         for (int j = 0; j < 16; j++) {
                             if (j >= rows) continue;
                             const size_t at = (size_t)(m + j) * ld + n;
-                            if (p.y_bf16) static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(__uint_as_float(v[j]));
-                            else static_cast<float*>(p.y)[at] = __uint_as_float(v[j]);
+                            if (p.y_bf16) static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(o[j]);
+                            else static_cast<float*>(p.y)[at] = o[j];
                         }
                     }
                 }

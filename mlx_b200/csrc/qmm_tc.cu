@@ -72,19 +72,29 @@ struct GemmParams {
 // The epilogue of qmatmul_epi on CNT rows of x from row m (of which `rows` are there) of column n: act(sum + bias) + residual.  The lanes of a warp
 // hold neighbouring columns: a residual row is read in whole 64- or 128-byte pieces, CNT of them under way.
 template <int CNT>
-__device__ __forceinline__ void finish(const GemmParams& p, uint32_t* v, int m, int rows, int n) {
+__device__ __forceinline__ void finish(const GemmParams& p, uint32_t (&raw)[CNT], int m, int rows, int n) {
     if (n >= p.N) return;
-    const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
-    float r[CNT];
+    float r[CNT], v[CNT];
+    const size_t at = (size_t)m * p.N + n;
+    if (p.residual && p.r_bf16) {
+        const uint16_t* q = static_cast<const uint16_t*>(p.residual) + at;
 #pragma unroll
-    for (int j = 0; j < CNT; j++) {
-        const size_t at = (size_t)(m + j) * p.N + n;
-        r[j] = !p.residual || j >= rows ? 0.0f
-               : p.r_bf16              ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.residual)[at])
-                                       : static_cast<const float*>(p.residual)[at];
+        for (int j = 0; j < CNT; j++, q += p.N) r[j] = j < rows ? __uint_as_float((uint32_t)*q << 16) : 0.0f;
+    } else if (p.residual) {
+        const float* q = static_cast<const float*>(p.residual) + at;
+#pragma unroll
+        for (int j = 0; j < CNT; j++, q += p.N) r[j] = j < rows ? *q : 0.0f;
+    }
+    const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < CNT; j++) v[j] = __uint_as_float(raw[j]) + b;
+    activate(p.act, v);
+    if (p.residual) {
+#pragma unroll
+        for (int j = 0; j < CNT; j++) v[j] += r[j];
     }
 #pragma unroll
-    for (int j = 0; j < CNT; j++) v[j] = __float_as_uint(activate(p.act, __uint_as_float(v[j]) + b) + r[j]);
+    for (int j = 0; j < CNT; j++) raw[j] = __float_as_uint(v[j]);
 }
 
 // The work of a launch is the sequence of (tile, k-stage) units, tile after tile.  Two schedules:
@@ -393,7 +403,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                                 for (int j = 0; j < 16; j++) pv[j] = __ldcg(ws + (size_t)j * kTileN);
                             }
                         }
-                        if constexpr (EPI) finish<16>(p, v, m0 + c0, m_end - c0, n);
+                        if constexpr (EPI) finish<16>(p, reinterpret_cast<uint32_t(&)[16]>(v), m0 + c0, m_end - c0, n);
                         store_rows(v, c0, 16);
                     }
                 }

@@ -558,13 +558,14 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                             sts_v4(run, s);
                         } else {
                             if constexpr (EPI == 1) {
-                                s.x = __float_as_uint(activate(p.act, __uint_as_float(s.x) + bias[0]) + res[0][0]);
-                                s.y = __float_as_uint(activate(p.act, __uint_as_float(s.y) + bias[0]) + res[0][1]);
-                                s.z = __float_as_uint(activate(p.act, __uint_as_float(s.z) + bias[1]) + res[1][0]);
-                                s.w = __float_as_uint(activate(p.act, __uint_as_float(s.w) + bias[1]) + res[1][1]);
+                                float o[4] = {__uint_as_float(s.x) + bias[0], __uint_as_float(s.y) + bias[0], __uint_as_float(s.z) + bias[1], __uint_as_float(s.w) + bias[1]};
+                                activate(p.act, o);
+                                s = make_uint4(__float_as_uint(o[0] + res[0][0]), __float_as_uint(o[1] + res[0][1]), __float_as_uint(o[2] + res[1][0]), __float_as_uint(o[3] + res[1][1]));
                             } else if constexpr (kGated) {
-                                s.x = __float_as_uint(activate(p.act, __uint_as_float(s.x) + bias[0]) * (__uint_as_float(s.z) + bias[1]));
-                                s.y = __float_as_uint(activate(p.act, __uint_as_float(s.y) + bias[0]) * (__uint_as_float(s.w) + bias[1]));
+                                float o[2] = {__uint_as_float(s.x) + bias[0], __uint_as_float(s.y) + bias[0]};
+                                activate(p.act, o);
+                                s.x = __float_as_uint(o[0] * (__uint_as_float(s.z) + bias[1]));
+                                s.y = __float_as_uint(o[1] * (__uint_as_float(s.w) + bias[1]));
                             }
                             const int n = (tile0 + ti) * (kGated ? 8 : 16) + n0, m = mt * 8 + m0;
                             const bool two = !kGated && n + 8 < p.N;
