@@ -28,6 +28,7 @@ struct GemmShape {
     int M, K, N, bits, group;
     bool y_bf16, sharded;
     int ld, col0;
+    bool residual = false;  // qmatmul_epi with a residual
 };
 struct GemmForce {  // overrides: 0, 1, or -1 for the plan's own choice
     int streamk = -1;  // stream-K or whole tiles
@@ -52,6 +53,8 @@ struct GemmPlan {
 //   whole tiles: ceil(T/G) rounds, each with an epilogue of 3 * bm/256 that nothing else overlaps;
 //   CTA pairs:   rounds of pair tiles; the epilogue overlaps where y leaves by TMA; 3 to set up;
 //   stream-K:    T*nst/G stages of up to 1.6 times the cost, an epilogue more, and the exchange of partials.
+// A residual makes every epilogue longer, least where it is no more than that of whole tiles of one CTA (2048 x 4096 x 4096, bf16: 61.8 us; pairs,
+// whose stores no longer hide it, 66.1; stream-K, which spills, 109; 64 rows 24.7, 26.9, 27.1).
 inline bool choose_gemm_plan(const GemmShape& a, int sm_count, const GemmForce& force, bool no_ytma, GemmPlan* pl) {
     pl->n_tiles = (a.N + kTileN - 1) / kTileN;
     const double G = sm_count, nst = (a.K / kBK + kSub - 1) / kSub;
@@ -68,14 +71,14 @@ inline bool choose_gemm_plan(const GemmShape& a, int sm_count, const GemmForce& 
             const double h = bm / 256.0, stage = 0.45 + 0.001 * bm, e = 3.0 * h, T = (double)pl->n_tiles * mt, rounds = std::ceil(T / G);
             double cost;
             if (k == 0) {
-                cost = rounds * (nst * stage + e);
+                cost = rounds * (nst * stage + e + (a.residual ? 3.0 * h : 0.0));
             } else if (k == 1) {
                 if (sm_count & 1) continue;
                 const double prounds = std::ceil((pl->n_tiles + 1) / 2 * (double)mt / (sm_count / 2));
-                cost = 3.0 + prounds * (nst * stage + (y_fast ? 0.5 : e));
+                cost = 3.0 + prounds * (nst * stage + (y_fast ? 0.5 : e) + (a.residual ? 6.0 * h : 0.0));
             } else {
                 if (T * nst < G && !(force.streamk == 1 && mt == m0)) continue;
-                cost = 2.0 + (1.1 + 0.5 * h) * T * nst / G * stage + (rounds + 1.0) * e + 4.0 * h * (T < G ? std::ceil(G / T) : 1.0);
+                cost = 2.0 + (1.1 + 0.5 * h) * T * nst / G * stage + (rounds + 1.0) * e + 4.0 * h * (T < G ? std::ceil(G / T) : 1.0) + (a.residual ? (rounds + 1.0) * 10.0 * h : 0.0);
             }
             if (found && cost >= best) continue;
             found = true;

@@ -69,32 +69,82 @@ struct GemmParams {
     int act, r_bf16;
 };
 
-// The epilogue of qmatmul_epi on CNT rows of x from row m (of which `rows` are there) of column n: act(sum + bias) + residual.  The lanes of a warp
-// hold neighbouring columns: a residual row is read in whole 64- or 128-byte pieces, CNT of them under way.
-template <int CNT>
-__device__ __forceinline__ void finish(const GemmParams& p, uint32_t (&raw)[CNT], int m, int rows, int n) {
-    if (n >= p.N) return;
-    float r[CNT], v[CNT];
+// ---- the epilogue of qmatmul_epi: act(sum + bias) + residual ----
+// The residual is the tile's size again in bytes, read by the warps that nothing overlaps: into L2 while the tile's MMAs run, then sixteen rows ahead
+// of the accumulator.  (Neither, 32 rows at a time: 2048 x 4096 x 4096 onto an fp32 stream 117 us, without the stream 61.)
+//
+// All epilogue threads, ahead of their wait for the accumulator: the rows [m0, m0 + rows) of the tile's columns from n0 on into L2, a row per copy.
+__device__ __forceinline__ void prefetch_residual(const GemmParams& p, int m0, int rows, int n0, int thread) {
+    const size_t es = p.r_bf16 ? 2 : 4;
+    if (!p.residual || n0 >= p.N || ((uintptr_t)p.residual | p.N * es) & 15) return;
+    const uint32_t bytes = (uint32_t)(min(kTileN, p.N - n0) * es);  // (a multiple of 16, as the rows are)
+    for (int row = thread; row < rows; row += kEpiWarps * 32)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(static_cast<const char*>(p.residual) + ((size_t)(m0 + row) * p.N + n0) * es), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t ldg_u16_plain(const uint16_t* p) {  // (not .nc: y may be the residual)
+    uint32_t v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// Column n of the residual, rows m .. m + 15 (of which `rows` are there), as it lies: converted here, each load would be waited for ahead of the next
+__device__ __forceinline__ void load_residual(const GemmParams& p, int m, int rows, int n, uint32_t (&r)[16]) {
+    if (!p.residual || n >= p.N) return;
     const size_t at = (size_t)m * p.N + n;
-    if (p.residual && p.r_bf16) {
+    if (p.r_bf16) {
         const uint16_t* q = static_cast<const uint16_t*>(p.residual) + at;
 #pragma unroll
-        for (int j = 0; j < CNT; j++, q += p.N) r[j] = j < rows ? __uint_as_float((uint32_t)*q << 16) : 0.0f;
-    } else if (p.residual) {
-        const float* q = static_cast<const float*>(p.residual) + at;
+        for (int j = 0; j < 16; j++, q += p.N) r[j] = j < rows ? ldg_u16_plain(q) : 0u;
+    } else {
+        const uint32_t* q = static_cast<const uint32_t*>(p.residual) + at;
 #pragma unroll
-        for (int j = 0; j < CNT; j++, q += p.N) r[j] = j < rows ? *q : 0.0f;
+        for (int j = 0; j < 16; j++, q += p.N) r[j] = j < rows ? *q : 0u;
     }
-    const float b = p.bias ? __ldg(p.bias + n) : 0.0f;
+}
+__device__ __forceinline__ void finish(const GemmParams& p, uint32_t* raw, const uint32_t (&r)[16], float bias) {
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < CNT; j++) v[j] = __uint_as_float(raw[j]) + b;
+    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(raw[j]) + bias;
     activate(p.act, v);
     if (p.residual) {
 #pragma unroll
-        for (int j = 0; j < CNT; j++) v[j] += r[j];
+        for (int j = 0; j < 16; j++) v[j] += __uint_as_float(r[j] << (p.r_bf16 ? 16 : 0));
     }
 #pragma unroll
-    for (int j = 0; j < CNT; j++) raw[j] = __float_as_uint(v[j]);
+    for (int j = 0; j < 16; j++) raw[j] = __float_as_uint(v[j]);
+}
+// A warp's share of a tile, rows [c_lo, c_hi) of x (whole sixteens; m_end of the tile's rows are there) of its lanes' columns n: put(sums, row of the tile)
+// takes sixteen at a time.
+template <class Put>
+__device__ __forceinline__ void finish_rows(const GemmParams& p, uint32_t lanes, int c_lo, int c_hi, int m0, int m_end, int n, const Put& put) {
+    const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f;
+    uint32_t r[16], next[16];
+    load_residual(p, m0 + c_lo, m_end - c_lo, n, next);
+    for (int c0 = c_lo; c0 < min(c_hi, m_end); c0 += 16) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) r[j] = next[j];
+        if (c0 + 16 < c_hi) load_residual(p, m0 + c0 + 16, m_end - c0 - 16, n, next);
+        uint32_t v[16];
+        __syncwarp();
+        tmem_ld16(lanes + c0, v);
+        finish(p, v, r, bias);
+        put(v, c0);
+    }
+}
+// sixteen rows straight to y (one copy of it)
+__device__ __forceinline__ void put_direct(const GemmParams& p, const uint32_t* v, int m, int rows, int n) {
+    if (n >= p.N) return;
+    const size_t at = (size_t)m * p.N + n;
+    if (p.y_bf16) {
+        __nv_bfloat16* q = static_cast<__nv_bfloat16*>(p.y) + at;
+#pragma unroll
+        for (int j = 0; j < 16; j++, q += p.N)
+            if (j < rows) *q = __float2bfloat16_rn(__uint_as_float(v[j]));
+    } else {
+        float* q = static_cast<float*>(p.y) + at;
+#pragma unroll
+        for (int j = 0; j < 16; j++, q += p.N)
+            if (j < rows) *q = __uint_as_float(v[j]);
+    }
 }
 
 // The work of a launch is the sequence of (tile, k-stage) units, tile after tile.  Two schedules:
@@ -263,6 +313,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
             const int tile = seg.tile(), s_lo = seg.s_lo(), s_hi = seg.s_hi();
             const int n = (tile / p.m_tiles) * kTileN + nl;
             const int m0 = (tile % p.m_tiles) * p.bm;
+            if (EPI && s_lo == 0) prefetch_residual(p, m0, min(p.bm, p.M - m0), n - nl, et);
             if (!mbar_wait(&sl->tmem_full, tile_i & 1, abort_flag)) break;
             tc_fence_after();
             const int m_end = min(p.bm, p.M - m0);
@@ -366,13 +417,17 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                         }
                     }
                 };
-                if (parts == 0 && y_vec) {
+                if (EPI && parts == 0) {
+                    finish_rows(p, tmem_base + ((uint32_t)(q * 32) << 16), blk_lo * 32, blk_hi * 32, m0, m_end, n, [&](uint32_t* v, int c0) {
+                        if (y_vec) store_rows(v, c0, 16);
+                        else put_direct(p, v, m0 + c0, m_end - c0, n);
+                    });
+                } else if (parts == 0 && y_vec) {
                     // (requesting the next sixteen columns before the current ones are stored was tried: 3 % slower)
                     for (int c0 = blk_lo * 32; c0 < blk_hi * 32; c0 += 16) {
                         uint32_t v[16];
                         __syncwarp();
                         tmem_ld16(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
-                        if constexpr (EPI) finish<16>(p, v, m0 + c0, m_end - c0, n);
                         store_rows(v, c0, 16);
                     }
                 } else if (parts == 0) {
@@ -380,7 +435,6 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                         uint32_t v[32];
                         __syncwarp();
                         tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + blk * 32, v);
-                        if constexpr (EPI) finish<32>(p, v, m0 + blk * 32, m_end - blk * 32, n);
                         store_rows(v, blk * 32, 32);
                     }
                 } else {
@@ -403,7 +457,11 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
                                 for (int j = 0; j < 16; j++) pv[j] = __ldcg(ws + (size_t)j * kTileN);
                             }
                         }
-                        if constexpr (EPI) finish<16>(p, reinterpret_cast<uint32_t(&)[16]>(v), m0 + c0, m_end - c0, n);
+                        if constexpr (EPI) {
+                            uint32_t r[16];
+                            load_residual(p, m0 + c0, m_end - c0, n, r);
+                            finish(p, v, r, p.bias && n < p.N ? __ldg(p.bias + n) : 0.0f);
+                        }
                         store_rows(v, c0, 16);
                     }
                 }
@@ -544,16 +602,18 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, tile_i++) {
             const int n = (tile / p.m_tiles) * kTileN + q * 32 + lane;
             const int m0 = (tile % p.m_tiles) * p.bm;
+            if (EPI) prefetch_residual(p, m0, min(p.bm, p.M - m0), (tile / p.m_tiles) * kTileN, tid);
             if (!mbar_wait(&sl->tmem_full, tile_i & 1, abort_flag)) break;
             tc_fence_after();
             // this thread: column n of y, rows m0 + c (32 consecutive n per warp: 64-byte row segments)
             const int m_end = min(p.bm, p.M - m0);
-            for (int blk = blk_lo; blk < blk_hi; blk++) {
+            if (EPI)
+                finish_rows(p, tmem_base + ((uint32_t)(q * 32) << 16), blk_lo * 32, blk_hi * 32, m0, m_end, n, [&](uint32_t* v, int c0) { put_direct(p, v, m0 + c0, m_end - c0, n); });
+            for (int blk = blk_lo; !EPI && blk < blk_hi; blk++) {
                 const int c0 = blk * 32;
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
-                if constexpr (EPI) finish<32>(p, v, m0 + c0, m_end - c0, n);
                 if (n < p.N) {
                     // column-sharded layers: the tile goes into every rank's copy of y (peer stores over NVLink)
                     const size_t idx0 = (size_t)(m0 + c0) * p.ld + p.col0 + n;
@@ -737,6 +797,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         for (int tile = cl; tile < total_tiles; tile += ncl, tile_i++) {
             const int n = n0_of(tile) + q * 32 + lane;
             const int m0 = (tile % p.m_tiles) * p.bm;
+            if (EPI) prefetch_residual(p, m0, min(p.bm, p.M - m0), n0_of(tile), tid);
             if (p.y_tma && tile_i > 0) {
                 // the copy engine has finished reading the previous tile out of the staging buffer
                 if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -747,12 +808,17 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             if (p.y_tma) {
                 // The accumulator goes to shared memory as bf16, [row of x][column], and is released at once; the
                 // copy engine takes the tile to y while the next tile's MMAs run.
-                for (int blk = blk_lo; blk < blk_hi; blk++) {
+                if (EPI)
+                    finish_rows(p, tmem_base + ((uint32_t)(q * 32) << 16), blk_lo * 32, blk_hi * 32, m0, min(p.bm, p.M - m0), n, [&](uint32_t* v, int c0) {
+                        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(sY + (size_t)c0 * 256) + q * 32 + lane;
+#pragma unroll
+                        for (int j = 0; j < 16; j++) dst[j * 128] = __float2bfloat16_rn(__uint_as_float(v[j]));
+                    });
+                for (int blk = blk_lo; !EPI && blk < blk_hi; blk++) {
                     const int c0 = blk * 32;
                     uint32_t v[32];
                     __syncwarp();
                     tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
-                    if constexpr (EPI) finish<32>(p, v, m0 + c0, min(p.bm, p.M - m0) - c0, n);
                     __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(sY + (size_t)c0 * 256) + q * 32 + lane;
 #pragma unroll
                     for (int j = 0; j < 32; j++) dst[j * 128] = __float2bfloat16_rn(__uint_as_float(v[j]));
@@ -791,12 +857,13 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             }
             // this thread: column n of y, rows m0 + c (32 consecutive n per warp: 64-byte row segments)
             const int m_end = min(p.bm, p.M - m0);
-            for (int blk = blk_lo; blk < blk_hi; blk++) {
+            if (EPI)
+                finish_rows(p, tmem_base + ((uint32_t)(q * 32) << 16), blk_lo * 32, blk_hi * 32, m0, m_end, n, [&](uint32_t* v, int c0) { put_direct(p, v, m0 + c0, m_end - c0, n); });
+            for (int blk = blk_lo; !EPI && blk < blk_hi; blk++) {
                 const int c0 = blk * 32;
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + c0, v);
-                if constexpr (EPI) finish<32>(p, v, m0 + c0, m_end - c0, n);
                 if (n < p.N) {
                     // column-sharded layers: the tile goes into every rank's copy of y (peer stores over NVLink)
                     const size_t idx0 = (size_t)(m0 + c0) * p.ld + p.col0 + n;
@@ -884,7 +951,7 @@ bool make_gemm_plan(const QmmArgs& a, int sm_count, const ShardPush* push, GemmP
     GemmForce force;
     if (schedule) force.streamk = schedule[0] == 's';
     if (pair) force.pair = pair[0] == '1';
-    const GemmShape shape{a.M, a.K, a.N, a.bits, a.group, a.y_dtype == LUX_DTYPE_BFLOAT16, push != nullptr, push ? push->ld : a.N, push ? push->col0 : 0};
+    const GemmShape shape{a.M, a.K, a.N, a.bits, a.group, a.y_dtype == LUX_DTYPE_BFLOAT16, push != nullptr, push ? push->ld : a.N, push ? push->col0 : 0, a.residual != nullptr};
     return choose_gemm_plan(shape, sm_count, force, getenv("LUXCUDA_QMM_NO_YTMA") != nullptr, pl) && encode_tiled_fn() != nullptr;
 }
 
