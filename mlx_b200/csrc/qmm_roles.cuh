@@ -206,8 +206,9 @@ __device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s_bits, u
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             if (FAST) {
+                const uint32_t lo = w[c] & 0x0F0F0F0Fu, hi = w[c] & 0xF0F0F0F0u;
 #pragma unroll
-                for (int i = 0; i < 4; i++) out[4 * c + i] = fma_bf16x2(prmt(w[c], 0u, 0x4040u + 0x0101u * i) & 0x00F0000Fu, s2, b2);
+                for (int i = 0; i < 4; i++) out[4 * c + i] = fma_bf16x2(prmt(lo, hi, 0x8480u + 0x1111u * i), s2, b2);
             } else {
                 uint32_t r[4];  // r[i] = (w^_i, w^_{i+4})
                 dequant4_general(w[c], s2, b2, r);
