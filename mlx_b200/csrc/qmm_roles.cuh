@@ -195,9 +195,10 @@ __device__ __forceinline__ uint32_t ldg_u16(const uint16_t* p) {  // zero-extend
 // 32 weights of one row (one scale) -> 16 registers of bf16 pairs in natural k order.
 // The matrix instruction wants neighbours in k side by side, which dequant.cuh's masks do not yield (they pair weights 4
 // apart, and a byte permute per pair put them in order afterwards: 9 integer operations per 8 weights at 4 bit, 10 at 8
-// bit).  Here a permute comes first.  4 bit: byte i of the word into both halves, one mask, q_2i in the low half and
-// 16 * q_2i+1 in the high one, whose scale is 2^-4 of the low one's: 8 operations.  8 bit: two bytes into the two halves,
-// which is all: 4 operations.  The products are the same (see dequant.cuh for the 2^-133 form).
+// bit).  Here a permute puts them there.  4 bit: the low codes of all bytes by one mask, the high ones by another; then byte i of
+// the first into the low half, q_2i, and of the second into the high one, 16 * q_2i+1, whose scale is 2^-4 of the low one's, and
+// above either the first's sign, zero: 6 operations.  8 bit: two bytes into the two halves, which is all: 4 operations.  The
+// products are the same (see dequant.cuh for the 2^-133 form).
 template <int BITS, bool FAST>
 __device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s_bits, uint32_t b_bits, uint32_t (&out)[16]) {
     const uint32_t b2 = dup_bf16(b_bits);
@@ -376,7 +377,8 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
         if (UPS == 2 && more) fetch_sb();
         uint32_t w[WPS], wn[8];  // this sub-block's words; 4 bit: the next one's, from the same unit
         bool ok = true;
-#pragma unroll 1
+        // (one copy of the code for both, where the ring has one slot a group: two cost 512 x 4096 x 4096 21 -> 22 us; with two slots, 3 % faster)
+#pragma unroll (BITS == 4 && SLOTS > 1 ? 2 : 1)
         for (int u = 0; u < kSub; u++) {
             if (UPS == 1 && u >= nsub) break;
             if (UPS == 2 || u == 0) {
