@@ -13,7 +13,7 @@ struct ExpertsShape {
     int experts, K, N, bits;
     bool gather;  // rows of x are fetched by index
 };
-constexpr int kPairMean = 65;  // rows an expert on average from which on the GEMM runs on pairs of CTAs
+constexpr int kPairMean = 80;  // rows an expert on average from which on the GEMM runs on pairs of CTAs
 inline bool experts_in_pairs(const ExpertsShape& s, int sm_count) {
     const size_t mean = (s.rows + s.experts - 1) / s.experts;
     return sm_count % 2 == 0 && s.N > 128 && mean >= (size_t)kPairMean;
@@ -43,10 +43,9 @@ inline bool experts_have_many_rows(const ExpertsShape& s, int sm_count) {
     return many < few;
 }
 
-// The GEMM: stages of its ring (see qmm_experts.cu), rows of x per tile, at most.
-constexpr int stages(bool pair) { return pair ? 3 : 6; }
-constexpr int kLowRows = 128, kTwoAccRows = 64;  // tiles of single CTAs; with two accumulators
-constexpr int y_pitch(bool gated) { return (gated ? kTileN / 2 : kTileN) * 2 + 16; }  // of a finished tile in shared memory, bytes a row of x
+constexpr int kExpertStages = 4, kExpertGroups = 4, kExpertEpis = 4;  // of the GEMM (see qmm_experts.cu)
+constexpr int kLowRows = 128;                                         // rows of x of a single CTA's tile, at most: half an accumulator's columns
+constexpr int y_pitch(bool gated) { return gated ? kTileN + 16 : 2 * kTileN; }  // of a finished tile in shared memory, bytes a row of x (gated: off the banks)
 struct ExpertsPlan {
     int bm, box, w_slots, n_tiles;  // box: rows of x per TMA box, a divisor of what a CTA fetches; n_tiles: of pairs two
     bool pair, y_staged;
@@ -65,9 +64,9 @@ inline ExpertsPlan plan_experts(const ExpertsShape& s, bool gated, bool y_pieces
     p.w_slots = s.bits == 8 ? 2 : 1;
     const int step = p.pair ? 32 : 16;
     p.bm = (int)std::min<size_t>(p.pair ? kMaxBM : kLowRows, std::max<size_t>(32, (2 * mean + step - 1) / step * step));
-    for (;; p.bm -= step) {  // (single CTAs: 8 bit and long tables cost some rows)
-        p.smem = 1024 + kGemmCtlBytes + (size_t)stages(p.pair) * kSub * (p.pair ? p.bm / 2 : p.bm) * 128 + (size_t)p.w_slots * kDqGroups * kWUnitBytes +
-                 (p.pair ? (size_t)(p.y_staged ? p.bm * y_pitch(gated) : 0) : (size_t)kEpiWarps * kEpiStageBytes) + (size_t)8 * (s.experts + 1);
+    for (;; p.bm -= step) {  // (pairs without a gate: their finished tiles cost some rows, at 8 bit more)
+        p.smem = 1024 + kGemmCtlBytes + (size_t)kExpertStages * kSub * (p.pair ? p.bm / 2 : p.bm) * 128 + (size_t)p.w_slots * kExpertGroups * kWUnitBytes +
+                 (p.pair ? (size_t)(p.y_staged ? p.bm * y_pitch(gated) : 0) : (size_t)kExpertEpis * kEpiStageBytes) + (size_t)8 * (s.experts + 1);
         if (p.smem <= (size_t)kGemmSmemLimit) break;
     }
     const int half = p.pair ? p.bm / 2 : p.bm;  // rows a CTA fetches

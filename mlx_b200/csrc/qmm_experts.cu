@@ -6,7 +6,7 @@
 //     bm allows, all of one height), then takes every gridDim.x-th tile of the whole list; neighbouring CTAs share an expert's weights or
 //     rows of x at the same time.
 //   * Many rows an expert: pairs of CTAs (cta_group::2), each with half of the rows of x and 128 rows of W of its own; the finished tile goes through
-//     shared memory, so that the next one's MMAs run while it is stored.  Fewer: single CTAs with twice as many stages.
+//     shared memory, so that the next one's MMAs run while it is stored.  Fewer: single CTAs with two accumulators.
 //   * The matrix instruction's N is the tile's own height, rounded up to 16: a tile of 40 rows takes 48 rows' time.
 //   * Rows of x come by TMA, a box of 16 to 64 rows per lane of a warp.  With an order they are copied side by side first, a launch of its own
 //     (2048 tokens x 8 experts x 4096: 134 MB, 27 us).  Fetched by index in here they cost more, since every tile of W does it again: TMA gathers of
@@ -28,12 +28,14 @@ namespace luxcuda {
 
 namespace {
 
-// A ring of stages: A in tensor memory (64 columns a stage), B in shared memory.  Low tiles leave room for twice as many, two to a group of
-// dequantising warps, which then does not wait for the MMAs of its last stage before it writes the next; and tiles of up to 64 rows for a
-// second accumulator, whose MMAs run under the epilogue of the first.
-constexpr uint32_t acc_cols(bool pair) { return pair ? 256 : 128; }  // of tensor memory; the ring lies behind them
-static_assert(stages(true) % kDqGroups == 0 && stages(false) % kDqGroups == 0, "a group always owns the same slots");
-static_assert(acc_cols(true) + stages(true) * kAColsPerSlot <= kTmemCols && acc_cols(false) + stages(false) * kAColsPerSlot <= kTmemCols, "tensor memory");
+// Four groups of dequantising warps and four epilogue warps (qmm_tc.cu: three and eight, as many threads): what bounds tiles that are not high is how
+// fast a group gets through a stage (0.43 us of 0.47 for three groups; without the tensor cores' part no less, without dequantisation 0.37), and the epilogue
+// has a second accumulator or a copy in shared memory to run beside.  Stages as groups: A in tensor memory, 64 columns each, behind the accumulators.
+constexpr int kGroups = 4, kStages = kGroups, kEpis = 4;
+constexpr int kXWarp = kEpis + 4 * kGroups, kIssueWarp = kXWarp + 1, kFetchWarp = kXWarp + 2, kThreads = (kXWarp + 3) * 32;
+static_assert(kStages == kExpertStages && kGroups == kExpertGroups && kEpis == kExpertEpis, "the plan's");
+constexpr uint32_t kACol = 256;  // one accumulator of up to 256 columns, or two
+static_assert(kACol + kStages * kAColsPerSlot <= kTmemCols, "tensor memory");
 
 struct ExpertGemm {
     const __nv_bfloat16* scales;
@@ -49,7 +51,7 @@ struct ExpertGemm {
 };
 
 struct Control {
-    uint64_t full[stages(false)], empty[stages(false)], wfull[kDqGroups * kMaxWSlots], wempty[kDqGroups * kMaxWSlots], tmem_full[2], tmem_empty[2];
+    uint64_t full[kStages], empty[kStages], wfull[kGroups * kMaxWSlots], wempty[kGroups * kMaxWSlots], tmem_full[2], tmem_empty[2];
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -110,18 +112,17 @@ __device__ __forceinline__ void tmem_ld_16x256b_x2(uint32_t taddr, uint32_t (&r)
 
 template <int BITS, bool GATED, bool PAIR>
 __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CUtensorMap& tmap_w, const ExpertGemm& p) {
-    constexpr int kStages = stages(PAIR), kCtas = PAIR ? 2 : 1, kAlign = 16 * kCtas;
-    constexpr uint32_t kACol = acc_cols(PAIR);
+    constexpr int kCtas = PAIR ? 2 : 1, kAlign = 16 * kCtas;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;  // of this CTA in its pair: 0 issues the MMAs of both
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sB = smem;  // [kStages][kSub][bm rows (pair: half of them)][128 B], swizzled (TMA)
     const uint32_t b_bytes = (uint32_t)(p.bm / kCtas) * 128;
-    unsigned char* sW = sB + (size_t)kStages * kSub * b_bytes;  // [kDqGroups][w_slots][128 rows][64 B], 64-byte swizzle (TMA)
-    unsigned char* sEpi = sW + (size_t)kDqGroups * p.w_slots * kWUnitBytes;  // [kEpiWarps][16 rows of x][32 columns] bf16
+    unsigned char* sW = sB + (size_t)kStages * kSub * b_bytes;  // [kGroups][w_slots][128 rows][64 B], 64-byte swizzle (TMA)
+    unsigned char* sEpi = sW + (size_t)kGroups * p.w_slots * kWUnitBytes;  // [kEpis][16 rows of x][32 columns] bf16
     // (pairs: [bm rows of x][kYPitch bytes]: a finished tile on its way out; the pitch keeps the rows on different banks)
     constexpr int kYCols = GATED ? kTileN / 2 : kTileN, kYPitch = y_pitch(GATED);
-    Control* ctl = reinterpret_cast<Control*>(sEpi + (PAIR ? (size_t)(p.y_staged ? p.bm * kYPitch : 0) : (size_t)kEpiWarps * kEpiStageBytes));
+    Control* ctl = reinterpret_cast<Control*>(sEpi + (PAIR ? (size_t)(p.y_staged ? p.bm * kYPitch : 0) : (size_t)kEpis * kEpiStageBytes));
     int* off = reinterpret_cast<int*>(reinterpret_cast<unsigned char*>(ctl) + kGemmCtlBytes);  // tables of GroupTiles
     int* first = off + p.experts + 1;
     volatile int* abort_flag = &ctl->abort_flag;
@@ -136,20 +137,20 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
             mbar_init(&ctl->full[s], 4 * kCtas + 1);
             mbar_init(&ctl->empty[s], 1);  // one tcgen05.commit (pairs: multicast to both CTAs)
         }
-        for (int g = 0; g < kDqGroups * kMaxWSlots; g++) {
+        for (int g = 0; g < kGroups * kMaxWSlots; g++) {
             mbar_init(&ctl->wfull[g], 1);
             mbar_init(&ctl->wempty[g], 4);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&ctl->tmem_full[b], 1);
-            mbar_init(&ctl->tmem_empty[b], kEpiWarps * kCtas);
+            mbar_init(&ctl->tmem_empty[b], kEpis * kCtas);
         }
         ctl->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // (tensor memory behind the wait: a kernel before this one may still want it)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp == kMmaWarp) {
+    if (warp == kIssueWarp) {
         if constexpr (PAIR) tmem_alloc_pair(&ctl->tmem_base, kTmemCols);
         else tmem_alloc(&ctl->tmem_base, kTmemCols);
     }
@@ -160,9 +161,8 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
     // accumulator and phase of the CTA's i-th tile
-    const bool two_acc = !PAIR && p.bm <= kTwoAccRows;
-    auto acc_of = [&](uint32_t i) { return two_acc ? i & 1 : 0u; };
-    auto phase_of = [&](uint32_t i) { return (two_acc ? i >> 1 : i) & 1; };
+    auto acc_of = [](uint32_t i) { return PAIR ? 0u : i & 1; };
+    auto phase_of = [](uint32_t i) { return (PAIR ? i : i >> 1) & 1; };
     GroupSeg seg;
     seg.p = &p;
     seg.init(p, off, nst, blockIdx.x / kCtas, gridDim.x / kCtas, kAlign);
@@ -173,7 +173,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
         else mbar_arrive(&ctl->full[s]);
     };
 
-    if (warp == kTmaWarp) {
+    if (warp == kXWarp) {
         // ---------------- rows of x: the whole warp, a box per lane and stage ----------------
         if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_x) : "memory");
         uint32_t slot = 0, ph = 1;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 if (++slot == kStages) { slot = 0; ph ^= 1; }
             }
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kIssueWarp) {
         // ---------------- MMA issuer: the whole warp, one elected lane issues ----------------
         auto mma = [](uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
             if constexpr (PAIR) tc_mma_ts_pair(d, a, b, idesc, acc);
@@ -212,7 +212,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
         bool ok = true;
         for (; rank == 0 && seg.valid() && ok; seg.next(), tile_i++) {
             const uint32_t idesc = umma_idesc(kTileN * kCtas, (seg.rows + kAlign - 1) & -kAlign);
-            const uint32_t acc = acc_of(tile_i), d_tmem = tmem_base + acc * kTwoAccRows;
+            const uint32_t acc = acc_of(tile_i), d_tmem = tmem_base + acc * kLowRows;
             if (!mbar_wait_warp(&ctl->tmem_empty[acc], phase_of(tile_i) ^ 1, abort_flag)) break;
             tc_fence_after();
             for (int st = 0; st < nst; st++) {
@@ -236,21 +236,21 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
             if (ok && elect_one()) commit(&ctl->tmem_full[acc]);
             __syncwarp();
         }
-    } else if (warp == kWWarp) {
+    } else if (warp == kFetchWarp) {
         // ---------------- packed weights ----------------
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_w) : "memory");
-            weight_producer<BITS>(p, seg, nks, sW, ctl->wfull, ctl->wempty, abort_flag,
+            weight_producer<BITS, kGroups>(p, seg, nks, sW, ctl->wfull, ctl->wempty, abort_flag,
                                   [&](const GroupSeg& s) { return GATED ? make_int2(n_tile(s) * 8, s.e) : make_int2(s.e * p.N + n_tile(s) * kTileN, 0); },
                                   [&](void* dst, int x, int2 at, uint64_t* bar) {
                                       if constexpr (GATED) tma_load_5d(dst, &tmap_w, x, 0, 0, at.x, at.y, bar);
                                       else tma_load_2d(dst, &tmap_w, x, at.x, bar);
                                   });
         }
-    } else if (warp >= kEpiWarps) {
+    } else if (warp >= kEpis) {
         // ---------------- dequantisers ----------------
-        const int q = warp & 3, grp = (warp - kEpiWarps) >> 2;
-        dequant_role<BITS, kStages / kDqGroups>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &ctl->wfull[grp * kMaxWSlots],
+        const int q = warp & 3, grp = (warp - kEpis) >> 2;
+        dequant_role<BITS, kGroups>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &ctl->wfull[grp * kMaxWSlots],
                            &ctl->wempty[grp * kMaxWSlots], &ctl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kACol + grp * kAColsPerSlot, abort_flag,
                            // (rows past the expert's last: the last one's scales, for lanes whose results are not stored)
@@ -262,20 +262,20 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                                    return s.e * p.N + min(n_tile(s) * kTileN + r, p.N - 1);
                                }
                            },
-                           [&](int i) { arrive_full(grp + i * kDqGroups); });
+                           [&]() { arrive_full(grp); });
     } else {
-        // ---------------- epilogue: warp w reads a quarter of the lanes, half of the columns (rows of x), 16 at a time ----------------
-        const int q = warp & 3, half = warp >> 2;
+        // ---------------- epilogue: a warp reads a quarter of the lanes, 16 columns (rows of x) at a time ----------------
+        const int q = warp;
         unsigned char* stg = sEpi + (size_t)warp * kEpiStageBytes;
         const bool staged = PAIR && p.y_staged;
         constexpr int kEpiBar = 1;  // named barrier of these warps
         uint32_t tile_i = 0;
         for (; seg.valid(); seg.next(), tile_i++) {
             const int tile_n = n_tile(seg);
-            if (staged && tile_i) asm volatile("bar.sync %0, %1;" ::"n"(kEpiBar), "n"(kEpiWarps * 32) : "memory");  // the previous tile has left
-            const int blocks = (seg.rows + 15) >> 4, lo = half ? (blocks + 1) >> 1 : 0, hi = half ? blocks : (blocks + 1) >> 1;
+            if (staged && tile_i) asm volatile("bar.sync %0, %1;" ::"n"(kEpiBar), "n"(kEpis * 32) : "memory");  // the previous tile has left
+            const int blocks = (seg.rows + 15) >> 4;
             const size_t ld = GATED ? p.N >> 1 : p.N;
-            const uint32_t acc = acc_of(tile_i), quarter = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kTwoAccRows;
+            const uint32_t acc = acc_of(tile_i), quarter = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kLowRows;
             if constexpr (GATED) {
                 // this thread: columns f[0], f[1] of y
                 const int F = p.N >> 1;
@@ -291,7 +291,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 }
                 if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
                 tc_fence_after();
-                for (int blk = lo; blk < hi; blk++) {
+                for (int blk = 0; blk < blocks; blk++) {
                     uint32_t v[2][8];
                     __syncwarp();
                     tmem_ld_16x256b_x2(quarter + blk * 16, v[0]);
@@ -339,7 +339,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 const float b = p.bias && n < p.N ? __ldg(p.bias + (size_t)seg.e * p.N + n) : 0.0f;
                 if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
                 tc_fence_after();
-                for (int blk = lo; blk < hi; blk++) {
+                for (int blk = 0; blk < blocks; blk++) {
                     uint32_t v[16];
                     __syncwarp();
                     tmem_ld16(quarter + blk * 16, v);
@@ -380,11 +380,11 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 else mbar_arrive(&ctl->tmem_empty[acc]);
             }
             if (staged) {  // the accumulator is free: the tile leaves, 16 bytes a store, while the next one's MMAs run
-                asm volatile("bar.sync %0, %1;" ::"n"(kEpiBar), "n"(kEpiWarps * 32) : "memory");
+                asm volatile("bar.sync %0, %1;" ::"n"(kEpiBar), "n"(kEpis * 32) : "memory");
                 constexpr int kPieces = kYCols / 8;
                 const int piece = tid % kPieces, col = tile_n * kYCols + piece * 8;
                 if (col < (int)ld)
-                    for (int row = tid / kPieces; row < seg.rows; row += kEpiWarps * 32 / kPieces)
+                    for (int row = tid / kPieces; row < seg.rows; row += kEpis * 32 / kPieces)
                         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.y) + (size_t)(seg.m0 + row) * ld + col) = *reinterpret_cast<const uint4*>(sEpi + row * kYPitch + piece * 16);
             }
         }
@@ -395,7 +395,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
     settle_after_abort(abort_flag);
     if constexpr (PAIR) cluster_sync();  // neither CTA leaves (or frees tensor memory) while the other may still reach into it
     if (tid == 0 && ctl->abort_flag) *p.error = 1;
-    if (warp == kMmaWarp) {
+    if (warp == kIssueWarp) {
         tc_fence_after();
         if constexpr (PAIR) tmem_dealloc_pair(tmem_base, kTmemCols);
         else tmem_dealloc(tmem_base, kTmemCols);
@@ -403,12 +403,12 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
 }
 
 template <int BITS, bool GATED>
-__global__ void __launch_bounds__(kNumThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
 qmm_experts_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ ExpertGemm p) {
     experts_body<BITS, GATED, false>(tmap_x, tmap_w, p);
 }
 template <int BITS, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 qmm_experts_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ ExpertGemm p) {
     experts_body<BITS, GATED, true>(tmap_x, tmap_w, p);
 }
@@ -421,7 +421,7 @@ cudaError_t launch_t(const CUtensorMap& tmap_x, const CUtensorMap& tmap_w, const
     if (cudaError_t e = allow_smem(kern, kGemmSmemLimit, attr_set)) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kNumThreads);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

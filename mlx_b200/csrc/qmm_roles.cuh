@@ -247,24 +247,24 @@ struct TileIter {
     __device__ __forceinline__ void next() { tile_ += step; }
 };
 // The CTA's stages are counted 0, 1, 2, ... along its sequence of segments, alike in every role; dequantising group g owns
-// the counts = g (mod kDqGroups).
+// the counts = g (mod GROUPS).
 //
 // One thread: the packed weights, unit after unit into the ring of the group that owns the stage.  Three stages at a time,
 // one for each group: first units first, so that with a single slot per group no group waits for another's second unit
 // (8 bit).  Every stage is UPS units, so that the rings advance alike; the odd sub-block's partner is announced without a load.
 // at(seg): where the tile's weights lie (two ints, whatever they mean to load); load(dst, first byte of the rows, at, barrier).
-template <int BITS, class Prm, class Seg, class At, class Load>
+template <int BITS, int GROUPS = kDqGroups, class Prm, class Seg, class At, class Load>
 __device__ __forceinline__ void weight_producer(const Prm& p, Seg seg, int nks, unsigned char* ring, uint64_t* wfull, uint64_t* wempty,
                                                 volatile int* abort_flag, const At& at, const Load& load) {
     constexpr int UPS = BITS == 8 ? 2 : 1;  // weight units (128 rows x 64 packed bytes) per pipeline stage
-    int2 row[kDqGroups];
-    int stage[kDqGroups], cnt = 0, slot = 0;
+    int2 row[GROUPS];
+    int stage[GROUPS], cnt = 0, slot = 0;
     uint32_t ph = 1;
     auto flush = [&]() {
 #pragma unroll
         for (int u = 0; u < UPS; u++) {
 #pragma unroll
-            for (int g = 0; g < kDqGroups; g++) {
+            for (int g = 0; g < GROUPS; g++) {
                 if (g >= cnt) break;
                 const int i = g * kMaxWSlots + slot;
                 if (!mbar_wait(wempty + i, ph, abort_flag)) return false;
@@ -285,20 +285,20 @@ __device__ __forceinline__ void weight_producer(const Prm& p, Seg seg, int nks, 
         const int s_hi = seg.s_hi();
         for (int st = seg.s_lo(); st < s_hi; st++) {
 #pragma unroll
-            for (int g = 0; g < kDqGroups; g++)
+            for (int g = 0; g < GROUPS; g++)
                 if (g == cnt) { row[g] = n0; stage[g] = st; }
-            if (++cnt == kDqGroups && !flush()) return;
+            if (++cnt == GROUPS && !flush()) return;
         }
     }
     flush();
 }
 // One warp (lane quarter of group grp; a warp may only touch its own quarter of the TMEM lanes): the thread owns row r of
-// every tile.  A group always writes the same slots.
+// every tile.  There are as many stages in flight as groups, so a group always writes the same slot.
 // What bounds it is its instructions, three such warps to a scheduler, and the instruction caches that all roles share;
 // hence row pointers per tile (a division each), one copy of the code for both sub-blocks, one arrival per warp.
-// SLOTS: how many slots of the A ring the group owns, kDqGroups apart; `empty` and a_tmem are the first one's, arrive(i) says that the i-th is full.
+// A group always writes the same slot of the A ring: `empty` and a_tmem are its, arrive() says that it is full.
 // row_of(seg, r): the row of wq, scales and biases that is row r of the tile.
-template <int BITS, int SLOTS = 1, class Prm, class Seg, class RowOf, class Arrive>
+template <int BITS, int GROUPS = kDqGroups, class Prm, class Seg, class RowOf, class Arrive>
 __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int r, int nks, const unsigned char* wring, uint64_t* wfull,
                                              uint64_t* wempty, uint64_t* empty, uint32_t a_tmem, volatile int* abort_flag,
                                              const RowOf& row_of, const Arrive& arrive) {
@@ -365,20 +365,19 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
     if (more) fetch_sb();
     const int half_shift = p.gshift == 5 ? 16 : 0, sub_shift = p.gshift == 6 ? 16 : 0;  // where the next half's, the next sub-block's scale is
     int wslot = 0;
-    uint32_t wphase = 0, phase = 1, own = 0;
+    uint32_t wphase = 0, phase = 1;
     while (more) {
         const int nsub = min(kSub, nks - st * kSub);
         uint32_t s_lo = sp[0], b_lo = bp[0];
         const uint32_t s_hi = sp[1], b_hi = bp[1];
-        st += kDqGroups;
+        st += GROUPS;
         if (st >= end) settle();
         // Three stages ahead of its use.  At 4 bit behind the proxy fence, which would wait for these loads too (777 rows in
         // groups of 32: 30.9 against 33-40 us); at 8 bit, with a fence per sub-block, here (512 x 8192 x 28672: 204 against 257).
         if (UPS == 2 && more) fetch_sb();
         uint32_t w[WPS], wn[8];  // this sub-block's words; 4 bit: the next one's, from the same unit
         bool ok = true;
-        // (one copy of the code for both, where the ring has one slot a group: two cost 512 x 4096 x 4096 21 -> 22 us; with two slots, 3 % faster)
-#pragma unroll (BITS == 4 && SLOTS > 1 ? 2 : 1)
+#pragma unroll 1
         for (int u = 0; u < kSub; u++) {
             if (UPS == 1 && u >= nsub) break;
             if (UPS == 2 || u == 0) {
@@ -400,8 +399,8 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
             }
             if (u >= nsub) break;  // (the odd sub-block's partner at 8 bit: nothing in it)
             if (u == 0) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty + own * kDqGroups, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
-                if (SLOTS == 1) phase ^= 1;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
+                phase ^= 1;
                 tc_fence_after();
                 if (!ok) break;
             }
@@ -413,7 +412,7 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
                 if (scale_fast_ok(sv)) dequant_32<BITS, true>(w + h * (WPS / 2), sv, bv, out);
                 else dequant_32<BITS, false>(w + h * (WPS / 2), sv, bv, out);  // whole-block branch: not if-converted
                 __syncwarp();
-                tmem_st16(a_tmem + own * (kDqGroups * kAColsPerSlot) + u * kAColsPerSub + h * 16, out);
+                tmem_st16(a_tmem + u * kAColsPerSub + h * 16, out);
             }
             if (UPS == 1) {
 #pragma unroll
@@ -430,11 +429,7 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
         tmem_st_wait();  // once per stage: both sub-blocks are in tensor memory
         tc_fence_before();
         __syncwarp();
-        if ((r & 31) == 0) arrive((int)own);
-        if (SLOTS > 1 && ++own == SLOTS) {
-            own = 0;
-            phase ^= 1;
-        }
+        if ((r & 31) == 0) arrive();
     }
 }
 

@@ -298,7 +298,7 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&](int) { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -593,7 +593,7 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&](int) { mbar_arrive(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min((s.tile() / p.m_tiles) * kTileN + r, p.N - 1); }, [&]() { mbar_arrive(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
@@ -788,7 +788,7 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         dequant_role<BITS>(p, seg, grp, q * 32 + lane, nks, sW + (size_t)grp * p.w_slots * kWUnitBytes, &sl->wfull[grp * kMaxWSlots],
                            &sl->wempty[grp * kMaxWSlots], &sl->empty[grp],
                            tmem_base + ((uint32_t)(q * 32) << 16) + kAColBase + grp * kAColsPerSlot, abort_flag,
-                           [&](const auto& s, int r) { return min(n0_of(s.tile()) + r, p.N - 1); }, [&](int) { mbar_arrive_cta0(&sl->full[grp]); });
+                           [&](const auto& s, int r) { return min(n0_of(s.tile()) + r, p.N - 1); }, [&]() { mbar_arrive_cta0(&sl->full[grp]); });
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32*(w%4).., half w/4 of the column blocks ----------------
         const int q = warp & 3, half = warp >> 2;
