@@ -810,9 +810,10 @@ bool make_plan(const QmmArgs& a, int mmax, int sm_count, Plan* pl, int experts =
     pl->kbc = (pl->nkb + pl->nch - 1) / pl->nch;
     pl->nch = (pl->nkb + pl->kbc - 1) / pl->kbc;
     pl->tile_bytes = pl->kbc * 2048;
-    // bulk copies of scales where a stage holds several tiles; one long tile's leave the warp time enough, and their rows meet in the same banks
-    // (64 experts x 4 rows: 1408 x 4096 54.8 us against 81.3, 2048 x 4096 65.4 against 70.3; 4096 x 4096 113.6 against 101.6)
-    pl->sb_bulk = experts && pl->kbc <= kWarps / 2 && pl->nch == 1 && a.N % 16 == 0;
+    // Scales by bulk copies, but for a long tile whose rows are whole multiples of 128 bytes of them: the eight rows that a warp reads then meet in
+    // one bank (64 experts x 4 rows, groups of 64, N = 4096: K = 1408 54.8 us against 81.3 by pieces, 2048 61.2 against 70.3, 3840 101.3 against 104.2;
+    // 4096 111.5 against 105.2, in groups of 128 103.9 against 105.9).
+    pl->sb_bulk = experts && pl->nch == 1 && a.N % 16 == 0 && (pl->kbc <= kWarps / 2 || a.K / a.group % 64 != 0);
     const int sb = pl->sb_bulk ? 64 * (a.K / a.group) : 32 * sb_row(a.bits == 4 && a.group == 32 ? 2 : 1), xs = kWarps * x_frags(a.bits) * 512 / (mt == 1 ? 2 : 1), bars = 8 * 3 * kMaxStages;
     // K in one chunk: nothing is kept per tile (4096: as far as Walk::groups divides exactly); in several: the tiles' running sums
     pl->tb = std::min(tiles_max, pl->nch == 1 ? 4096 : 16 * 1024 / (mt * 512));

