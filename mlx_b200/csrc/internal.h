@@ -382,7 +382,7 @@ struct MoeRouteArgs {
     bool logits_bf16;
     float scale;
 };
-int moe_route_blocks(const MoeRouteArgs& a);  // more than one: the workspace is needed
+int moe_route_blocks(const MoeRouteArgs& a, int sm_count);  // more than one: the workspace is needed
 size_t moe_route_workspace_bytes();
 cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, int* launches);
 struct MoeCombineArgs {

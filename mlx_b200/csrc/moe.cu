@@ -2,16 +2,16 @@
 // token's expert outputs (moe_combine).
 //
 // moe_route.  One warp takes a token: lane l holds the logits of experts l, l + 32, ... as unsigned keys in the order of the numbers (0: not to
-// be chosen), and top_k times the warp's largest key goes, of equal ones the lowest expert's.  Then a counting sort that keeps
+// be chosen); those above a threshold that the lanes' largest give are ranked among themselves (choose).  Then a counting sort that keeps
 // the order of the pairs: a block ranks its own pairs (ballots of equal experts within 32 pairs, counts per warp and expert in shared memory),
 // and adds where its share of each expert begins.
 //   * Few tokens: one block does it all, one launch.
-//   * More: a block takes as many neighbouring tokens as it has warps (more where that would be over kMaxBlocks blocks) and leaves its counts per
+//   * More: a block takes as many neighbouring tokens as it has warps (more where that would be more blocks than SMs) and leaves its counts per
 //     expert in a workspace; a second launch adds them up along the blocks, for 32 experts a block; a third puts the pairs in their places.  Up to
 //     kFewBlocks blocks the last two are one launch, whose blocks each add up for themselves.  No atomics: a pair's rank must not depend
 //     on who comes first.
 // Bytes: tokens * experts logits once, 16 bytes a pair out.  Bound by the instructions of the choice (about a thousand a token at 256 experts, best
-// 8; 60 % of the issue slots): 8192 tokens 20.5 us, with sigmoid and bias 22.7.  Few tokens: by the latency of a launch, 4 us.
+// 8; 60 % of the issue slots): 8192 tokens 18.2 us, with sigmoid and bias 20.0.  Few tokens: by the latency of a launch, 4 us.
 //
 // moe_combine.  HBM-bound: a thread takes 8 neighbouring columns of a token, with the loads of up to 8 slots under way (4096 tokens x 8 x 4096,
 // fp32 stream: 65 us, 6.0 TB/s).
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(THREADS) moe_route_kernel(const MoeRouteArgs a
 
 // The second launch: 32 experts a block, warp w a run of the B blocks' counts.  Behind it hist[b][e] is the sum of the blocks before b, hist[B][e] that of
 // all.
-constexpr int kMaxBlocks = 296;  // two of 1024 threads on each of 148 SMs
+constexpr int kMaxBlocks = 160;  // (one on each SM, whose registers hold one of 1024 threads: in two rounds, 8192 x 256 22.6 us against 20.0)
 __global__ void __launch_bounds__(1024) moe_count_kernel(int* hist, int E, int B) {
     __shared__ int part[32][33];
     wait_previous();
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kPlaceThreads) moe_place_kernel(const MoeRoute
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= E; i += kPlaceThreads) a.offsets[i] = all[i];
 }
-// Few blocks: every block adds up the counts itself, for its own pairs.  One launch less.
+// Few blocks: every block adds up the counts itself, for its own pairs.  One launch less (with 147 blocks 2.5 us more than it saves).
 constexpr int kFewBlocks = 64, kCountThreads = 1024;
 __global__ void __launch_bounds__(kCountThreads) moe_count_place_kernel(const MoeRouteArgs a, int chunk) {
     extern __shared__ int smem[];
@@ -512,15 +512,15 @@ cudaError_t launch_route_v(const MoeRouteArgs& a, int blocks, int chunk, cudaStr
 }  // namespace
 
 // One block: as long as its warps have no more than a token each (64 tokens, two each: 10.4 us against 9.0 in several) and the pairs fit a round.
-int moe_route_blocks(const MoeRouteArgs& a) {
+int moe_route_blocks(const MoeRouteArgs& a, int sm_count) {
     if (a.tokens <= 32 && a.tokens * a.top_k <= (size_t)kRoundPairs) return 1;
-    const size_t per = std::max<size_t>(route_warps(a.experts), (a.tokens + kMaxBlocks - 1) / kMaxBlocks);
+    const size_t most = std::min(sm_count, kMaxBlocks), per = std::max<size_t>(route_warps(a.experts), (a.tokens + most - 1) / most);
     return (int)std::max<size_t>((a.tokens + per - 1) / per, 2);
 }
 size_t moe_route_workspace_bytes() { return (size_t)(kMaxBlocks + 1) * LUX_CUDA_MAX_EXPERTS * sizeof(int); }
 
 cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev, int* launches) {
-    const int blocks = moe_route_blocks(a), chunk = std::max(1, (int)((a.tokens + blocks - 1) / blocks));
+    const int blocks = moe_route_blocks(a, sm_count), chunk = std::max(1, (int)((a.tokens + blocks - 1) / blocks));
     cudaError_t e;
     *launches = 1;
     if (!a.logits) e = launch_route_t<0, false, false>(a, blocks, chunk, stream, overlap_prev);

@@ -171,7 +171,7 @@ LuxBackendError moe_route(LuxBackendContext* ctx, const lux_moe_route_params* pa
     DeviceGuard g(c->dev->device());
     MoeRouteArgs a{o[LOGITS].ptr(), (const float*)o[BIAS].ptr(), (int*)o[IDS].ptr(), (float*)o[WEIGHTS].ptr(), (int*)o[ORDER].ptr(), (int*)o[POS].ptr(),
                    (int*)o[OFFSETS].ptr(), nullptr, (size_t)p.tokens, ld, p.experts, p.top_k, p.score, p.renorm, ls == 2, p.scale};
-    if (moe_route_blocks(a) > 1) {
+    if (moe_route_blocks(a, c->dev->sm_count) > 1) {
         if (LuxBackendError e = grow_workspace(c, &c->moe_ws, nullptr, moe_route_workspace_bytes(), "moe_route")) return e;
         a.hist = (int*)c->moe_ws->ptr;
     }
