@@ -285,8 +285,8 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 for (int j = 0; j < 2; j++) {
                     f[j] = tile_n * 64 + q * 16 + j * 8 + (lane >> 2);
                     if (p.bias && f[j] < F) {
-                        bg[j] = __ldg(p.bias + (size_t)seg.e * p.N + f[j]);
-                        bu[j] = __ldg(p.bias + (size_t)seg.e * p.N + F + f[j]);
+                        bg[j] = __ldcg(p.bias + (size_t)seg.e * p.N + f[j]);
+                        bu[j] = __ldcg(p.bias + (size_t)seg.e * p.N + F + f[j]);
                     }
                 }
                 if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
@@ -336,7 +336,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                 }
             } else {
                 const int n = tile_n * kTileN + q * 32 + lane;
-                const float b = p.bias && n < p.N ? __ldg(p.bias + (size_t)seg.e * p.N + n) : 0.0f;
+                const float b = p.bias && n < p.N ? __ldcg(p.bias + (size_t)seg.e * p.N + n) : 0.0f;
                 if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
                 tc_fence_after();
                 for (int blk = 0; blk < blocks; blk++) {
@@ -437,7 +437,8 @@ cudaError_t launch_b(const ExpertsArgs& a, const CUtensorMap& tmap_x, const CUte
 }
 
 // Rows of x side by side: row i of out is row order[i] / top_k of x, zeros where there is none (which behind the last pair is anything).  A warp takes
-// a row at a time, 64 bytes a lane under way.
+// a row at a time, 64 bytes a lane under way.  (Loads past L1, here and of what the GEMM reads besides weights: the kernel before may have written it while
+// this one was already on the SM.)
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, uint4* out, const int* order, int rows, int x_rows, int pieces, uint32_t top_k) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint4* x, uint4*
         for (int c = lane; c < pieces; c += 128) {
             uint4 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = there && c + 32 * u < pieces ? __ldg(src + c + 32 * u) : make_uint4(0, 0, 0, 0);
+            for (int u = 0; u < 4; u++) v[u] = there && c + 32 * u < pieces ? __ldcg(src + c + 32 * u) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int u = 0; u < 4; u++)
                 if (c + 32 * u < pieces) dst[c + 32 * u] = v[u];

@@ -110,6 +110,44 @@ def test_odd_gated_sizes(ctx, oracle, bits, group, K, N, rows):
     run(ctx, oracle, w, values, x, groups(rng, E, rows, "ragged"), E, K, N, bits, group, act=P.ACT_GELU, gated=True)
 
 
+# one sub-block of k, an odd number of them, odd groups a row; single CTAs and pairs; tiles of W short of 128 rows, of two tiles, and an odd number of tiles
+@pytest.mark.parametrize("bits,group,K", [(4, 64, 64), (8, 32, 192), (4, 32, 320), (4, 128, 1408), (8, 128, 640)])
+@pytest.mark.parametrize("N,gated", [(120, False), (131, False), (400, False), (16, True), (272, True)])
+@pytest.mark.parametrize("rows", [250, 1500])
+@pytest.mark.parametrize("pair", ["0", "1"])
+def test_many_rows(ctx, oracle, monkeypatch, bits, group, K, N, gated, rows, pair):
+    monkeypatch.setenv("LUXCUDA_EXPERTS", "many")
+    monkeypatch.setenv("LUXCUDA_EXPERTS_PAIR", pair)
+    rng = np.random.default_rng(K + N + rows)
+    E = 4
+    w, values = layer(oracle, E, N, K, bits, group)
+    x = oracle.make_x(rows, K, oracle.BF16, tag=N)
+    offsets = groups(rng, E, rows, "ragged")
+    order = rng.permutation(rows).astype(np.int32)
+    run(ctx, oracle, w, values, x, offsets, E, K, N, bits, group, order=order, act=P.ACT_GELU_TANH, gated=gated)
+    assert ctx.last_kernel() == f"qmm_experts<{bits}{',pairs' if pair == '1' else ''}>"
+    run(ctx, oracle, w, values, x, groups(rng, E, rows, "tail"), E, K, N, bits, group, gated=gated, y_dtype=F32)
+
+
+@pytest.mark.parametrize("rows", [11, 250, 1000])
+@pytest.mark.parametrize("y_dtype", [BF16, F32])
+@pytest.mark.parametrize("gated", [False, True])
+def test_y_on_no_wide_boundary(ctx, oracle, rows, y_dtype, gated):
+    """One element past a 16-byte boundary: the same bits."""
+    E, K, N = 3, 256, 160
+    w, values = layer(oracle, E, N, K, 4, 64)
+    x = oracle.make_x(rows, K, oracle.BF16)
+    offsets = groups(None, E, rows, "even")
+    want = run(ctx, oracle, w, values, x, offsets, E, K, N, 4, 64, gated=gated, y_dtype=y_dtype)
+    kind, size = (np.uint16, 2) if y_dtype == BF16 else (np.float32, 4)
+    room = ctx.upload(np.zeros(want.size + 2, kind))
+    ctx.qmatmul_experts(ctx.experts_params(rows, rows, E, K, N, 4, 64, gated=gated, y_dtype=y_dtype), ctx.upload(x), None, ctx.upload(offsets), *(ctx.upload(a) for a in w), None,
+                        ctx.wrap(room.device_ptr + size, want.nbytes))
+    got = room.to_host()
+    np.testing.assert_array_equal(got[1:-1].reshape(want.shape), want)
+    assert got[0] == 0 and got[-1] == 0
+
+
 @pytest.mark.parametrize("act", [P.ACT_NONE, P.ACT_RELU, P.ACT_SILU, P.ACT_GELU, P.ACT_GELU_TANH])
 @pytest.mark.parametrize("y_dtype", [BF16, F32])
 @pytest.mark.parametrize("rows", [20, 400])
