@@ -229,6 +229,32 @@ def test_infinite_and_missing_weights_of_other_experts(ctx, oracle):
         assert np.isnan(oracle.from_bf16(got[offsets[1]:offsets[2]])).all()
 
 
+@pytest.mark.parametrize("bits,group,K", [(4, 32, 32), (4, 32, 96), (4, 64, 320), (4, 128, 4224), (8, 32, 160), (8, 64, 192)])
+@pytest.mark.parametrize("N,gated", [(19, False), (48, False), (32, True)])
+@pytest.mark.parametrize("rows", [7, 300])
+def test_an_infinite_scale_stays_in_its_row(ctx, oracle, bits, group, K, N, gated, rows):
+    """K ends inside a block of the kernels': what lies behind it there is the next row's."""
+    E = 2
+    w, _ = layer(oracle, E, N, K, bits, group)
+    x, offsets = oracle.make_x(rows, K, oracle.BF16), groups(None, E, rows, "even")
+    prm = ctx.experts_params(rows, rows, E, K, N, bits, group, gated=gated, y_dtype=F32)
+    xb, off, y = ctx.upload(x), ctx.upload(offsets), ctx.empty((rows, N // 2 if gated else N), np.float32)
+
+    def call(scales, biases):
+        ctx.qmatmul_experts(prm, xb, None, off, ctx.upload(w[0]), ctx.upload(scales), ctx.upload(biases), None, y)
+        return y.to_host()
+
+    want = call(w[1], w[2])
+    for n in (0, 5, N - 1):
+        s, b = w[1].reshape(E * N, -1).copy(), w[2].reshape(E * N, -1).copy()
+        s[n], b[n] = 0x7F80, 0xFF80  # infinity, minus infinity: of expert 0
+        got = call(s, b)
+        cols = [c for c in range(want.shape[1]) if c != n and not (gated and c + N // 2 == n)]
+        np.testing.assert_array_equal(got[:, cols], want[:, cols])
+        np.testing.assert_array_equal(got[offsets[1]:], want[offsets[1]:])
+        assert not np.isfinite(got[:offsets[1], n % want.shape[1]]).any()
+
+
 @pytest.mark.parametrize("rows", [16, 500])
 def test_recorded(ctx, oracle, rows):
     """Recorded once, replayed with other offsets in the same buffer."""
