@@ -21,20 +21,20 @@ inline bool experts_in_pairs(const ExpertsShape& s, int sm_count) {
 
 // Estimates of the times in microseconds, for experts that share the rows evenly: the host does not know better.  Fitted to 170 shapes (2 to 128
 // experts, K 512 to 4096, N 128 to 8192, 0.5 to 90 rows an expert, 4 and 8 bit; calls from a host, launches included): the faster of the two, or
-// one within 5 % of it, is taken on 159 of them, all in all 0.8 % is lost, 34 % at worst; the times are off by a seventh on average.
+// one within 5 % of it, is taken on 162 of them, all in all 0.8 % is lost, 37 % at worst; the times are off by a seventh on average.
 //   few rows (qmv_stream.cu): the row tiles of all items of eight rows, dealt over the SMs, a tile at the rate of its packed bytes but
 //   not below what starting one costs; x is loaded again for every item a CTA works on;
 //   many (qmm_experts.cu): rounds of tiles, a k-stage of 128 bound by dequantisation until the tiles are high; gathered rows first.
 inline void experts_estimates(const ExpertsShape& s, int sm_count, double* few, double* many) {
     const double mean = (double)s.rows / s.experts, active = s.experts * (1.0 - std::exp(-mean)), m = s.rows / active;
-    const double row_tiles = (s.N + 15) / 16, items = active * std::max(1.0, m / 8 + 0.14), tiles = items * row_tiles / sm_count;
-    const double tile = std::max(0.16 + 0.057 * (s.K * (double)s.bits / 1024), 0.46);
-    *few = 5.9 + std::max(1.0, tiles) * tile + 0.30 * std::max(1.0, tiles / row_tiles);
+    const double row_tiles = (s.N + 15) / 16, items = active * std::max(1.0, m / 8 + 0.29), tiles = items * row_tiles / sm_count;
+    const double tile = std::max(0.15 + 0.063 * (s.K * (double)s.bits / 1024), 0.49);
+    *few = 5.9 + std::max(1.0, tiles) * tile + 0.07 * std::max(1.0, tiles / row_tiles);
     const bool pairs = experts_in_pairs(s, sm_count);
     const double n_tiles = (s.N + 127) / 128, G = pairs ? sm_count / 2 : sm_count, bm = std::min(pairs ? 256.0 : 128.0, std::max(32.0, 2 * mean));
     const double T = active * std::max(1.0, m / bm + 0.35) * (pairs ? std::ceil(n_tiles / 2) : n_tiles);
-    const double high = std::max(0.0, std::min(m, bm) - 48), stage = pairs ? 0.49 + 0.002 * high : 0.42 + 0.0116 * high;
-    *many = 6.2 + (s.gather ? 0.6 + s.rows * (double)s.K * 4 / 2.0e6 : 0.0) + std::ceil(T / G) * (std::ceil(s.K / 128.0) * stage + 1.0);
+    const double high = std::max(0.0, std::min(m, bm) - 48), stage = pairs ? 0.44 + 0.0017 * high : (s.bits == 8 ? 0.53 : 0.33) + 0.0051 * high;
+    *many = 5.5 + (s.gather ? 0.67 + s.rows * (double)s.K * 4 / 1.85e6 : 0.0) + std::ceil(T / G) * (std::ceil(s.K / 128.0) * stage + 1.2);
 }
 inline bool experts_have_many_rows(const ExpertsShape& s, int sm_count) {
     if (!s.rows) return false;

@@ -1,7 +1,8 @@
 // Products grouped by expert for many rows an expert (qmatmul_experts), bf16 activations, affine weights:
 //   y[i] = epilogue(x[row(i)] . dequant(Wq[e])^T + bias[e]),   offsets[e] <= i < offsets[e+1]
 // The roles of qmm_tc.cu's kernels on tiles of 128 rows of an expert's W (on pairs of CTAs: two neighbouring ones) against up to bm of its rows of x;
-// tensor-bound where experts have 150 rows and more, bound by dequantisation below (a k-stage of 128 takes 0.45 us of it whatever the rows).
+// tensor-bound where experts have 150 rows and more, bound by dequantisation below (a k-stage of 128 takes 0.36 us of it at
+// 4 bit, 0.46 at 8, whatever the rows).
 //   * The tiles follow from the offsets in device memory: every CTA scans them at its start (an expert's rows are cut into as few tiles as
 //     bm allows, all of one height), then takes every gridDim.x-th tile of the whole list; neighbouring CTAs share an expert's weights or
 //     rows of x at the same time.
@@ -29,8 +30,9 @@ namespace luxcuda {
 namespace {
 
 // Four groups of dequantising warps and four epilogue warps (qmm_tc.cu: three and eight, as many threads): what bounds tiles that are not high is how
-// fast a group gets through a stage (0.43 us of 0.47 for three groups; without the tensor cores' part no less, without dequantisation 0.37), and the epilogue
-// has a second accumulator or a copy in shared memory to run beside.  Stages as groups: A in tensor memory, 64 columns each, behind the accumulators.
+// fast a group gets through a stage (64 experts x 8 rows, 4096 x 2816: without the tensor cores' part 5 % less time, without the arithmetic on codes
+// 12 %, with all weights in L2 no less; the rest are the instructions of the hand-overs), and the epilogue has a second accumulator or a copy
+// in shared memory to run beside.  Stages as groups: A in tensor memory, 64 columns each, behind the accumulators.
 constexpr int kGroups = 4, kStages = kGroups, kEpis = 4;
 constexpr int kXWarp = kEpis + 4 * kGroups, kIssueWarp = kXWarp + 1, kFetchWarp = kXWarp + 2, kThreads = (kXWarp + 3) * 32;
 static_assert(kStages == kExpertStages && kGroups == kExpertGroups && kEpis == kExpertEpis, "the plan's");

@@ -192,6 +192,12 @@ __device__ __forceinline__ uint32_t ldg_u16(const uint16_t* p) {  // zero-extend
     return v;
 }
 
+// scale_fast_ok of two
+__device__ __forceinline__ bool scales_fast_ok(uint32_t s) {
+    const uint32_t u = (s & 0x7FFF7FFFu) - 0x00800080u;  // (a borrow leaves the low half's top bit)
+    return ((u | (u + 0x43804380u)) & 0x80008000u) == 0;
+}
+
 // 32 weights of one row (one scale) -> 16 registers of bf16 pairs in natural k order.
 // The matrix instruction wants neighbours in k side by side, which dequant.cuh's masks do not yield (they pair weights 4
 // apart, and a byte permute per pair put them in order afterwards: 9 integer operations per 8 weights at 4 bit, 10 at 8
@@ -200,10 +206,9 @@ __device__ __forceinline__ uint32_t ldg_u16(const uint16_t* p) {  // zero-extend
 // above either the first's sign, zero: 6 operations.  8 bit: two bytes into the two halves, which is all: 4 operations.  The
 // products are the same (see dequant.cuh for the 2^-133 form).
 template <int BITS, bool FAST>
-__device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s_bits, uint32_t b_bits, uint32_t (&out)[16]) {
-    const uint32_t b2 = dup_bf16(b_bits);
+__device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s, uint32_t b2, uint32_t (&out)[16]) {
     if (BITS == 4) {
-        const uint32_t s2 = FAST ? imad(s_bits, 0x00010001u, 0x40804280u) : dup_bf16(s_bits);  // FAST: (s * 2^133, s * 2^129)
+        const uint32_t s2 = FAST ? s + 0x40804280u : s;  // FAST: (s * 2^133, s * 2^129)
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             if (FAST) {
@@ -220,7 +225,7 @@ __device__ __forceinline__ void dequant_32(const uint32_t* w, uint32_t s_bits, u
             }
         }
     } else {
-        const uint32_t s2 = FAST ? scale_x2_133(s_bits) : dup_bf16(s_bits);
+        const uint32_t s2 = FAST ? s + 0x42804280u : s;
 #pragma unroll
         for (int c = 0; c < 8; c++) {
             if (FAST) {
@@ -302,7 +307,7 @@ template <int BITS, int GROUPS = kDqGroups, class Prm, class Seg, class RowOf, c
 __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int r, int nks, const unsigned char* wring, uint64_t* wfull,
                                              uint64_t* wempty, uint64_t* empty, uint32_t a_tmem, volatile int* abort_flag,
                                              const RowOf& row_of, const Arrive& arrive) {
-    constexpr int WPS = kBK * BITS / 32;    // packed words per row per sub-block: 8 | 16
+    constexpr int UB = 16 / BITS;           // blocks of 32 weights in a unit's 64 bytes of a row
     constexpr int UPS = BITS == 8 ? 2 : 1;  // weight units (128 rows x 64 packed bytes) per pipeline stage
     const int gpr = p.K >> p.gshift;
     const int ng_full = (kSub * kBK) >> p.gshift;  // scale groups per full stage: 4, 2 or 1
@@ -363,63 +368,80 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
     if (st >= end) settle();
     else new_rows();
     if (more) fetch_sb();
-    const int half_shift = p.gshift == 5 ? 16 : 0, sub_shift = p.gshift == 6 ? 16 : 0;  // where the next half's, the next sub-block's scale is
+    // where a block's scale is among the stage's four, twice over; and those of two neighbouring blocks
+    const bool g32 = p.gshift == 5, g64 = p.gshift == 6;
+    const uint32_t at1 = g32 ? 0x3232u : 0x1010u, at2 = g32 ? 0x5454u : g64 ? 0x3232u : 0x1010u, at3 = g32 ? 0x7676u : at2, two0 = g32 ? 0x3210u : 0x1010u, two2 = g32 ? 0x7654u : at2;
     int wslot = 0;
     uint32_t wphase = 0, phase = 1;
     while (more) {
         const int nsub = min(kSub, nks - st * kSub);
-        uint32_t s_lo = sp[0], b_lo = bp[0];
-        const uint32_t s_hi = sp[1], b_hi = bp[1];
+        const uint32_t s_lo = sp[0], b_lo = bp[0], s_hi = sp[1], b_hi = bp[1];
         st += GROUPS;
         if (st >= end) settle();
         // Three stages ahead of its use.  At 4 bit behind the proxy fence, which would wait for these loads too (777 rows in
         // groups of 32: 30.9 against 33-40 us); at 8 bit, with a fence per sub-block, here (512 x 8192 x 28672: 204 against 257).
         if (UPS == 2 && more) fetch_sb();
-        uint32_t w[WPS], wn[8];  // this sub-block's words; 4 bit: the next one's, from the same unit
         bool ok = true;
 #pragma unroll 1
-        for (int u = 0; u < kSub; u++) {
-            if (UPS == 1 && u >= nsub) break;
-            if (UPS == 2 || u == 0) {
-                ok = mbar_wait(wfull + wslot, wphase, abort_flag) && ok;
-                const unsigned char* wrow = wrow0 + wslot * kWUnitBytes;
+        for (int u = 0; u < UPS; u++) {
+            ok = mbar_wait(wfull + wslot, wphase, abort_flag) && ok;
+            uint32_t w[16];
+            const unsigned char* wrow = wrow0 + wslot * kWUnitBytes;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((c ^ wsw) << 4));
-                    uint32_t* d = UPS == 2 ? w + (4 * c) % WPS : (c < 2 ? w + 4 * c : wn + 4 * (c - 2));
-                    d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
-                }
-                // The reads above are generic-proxy accesses, the refill is an async-proxy write: the proxy
-                // fence orders the two (without it a read still in the load pipe could see the next unit).
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if ((r & 31) == 0) mbar_arrive(wempty + wslot);
-                if (++wslot == p.w_slots) { wslot = 0; wphase ^= 1; }
-                if (UPS == 1 && more) fetch_sb();
+            for (int c = 0; c < 4; c++) {
+                const uint4 v = *reinterpret_cast<const uint4*>(wrow + ((c ^ wsw) << 4));
+                w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
             }
-            if (u >= nsub) break;  // (the odd sub-block's partner at 8 bit: nothing in it)
+            // The reads above are generic-proxy accesses, the refill is an async-proxy write: the proxy
+            // fence orders the two (without it a read still in the load pipe could see the next unit).
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if ((r & 31) == 0) mbar_arrive(wempty + wslot);
+            if (++wslot == p.w_slots) { wslot = 0; wphase ^= 1; }
+            if (UPS == 1 && more) fetch_sb();
+            if (u >= nsub) break;  // (8 bit: an odd sub-block's partner, with nothing in it)
             if (u == 0) {
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty, phase, abort_flag) && ok);  // tcgen05.st below is warp-collective
                 phase ^= 1;
                 tc_fence_after();
                 if (!ok) break;
             }
-            // the two 32-weight halves of the sub-block: in one group, or (groups of 32) in one each
+            // the unit's blocks of 32 weights, each in one group
+            const int blocks = UPS == 1 ? 2 * nsub : 2;
+            const uint32_t a_unit = a_tmem + u * kAColsPerSub;
+            uint32_t sv[UB], bv[UB];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t sv = (h ? s_lo >> half_shift : s_lo) & 0xFFFFu, bv = (h ? b_lo >> half_shift : b_lo) & 0xFFFFu;
-                uint32_t out[16];
-                if (scale_fast_ok(sv)) dequant_32<BITS, true>(w + h * (WPS / 2), sv, bv, out);
-                else dequant_32<BITS, false>(w + h * (WPS / 2), sv, bv, out);  // whole-block branch: not if-converted
-                __syncwarp();
-                tmem_st16(a_tmem + u * kAColsPerSub + h * 16, out);
+            for (int i = 0; i < UB; i++) {
+                const uint32_t at = UPS == 1 ? (i == 0 ? 0x1010u : i == 1 ? at1 : i == 2 ? at2 : at3) : (u == 0 ? (i == 0 ? 0x1010u : at1) : (i == 0 ? at2 : at3));
+                sv[i] = prmt(s_lo, s_hi, at);
+                bv[i] = prmt(b_lo, b_hi, at);
             }
-            if (UPS == 1) {
+            bool fast = scales_fast_ok(prmt(s_lo, s_hi, UPS == 2 && u == 1 ? two2 : two0));
+            if (UPS == 1) fast = fast && (blocks == 2 || scales_fast_ok(prmt(s_lo, s_hi, two2)));
+            // Scales out of the fast form's range are rare: one vote per unit and a loop of one copy whose operands move up, out of the way.  (A
+            // branch per block, both forms side by side, and scales by shifts: 2330 instructions a stage, not 1740; 64 experts x 8 rows, 4096 x 2816,
+            // 153 us against 132, 256 x 4096 x 4096 20.6 against 18.6.)
+            if (__all_sync(0xFFFFFFFFu, fast)) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] = wn[i];
+                for (int i = 0; i < UB; i++) {
+                    if (i == 2 && blocks == 2) break;
+                    uint32_t out[16];
+                    dequant_32<BITS, true>(w + i * BITS, sv[i], bv[i], out);
+                    tmem_st16(a_unit + i * 16, out);
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < blocks; i++) {
+                    uint32_t out[16];
+                    dequant_32<BITS, false>(w, sv[0], bv[0], out);
+                    __syncwarp();
+                    tmem_st16(a_unit + i * 16, out);
+#pragma unroll
+                    for (int k = 0; k + BITS < 16; k++) w[k] = w[k + BITS];
+#pragma unroll
+                    for (int k = 0; k + 1 < UB; k++) { sv[k] = sv[k + 1]; bv[k] = bv[k + 1]; }
+                }
             }
-            s_lo = half_shift ? s_hi : s_lo >> sub_shift;
-            b_lo = half_shift ? b_hi : b_lo >> sub_shift;
         }
         ok = __all_sync(0xFFFFFFFFu, ok);  // (8 bit: the second unit's wait)
         if (!ok) {

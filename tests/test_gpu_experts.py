@@ -229,6 +229,26 @@ def test_infinite_and_missing_weights_of_other_experts(ctx, oracle):
         assert np.isnan(oracle.from_bf16(got[offsets[1]:offsets[2]])).all()
 
 
+@pytest.mark.parametrize("bits,group", [(4, 32), (4, 64), (4, 128), (8, 32), (8, 64), (8, 128)])
+@pytest.mark.parametrize("which,pair", [("few", "0"), ("many", "0"), ("many", "1")])
+def test_scales_of_any_size(ctx, oracle, monkeypatch, bits, group, which, pair):
+    """Zero, negative, the smallest normal one, on both sides of 2^-5 and large: where the kernels' short dequantisation ends, alone in a row and mixed."""
+    monkeypatch.setenv("LUXCUDA_EXPERTS", which)
+    monkeypatch.setenv("LUXCUDA_EXPERTS_PAIR", pair)
+    E, K, N, rows = 2, 640, 200, 90
+    (wq, s, b), _ = layer(oracle, E, N, K, bits, group)
+    rng = np.random.default_rng(group + bits)
+    sizes = oracle.to_bf16(np.array([0.0, 2.0 ** -126, 1e-3, -1e-3, 0.0311, 0.03125, -0.03125, 0.7, 9.0], np.float32))
+    s = s.reshape(E * N, -1).copy()
+    for n in range(E * N):
+        if n % 40 < 9:
+            s[n] = sizes[n % 40]
+        elif n % 40 < 20 or n % 80 == 47:
+            s[n] = rng.choice(sizes, s.shape[1])
+    values = oracle.from_bf16(oracle.dequantize(wq, s, b, K, bits, group, oracle.BF16)).reshape(E, N, K)
+    run(ctx, oracle, (wq, s, b), values, oracle.make_x(rows, K, oracle.BF16), groups(None, E, rows, "even"), E, K, N, bits, group, y_dtype=F32)
+
+
 @pytest.mark.parametrize("bits,group,K", [(4, 32, 32), (4, 32, 96), (4, 64, 320), (4, 128, 4224), (8, 32, 160), (8, 64, 192)])
 @pytest.mark.parametrize("N,gated", [(19, False), (48, False), (32, True)])
 @pytest.mark.parametrize("rows", [7, 300])
