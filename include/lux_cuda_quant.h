@@ -398,9 +398,10 @@ typedef struct lux_gpu_quant_vtbl {
     /* --- a product with its epilogue (LUX_CUDA_QUANT_HAS) ---
      * y[M,N] = act(x[M,K] . dequant(wq[N,K])^T + bias[n]) + residual[M,N]
      * x, scales and biases BF16; bias fp32 [N]; residual F32 or BF16; y F32 or BF16.  The sum, the bias, the activation and the residual
-     * are taken in fp32 and rounded once.  bias or residual may be NULL: nothing is added.  y may be residual itself (of the same
-     * type); otherwise it overlaps nothing that is read.  Any M.  (The reference has op_matmul_f32, backend_plugin.h:129, then op_add_f32
-     * and the unary ops as calls of their own.) */
+     * are taken in fp32 and rounded once (for many rows, as in qmatmul and qmatmul_experts, by the tensor cores, whose fp32 sums cut off what
+     * does not fit: 1 to 3e-6 of y).  bias or residual may be NULL: nothing is added.  y may be residual itself (of the same type);
+     * otherwise it overlaps nothing that is read.  Any M.  (The reference has op_matmul_f32, backend_plugin.h:129, then op_add_f32 and the
+     * unary ops as calls of their own.) */
     LuxBackendError (*qmatmul_epi)(LuxBackendContext* ctx, const lux_qmm_epi_params* params, LuxBackendBuffer* x, LuxBackendBuffer* wq,
                                    LuxBackendBuffer* scales, LuxBackendBuffer* biases, LuxBackendBuffer* bias, LuxBackendBuffer* residual,
                                    LuxBackendBuffer* y);

@@ -13,6 +13,8 @@
 //     (2048 tokens x 8 experts x 4096: 134 MB, 27 us).  Fetched by index in here they cost more, since every tile of W does it again: TMA gathers of
 //     four rows take 29 ns each, 128 of them a stage of 256 rows (1692 us for the 4096 x 2816 product); 16-byte copies by two warps 588, and on pairs of
 //     CTAs 690 (their writes have to be waited for and fenced before the MMAs, two stages instead of three are under way).
+//   * The sums are the tensor cores' fp32 accumulators, which cut off instead of rounding: fp32 y is off by 1 to 3e-6 (2-norm).  Shorter sums added
+//     up outside would cost a second accumulator for every tile, in registers or memory.
 //   * Gated: a tile is eight groups of eight rows of gate and the eight of up that go with them, one TMA box of the weights seen as
 //     [expert][group of 8][half][8][byte].  Tensor memory is then read in the shape that leaves a row and the row eight further on in one
 //     thread: no exchange between the two halves.
