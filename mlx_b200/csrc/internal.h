@@ -393,7 +393,8 @@ struct MoeCombineArgs {
     void* out;
     size_t tokens, dim, y_rows;
     int top_k;
-    bool y_bf16, out_bf16, vec;  // vec: every row of every buffer starts on a 16-byte boundary and is whole pieces of 8
+    bool y_bf16, out_bf16;
+    int vec;  // 8, 4, 2 or 1: a row is whole pieces of so many columns, each on a boundary of its bytes (16 at most) in every buffer
 };
 cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev);
 // products grouped by expert (qmv_stream.cu: few rows an expert; qmm_experts.cu: many)

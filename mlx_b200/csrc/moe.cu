@@ -14,7 +14,8 @@
 // 8; 60 % of the issue slots): 8192 tokens 18.2 us, with sigmoid and bias 20.0.  Few tokens: by the latency of a launch, 4 us.
 //
 // moe_combine.  HBM-bound: a thread takes 8 neighbouring columns of a token, with the loads of up to 8 slots under way (4096 tokens x 8 x 4096,
-// fp32 stream: 65 us, 6.0 TB/s).
+// fp32 stream: 64 us, 6.1 TB/s); rows that are no whole pieces of 8 on 16-byte boundaries go in several of 4, 2 or 1 (1.3 to 2.9 times the floor,
+// 2 x 5003 bf16 the worst).
 #include <algorithm>
 #include <type_traits>
 
@@ -396,47 +397,79 @@ __global__ void __launch_bounds__(kCountThreads) moe_count_place_kernel(const Mo
 }
 
 // ---- the weighted sum -------------------------------------------------------------------------------------------------
-template <bool BF16>
-__device__ __forceinline__ float load1(const void* p, size_t i) {
-    if (BF16) return __uint_as_float((uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << 16);
-    return reinterpret_cast<const float*>(p)[i];
-}
-// V neighbouring elements (8 from a 16-byte boundary, or one)
+// V neighbouring elements, on a boundary of as many bytes as they have (16 at most)
 template <int V, bool BF16>
 struct Piece {
-    uint4 raw[BF16 ? 1 : 2];
+    static constexpr int kWords = BF16 ? (V + 1) / 2 : V;
+    uint32_t raw[kWords];
     __device__ __forceinline__ void load(const void* p, size_t i) {
-        if constexpr (V == 1) {
-            raw[0].x = __float_as_uint(load1<BF16>(p, i));
-        } else if constexpr (BF16) {
-            raw[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+        const char* q = static_cast<const char*>(p) + i * (BF16 ? 2 : 4);
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int k = 0; k < kWords; k += 4) {
+                const uint4 v = reinterpret_cast<const uint4*>(q)[k / 4];
+                raw[k] = v.x; raw[k + 1] = v.y; raw[k + 2] = v.z; raw[k + 3] = v.w;
+            }
+        } else if constexpr (kWords == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(q);
+            raw[0] = v.x; raw[1] = v.y;
+        } else if constexpr (BF16 && V == 1) {
+            raw[0] = *reinterpret_cast<const uint16_t*>(q);
         } else {
-            const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + i);
-            raw[0] = q[0];
-            raw[1] = q[1];
+            raw[0] = *reinterpret_cast<const uint32_t*>(q);
         }
     }
     __device__ __forceinline__ float at(int j) const {
-        if constexpr (V == 1) return __uint_as_float(raw[0].x);
-        const uint32_t* w = &raw[0].x;
-        if constexpr (BF16) return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
-        return __uint_as_float(w[j]);
+        if constexpr (BF16) return __uint_as_float(j & 1 ? raw[j >> 1] & 0xFFFF0000u : raw[j >> 1] << 16);
+        return __uint_as_float(raw[j]);
+    }
+    __device__ __forceinline__ void put(const float (&v)[V]) {
+        if constexpr (BF16) {
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[j], V > 1 ? v[j + (V > 1)] : 0.0f);
+                raw[j / 2] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++) raw[j] = __float_as_uint(v[j]);
+        }
+    }
+    __device__ __forceinline__ void store(void* p, size_t i) const {
+        char* q = static_cast<char*>(p) + i * (BF16 ? 2 : 4);
+        if constexpr (kWords >= 4) {
+#pragma unroll
+            for (int k = 0; k < kWords; k += 4) reinterpret_cast<uint4*>(q)[k / 4] = make_uint4(raw[k], raw[k + 1], raw[k + 2], raw[k + 3]);
+        } else if constexpr (kWords == 2) {
+            *reinterpret_cast<uint2*>(q) = make_uint2(raw[0], raw[1]);
+        } else if constexpr (BF16 && V == 1) {
+            *reinterpret_cast<uint16_t*>(q) = (uint16_t)raw[0];
+        } else {
+            *reinterpret_cast<uint32_t*>(q) = raw[0];
+        }
     }
 };
-template <int V, bool YB, bool OB>
-__global__ void __launch_bounds__(256) moe_combine_kernel(const MoeCombineArgs a) {
+// A thread: R pieces of V columns of a token, `groups` pieces apart; U: slots whose loads are under way together.
+template <int V, int R, int U, bool YB, bool OB>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const MoeCombineArgs a, size_t groups) {
     wait_previous();
-    const size_t per_row = (a.dim + V - 1) / V, i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= per_row * a.tokens) return;
-    const size_t t = per_row * a.tokens <= 0xffffffffu ? (uint32_t)i / (uint32_t)per_row : i / per_row, col = (i - t * per_row) * V;
-    constexpr int U = YB || V == 1 ? 8 : 4;  // slots whose loads are under way together
-    float s[V];
-    Piece<V, OB> r;
-    if (a.residual) r.load(a.residual, t * a.dim + col);
+    const size_t pieces = a.dim / V, i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= groups * a.tokens) return;
+    const size_t t = groups * a.tokens <= 0xffffffffu ? (uint32_t)i / (uint32_t)groups : i / groups, c0 = i - t * groups;
+    float s[R][V];
+    bool in[R];
+    Piece<V, OB> o[R];
 #pragma unroll
-    for (int j = 0; j < V; j++) s[j] = a.residual ? r.at(j) : 0.0f;
+    for (int r = 0; r < R; r++) {
+        in[r] = R == 1 || c0 + r * groups < pieces;
+        if (a.residual && in[r]) o[r].load(a.residual, t * a.dim + (c0 + r * groups) * V);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < V; j++) s[r][j] = a.residual && in[r] ? o[r].at(j) : 0.0f;
     for (int j0 = 0; j0 < a.top_k; j0 += U) {
-        Piece<V, YB> y[U];
+        Piece<V, YB> y[U][R];
         float w[U];
         bool there[U];
 #pragma unroll
@@ -446,33 +479,25 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const MoeCombineArgs a
             const int at = slot ? a.pos[p] : -1;
             there[u] = at >= 0 && (size_t)at < a.y_rows;
             w[u] = slot && a.weights ? a.weights[p] : 1.0f;
-            if (there[u]) y[u].load(a.y, (size_t)at * a.dim + col);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (there[u] && in[r]) y[u][r].load(a.y, (size_t)at * a.dim + (c0 + r * groups) * V);
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (there[u]) {
 #pragma unroll
-                for (int j = 0; j < V; j++) s[j] = fmaf(w[u], y[u].at(j), s[j]);
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int j = 0; j < V; j++) s[r][j] = in[r] ? fmaf(w[u], y[u][r].at(j), s[r][j]) : 0.0f;
             }
     }
-    const size_t o = t * a.dim + col;
-    if constexpr (V == 1) {
-        if (OB) reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(s[0]);
-        else reinterpret_cast<float*>(a.out)[o] = s[0];
-    } else if constexpr (OB) {
-        uint4 v;
-        uint32_t* w = &v.x;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(s[2 * j], s[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+    for (int r = 0; r < R; r++)
+        if (in[r]) {
+            o[r].put(s[r]);
+            o[r].store(a.out, t * a.dim + (c0 + r * groups) * V);
         }
-        *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o) = v;
-    } else {
-        float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o);
-        q[0] = make_float4(s[0], s[1], s[2], s[3]);
-        q[1] = make_float4(s[4], s[5], s[6], s[7]);
-    }
 }
 
 cudaLaunchConfig_t config(unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, bool overlap_prev, cudaLaunchAttribute* attr) {
@@ -546,16 +571,32 @@ cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t s
     return cudaLaunchKernelEx(&place, moe_place_kernel, a, chunk, blocks);
 }
 
-cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {
-    const size_t pieces = (a.vec ? a.dim / 8 : a.dim) * a.tokens;
-    const unsigned threads = pieces >= 148 * 256 ? 256 : 64;  // (few pieces: more blocks, on more SMs)
+namespace {
+template <int V, int R, int U>
+cudaError_t launch_combine_t(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {
+    const size_t groups = (a.dim / V + R - 1) / R, all = groups * a.tokens;
+    const unsigned threads = all >= 148 * 256 ? 256 : 64;  // (few: more blocks, on more SMs)
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = config((unsigned)((pieces + threads - 1) / threads), threads, 0, stream, overlap_prev, &attr);
-    void (*kern)(MoeCombineArgs) = a.vec ? (a.y_bf16 ? (a.out_bf16 ? moe_combine_kernel<8, true, true> : moe_combine_kernel<8, true, false>)
-                                                     : (a.out_bf16 ? moe_combine_kernel<8, false, true> : moe_combine_kernel<8, false, false>))
-                                         : (a.y_bf16 ? (a.out_bf16 ? moe_combine_kernel<1, true, true> : moe_combine_kernel<1, true, false>)
-                                                     : (a.out_bf16 ? moe_combine_kernel<1, false, true> : moe_combine_kernel<1, false, false>));
-    return cudaLaunchKernelEx(&cfg, kern, a);
+    const cudaLaunchConfig_t cfg = config((unsigned)((all + threads - 1) / threads), threads, 0, stream, overlap_prev, &attr);
+    constexpr int UF = V == 8 ? (U + 1) / 2 : U;  // (fp32: as many bytes)
+    void (*kern)(MoeCombineArgs, size_t) = a.y_bf16 ? (a.out_bf16 ? moe_combine_kernel<V, R, U, true, true> : moe_combine_kernel<V, R, U, true, false>)
+                                                    : (a.out_bf16 ? moe_combine_kernel<V, R, UF, false, true> : moe_combine_kernel<V, R, UF, false, false>);
+    return cudaLaunchKernelEx(&cfg, kern, a, groups);
+}
+}  // namespace
+
+// Rows of whole pieces of eight: eight slots under way, or two and more columns where there are no more slots.  Others: two slots of more columns, which
+// leaves room for more threads and wastes less on slots that are not there (3565 x 6 x 7684 bf16 90 us, eight slots 123, one column a thread
+// 284; 4463 x 2 x 7772 62, eight 135, 329); eight where there are no more columns than the card has threads (16 x 8 x 5003 4.2 us, two slots 5.1;
+// 128 x 8 x 4098 6.6, two slots 5.8).
+cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {
+    const bool two = a.top_k <= 2 || a.dim * a.tokens > 148 * 2048;
+    switch (a.vec) {
+        case 8: return a.top_k <= 2 ? launch_combine_t<8, 2, 2>(a, stream, overlap_prev) : launch_combine_t<8, 1, 8>(a, stream, overlap_prev);
+        case 4: return two ? launch_combine_t<4, 4, 2>(a, stream, overlap_prev) : launch_combine_t<4, 2, 8>(a, stream, overlap_prev);
+        case 2: return two ? launch_combine_t<2, 8, 2>(a, stream, overlap_prev) : launch_combine_t<2, 4, 8>(a, stream, overlap_prev);
+        default: return two ? launch_combine_t<1, 8, 2>(a, stream, overlap_prev) : launch_combine_t<1, 4, 8>(a, stream, overlap_prev);
+    }
 }
 
 }  // namespace luxcuda

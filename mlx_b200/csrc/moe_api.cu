@@ -251,9 +251,11 @@ LuxBackendError moe_combine(LuxBackendContext* ctx, const lux_moe_combine_params
     o[OUT].written = true;
     if (LuxBackendError e = check(o, COUNT, "moe_combine", OUT, RES)) return e;
     if (!p.tokens || !p.dim) return LUX_BACKEND_OK;
-    auto vec = [&](int i) { return !o[i].b || ((uintptr_t)o[i].b->ptr & 15) == 0; };
+    int vec = 8;  // columns that lie together on a boundary of theirs in every row
+    auto fits = [&](int i, size_t es) { return !o[i].b || ((uintptr_t)o[i].b->ptr & (std::min<size_t>(vec * es, 16) - 1)) == 0; };
+    while (vec > 1 && !(p.dim % vec == 0 && fits(Y, ys) && fits(RES, os) && fits(OUT, os))) vec /= 2;
     const MoeCombineArgs a{o[Y].ptr(), (const int*)o[POS].ptr(), (const float*)o[WEIGHTS].ptr(), o[RES].ptr(), o[OUT].ptr(), (size_t)p.tokens, (size_t)p.dim, (size_t)p.y_rows,
-                           p.top_k, ys == 2, os == 2, p.dim % 8 == 0 && vec(Y) && vec(RES) && vec(OUT)};
+                           p.top_k, ys == 2, os == 2, vec};
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
     LUX_CUDA_TRY(launch_moe_combine(a, c->stream, chain_is_open(c)));

@@ -49,6 +49,33 @@ def test_combine(ctx, oracle, y_dtype, out_dtype, T, dim, k, shift):
             res.from_host(oracle.to_bf16(rv.astype(np.float32)) if out_dtype == BF16 else rv.astype(np.float32))
 
 
+@pytest.mark.parametrize("y_dtype", [F32, BF16])
+@pytest.mark.parametrize("out_dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [4, 12, 2, 6, 3, 5, 1028, 1030, 1031])
+@pytest.mark.parametrize("T,k,shift", [(9, 5, 0), (9, 5, 2), (9, 5, 4), (9, 2, 0), (9, 1, 2), (700, 5, 0)])
+def test_pieces_of_a_row(ctx, oracle, y_dtype, out_dtype, dim, T, k, shift):
+    """Pieces of 4, 2 and single columns, buffers that begin so many elements past a 16-byte boundary: the bits of a row of the same values whose
+    pieces are wide ones."""
+    rng = np.random.default_rng(dim + shift)
+    wide = (dim + 7) // 8 * 8
+    v, r = rng.standard_normal((T * k, wide)).astype(np.float32), rng.standard_normal((T, wide)).astype(np.float32)
+    pos, w = ctx.upload(rng.permutation(T * k).astype(np.int32)), ctx.upload(rng.standard_normal(T * k).astype(np.float32))
+
+    def run(n, shift):
+        bufs = []
+        for a, dt in ((v, y_dtype), (r, out_dtype), (np.zeros_like(r), out_dtype)):
+            raw = a[:, :n].reshape(-1)
+            raw = oracle.to_bf16(raw) if dt == BF16 else raw
+            room = ctx.upload(np.concatenate([np.full(shift, 7, raw.dtype), raw, np.full(8, 7, raw.dtype)]))
+            bufs.append((room, ctx.wrap(room.device_ptr + shift * raw.itemsize, raw.nbytes)))
+        ctx.moe_combine(ctx.moe_combine_params(T, n, k, T * k, y_dtype=y_dtype, out_dtype=out_dtype), bufs[0][1], pos, w, bufs[1][1], bufs[2][1])
+        got = bufs[2][0].to_host()
+        assert (got[:shift] == 7).all() and (got[-8:] == 7).all()
+        return got[shift:-8].reshape(T, n)
+
+    np.testing.assert_array_equal(run(dim, shift), run(wide, 0)[:, :dim])
+
+
 def test_rows_of_nobody_are_not_read(ctx):
     """Infinities and NaN in rows that no pair stands for do not come through."""
     T, dim, k = 5, 64, 2
