@@ -13,10 +13,12 @@ struct ExpertsShape {
     int experts, K, N, bits;
     bool gather;  // rows of x are fetched by index
 };
-constexpr int kPairMean = 80;  // rows an expert on average from which on the GEMM runs on pairs of CTAs
+// Pairs of CTAs: from so many rows an expert on average, where single ones would have so many tiles each (64 experts x 256 rows, 4096 x 2816: pairs 372 us, single
+// ones 410; 64 rows: 163 and 160; 150 shapes with 32 to 1000 rows an expert and mostly fewer tiles: 3 % lost all in all, by the rows alone 12).
+constexpr int kPairMean = 80, kPairTiles = 3;
 inline bool experts_in_pairs(const ExpertsShape& s, int sm_count) {
-    const size_t mean = (s.rows + s.experts - 1) / s.experts;
-    return sm_count % 2 == 0 && s.N > 128 && mean >= (size_t)kPairMean;
+    const size_t mean = (s.rows + s.experts - 1) / s.experts, tiles = (size_t)s.experts * ((mean + 127) / 128) * ((s.N + 127) / 128);
+    return sm_count % 2 == 0 && s.N > 128 && mean >= (size_t)kPairMean && tiles > (size_t)kPairTiles * sm_count;
 }
 
 // Estimates of the times in microseconds, for experts that share the rows evenly: the host does not know better.  Fitted to 170 shapes (2 to 128

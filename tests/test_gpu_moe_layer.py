@@ -141,9 +141,9 @@ def test_chained_with_the_rest(ctx, oracle):
 
 
 def test_the_kernels_that_take_a_layer(ctx, oracle):
-    """Few rows an expert: the decode kernel; many: the GEMM, pairs of CTAs where they are many more."""
-    for T, first in ((1, "qmv_experts<4>"), (150, "qmm_experts<4>"), (600, "qmm_experts<4,pairs>")):
-        layer = Layer(ctx, oracle, T, 4, 2, 512, 512)
+    """Few rows an expert: the decode kernel; many: the GEMM, pairs of CTAs where they are many more and single ones would have several tiles each."""
+    for T, E, k, F, first in ((1, 4, 2, 512, "qmv_experts<4>"), (150, 4, 2, 512, "qmm_experts<4>"), (600, 4, 2, 512, "qmm_experts<4>"), (300, 16, 8, 1024, "qmm_experts<4,pairs>")):
+        layer = Layer(ctx, oracle, T, E, k, 512, F)
         layer.step()
         ctx.qmatmul_experts(layer.prm[1], layer.b["x"], layer.b["order"], layer.b["offsets"], *layer.b["up"], None, layer.b["h"])
         assert ctx.last_kernel() == first
