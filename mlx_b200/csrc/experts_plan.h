@@ -45,6 +45,25 @@ inline bool experts_have_many_rows(const ExpertsShape& s, int sm_count) {
     return many < few;
 }
 
+// The decode kernel's boxes (qmv_stream.cu) of the packed weights [expert][half][row][byte]: a tile is 16 rows, eight of either half where gated.
+// What a box of whole 128-byte k-blocks holds behind a row's end is the start of the row after it, which must be there: so rows below 128 bytes end
+// with themselves (the k-block is filled up with zeros), and the last tile of all takes single k-blocks of a map that ends with the rows, `end`.
+struct ExpertsMap {
+    unsigned long long dims[4], strides[3];
+    unsigned box[4];
+};
+inline ExpertsMap experts_map(int experts, int K, int N, int bits, bool gated, int kbc) {
+    const unsigned long long row = (unsigned long long)K * bits / 8, halves = gated ? 2 : 1, rows = N / halves;
+    return {{row < 128 ? row : 128, rows, halves * experts, (row + 127) / 128}, {row, rows * row, 128}, {128, (unsigned)(16 / halves), (unsigned)halves, (unsigned)kbc}};
+}
+inline ExpertsMap experts_map_end(int experts, int K, int N, int bits, bool gated) {  // (three dimensions)
+    ExpertsMap m = experts_map(experts, K, N, bits, gated, 1);
+    m.dims[0] = m.strides[0];
+    return m;
+}
+// of `tiles` tiles from tile0 on of expert e: those that take the first of the two maps
+constexpr int experts_whole(bool k_tail, int e, int experts, int tile0, int tiles, int n_rt) { return k_tail && e + 1 == experts && tile0 + tiles == n_rt ? tiles - 1 : tiles; }
+
 constexpr int kExpertStages = 4, kExpertGroups = 4, kExpertEpis = 4;  // of the GEMM (see qmm_experts.cu)
 constexpr int kLowRows = 128;                                         // rows of x of a single CTA's tile, at most: half an accumulator's columns
 constexpr int y_pitch(bool gated) { return gated ? kTileN + 16 : 2 * kTileN; }  // of a finished tile in shared memory, bytes a row of x (gated: off the banks)

@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "epilogue.cuh"
+#include "experts_plan.h"
 #include "groups.cuh"
 #include "internal.h"
 #include "qmv_frag.cuh"
@@ -169,8 +170,8 @@ struct GroupParams<kGroups> {
     // The scales of a tile's rows lie side by side, and its biases: one bulk copy each (two where gated) into [16 rows][groups], without padding; for K
     // in one chunk and N in whole tiles.  (By pieces as above the one warp that fetches them takes 0.5 us per tile, whatever K.)
     int sb_bulk;
-    // K inside a k-block: the boxes are whole all the same, and what they hold behind a row's end is the row after it (with scales of zero); but the
-    // last tile of all, behind which nothing need be, takes single k-blocks of this map, which ends with the rows.
+    // K inside a k-block: the boxes are whole all the same (what they hold behind a row's end has scales of zero); but the last tile of all takes single
+    // k-blocks of this map, which ends with the rows (experts_map).
     alignas(64) CUtensorMap map_end;
 };
 // NI: how many matmuls of a batch, at most; 1: one; 0: one whose rows of x are n_items items of 16 (M: all of them); kGroups: experts.
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 if constexpr (kExperts) {
                     constexpr int TR = kGated ? 8 : 16;
                     const int z = kGated ? 2 * wk.e : wk.e, kb0 = wk.c * p.kbc, ops = wk.kb_cnt(p);
-                    const int whole = p.k_tail && wk.e + 1 == p.experts && tile0 + tiles == p.n_rt ? tiles - 1 : tiles;
+                    const int whole = experts_whole(p.k_tail, wk.e, p.experts, tile0, tiles, p.n_rt);
                     if (lane == 0) bar_expect(full + 8 * st, (whole * p.kbc + (tiles - whole) * ops) * 2048 + more);
                     __syncwarp();
                     if (lane < whole) tma_load_4d(stage + lane * p.tile_bytes, &p.maps[0], 0, (tile0 + lane) * TR, z, kb0, full + 8 * st);
@@ -988,21 +989,19 @@ cudaError_t launch_qmv_experts(const ExpertsArgs& a, int sm_count, cudaStream_t 
     Plan pl;
     const EncodeTiledFn encode = encode_tiled_fn();
     if (!encode || !make_plan(one_expert(a), kGroupRows, sm_count, &pl, a.experts)) return cudaErrorInvalidValue;
-    // The packed weights [expert][half][row][byte], a tile being eight rows of either half, or 16 of the only one: boxes as encode_weights'
-    const cuuint64_t row_bytes = (cuuint64_t)a.K * a.bits / 8, halves = a.gated ? 2 : 1, rows = a.N / halves;
-    const cuuint32_t estr[4] = {1, 1, 1, 1}, box_rows = 16 / (cuuint32_t)halves;
+    auto encode_map = [&](const ExpertsMap& m, int n, CUtensorMap* map) {
+        cuuint64_t dims[4], strides[3];
+        cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
+        std::copy(m.dims, m.dims + 4, dims);
+        std::copy(m.strides, m.strides + 3, strides);
+        std::copy(m.box, m.box + 4, box);
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
     CUtensorMap map, map_end;
-    const cuuint64_t dims[4] = {128, rows, halves * a.experts, (row_bytes + 127) / 128}, strides[3] = {row_bytes, rows * row_bytes, 128};
-    const cuuint32_t box[4] = {128, box_rows, (cuuint32_t)halves, (cuuint32_t)pl.kbc};
-    CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint32_t*>(a.wq), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CUresult r = encode_map(experts_map(a.experts, a.K, a.N, a.bits, a.gated, pl.kbc), 4, &map);
     map_end = map;
-    if (r == CUDA_SUCCESS && row_bytes % 128) {  // (see GroupParams::map_end)
-        const cuuint64_t edims[3] = {row_bytes, rows, halves * a.experts}, estrides[2] = {row_bytes, rows * row_bytes};
-        const cuuint32_t ebox[3] = {128, box_rows, (cuuint32_t)halves};
-        r = encode(&map_end, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint32_t*>(a.wq), edims, estrides, ebox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    }
+    if (r == CUDA_SUCCESS && (size_t)a.K * a.bits / 8 % 128) r = encode_map(experts_map_end(a.experts, a.K, a.N, a.bits, a.gated), 3, &map_end);
     if (r != CUDA_SUCCESS) {
         set_last_error("cuTensorMapEncodeTiled (experts' weights) failed (%d)", (int)r);
         return cudaErrorInvalidValue;
