@@ -273,10 +273,12 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
         unsigned char* stg = sEpi + (size_t)warp * kEpiStageBytes;
         const bool staged = PAIR && p.y_staged;
         constexpr int kEpiBar = 1;  // named barrier of these warps
+        auto wait_tile = [&](uint32_t acc, uint32_t i) {  // (staged: and the previous tile has left)
+            return staged ? mbar_wait_epis<kEpiBar, kEpis>(&ctl->tmem_full[acc], phase_of(i), abort_flag) : mbar_wait_epi(&ctl->tmem_full[acc], phase_of(i), abort_flag);
+        };
         uint32_t tile_i = 0;
         for (; seg.valid(); seg.next(), tile_i++) {
             const int tile_n = n_tile(seg);
-            if (staged && tile_i) asm volatile("bar.sync %0, %1;" ::"n"(kEpiBar), "n"(kEpis * 32) : "memory");  // the previous tile has left
             const int blocks = (seg.rows + 15) >> 4;
             const size_t ld = GATED ? p.N >> 1 : p.N;
             const uint32_t acc = acc_of(tile_i), quarter = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kLowRows;
@@ -293,7 +295,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
                         bu[j] = __ldcg(p.bias + (size_t)seg.e * p.N + F + f[j]);
                     }
                 }
-                if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
+                if (!wait_tile(acc, tile_i)) break;
                 tc_fence_after();
                 for (int blk = 0; blk < blocks; blk++) {
                     uint32_t v[2][8];
@@ -341,7 +343,7 @@ __device__ __forceinline__ void experts_body(const CUtensorMap& tmap_x, const CU
             } else {
                 const int n = tile_n * kTileN + q * 32 + lane;
                 const float b = p.bias && n < p.N ? __ldcg(p.bias + (size_t)seg.e * p.N + n) : 0.0f;
-                if (!mbar_wait(&ctl->tmem_full[acc], phase_of(tile_i), abort_flag)) break;
+                if (!wait_tile(acc, tile_i)) break;
                 tc_fence_after();
                 for (int blk = 0; blk < blocks; blk++) {
                     uint32_t v[16];

@@ -64,6 +64,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, vol
     *abort_flag = 1;
     return false;
 }
+// The epilogue warps' wait.  One answer for a warp, whose loads from tensor memory are collective: a lane may still have seen the barrier flip when
+// others gave up.
+__device__ __forceinline__ bool mbar_wait_epi(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag));
+}
+// ... and one for all WARPS warps where they meet at the named barrier BAR before they wait again (and they meet there now).
+template <int BAR, int WARPS>
+__device__ __forceinline__ bool mbar_wait_epis(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+    uint32_t all;
+    asm volatile("{ .reg .pred p, q; setp.ne.u32 q, %1, 0; bar.red.and.pred p, %2, %3, q; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(all) : "r"((uint32_t)mbar_wait(b, parity, abort_flag)), "n"(BAR), "n"(WARPS * 32) : "memory");
+    return all != 0;
+}
 // After an abort nobody waits for the copies and MMAs in flight any more; before the CTA frees its tensor memory and ends
 // they get two milliseconds, far more than they take.  Every thread, behind the barrier at which all roles have returned.
 __device__ __forceinline__ void settle_after_abort(volatile int* abort_flag) {

@@ -314,7 +314,10 @@ qmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant_
             const int n = (tile / p.m_tiles) * kTileN + nl;
             const int m0 = (tile % p.m_tiles) * p.bm;
             if (EPI && s_lo == 0) prefetch_residual(p, m0, min(p.bm, p.M - m0), n - nl, et);
-            if (!mbar_wait(&sl->tmem_full, tile_i & 1, abort_flag)) break;
+            // (split tiles: these warps meet at a barrier below)
+            if (!(s_lo != 0 || s_hi != nst ? mbar_wait_epis<kEpiBar, kEpiWarps>(&sl->tmem_full, tile_i & 1, abort_flag)
+                                           : mbar_wait_epi(&sl->tmem_full, tile_i & 1, abort_flag)))
+                break;
             tc_fence_after();
             const int m_end = min(p.bm, p.M - m0);
             if (s_lo != 0) {
@@ -603,7 +606,7 @@ qmm_tc_tiles_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_con
             const int n = (tile / p.m_tiles) * kTileN + q * 32 + lane;
             const int m0 = (tile % p.m_tiles) * p.bm;
             if (EPI) prefetch_residual(p, m0, min(p.bm, p.M - m0), (tile / p.m_tiles) * kTileN, tid);
-            if (!mbar_wait(&sl->tmem_full, tile_i & 1, abort_flag)) break;
+            if (!mbar_wait_epi(&sl->tmem_full, tile_i & 1, abort_flag)) break;
             tc_fence_after();
             // this thread: column n of y, rows m0 + c (32 consecutive n per warp: 64-byte row segments)
             const int m_end = min(p.bm, p.M - m0);
@@ -798,12 +801,13 @@ qmm_tc_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             const int n = n0_of(tile) + q * 32 + lane;
             const int m0 = (tile % p.m_tiles) * p.bm;
             if (EPI) prefetch_residual(p, m0, min(p.bm, p.M - m0), n0_of(tile), tid);
-            if (p.y_tma && tile_i > 0) {
+            if (p.y_tma) {
                 // the copy engine has finished reading the previous tile out of the staging buffer
-                if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                asm volatile("bar.sync %0, %1;" ::"n"(kPairEpiBar), "n"(kEpiWarps * 32) : "memory");
+                if (tid == 0 && tile_i > 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                if (!mbar_wait_epis<kPairEpiBar, kEpiWarps>(&sl->tmem_full, tile_i & 1, abort_flag)) break;
+            } else if (!mbar_wait_epi(&sl->tmem_full, tile_i & 1, abort_flag)) {
+                break;
             }
-            if (!mbar_wait(&sl->tmem_full, tile_i & 1, abort_flag)) break;
             tc_fence_after();
             if (p.y_tma) {
                 // The accumulator goes to shared memory as bf16, [row of x][column], and is released at once; the
