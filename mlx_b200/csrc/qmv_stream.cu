@@ -82,19 +82,20 @@ __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
                  : "=r"(ok) : "r"(b), "r"(parity), "r"(20000u) : "memory");
     return ok != 0;
 }
-// Bounded wait (about two seconds of SM clock).  False: it ran out, or another role has given up; *abort is set.
+// Bounded wait (about two seconds of SM clock).  False: it ran out, or another role has given up; *abort is set.  The answer is a lane's own: one may
+// still have seen the barrier flip when others gave up.  What a warp does together behind a wait needs the answer of all (a vote, which costs 1 % in
+// the working warps' loop) or none: those and the summing warps go on over what there is in shared memory, with short waits from then on.
 // SLEEP: of the helper warps, which are never in a hurry.
 template <bool SLEEP>
 __device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int* abort) {
     if (bar_try(b, parity)) return true;
     const uint32_t t0 = clock();
-    for (;;) {
+    while (!*abort && (uint32_t)clock() - t0 <= 4000000000u) {
 #pragma unroll 1
         for (int i = 0; i < 64; i++) {
             if (SLEEP) __nanosleep(32);
             if (bar_try(b, parity)) return true;
         }
-        if (*abort || (uint32_t)clock() - t0 > 4000000000u) break;
     }
     *abort = 1;
     return false;
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 do {
                     for (int g = 0; g < wk.ng && ok; g++) {
                         const int tile0 = wk.b0 + g * p.ts, tiles = min(p.ts, wk.tile_end(p) - tile0);
-                        ok = bar_wait<true>(empty + 8 * st, ph ^ 1, abort);
+                        ok = __all_sync(0xffffffffu, bar_wait<true>(empty + 8 * st, ph ^ 1, abort));
                         if (!ok) break;
                         const uint32_t stage = ring + st * p.stage_bytes;
                         expert_boxes(stage, tile0, tiles, tiles * 64 * gpr);
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                     const int tile0 = wk.b0 + g * p.ts, tiles = min(p.ts, t_end - tile0);
                     // (the ring is full and nobody works on it before the previous kernel has ended: see the summing warps)
                     if (issued == p.stages) asm volatile("griddepcontrol.wait;" ::: "memory");
-                    ok = bar_wait<true>(empty + 8 * st, ph ^ 1, abort);
+                    ok = __all_sync(0xffffffffu, bar_wait<true>(empty + 8 * st, ph ^ 1, abort));
                     if (!ok) break;
                     const uint32_t stage = ring + st * p.stage_bytes;
                     if constexpr (kExperts) {
@@ -506,14 +507,13 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 }
                 // lane (g, t) of the MMA: rows n = g, g+8 of the tile, rows of x 2t, 2t+1 (and 8 more)
                 const int m0 = 2 * (lane & 3), n0 = lane >> 2;
-                for (int g = 0; g < wk.ng && ok; g++) {
+                for (int g = 0; g < wk.ng; g++) {
                     if (turn-- != 0) {
                         next_stage();
                         continue;
                     }
                     turn = p.sum_warps - 1;
-                    ok = bar_wait<true>(sums + 8 * st, ph, abort);
-                    if (!ok) break;
+                    bar_wait<true>(sums + 8 * st, ph, abort);
                     const int tile0 = wk.b0 + g * p.ts, tiles = min(p.ts, t_end - tile0);
                     for (int i = 0; i < tiles * MT; i++) {
                         const int ti = MT == 1 ? i : i >> 1, mt = MT == 1 ? 0 : i & 1;
@@ -744,7 +744,11 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
             }
 #pragma unroll 1
             for (int gi = 0; gi < mine; gi++) {
-                if (!bar_wait<false>(bar, ph, abort)) { ok = false; break; }
+                if constexpr (MT == 2 && SPL == 2) {  // (16 rows in groups of 32: without a way out the compiler spills 88 bytes, 5 % of the time)
+                    if (!__all_sync(0xffffffffu, bar_wait<false>(bar, ph, abort))) { ok = false; break; }
+                } else {
+                    bar_wait<false>(bar, ph, abort);
+                }
                 uint32_t w[2][8], s[2][SPL], b[2][SPL];
 #pragma unroll
                 for (int r = 0; r < 2; r++)
@@ -779,8 +783,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
                 next_stage();
             }
             for (int gi = mine; gi < ng && ok; gi++) {  // groups without a tile of this warp
-                ok = bar_wait<false>(bar, ph, abort);
-                if (ok && lane == 0) bar_arrive(bar + 8 * kMaxStages);
+                bar_wait<false>(bar, ph, abort);
+                if (lane == 0) bar_arrive(bar + 8 * kMaxStages);
                 next_stage();
             }
             if (!ok || !wk.next_run(p)) break;
