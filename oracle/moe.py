@@ -4,9 +4,9 @@ import numpy as np
 NONE, RELU, SILU, GELU, GELU_TANH = range(5)
 
 
-def _erf(v):
-    from math import erf
-    return np.vectorize(erf, otypes=[np.float64])(v)
+def _erfc(v):
+    from math import erfc
+    return np.vectorize(erfc, otypes=[np.float64])(v)
 
 
 def act(kind, v):
@@ -17,7 +17,7 @@ def act(kind, v):
         if kind == SILU:
             return v / (1 + np.exp(-v))
         if kind == GELU:
-            return 0.5 * v * (1 + _erf(v / np.sqrt(2)))
+            return 0.5 * v * _erfc(-v / np.sqrt(2))
         if kind == GELU_TANH:
             return 0.5 * v * (1 + np.tanh(np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3)))
     return v
