@@ -67,17 +67,13 @@ def check(tile_end, E, K, N, bits, gated):
 
 
 @pytest.mark.parametrize("bits,K", [(4, 32), (4, 64), (4, 96), (4, 128), (4, 224), (4, 256), (4, 288), (4, 2912), (8, 32), (8, 64), (8, 96), (8, 128), (8, 160), (8, 2080)])
-@pytest.mark.parametrize("N", [1, 2, 15, 16, 17, 18, 31, 33, 129])
-@pytest.mark.parametrize("E", [1, 2, 3, 17])
-def test_no_box_ends_behind_the_weights(tile_end, bits, K, N, E):
+def test_no_box_ends_behind_the_weights(tile_end, bits, K):
     """Rows of 16 bytes and more, last tiles of one row and more, experts of one row: a box of whole k-blocks over them reaches up to seven rows further."""
-    check(tile_end, E, K, N, bits, False)
-
-
-@pytest.mark.parametrize("bits,K", [(4, 32), (4, 96), (4, 288), (8, 32), (8, 96), (8, 128)])
-@pytest.mark.parametrize("N", [16, 32, 272])
-def test_gated(tile_end, bits, K, N):
-    check(tile_end, 3, K, N, bits, True)
+    for E in (1, 2, 3, 17):
+        for N in (1, 2, 15, 16, 17, 18, 31, 33, 129):
+            check(tile_end, E, K, N, bits, False)
+        for N in (16, 32, 272):
+            check(tile_end, E, K, N, bits, True)
 
 
 def test_any_shape(tile_end):
