@@ -396,7 +396,7 @@ struct MoeCombineArgs {
     bool y_bf16, out_bf16;
     int vec;  // 8, 4, 2 or 1: a row is whole pieces of so many columns, each on a boundary of its bytes (16 at most) in every buffer
 };
-cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev);
+cudaError_t launch_moe_combine(const MoeCombineArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev);
 // products grouped by expert (qmv_stream.cu: few rows an expert; qmm_experts.cu: many)
 struct ExpertsArgs {
     const void* x;

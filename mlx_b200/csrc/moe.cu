@@ -536,7 +536,8 @@ cudaError_t launch_route_v(const MoeRouteArgs& a, int blocks, int chunk, cudaStr
 
 }  // namespace
 
-// One block: as long as its warps have no more than a token each (64 tokens, two each: 10.4 us against 9.0 in several) and the pairs fit a round.
+// One block: up to 32 tokens, a token a warp, or two above 256 experts, where a block has 16 warps (64 tokens of 64 experts, two a warp: 10.4 us against 9.0 in
+// several blocks), and pairs that fit a round.
 int moe_route_blocks(const MoeRouteArgs& a, int sm_count) {
     if (a.tokens <= 32 && a.tokens * a.top_k <= (size_t)kRoundPairs) return 1;
     const size_t most = std::min(sm_count, kMaxBlocks), per = std::max<size_t>(route_warps(a.experts), (a.tokens + most - 1) / most);
@@ -573,9 +574,9 @@ cudaError_t launch_moe_route(const MoeRouteArgs& a, int sm_count, cudaStream_t s
 
 namespace {
 template <int V, int R, int U>
-cudaError_t launch_combine_t(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {
+cudaError_t launch_combine_t(const MoeCombineArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev) {
     const size_t groups = (a.dim / V + R - 1) / R, all = groups * a.tokens;
-    const unsigned threads = all >= 148 * 256 ? 256 : 64;  // (few: more blocks, on more SMs)
+    const unsigned threads = all >= (size_t)sm_count * 256 ? 256 : 64;  // (few: more blocks, on more SMs)
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = config((unsigned)((all + threads - 1) / threads), threads, 0, stream, overlap_prev, &attr);
     constexpr int UF = V == 8 ? (U + 1) / 2 : U;  // (fp32: as many bytes)
@@ -589,13 +590,13 @@ cudaError_t launch_combine_t(const MoeCombineArgs& a, cudaStream_t stream, bool 
 // leaves room for more threads and wastes less on slots that are not there (3565 x 6 x 7684 bf16 90 us, eight slots 123, one column a thread
 // 284; 4463 x 2 x 7772 62, eight 135, 329); eight where there are no more columns than the card has threads (16 x 8 x 5003 4.2 us, two slots 5.1;
 // 128 x 8 x 4098 6.6, two slots 5.8).
-cudaError_t launch_moe_combine(const MoeCombineArgs& a, cudaStream_t stream, bool overlap_prev) {
-    const bool two = a.top_k <= 2 || a.dim * a.tokens > 148 * 2048;
+cudaError_t launch_moe_combine(const MoeCombineArgs& a, int sm_count, cudaStream_t stream, bool overlap_prev) {
+    const bool two = a.top_k <= 2 || a.dim * a.tokens > (size_t)sm_count * 2048;
     switch (a.vec) {
-        case 8: return a.top_k <= 2 ? launch_combine_t<8, 2, 2>(a, stream, overlap_prev) : launch_combine_t<8, 1, 8>(a, stream, overlap_prev);
-        case 4: return two ? launch_combine_t<4, 4, 2>(a, stream, overlap_prev) : launch_combine_t<4, 2, 8>(a, stream, overlap_prev);
-        case 2: return two ? launch_combine_t<2, 8, 2>(a, stream, overlap_prev) : launch_combine_t<2, 4, 8>(a, stream, overlap_prev);
-        default: return two ? launch_combine_t<1, 8, 2>(a, stream, overlap_prev) : launch_combine_t<1, 4, 8>(a, stream, overlap_prev);
+        case 8: return a.top_k <= 2 ? launch_combine_t<8, 2, 2>(a, sm_count, stream, overlap_prev) : launch_combine_t<8, 1, 8>(a, sm_count, stream, overlap_prev);
+        case 4: return two ? launch_combine_t<4, 4, 2>(a, sm_count, stream, overlap_prev) : launch_combine_t<4, 2, 8>(a, sm_count, stream, overlap_prev);
+        case 2: return two ? launch_combine_t<2, 8, 2>(a, sm_count, stream, overlap_prev) : launch_combine_t<2, 4, 8>(a, sm_count, stream, overlap_prev);
+        default: return two ? launch_combine_t<1, 8, 2>(a, sm_count, stream, overlap_prev) : launch_combine_t<1, 4, 8>(a, sm_count, stream, overlap_prev);
     }
 }
 

@@ -258,7 +258,7 @@ LuxBackendError moe_combine(LuxBackendContext* ctx, const lux_moe_combine_params
                            p.top_k, ys == 2, os == 2, vec};
     std::lock_guard<std::mutex> lk(c->mu);
     DeviceGuard g(c->dev->device());
-    LUX_CUDA_TRY(launch_moe_combine(a, c->stream, chain_is_open(c)));
+    LUX_CUDA_TRY(launch_moe_combine(a, c->dev->sm_count, c->stream, chain_is_open(c)));
     c->launches++;
     c->last_kernel = "moe_combine";
     note_outputs(c, o, COUNT);
