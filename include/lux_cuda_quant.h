@@ -400,7 +400,8 @@ typedef struct lux_gpu_quant_vtbl {
      * x, scales and biases BF16; bias fp32 [N]; residual F32 or BF16; y F32 or BF16.  The sum, the bias, the activation and the residual
      * are taken in fp32 and rounded once (for many rows, as in qmatmul and qmatmul_experts, by the tensor cores, whose fp32 sums cut off what
      * does not fit: 1 to 3e-6 of y).  bias or residual may be NULL: nothing is added.  y may be residual itself (of the same type);
-     * otherwise it overlaps nothing that is read.  Any M.  (The reference has op_matmul_f32, backend_plugin.h:129, then op_add_f32 and the
+     * otherwise it overlaps nothing that is read.  Any M; above 16 rows K should be a multiple of 64 and y begin on a 16-byte boundary, or the rows go
+     * sixteen at a time, the weights read again for each sixteen.  (The reference has op_matmul_f32, backend_plugin.h:129, then op_add_f32 and the
      * unary ops as calls of their own.) */
     LuxBackendError (*qmatmul_epi)(LuxBackendContext* ctx, const lux_qmm_epi_params* params, LuxBackendBuffer* x, LuxBackendBuffer* wq,
                                    LuxBackendBuffer* scales, LuxBackendBuffer* biases, LuxBackendBuffer* bias, LuxBackendBuffer* residual,
@@ -413,7 +414,7 @@ typedef struct lux_gpu_quant_vtbl {
      * moe_route: logits F32 or BF16 [tokens][experts].  A token's experts, best first, are those of the top_k largest logits or, with `bias`
      * (fp32 [experts], SCORE_SIGMOID only), of the largest sigmoid(logit) + bias, taken in fp64; of equals the lowest index first.  An
      * expert whose logit is -infinity or NaN is not chosen, nor one whose bias is; a slot for which no expert is left gets id -1 and weight 0.
-     *   SCORE_SOFTMAX: weight = exp(logit - max) / sum over the token's experts (logits equal to the largest count as exp(0), infinite ones too);
+     *   SCORE_SOFTMAX: weight = exp(logit - max) / sum of that over all experts, chosen or not (logits equal to the largest count as exp(0), infinite ones too);
      *   SCORE_SIGMOID: weight = 1 / (1 + exp(-logit));
      *   renorm: divided by the sum of the token's weights (0 where that is 0);     all times `scale`.  Weights are taken in fp32.
      * ids int32 [tokens][top_k], weights fp32 [tokens][top_k];
@@ -432,7 +433,8 @@ typedef struct lux_gpu_quant_vtbl {
      * wq, scales and biases as qmatmul's, one expert's [N][...] after the other's; x, scales, biases BF16; bias fp32 [experts][N] or NULL; y F32
      * or BF16, sums, bias and activation in fp32 and rounded once.  Rows of y that belong to no expert are left as they were.  Offsets
      * are cut to [0, rows] and an expert whose offsets fall has no rows (where the cut ones overlap, it is not said which rows are computed); x
-     * counts as zero where a row of it does not exist.  K a multiple of the group.  A row's result depends on nothing but the row and its
+     * counts as zero where a row of it does not exist.  K a multiple of the group; for more than a few rows an expert it should be one of 64, or the rows
+     * go eight at a time, the weights read again for each eight.  A row's result depends on nothing but the row and its
      * expert, in calls with the same parameters. */
     LuxBackendError (*qmatmul_experts)(LuxBackendContext* ctx, const lux_experts_params* params, LuxBackendBuffer* x, LuxBackendBuffer* order,
                                        LuxBackendBuffer* offsets, LuxBackendBuffer* wq, LuxBackendBuffer* scales, LuxBackendBuffer* biases,

@@ -1,8 +1,9 @@
 // Products grouped by expert for many rows an expert (qmatmul_experts), bf16 activations, affine weights:
 //   y[i] = epilogue(x[row(i)] . dequant(Wq[e])^T + bias[e]),   offsets[e] <= i < offsets[e+1]
 // The roles of qmm_tc.cu's kernels on tiles of 128 rows of an expert's W (on pairs of CTAs: two neighbouring ones) against up to bm of its rows of x;
-// tensor-bound where experts have 150 rows and more, bound by dequantisation below (a k-stage of 128 takes 0.36 us of it at
-// 4 bit, 0.46 at 8, whatever the rows).
+// bound by dequantisation for few rows (32 an expert: a k-stage of 128 takes 0.34 us at 4 bit, 0.53 at 8, the tensor pipe is active 12 and 10 % of the time), by
+// that and by last rounds of tiles that are not full for more (16 experts, 4096 x 2816 gated, 4 bit: 128 rows 41 % of the tensor pipe and 925 TFLOP/s, 256
+// rows 51 % and 1121, 512 rows 65 % and 1278; 256 rows at 8 bit 41 % and 865).
 //   * The tiles follow from the offsets in device memory: every CTA scans them at its start (an expert's rows are cut into as few tiles as
 //     bm allows, all of one height), then takes every gridDim.x-th tile of the whole list; neighbouring CTAs share an expert's weights or
 //     rows of x at the same time.

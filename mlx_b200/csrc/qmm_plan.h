@@ -46,15 +46,16 @@ struct GemmPlan {
 // memory) is documented for multiples of 32 only, so a pair's tiles are that high whatever is left of M.
 //
 // Schedule and height go by a rough estimate of the time in microseconds, not a fit: on 392 shapes (32 to 2048 rows, K 512 to
-// 8192, N 256 to 11008) it takes the fastest of the three kernels or one within 4 % of it on 377, within 20 % at worst, but
-// the times themselves are off by up to a third for low tiles (48 rows: 0.64 us a stage measured, 0.50 here).  A k-stage of a tile costs about 0.45 + 0.001 * bm whatever the kernel (dequantisation, then the
-// MMAs), so a lower tile pays where it saves no round of tiles: 777 x 2880 x 5003 took 35.6 us in 208-row tiles and
+// 8192, N 256 to 11008) it takes the fastest of the three kernels or one within 4 % of it on 356, 40 % off at worst (34 x 1792 x 2781 at 4
+// bit: stream-K 14.5 us, whole tiles 10.4), and the times themselves are off by up to a third for low tiles.  (On 377 and 20 % before
+// dequantisation last became faster, whole tiles most; kept, since another schedule adds in another order and would change calls' last bits.)
+// A k-stage of a tile costs about 0.45 + 0.001 * bm whatever the kernel (dequantisation, then the MMAs), so a lower tile pays where it saves no round of tiles: 777 x 2880 x 5003 took 35.6 us in 208-row tiles and
 // 30.8 in 112-row ones, two rounds either way.
 //   whole tiles: ceil(T/G) rounds, each with an epilogue of 3 * bm/256 that nothing else overlaps;
 //   CTA pairs:   rounds of pair tiles; the epilogue overlaps where y leaves by TMA; 3 to set up;
 //   stream-K:    T*nst/G stages of up to 1.6 times the cost, an epilogue more, and the exchange of partials.
 // A residual makes every epilogue longer, least where it is no more than that of whole tiles of one CTA (2048 x 4096 x 4096, bf16: 61.8 us; pairs,
-// whose stores no longer hide it, 66.1; stream-K, which spills, 109; 64 rows 24.7, 26.9, 27.1).
+// whose stores no longer hide it, 66.1; stream-K, which spills, 109; 64 rows 24.7, 26.9, 27.1).  Its terms rest on these two shapes.
 inline bool choose_gemm_plan(const GemmShape& a, int sm_count, const GemmForce& force, bool no_ytma, GemmPlan* pl) {
     pl->n_tiles = (a.N + kTileN - 1) / kTileN;
     const double G = sm_count, nst = (a.K / kBK + kSub - 1) / kSub;

@@ -267,7 +267,7 @@ struct TileIter {
 // The CTA's stages are counted 0, 1, 2, ... along its sequence of segments, alike in every role; dequantising group g owns
 // the counts = g (mod GROUPS).
 //
-// One thread: the packed weights, unit after unit into the ring of the group that owns the stage.  Three stages at a time,
+// One thread: the packed weights, unit after unit into the ring of the group that owns the stage.  GROUPS stages at a time,
 // one for each group: first units first, so that with a single slot per group no group waits for another's second unit
 // (8 bit).  Every stage is UPS units, so that the rings advance alike; the odd sub-block's partner is announced without a load.
 // at(seg): where the tile's weights lie (two ints, whatever they mean to load); load(dst, first byte of the rows, at, barrier).
@@ -312,7 +312,7 @@ __device__ __forceinline__ void weight_producer(const Prm& p, Seg seg, int nks, 
 }
 // One warp (lane quarter of group grp; a warp may only touch its own quarter of the TMEM lanes): the thread owns row r of
 // every tile.  There are as many stages in flight as groups, so a group always writes the same slot.
-// What bounds it is its instructions, three such warps to a scheduler, and the instruction caches that all roles share;
+// What bounds it is its instructions, GROUPS such warps to a scheduler, and the instruction caches that all roles share;
 // hence row pointers per tile (a division each), one copy of the code for both sub-blocks, one arrival per warp.
 // A group always writes the same slot of the A ring: `empty` and a_tmem are its, arrive() says that it is full.
 // row_of(seg, r): the row of wq, scales and biases that is row r of the tile.
@@ -391,7 +391,7 @@ __device__ __forceinline__ void dequant_role(const Prm& p, Seg seg, int grp, int
         const uint32_t s_lo = sp[0], b_lo = bp[0], s_hi = sp[1], b_hi = bp[1];
         st += GROUPS;
         if (st >= end) settle();
-        // Three stages ahead of its use.  At 4 bit behind the proxy fence, which would wait for these loads too (777 rows in
+        // GROUPS stages ahead of its use.  At 4 bit behind the proxy fence, which would wait for these loads too (777 rows in
         // groups of 32: 30.9 against 33-40 us); at 8 bit, with a fence per sub-block, here (512 x 8192 x 28672: 204 against 257).
         if (UPS == 2 && more) fetch_sb();
         bool ok = true;

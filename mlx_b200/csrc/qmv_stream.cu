@@ -335,7 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) qmv_stream_kernel(const __grid_co
 
     std::conditional_t<kExperts, GroupWalk<kGroupRows>, Walk> wk;
     if constexpr (kExperts) {
-        // (which weights are wanted is the previous kernel's answer: there is nothing to fetch ahead of it)
+        // (which weights are wanted stands in the offsets, which a kernel still at work may be writing; so nothing is fetched ahead of the wait, not even
+        // where that kernel, as ahead of a layer's second product, writes x alone)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         int* const off = reinterpret_cast<int*>(smem + p.tables_off);
